@@ -505,6 +505,87 @@ int mfq_low_rank_gradient(const void* g, const void* bf, const void* tf, int dty
 int mfq_low_rank_up(const void* x, const void* tf, int dtype, int64_t M, int64_t K, int64_t rank, int64_t R,
                     void* out, void* stream);
 
+/*
+ * Rotary tables: cos[i][p] = factor * cos(positions[i][axis[p]] * frequencies[p]), sin the same, evaluated in
+ * float64 and rounded once.  positions [n, axes] int32; frequencies and axis: `pairs` values each, HOST
+ * pointers, read before the call returns; cos, sin [n, pairs] float32.  At most MFQ_ROTARY_MAX_PAIRS pairs.
+ */
+#define MFQ_ROTARY_MAX_PAIRS 256
+int mfq_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, const double* frequencies,
+                      const uint8_t* axis, float factor, float* cos, float* sin, void* stream);
+
+/*
+ * Rotary positions of q and k with the RMS norm of their heads in front (AttentionUtils.process_qkv and
+ * apply_rope, src/mflux/models/flux/model/flux_transformer/common/attention_utils.py), and the gradients.
+ *   x       [batch, tokens, heads, dim], the last axis dense, the others by x_stride (elements)
+ *   weight  [dim] of the norm, NULL: no norm
+ *   out     forward: the result, backward: the gradient of x (NULL: not wanted); densely packed
+ *   dy      backward: the gradient of the result, as x by dy_stride
+ *   dweight backward: [dim], NULL: not wanted; needs weight
+ * k.heads == 0: no second tensor.  Backward reads x where there is a weight, and not otherwise.
+ * The first `rotated` channels (even) turn, pairs (i, i + rotated / 2) for MFQ_ROTARY_HALF, (2i, 2i + 1) for
+ * MFQ_ROTARY_INTERLEAVED; the others pass.  cos, sin [table_rows, rotated / 2] float32; a token's row is
+ * positions[b * position_batch + token], or its place in its entry without positions, clamped to the table.
+ * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16; dim even, at most 512.  Any alignment of elements; 16-byte aligned
+ * pointers and strides of whole 16 bytes load wider.  No array may overlap another that is written.
+ * workspace: mfq_rotary_workspace_bytes() of it, 16-byte aligned, for the backward pass of a weight.
+ */
+enum mfq_rotary_layout { MFQ_ROTARY_INTERLEAVED = 0, MFQ_ROTARY_HALF = 1 };
+typedef struct mfq_rotary_tensor {
+  const void *x, *dy, *weight;
+  void *out, *dweight;
+  int64_t x_stride[3], dy_stride[3]; /* batch, token, head */
+  int64_t heads;
+} mfq_rotary_tensor;
+typedef struct mfq_rotary_args {
+  int32_t dtype, layout, dim, rotated;
+  int64_t batch, tokens, table_rows, position_batch;
+  const float *cos, *sin;
+  const int32_t* positions;
+  float eps;
+  mfq_rotary_tensor q, k;
+} mfq_rotary_args;
+size_t mfq_rotary_workspace_bytes(const mfq_rotary_args* args);
+int mfq_rotary(const mfq_rotary_args* args, void* stream);
+int mfq_rotary_backward(const mfq_rotary_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * y = softmax(scale q k^T + mask) v (mx.fast.scaled_dot_product_attention,
+ * src/mflux/models/flux/model/flux_transformer/common/attention_utils.py:49), and its gradients.
+ *   q, y, dy  [batch, q_tokens, heads, dim]      packed: [q_tokens, heads, dim]
+ *   k, v      [batch, k_tokens, kv_heads, dim]   packed: [k_tokens, kv_heads, dim]
+ * 16-bit type dtype, the last axis dense, the others by stride (elements, multiples of 8; the token's below
+ * 2^24), 16-byte aligned; out, dq, dk, dv densely packed.  heads a multiple of kv_heads: head h reads key
+ * head h / (heads / kv_heads).  dim a multiple of 8 up to 256.
+ * Sequences: an entry each, of q_lengths[b] queries and k_lengths[b] keys (NULL: all); or packed, q_offsets and
+ * k_offsets non-NULL, batch + 1 non-decreasing values each, sequence s having the rows [offsets[s], offsets[s + 1]).
+ * Both are device memory: values outside the tensors are clamped to them (decreasing offsets give
+ * unspecified values, never an access outside the arrays).
+ * causal: query i of n sees the keys up to i + m - n of m.  A query that sees no key, and every row that no
+ * sequence holds, gets zeros.  What a query does not see does not reach it, infinities and NaN included.
+ * Softmax and sums in float32, the probabilities rounded to dtype for the second product.  scale > 0.
+ *   lse    [heads, rows] float32, rows = q_tokens or batch * q_tokens: written by the forward pass if not NULL,
+ *          read by the backward pass (which needs it, y, dy, and delta of the same size to write to)
+ *   dq, dk, dv  backward: NULL where not wanted
+ * workspace: mfq_attention_workspace_bytes() of it (few queries against many keys), 16-byte aligned.
+ */
+typedef struct mfq_attention_tensor {
+  const void* p;
+  int64_t stride[3]; /* batch, token, head */
+} mfq_attention_tensor;
+typedef struct mfq_attention_args {
+  int32_t dtype, causal, dim;
+  float scale;
+  int64_t batch, heads, kv_heads, q_tokens, k_tokens;
+  mfq_attention_tensor q, k, v, y, dy;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;
+  const int32_t *q_offsets, *k_offsets, *q_lengths, *k_lengths;
+} mfq_attention_args;
+size_t mfq_attention_workspace_bytes(const mfq_attention_args* args);
+int mfq_attention(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int mfq_attention_backward(const mfq_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

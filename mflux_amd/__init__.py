@@ -6,8 +6,10 @@ from . import lora, nn, weights
 from .core import (PreparedWeights, dequantize, dequantize_rows, gelu_approx, layer_norm_modulate, prepare_weights, quantize,
                    quantized_matmul,
                    quantized_matmul_epilogue, quantized_matmul_prepared, silu, silu_quantized_matmul)
+from .heads import attention, rotary, rotary_tables
 
 __all__ = ["nn", "lora", "weights", "quantize", "dequantize", "dequantize_rows", "quantized_matmul",
            "quantized_matmul_epilogue", "silu", "gelu_approx", "silu_quantized_matmul", "layer_norm_modulate",
-           "prepare_weights", "quantized_matmul_prepared", "PreparedWeights"]
+           "prepare_weights", "quantized_matmul_prepared", "PreparedWeights",
+           "rotary_tables", "rotary", "attention"]
 __version__ = "0.1.0"

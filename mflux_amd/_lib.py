@@ -18,6 +18,32 @@ EPILOGUE_GELU, EPILOGUE_GATE_RESIDUAL, EPILOGUE_SWIGLU = 1, 2, 3
 KERNEL_MATVEC, KERNEL_SLICED, KERNEL_WIDE, KERNEL_TILES_128, KERNEL_TILES_256, KERNEL_TWO_KERNELS = range(1, 7)
 MFQ_ESCRATCH = -9  # mfq_qmm_t_static: the K split needs more than the built-in buffer
 
+ROTARY_LAYOUTS = {"interleaved": 0, "half": 1}
+
+
+class RotaryTensor(ctypes.Structure):  # mfq_rotary_tensor
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "dy", "weight", "out", "dweight")] + [
+        ("x_stride", ctypes.c_int64 * 3), ("dy_stride", ctypes.c_int64 * 3), ("heads", ctypes.c_int64)]
+
+
+class RotaryArgs(ctypes.Structure):  # mfq_rotary_args
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "layout", "dim", "rotated")] + [
+        (n, ctypes.c_int64) for n in ("batch", "tokens", "table_rows", "position_batch")] + [
+        (n, ctypes.c_void_p) for n in ("cos", "sin", "positions")] + [
+        ("eps", ctypes.c_float), ("q", RotaryTensor), ("k", RotaryTensor)]
+
+
+class AttentionTensor(ctypes.Structure):  # mfq_attention_tensor
+    _fields_ = [("p", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
+
+
+class AttentionArgs(ctypes.Structure):  # mfq_attention_args
+    _fields_ = [("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("dim", ctypes.c_int32), ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_tokens", "k_tokens")] + [
+        (n, AttentionTensor) for n in ("q", "k", "v", "y", "dy")] + [
+        (n, ctypes.c_void_p) for n in ("out", "dq", "dk", "dv", "lse", "delta", "q_offsets", "k_offsets", "q_lengths", "k_lengths")]
+
+
 # every symbol include/mfq.h declares, with its ctypes signature
 _I64, _INT, _PTR = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
 SIGNATURES = {
@@ -57,6 +83,13 @@ SIGNATURES = {
     "mfq_low_rank_forward": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _I64, _PTR, _PTR, _PTR]),
     "mfq_low_rank_gradient": (_INT, [_PTR, _PTR, _PTR, _INT, _I64, _I64, _I64, _I64, ctypes.c_float, _PTR, _PTR, _PTR, _PTR]),
     "mfq_low_rank_up": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _I64, _PTR, _PTR]),
+    "mfq_rotary_tables": (_INT, [_PTR, _I64, _INT, _INT, _PTR, _PTR, ctypes.c_float, _PTR, _PTR, _PTR]),
+    "mfq_rotary_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RotaryArgs)]),
+    "mfq_rotary": (_INT, [ctypes.POINTER(RotaryArgs), _PTR]),
+    "mfq_rotary_backward": (_INT, [ctypes.POINTER(RotaryArgs), _PTR, ctypes.c_size_t, _PTR]),
+    "mfq_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+    "mfq_attention": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
+    "mfq_attention_backward": (_INT, [ctypes.POINTER(AttentionArgs), _PTR]),
     "mfq_low_rank_add": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _PTR, _INT, _PTR]),
 }
 

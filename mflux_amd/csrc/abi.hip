@@ -1,6 +1,7 @@
 // C ABI of libmfq.so: argument validation and dispatch.  No kernel is
 // launched unless every check has passed, so a caller's mistake is an error
 // code and never a device fault.
+#include "attention.h"
 #include "common.h"
 
 namespace {
@@ -447,6 +448,135 @@ int mfq_low_rank_add(const void* t, const void* bs, int dtype, int64_t M, int64_
   low_rank.bs = bs;
   low_rank.R = (int)rank;
   return mfq::launch_low_rank_add(dtype, low_rank, M, N, y, y_dtype, (hipStream_t)stream);
+}
+
+int mfq_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, const double* frequencies, const uint8_t* axis, float factor,
+                      float* cos, float* sin, void* stream) {
+  if (n <= 0 || axes <= 0 || axes > 255 || pairs <= 0 || pairs > MFQ_ROTARY_MAX_PAIRS || n > ((int64_t)1 << 31)) return MFQ_ESHAPE;
+  if (n * pairs > ((int64_t)1 << 38)) return MFQ_ESHAPE;
+  if (!positions || !frequencies || !axis || !cos || !sin) return MFQ_ENULL;
+  for (int i = 0; i < pairs; ++i)
+    if (axis[i] >= axes) return MFQ_ESHAPE;
+  return mfq::launch_rotary_tables(positions, n, axes, pairs, frequencies, axis, factor, cos, sin, (hipStream_t)stream);
+}
+
+static int check_rotary(const mfq_rotary_args* a, bool backward, bool* wide) {
+  if (!a) return MFQ_ENULL;
+  if (!known(a->dtype)) return MFQ_EDTYPE;
+  if (a->layout != MFQ_ROTARY_HALF && a->layout != MFQ_ROTARY_INTERLEAVED) return MFQ_ESHAPE;
+  if (a->dim <= 0 || a->dim > 512 || a->dim % 2 || a->rotated < 0 || a->rotated > a->dim || a->rotated % 2) return MFQ_ESHAPE;
+  if (a->batch <= 0 || a->tokens <= 0 || a->batch > INT32_MAX || a->tokens > INT32_MAX || a->batch * a->tokens > ((int64_t)1 << 40)) return MFQ_ESHAPE;
+  if (a->table_rows <= 0 || a->table_rows > INT32_MAX || a->position_batch < 0) return MFQ_ESHAPE;
+  if (a->q.heads <= 0 || a->k.heads < 0 || a->q.heads > 65536 || a->k.heads > 65536) return MFQ_ESHAPE;
+  if (!(a->eps >= 0.f)) return MFQ_ESHAPE;
+  if (a->rotated && (!a->cos || !a->sin)) return MFQ_ENULL;
+  const int64_t per16 = a->dtype == MFQ_F32 ? 4 : 8;
+  *wide = mfq::aligned16(a->cos) && mfq::aligned16(a->sin);
+  for (const mfq_rotary_tensor* t : {&a->q, &a->k}) {
+    if (!t->heads) continue;
+    if ((!backward || t->weight) && !t->x) return MFQ_ENULL;
+    if (!backward && !t->out) return MFQ_ENULL;
+    if (backward && !t->dy) return MFQ_ENULL;
+    if (t->dweight && !t->weight) return MFQ_ENULL;
+    for (int i = 0; i < 3; ++i) {
+      if (t->x_stride[i] < 0 || t->dy_stride[i] < 0) return MFQ_ESHAPE;
+      *wide = *wide && t->x_stride[i] % per16 == 0 && (!backward || t->dy_stride[i] % per16 == 0);
+    }
+    *wide = *wide && mfq::aligned16(t->x) && mfq::aligned16(t->out) && mfq::aligned16(t->weight) && (!backward || mfq::aligned16(t->dy));
+    *wide = *wide && a->dim % per16 == 0;  // rows of the result
+  }
+  return MFQ_OK;
+}
+
+size_t mfq_rotary_workspace_bytes(const mfq_rotary_args* args) { return args ? mfq::rotary_workspace_bytes(*args) : 0; }
+
+int mfq_rotary(const mfq_rotary_args* args, void* stream) {
+  bool wide = false;
+  if (int rc = check_rotary(args, false, &wide)) return rc;
+  return mfq::launch_rotary(*args, wide, false, nullptr, (hipStream_t)stream);
+}
+
+int mfq_rotary_backward(const mfq_rotary_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  bool wide = false;
+  if (int rc = check_rotary(args, true, &wide)) return rc;
+  const size_t need = mfq::rotary_workspace_bytes(*args);
+  if (need && !workspace) return MFQ_ENULL;
+  if (need > workspace_bytes) return MFQ_ESCRATCH;
+  if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
+  return mfq::launch_rotary(*args, wide, true, static_cast<float*>(workspace), (hipStream_t)stream);
+}
+
+static int attention_call(const mfq_attention_args* a, bool backward, mfq::AttentionCall* c) {
+  if (!a) return MFQ_ENULL;
+  if (!is16(a->dtype)) return MFQ_EDTYPE;
+  if (a->dim <= 0 || a->dim > 256 || a->dim % 8) return MFQ_ESHAPE;
+  if (a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->heads > 65536) return MFQ_ESHAPE;
+  if (a->batch <= 0 || a->q_tokens <= 0 || a->k_tokens <= 0 || a->batch > (1 << 24)) return MFQ_ESHAPE;
+  if (a->q_tokens * a->heads > (1 << 30) || a->k_tokens > (1 << 30) || a->q_tokens > (1 << 30)) return MFQ_ESHAPE;
+  if (!(a->scale > 0.f) || a->scale > 1e30f) return MFQ_ESHAPE;
+  if ((a->q_offsets == nullptr) != (a->k_offsets == nullptr)) return MFQ_ENULL;
+  if (a->q_offsets && (a->q_lengths || a->k_lengths)) return MFQ_EUNSUPPORTED;
+  struct In {
+    const mfq_attention_tensor* t;
+    mfq::AttentionTensor* to;
+  } in[] = {{&a->q, &c->q}, {&a->k, &c->k}, {&a->v, &c->v}, {&a->y, &c->y}, {&a->dy, &c->dy}};
+  for (int i = 0; i < (backward ? 5 : 3); ++i) {
+    const mfq_attention_tensor& t = *in[i].t;
+    if (!t.p) return MFQ_ENULL;
+    if (!mfq::aligned16(t.p)) return MFQ_EALIGN;
+    for (int64_t s : t.stride)
+      if (s < 0) return MFQ_ESHAPE;
+      else if (s % 8) return MFQ_EALIGN;
+    if (t.stride[1] >= (1 << 24)) return MFQ_ESHAPE;
+    *in[i].to = {static_cast<const uint16_t*>(t.p), t.stride[0], t.stride[1], t.stride[2]};
+  }
+  if (!backward && !a->out) return MFQ_ENULL;
+  if (backward && (!a->lse || !a->delta || (!a->dq && !a->dk && !a->dv))) return MFQ_ENULL;
+  for (const void* p : {(const void*)a->out, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+    if (!mfq::aligned16(p)) return MFQ_EALIGN;
+  c->out = static_cast<uint16_t*>(a->out);
+  c->dq = static_cast<uint16_t*>(a->dq);
+  c->dk = static_cast<uint16_t*>(a->dk);
+  c->dv = static_cast<uint16_t*>(a->dv);
+  c->lse = a->lse;
+  c->delta = a->delta;
+  c->q_offsets = a->q_offsets;
+  c->k_offsets = a->k_offsets;
+  c->q_lengths = a->q_lengths;
+  c->k_lengths = a->k_lengths;
+  c->batch = (int)a->batch;
+  c->heads = (int)a->heads;
+  c->kv_heads = (int)a->kv_heads;
+  c->dim = a->dim;
+  c->q_tokens = (int)a->q_tokens;
+  c->k_tokens = (int)a->k_tokens;
+  c->causal = a->causal != 0;
+  c->scale = a->scale;
+  return MFQ_OK;
+}
+
+size_t mfq_attention_workspace_bytes(const mfq_attention_args* args) {
+  mfq::AttentionCall c;
+  if (attention_call(args, false, &c) != MFQ_OK) return 0;
+  return mfq::attention_split_bytes(c, mfq::attention_splits(c));
+}
+
+int mfq_attention(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  mfq::AttentionCall c;
+  if (int rc = attention_call(args, false, &c)) return rc;
+  const int splits = mfq::attention_splits(c);
+  if (!splits) return mfq::launch_attention(args->dtype, c, (hipStream_t)stream);
+  const size_t need = mfq::attention_split_bytes(c, splits);
+  if (need && !workspace) return MFQ_ENULL;
+  if (need > workspace_bytes) return MFQ_ESCRATCH;
+  if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
+  return mfq::launch_attention_split(args->dtype, c, splits, workspace, (hipStream_t)stream);
+}
+
+int mfq_attention_backward(const mfq_attention_args* args, void* stream) {
+  mfq::AttentionCall c;
+  if (int rc = attention_call(args, true, &c)) return rc;
+  return mfq::launch_attention_backward(args->dtype, c, (hipStream_t)stream);
 }
 
 }  // extern "C"

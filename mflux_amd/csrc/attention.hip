@@ -1,0 +1,103 @@
+// Attention over whole prompts and images: y = softmax(scale q k^T + mask) v for
+// batched or packed sequences, grouped heads, causal or not
+// (mx.fast.scaled_dot_product_attention in the reference,
+// src/mflux/models/flux/model/flux_transformer/common/attention_utils.py:49).
+//
+// One pass over the keys with the softmax's running maximum and sum in float32; the scores never leave the registers.
+// A workgroup of four wavefronts has 128 queries of one head, 32 a wavefront, and walks the keys 64 at a time: K and V
+// tiles go straight from memory into LDS (two of each, the next pair in flight while the current one is multiplied) and are
+// read by all four wavefronts.  See attention.h for the orientation of the products.
+#include "attention.h"
+
+namespace mfq {
+namespace {
+
+constexpr int kQueries = 128;  // of a workgroup
+constexpr int kKeys = 64;      // of a step
+
+constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, int kDim>
+__global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
+  constexpr int kPitch = pitch_of(kDim);
+  constexpr int kTileBytes = kKeys * kPitch * 2;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // K, V, K, V
+  const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
+  int head, index;
+  head_and_tile(blockIdx.x, c.heads, tiles, head, index);
+  const Run run = find_run<kQueries>(c, index, false, c.causal);
+  if (!run.valid) return;
+  const int kv_head = head / (c.heads / c.kv_heads);
+
+  const int row = run.tile * kQueries + wave * 32 + (lane & 31);  // of the run: the lane's query
+  const int limit = visible_keys(run, row, c.causal);
+  // keys that any query of the workgroup sees: the last one's, as limits grow along the rows
+  const int keys = uniform(run.tile * kQueries < run.nq ? visible_keys(run, min(run.tile * kQueries + kQueries, run.nq) - 1, c.causal) : 0);
+  const int least = wave_min(limit), most = wave_max(limit);
+
+  QueryState<T, kDim, kPitch> state;
+  state.init();
+  if (keys > 0) {
+    const int64_t q_at = run.batch * c.q.batch + (int64_t)(run.q0 + min(row, run.nq - 1)) * c.q.token + head * c.q.head;
+    state.load_row(state.q, c.q.p + q_at, c.dim, lane);
+    const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
+    const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
+    TileLoader<kPitch, kKeys, 256> load_k, load_v;
+    load_k.init(thread, c.k.token, c.dim);
+    load_v.init(thread, c.v.token, c.dim);
+    const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
+    const float scale = c.scale * kLog2e;
+    load_k.load(k, lds_at, keys, thread);
+    load_v.load(v, lds_at + kTileBytes, keys, thread);
+    for (int first = 0, buffer = 0; first < keys; first += kKeys, buffer ^= 1) {
+      arrive_and_sync();
+      const int next = first + kKeys;
+      if (next < keys) {
+        const uint32_t to = lds_at + (buffer ^ 1) * 2 * kTileBytes;
+        load_k.load(k + (int64_t)next * c.k.token, to, keys - next, thread);
+        load_v.load(v + (int64_t)next * c.v.token, to + kTileBytes, keys - next, thread);
+      }
+      const char* k_tile = lds + buffer * 2 * kTileBytes;
+      if (next <= least) state.template step<2, false>(k_tile, k_tile + kTileBytes, kKeys, scale, lane);
+      else if (first < most) state.template step<2, true>(k_tile, k_tile + kTileBytes, limit - first, scale, lane);
+    }
+  }
+  if (row >= run.rows) return;
+  const float sum = sum_halves(state.sum);
+  const int64_t at = (int64_t)run.batch * c.q_tokens + run.q0 + row;  // of the densely packed result
+  const bool seen = limit > 0;
+  store_row<T, kDim / 32>(c.out + (at * c.heads + head) * c.dim, state.o, seen ? 1.0f / sum : 0.f, c.dim, lane);
+  if (c.lse && lane < 32) {
+    const int64_t rows = (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens;
+    c.lse[head * rows + at] = seen ? state.top * (c.scale * kLog2e) + __builtin_amdgcn_logf(sum) : __builtin_inff();
+  }
+}
+
+template <typename T, int kDim>
+int launch(const AttentionCall& c, hipStream_t stream) {
+  constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
+  static PerDeviceInt configured;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim>), kBytes)) return MFQ_ELAUNCH;
+  // packed: a tile that is not full for every sequence at most, and for the rows in front of and behind them
+  const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
+  if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
+  hipLaunchKernelGGL((attention_kernel<T, kDim>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+  return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+}
+
+template <typename T>
+int launch_dim(const AttentionCall& c, hipStream_t stream) {
+  if (c.dim <= 64) return launch<T, 64>(c, stream);
+  if (c.dim <= 96) return launch<T, 96>(c, stream);
+  if (c.dim <= 128) return launch<T, 128>(c, stream);
+  if (c.dim <= 192) return launch<T, 192>(c, stream);
+  return launch<T, 256>(c, stream);
+}
+
+}  // namespace
+
+int launch_attention(int dtype, const AttentionCall& c, hipStream_t stream) {
+  return dtype == MFQ_BF16 ? launch_dim<BF16>(c, stream) : launch_dim<F16>(c, stream);
+}
+
+}  // namespace mfq

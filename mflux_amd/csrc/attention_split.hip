@@ -1,0 +1,223 @@
+// Attention of few queries against many keys (single tokens over a cache): y = softmax(scale q k^T + mask) v with the key axis
+// split over workgroups and joined behind them.
+//
+// Bound by the bytes of K and V, which are read once: the query heads that share a key head are the columns of one product (32
+// rows = tokens x heads of a group to a workgroup), and every wavefront streams key tiles of its own through a ring in LDS
+// that no other wavefront waits for.  The wavefronts of a workgroup are joined in LDS, the workgroups of a sequence by a second
+// launch over their float32 partial results (none if the axis is not split).
+#include "attention.h"
+
+#include <algorithm>
+
+namespace mfq {
+namespace {
+
+constexpr int kRows = 32;  // of a workgroup: (token, head of the group) pairs
+constexpr int kStep = 32;  // keys of a step of a wavefront
+
+constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+constexpr int waves_of(int dim) { return dim <= 128 ? 4 : 2; }
+
+template <typename T, int kDim>
+struct SplitShape {
+  static constexpr int kPitch = pitch_of(kDim), kWaves = waves_of(kDim), kStages = 2;
+  static constexpr int kTile = kStep * kPitch * 2;            // bytes
+  static constexpr int kRing = kStages * 2 * kTile;           // of a wavefront: K, V of each stage
+  static constexpr int kPart = kRows * (kDim + 4) * 4;        // a wavefront's result on its way to the others
+  static constexpr int kStats = kWaves * kRing;               // where its statistics lie
+  static constexpr int kLds = kStats + kWaves * kRows * 8;
+  static_assert(kPart <= kRing, "a wavefront's result fits its ring");
+};
+
+template <typename T, int kDim>
+__global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel(AttentionCall c, int tiles, int splits, float* part_o,
+                                                                                 float2* part_stats) {
+  using S = SplitShape<T, kDim>;
+  constexpr int kPitch = S::kPitch, kWaves = S::kWaves;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
+  // workgroups are dealt round-robin to the XCDs: the splits of a tile and head behind each other
+  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
+  const int kv_head = item % c.kv_heads, group = c.heads / c.kv_heads;
+  const Run run = find_run<kRows>(c, item / c.kv_heads, false, false, group);
+  if (!run.valid) return;
+
+  const int row = run.tile * kRows + (lane & 31), token = row / group, head = kv_head * group + row % group;
+  const int limit = visible_keys(run, token, c.causal);
+  const int most = wave_max(limit), least = wave_min(token < run.rows ? limit : INT32_MAX);
+  const int chunk = ((run.nk + splits - 1) / splits + kStep - 1) / kStep * kStep;
+  const int begin = split * chunk, end = min(min(begin + chunk, run.nk), most);
+
+  QueryState<T, kDim, kPitch> state;
+  state.init();
+  if (begin < end) {
+    const int64_t q_at = run.batch * c.q.batch + (int64_t)(run.q0 + min(token, run.nq - 1)) * c.q.token + head * c.q.head;
+    state.load_row(state.q, c.q.p + q_at, c.dim, lane);
+    const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
+    const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
+    TileLoader<kPitch, kStep, 64> load_k, load_v;
+    load_k.init(lane, c.k.token, c.dim);
+    load_v.init(lane, c.v.token, c.dim);
+    char* ring = lds + wave * S::kRing;
+    const uint32_t ring_at = (uint32_t)(uintptr_t)lds + wave * S::kRing;
+    const float scale = c.scale * kLog2e;
+    constexpr int kRequests = 2 * TileLoader<kPitch, kStep, 64>::kLoads;
+    auto request = [&](int first, int stage) __attribute__((always_inline)) {
+      load_k.load(k + (int64_t)first * c.k.token, ring_at + stage * 2 * S::kTile, run.nk - first, lane);
+      load_v.load(v + (int64_t)first * c.v.token, ring_at + stage * 2 * S::kTile + S::kTile, run.nk - first, lane);
+    };
+    const int first_tile = begin + wave * kStep;
+    if (first_tile < end) request(first_tile, 0);
+    int stage = 0;
+    for (int first = first_tile; first < end; first += kWaves * kStep, stage ^= 1) {
+      const int next = first + kWaves * kStep;
+      if (next < end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is overwritten
+        request(next, stage ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const char* tile = ring + stage * 2 * S::kTile;
+      if (first + kStep <= least) state.template step<1, false>(tile, tile + S::kTile, kStep, scale, lane);
+      else state.template step<1, true>(tile, tile + S::kTile, limit - first, scale, lane);
+    }
+  }
+
+  // join the wavefronts: their accumulators and statistics through LDS, rows of kDim + 4 floats
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  constexpr int kFloats = kDim + 4;
+  float* mine = reinterpret_cast<float*>(lds + wave * S::kRing) + (lane & 31) * kFloats;
+#pragma unroll
+  for (int b = 0; b < kDim / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4*>(mine + 32 * b + result_row(i, lane)) = f32x4{state.o[b][i], state.o[b][i + 1], state.o[b][i + 2], state.o[b][i + 3]};
+  float2* stats = reinterpret_cast<float2*>(lds + S::kStats);
+  const float sum = sum_halves(state.sum);
+  if (lane < 32) stats[wave * kRows + lane] = make_float2(state.top, sum);
+  __syncthreads();
+  const float c2 = c.scale * kLog2e;
+  const int64_t rows = (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens;
+  // a thread: four elements of a row at a time
+  for (int i = thread; i < kRows * (kDim / 4); i += kWaves * kWave) {
+    const int r = i / (kDim / 4), d = i % (kDim / 4) * 4;
+    const int p = run.tile * kRows + r, tok = p / group;
+    if (tok >= run.rows || d >= c.dim) continue;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w * kRows + r].x);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 st = stats[w * kRows + r];
+      // a part without keys has the factor 0; where the reference is an infinity the scores' own NaN stay
+      const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * c2);
+      total += st.y * f;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * S::kRing) + r * kFloats + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += a[e] * f;
+    }
+    const int64_t at = ((int64_t)run.batch * c.q_tokens + run.q0 + tok) * c.heads + kv_head * group + p % group;
+    if (splits == 1) {
+      const bool seen = visible_keys(run, tok, c.causal) > 0;
+      const float f = seen ? 1.0f / total : 0.f;
+      *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = u32x2{T::pack2(o[0] * f, o[1] * f), T::pack2(o[2] * f, o[3] * f)};
+      if (c.lse && d == 0)
+        c.lse[(at % c.heads) * rows + at / c.heads] = seen ? top * c2 + __builtin_amdgcn_logf(total) : __builtin_inff();
+    } else {
+      const int64_t slot = (int64_t)split * rows * c.heads + at;
+      *reinterpret_cast<f32x4*>(part_o + slot * c.dim + d) = o;
+      if (d == 0) part_stats[slot] = make_float2(top, total);
+    }
+  }
+}
+
+// y = the partial results of a row joined: a wavefront to a row, the lanes along the head
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows, int splits, const float* part_o, const float2* part_stats) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (at >= rows * c.heads) return;
+  const float c2 = c.scale * kLog2e;
+  float top = -__builtin_inff();
+  for (int s = lane; s < splits; s += kWave) top = fmaxf(top, part_stats[(int64_t)s * rows * c.heads + at].x);
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const int d = lane * 4;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float total = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const int64_t slot = (int64_t)s * rows * c.heads + at;
+    const float2 st = part_stats[slot];
+    const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * c2);
+    total += st.y * f;
+    if (d < c.dim) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(part_o + slot * c.dim + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += a[e] * f;
+    }
+  }
+  // a row that sees no key has neither a maximum nor a sum (a sum that is NaN is a row's own)
+  const bool empty = top == -__builtin_inff() && total == 0.f;
+  const float f = empty ? 0.f : 1.0f / total;
+  if (d < c.dim)
+    *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = u32x2{T::pack2(o[0] * f, o[1] * f), T::pack2(o[2] * f, o[3] * f)};
+  if (c.lse && lane == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + __builtin_amdgcn_logf(total);
+}
+
+int64_t rows_of(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens; }
+int64_t tiles_of(const AttentionCall& c) {
+  const int64_t group = c.heads / c.kv_heads;
+  return c.q_offsets ? c.q_tokens * group / kRows + c.batch + 2 : (c.q_tokens * group + kRows - 1) / kRows * c.batch;
+}
+
+template <typename T, int kDim>
+int launch(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
+  using S = SplitShape<T, kDim>;
+  static PerDeviceInt configured;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_split_kernel<T, kDim>), S::kLds)) return MFQ_ELAUNCH;
+  const int64_t tiles = tiles_of(c), rows = rows_of(c), grid = tiles * c.kv_heads * splits;
+  if (grid > INT32_MAX) return MFQ_ESHAPE;
+  float* part_o = workspace;
+  float2* part_stats = splits > 1 ? reinterpret_cast<float2*>(workspace + splits * rows * c.heads * c.dim) : nullptr;
+  hipLaunchKernelGGL((attention_split_kernel<T, kDim>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, (int)tiles, splits,
+                     part_o, part_stats);
+  if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
+  if (splits == 1) return MFQ_OK;
+  hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((rows * c.heads + 3) / 4)), dim3(256), 0, stream, c, rows, splits, part_o, part_stats);
+  return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+}
+
+template <typename T>
+int launch_dim(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
+  if (c.dim <= 64) return launch<T, 64>(c, splits, workspace, stream);
+  if (c.dim <= 96) return launch<T, 96>(c, splits, workspace, stream);
+  if (c.dim <= 128) return launch<T, 128>(c, splits, workspace, stream);
+  if (c.dim <= 192) return launch<T, 192>(c, splits, workspace, stream);
+  return launch<T, 256>(c, splits, workspace, stream);
+}
+
+}  // namespace
+
+int attention_splits(const AttentionCall& c) {
+  const int64_t group = c.heads / c.kv_heads;
+  // mean queries of a sequence
+  const int64_t queries = c.q_offsets ? (c.q_tokens + c.batch - 1) / std::max(c.batch, 1) : c.q_tokens;
+  if (queries * group > kRows) return 0;
+  const int64_t keys = c.q_offsets ? (c.k_tokens + c.batch - 1) / std::max(c.batch, 1) : c.k_tokens;
+  const int64_t items = std::max<int64_t>(tiles_of(c) - (c.q_offsets ? 2 : 0), 1) * c.kv_heads;
+  const int64_t most = std::max<int64_t>(keys / 256, 1);  // a split has 256 keys at least
+  return (int)std::min({most, (4 * (int64_t)compute_units() + items - 1) / items, (int64_t)256});
+}
+
+size_t attention_split_bytes(const AttentionCall& c, int splits) {
+  return splits > 1 ? (size_t)(splits * rows_of(c) * c.heads) * (c.dim + 2) * 4 : 0;
+}
+
+int launch_attention_split(int dtype, const AttentionCall& c, int splits, void* workspace, hipStream_t stream) {
+  return dtype == MFQ_BF16 ? launch_dim<BF16>(c, splits, (float*)workspace, stream) : launch_dim<F16>(c, splits, (float*)workspace, stream);
+}
+
+}  // namespace mfq

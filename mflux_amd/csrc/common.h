@@ -528,4 +528,10 @@ int launch_layer_norm_modulate(const void* x, int dtype, int64_t M, int64_t K, c
 int launch_splitk_reduce(int dtype, const void* planes, int splits, int64_t M, int64_t N, const void* bias, void* y,
                          int y_dtype, hipStream_t stream, Epilogue epi = Epilogue());
 
+// rotary tables, rotary positions and the heads' norm: see include/mfq.h.  wide: every pointer and stride is of whole 16 bytes
+int launch_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, const double* frequencies, const uint8_t* axis, float factor,
+                         float* cos, float* sin, hipStream_t stream);
+size_t rotary_workspace_bytes(const mfq_rotary_args& a);
+int launch_rotary(const mfq_rotary_args& a, bool wide, bool backward, float* workspace, hipStream_t stream);
+
 }  // namespace mfq

@@ -12,7 +12,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <limits>
 #include <tuple>
+#include <vector>
 
 #include "../../include/mfq.h"
 
@@ -387,6 +389,252 @@ void low_rank_add_(Tensor& y, const Tensor& t, const Tensor& bs) {
                                 t.size(1), y.data_ptr(), dtype_code(y.scalar_type(), "y"), stream_of(y)));
 }
 
+// ---- the heads of an attention block (include/mfq.h, mfq_rotary and mfq_attention)
+Tensor device_int32(const char* fn, const char* name, const Tensor& t, const Tensor& like) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt, fn, ": ", name, " must be int32 on ", like.device());
+  return t.contiguous();
+}
+
+std::tuple<Tensor, Tensor> rotary_tables(const Tensor& positions, const std::vector<double>& frequencies, const std::vector<int64_t>& axis,
+                                         double factor) {
+  TORCH_CHECK(positions.dim() == 2 && positions.scalar_type() == at::kInt && positions.is_contiguous(),
+              "mfq::rotary_tables: positions must be a contiguous int32 matrix");
+  TORCH_CHECK(frequencies.size() == axis.size() && !axis.empty() && axis.size() <= MFQ_ROTARY_MAX_PAIRS,
+              "mfq::rotary_tables: an axis for every frequency");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(positions.device());
+  uint8_t of[MFQ_ROTARY_MAX_PAIRS];
+  for (size_t i = 0; i < axis.size(); ++i) {
+    TORCH_CHECK(axis[i] >= 0 && axis[i] < positions.size(1), "mfq::rotary_tables: no such axis");
+    of[i] = (uint8_t)axis[i];
+  }
+  const int64_t n = positions.size(0), pairs = (int64_t)axis.size();
+  Tensor cos = at::empty({n, pairs}, positions.options().dtype(at::kFloat)), sin = at::empty_like(cos);
+  if (n == 0) return {cos, sin};
+  check_status("mfq_rotary_tables",
+               mfq_rotary_tables(positions.data_ptr<int32_t>(), n, (int)positions.size(1), (int)pairs, frequencies.data(), of, (float)factor,
+                                 cos.data_ptr<float>(), sin.data_ptr<float>(), stream_of(positions)));
+  return {cos, sin};
+}
+
+// x [B, S, H, D]; what has no dense last axis is copied
+Tensor dense_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+void set_strides(int64_t (&to)[3], const Tensor& t) {
+  for (int i = 0; i < 3; ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+struct RotaryOperands {
+  mfq_rotary_args a = {};
+  std::vector<Tensor> keep;  // what the pointers point into
+
+  RotaryOperands(const char* fn, const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                 const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight, const c10::optional<Tensor>& k_weight,
+                 int64_t layout, double eps) {
+    TORCH_CHECK(q.dim() == 4 && cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": q [B, S, H, D], cos and sin [P, R / 2]");
+    TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.device() == q.device() && sin.device() == q.device(),
+                fn, ": cos and sin must be float32 on ", q.device());
+    a.dtype = dtype_code(q.scalar_type(), "q");
+    a.layout = (int32_t)layout;
+    a.dim = (int32_t)q.size(3);
+    a.rotated = (int32_t)cos.size(1) * 2;
+    a.batch = q.size(0);
+    a.tokens = q.size(1);
+    a.table_rows = cos.size(0);
+    a.eps = (float)eps;
+    keep.push_back(cos.contiguous());
+    a.cos = keep.back().data_ptr<float>();
+    keep.push_back(sin.contiguous());
+    a.sin = keep.back().data_ptr<float>();
+    if (positions.has_value()) {
+      TORCH_CHECK(positions->dim() == 2 && positions->size(1) == a.tokens && (positions->size(0) == a.batch || positions->size(0) == 1), fn,
+                  ": positions [B, S] or [1, S]");
+      keep.push_back(device_int32(fn, "positions", *positions, q));
+      a.positions = keep.back().data_ptr<int32_t>();
+      a.position_batch = positions->size(0) > 1 ? a.tokens : 0;
+    } else {
+      TORCH_CHECK(cos.size(0) >= a.tokens, fn, ": the tables are shorter than the tokens");
+    }
+    tensor(fn, a.q, q, q_weight, q);
+    if (k.has_value()) tensor(fn, a.k, *k, k_weight, q);
+  }
+  void tensor(const char* fn, mfq_rotary_tensor& to, const Tensor& t, const c10::optional<Tensor>& weight, const Tensor& q) {
+    TORCH_CHECK(t.dim() == 4 && t.scalar_type() == q.scalar_type() && t.device() == q.device() && t.size(0) == q.size(0) &&
+                    t.size(1) == q.size(1) && t.size(3) == q.size(3) && t.size(2) > 0,
+                fn, ": q and k must agree in type, device and all axes but the heads");
+    keep.push_back(dense_rows(t));
+    to.x = keep.back().data_ptr();
+    set_strides(to.x_stride, keep.back());
+    to.heads = t.size(2);
+    if (weight.has_value()) {
+      TORCH_CHECK(weight->dim() == 1 && weight->size(0) == q.size(3) && weight->scalar_type() == q.scalar_type() && weight->device() == q.device(),
+                  fn, ": a weight must be a [D] vector of q's type");
+      keep.push_back(weight->contiguous());
+      to.weight = keep.back().data_ptr();
+    }
+  }
+  void gradient(const char* fn, mfq_rotary_tensor& to, const Tensor& dy, const Tensor& x) {
+    TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(), fn,
+                ": a gradient must be as its tensor");
+    keep.push_back(dense_rows(dy));
+    to.dy = keep.back().data_ptr();
+    set_strides(to.dy_stride, keep.back());
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                                  const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
+                                  const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  RotaryOperands o("mfq::rotary", q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
+  Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.has_value() ? k->sizes() : at::IntArrayRef({0}), q.options());
+  if (q.numel() == 0) return {yq, yk};
+  o.a.q.out = yq.data_ptr();
+  if (k.has_value()) o.a.k.out = yk.data_ptr();
+  check_status("mfq_rotary", mfq_rotary(&o.a, stream_of(q)));
+  return {yq, yk};
+}
+
+// (dq, dk, the weights' gradients); what there is not comes back empty
+std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_backward(const Tensor& dyq, const c10::optional<Tensor>& dyk, const Tensor& q,
+                                                           const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                                                           const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
+                                                           const c10::optional<Tensor>& k_weight, int64_t layout, double eps, bool want_x,
+                                                           bool want_q_weight, bool want_k_weight) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  TORCH_CHECK(k.has_value() == dyk.has_value(), "mfq::rotary_backward: a gradient for each tensor");
+  TORCH_CHECK((!want_q_weight || q_weight.has_value()) && (!want_k_weight || k_weight.has_value()), "mfq::rotary_backward: no such weight");
+  RotaryOperands o("mfq::rotary_backward", q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
+  o.gradient("mfq::rotary_backward", o.a.q, dyq, q);
+  if (k.has_value()) o.gradient("mfq::rotary_backward", o.a.k, *dyk, *k);
+  const Tensor none = at::empty({0}, q.options());
+  Tensor dq = want_x ? at::empty(q.sizes(), q.options()) : none, dk = want_x && k.has_value() ? at::empty(k->sizes(), q.options()) : none;
+  Tensor dwq = want_q_weight ? at::empty({q.size(3)}, q.options()) : none, dwk = want_k_weight ? at::empty({q.size(3)}, q.options()) : none;
+  if (q.numel() == 0) return {dq, dk, dwq.zero_(), dwk.zero_()};
+  if (want_x) {
+    o.a.q.out = dq.data_ptr();
+    if (k.has_value()) o.a.k.out = dk.data_ptr();
+  }
+  if (want_q_weight) o.a.q.dweight = dwq.data_ptr();
+  if (want_k_weight) o.a.k.dweight = dwk.data_ptr();
+  const size_t bytes = mfq_rotary_workspace_bytes(&o.a);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_status("mfq_rotary_backward", mfq_rotary_backward(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  return {dq, dk, dwq, dwk};
+}
+
+// A tensor of mfq_attention: rows of whole 16 bytes at whole 16 bytes; anything else is copied
+void attention_tensor(std::vector<Tensor>& keep, mfq_attention_tensor& to, const Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= 0));
+  const int64_t token = t.dim() - 3;
+  ok = ok && (t.size(token) <= 1 || t.stride(token) < (1 << 24));
+  keep.push_back(ok ? t : t.clone(at::MemoryFormat::Contiguous));
+  const Tensor& k = keep.back();
+  to.p = k.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    const int64_t axis = token - 1 + i;
+    to.stride[i] = axis >= 0 && k.size(axis) > 1 ? k.stride(axis) : 0;
+  }
+}
+
+struct AttentionOperands {
+  mfq_attention_args a = {};
+  std::vector<Tensor> keep;
+
+  AttentionOperands(const char* fn, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                    const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
+                    bool causal, double scale) {
+    const bool packed = q_offsets.has_value();
+    const int64_t d = packed ? 3 : 4;
+    TORCH_CHECK(k_offsets.has_value() == packed && q.dim() == d && k.dim() == d && v.sizes() == k.sizes(), fn,
+                ": q [B, S, H, D] and k, v [B, S, Hkv, D], or packed without the batch and with both offsets");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && k.device() == q.device() && v.device() == q.device() &&
+                    q.size(-1) == k.size(-1) && (packed || q.size(0) == k.size(0)),
+                fn, ": q, k and v must agree in type, device, head size and batch");
+    a.dtype = dtype_code(q.scalar_type(), "q");
+    a.causal = causal;
+    a.dim = (int32_t)q.size(-1);
+    a.scale = (float)scale;
+    a.heads = q.size(-2);
+    a.kv_heads = k.size(-2);
+    a.q_tokens = q.size(-3);
+    a.k_tokens = k.size(-3);
+    keep.reserve(16);
+    if (packed) {
+      TORCH_CHECK(q_offsets->dim() == 1 && q_offsets->size(0) >= 2 && k_offsets->sizes() == q_offsets->sizes(), fn,
+                  ": offsets of one more value than there are sequences");
+      a.batch = q_offsets->size(0) - 1;
+      a.q_offsets = ints(fn, "q_offsets", q_offsets, q);
+      a.k_offsets = ints(fn, "k_offsets", k_offsets, q);
+    } else {
+      a.batch = q.size(0);
+      for (const auto* l : {&q_lengths, &k_lengths})
+        TORCH_CHECK(!l->has_value() || ((*l)->dim() == 1 && (*l)->size(0) == a.batch), fn, ": lengths of one value an entry");
+      a.q_lengths = ints(fn, "q_lengths", q_lengths, q);
+      a.k_lengths = ints(fn, "k_lengths", k_lengths, q);
+    }
+    attention_tensor(keep, a.q, q);
+    attention_tensor(keep, a.k, k);
+    attention_tensor(keep, a.v, v);
+  }
+  const int32_t* ints(const char* fn, const char* name, const c10::optional<Tensor>& t, const Tensor& q) {
+    if (!t.has_value()) return nullptr;
+    keep.push_back(device_int32(fn, name, *t, q));
+    return keep.back().data_ptr<int32_t>();
+  }
+  int64_t rows() const { return (a.q_offsets ? 1 : a.batch) * a.q_tokens; }
+};
+
+// (y, log-sum-exps or an empty tensor)
+std::tuple<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                                     const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
+                                     const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool want_lse) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  AttentionOperands o("mfq::attention", q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
+  Tensor y = at::empty(q.sizes(), q.options());
+  Tensor lse = want_lse ? at::empty({o.a.heads, o.rows()}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {y, lse};
+  if (k.numel() == 0) return {y.zero_(), lse.fill_(std::numeric_limits<float>::infinity())};
+  o.a.out = y.data_ptr();
+  if (want_lse) o.a.lse = lse.data_ptr<float>();
+  const size_t bytes = mfq_attention_workspace_bytes(&o.a);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_status("mfq_attention", mfq_attention(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  return {y, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& dy, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& y,
+                                                      const Tensor& lse, const c10::optional<Tensor>& q_offsets,
+                                                      const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
+                                                      const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool want_dq,
+                                                      bool want_dkv) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  AttentionOperands o("mfq::attention_backward", q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
+  TORCH_CHECK(dy.sizes() == q.sizes() && y.sizes() == q.sizes() && dy.scalar_type() == q.scalar_type() && y.scalar_type() == q.scalar_type() &&
+                  dy.device() == q.device() && y.device() == q.device(),
+              "mfq::attention_backward: dy and y must be as q");
+  const Tensor none = at::empty({0}, q.options());
+  Tensor dq = want_dq ? at::empty(q.sizes(), q.options()) : none;
+  Tensor dk = want_dkv ? at::empty(k.sizes(), q.options()) : none, dv = want_dkv ? at::empty(k.sizes(), q.options()) : none;
+  if (q.numel() == 0 || k.numel() == 0 || (!want_dq && !want_dkv)) return {dq.zero_(), dk.zero_(), dv.zero_()};
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == o.a.heads * o.rows() && lse.device() == q.device(),
+              "mfq::attention_backward: lse [H, rows] of the forward pass");
+  attention_tensor(o.keep, o.a.y, y);
+  attention_tensor(o.keep, o.a.dy, dy);
+  Tensor delta = at::empty_like(lse);
+  o.a.lse = lse.data_ptr<float>();
+  o.a.delta = delta.data_ptr<float>();
+  if (want_dq) o.a.dq = dq.data_ptr();
+  if (want_dkv) {
+    o.a.dk = dk.data_ptr();
+    o.a.dv = dv.data_ptr();
+  }
+  check_status("mfq_attention_backward", mfq_attention_backward(&o.a, stream_of(q)));
+  return {dq, dk, dv};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mfq, m) {
@@ -404,6 +652,11 @@ TORCH_LIBRARY(mfq, m) {
   m.def("low_rank_forward(Tensor x, Tensor af, int rank) -> (Tensor, Tensor)");
   m.def("low_rank_gradient(Tensor g, Tensor bf, Tensor tf, int rank, float scale, bool want_gt, bool want_db) -> (Tensor, Tensor, Tensor)");
   m.def("low_rank_up(Tensor x, Tensor tf, int rank) -> Tensor");
+  m.def("rotary_tables(Tensor positions, float[] frequencies, int[] axis, float factor) -> (Tensor, Tensor)");
+  m.def("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
+  m.def("rotary_backward(Tensor dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps, bool want_x, bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_lse) -> (Tensor, Tensor)");
+  m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA dispatch key
@@ -421,4 +674,9 @@ TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA d
   m.impl("low_rank_forward", low_rank_forward);
   m.impl("low_rank_gradient", low_rank_gradient);
   m.impl("low_rank_up", low_rank_up);
+  m.impl("rotary_tables", rotary_tables);
+  m.impl("rotary", rotary);
+  m.impl("rotary_backward", rotary_backward);
+  m.impl("attention", attention);
+  m.impl("attention_backward", attention_backward);
 }

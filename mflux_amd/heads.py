@@ -1,0 +1,317 @@
+"""What an attention block does to its heads between the stacked q/k/v product
+and the output projection: ``rotary_tables``, ``rotary`` (RMS norm of the heads
+and rotary positions) and ``attention``.
+
+In the reference: AttentionUtils.process_qkv, apply_rope and compute_attention
+(src/mflux/models/flux/model/flux_transformer/common/attention_utils.py:21-49,
+76-80), there with ``[B, H, S, D]`` arrays.  Here heads stay where the linear
+layers leave them, ``[B, S, H, D]`` (or packed ``[T, H, D]``), and are read through
+their strides: a slice of a stacked product needs no copy.
+
+The calls run on the current stream of their tensors' device and launch nothing
+anywhere else; sums are made in a fixed order, so the same inputs give the same
+bits.  All three can be captured into a graph.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .core import _DTYPE_CODE, _require_hip
+
+
+def _integers(fn: str, name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"[{fn}] {name} must be int32 or int64, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"[{fn}] {name} lives on {t.device}, expected {device}")
+    return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+
+
+def _is_integer(value) -> bool:
+    return isinstance(value, int) and not isinstance(value, bool)
+
+
+# ---- tables -----------------------------------------------------------------
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:
+    """The ``dim / 2`` angles a position adds, and what the tables are multiplied
+    by (1 except for ``"yarn"``).  ``scaling`` stretches them for contexts longer than the
+    ``rotary_tables`` docstring says."""
+    if not _is_integer(dim) or dim <= 0 or dim % 2:
+        raise ValueError(f"[rotary_tables] a dimension must be a positive even number, got {dim!r}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError(f"[rotary_tables] base must be positive, got {base!r}")
+    plain = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling is None:
+        return plain, 1.0
+    known = {"linear": {"type", "factor"}, "ntk": {"type", "factor"},
+             "yarn": {"type", "factor", "original_length", "beta_fast", "beta_slow", "attention_factor"}}
+    kind = scaling.get("type")
+    if kind not in known:
+        raise ValueError(f"[rotary_tables] scaling type must be 'linear', 'ntk' or 'yarn', got {kind!r}")
+    if set(scaling) - known[kind]:
+        raise ValueError(f"[rotary_tables] unknown scaling entries for '{kind}': {sorted(set(scaling) - known[kind])}")
+    factor = scaling.get("factor")
+    if not isinstance(factor, (int, float)) or not (factor >= 1 and math.isfinite(factor)):
+        raise ValueError(f"[rotary_tables] scaling factor must be at least 1, got {factor!r}")
+    if kind == "linear":
+        return [f / factor for f in plain], 1.0
+    if kind == "ntk":
+        if dim == 2:
+            raise ValueError("[rotary_tables] 'ntk' needs a dimension above 2")
+        return [(base * factor ** (dim / (dim - 2))) ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
+    length, fast, slow = scaling.get("original_length"), scaling.get("beta_fast", 32.0), scaling.get("beta_slow", 1.0)
+    if not isinstance(length, (int, float)) or length <= 0:
+        raise ValueError(f"[rotary_tables] 'yarn' needs a positive original_length, got {length!r}")
+    if not (fast >= slow > 0) or base <= 1:
+        raise ValueError("[rotary_tables] 'yarn' needs beta_fast >= beta_slow > 0 and a base above 1")
+
+    def pair_of(turns: float) -> float:
+        return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), dim - 1)
+    out = []
+    for i, f in enumerate(plain):
+        stretched = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+        out.append(f / factor * stretched + f * (1.0 - stretched))
+    tables = scaling.get("attention_factor")
+    return out, 0.1 * math.log(factor) + 1.0 if tables is None else float(tables)
+
+
+def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: float = 10000.0,
+                  scaling: dict | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(cos, sin)`` of the rotary angles of ``positions``, float32 ``[S, R / 2]``.
+
+    ``positions``: integers ``[S]`` with ``dims`` the number of channels that turn, or
+    ``[S, A]`` with one such number for each of ``A`` axes, whose pairs lie side by
+    side (an image token's id, row and column in the DiT blocks: ``(16, 56, 56)``).
+    Negative positions are fine.  At most 512 channels in all.
+
+    ``scaling`` stretches the angles for contexts longer than a model was trained
+    on: ``{"type": "linear", "factor": f}`` divides positions, ``"ntk"`` raises the base so
+    that the slowest pair is divided by ``f`` and the fastest by nothing, and ``"yarn"``
+    (``original_length``, ``beta_fast``, ``beta_slow``, ``attention_factor``) divides the pairs
+    that turn less than ``beta_slow`` times over the original length, leaves those that turn more
+    than ``beta_fast`` times, and multiplies the tables by ``0.1 ln f + 1``.
+
+    Angles are taken in float64: a float32 product is off by thousandths at far
+    positions."""
+    fn = "rotary_tables"
+    if not isinstance(positions, torch.Tensor) or positions.ndim not in (1, 2):
+        raise ValueError(f"[{fn}] positions must be a tensor [S] or [S, A]")
+    if positions.ndim == 1:
+        axes = (dims,)
+    else:
+        axes = tuple(dims) if isinstance(dims, (tuple, list)) else (dims,)
+        if len(axes) != positions.shape[1]:
+            raise ValueError(f"[{fn}] positions have {positions.shape[1]} axes, dims {len(axes)}")
+    if not all(_is_integer(d) for d in axes) or not axes:
+        raise ValueError(f"[{fn}] dims must be a number, or one for each axis, got {dims!r}")
+    frequencies, axis, factor = [], [], 1.0
+    for a, dim in enumerate(axes):
+        f, factor = rotary_frequencies(dim, base, scaling)
+        frequencies += f
+        axis += [a] * len(f)
+    if len(frequencies) > 256:
+        raise ValueError(f"[{fn}] at most 512 channels turn, got {2 * len(frequencies)}")
+    positions = _integers(fn, "positions", positions, positions.device)
+    _require_hip(fn, positions, "positions")
+    return _lib.ops().rotary_tables(positions.reshape(positions.shape[0], len(axes)).contiguous(), frequencies, axis, factor)
+
+
+# ---- RMS norm of the heads and rotary positions -------------------------------------
+
+class _RotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, q_weight, k_weight, layout, eps):
+        yq, yk = _lib.ops().rotary(q, k, cos, sin, positions, q_weight, k_weight, layout, eps)
+        # without a weight the gradient is the gradient turned back: nothing of the input is needed but its shape
+        ctx.save_for_backward(q, k, cos, sin, positions, q_weight, k_weight)
+        ctx.layout, ctx.eps = layout, eps
+        return yq if k is None else (yq, yk)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk=None):
+        q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if not any(need):
+            return (None,) * 9
+        dq, dk, dwq, dwk = _lib.ops().rotary_backward(dyq, dyk, q, k, cos, sin, positions, q_weight, k_weight, ctx.layout, ctx.eps,
+                                                      need[0] or need[1], need[5], need[6])
+        return (dq if need[0] else None, dk if need[1] else None, None, None, None, dwq if need[5] else None, dwk if need[6] else None,
+                None, None)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, *, layout: str = "interleaved",
+           positions: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+           eps: float = 1e-6):
+    """Rotary positions of ``q`` and ``k`` in one pass, with the RMS norm of their heads in
+    front where a weight is given.  Returns ``(q', k')``, or ``q'`` for ``k=None``.
+
+    ``q``: ``[B, S, H, D]`` or packed ``[T, H, D]``, ``k`` the same with its own number of
+    heads; float32, float16 or bfloat16, ``D`` even and up to 512; any strides (a last
+    axis that is not dense is copied), results densely packed.
+    ``cos``, ``sin``: float32 ``[P, R / 2]`` of ``rotary_tables``; the first ``R`` channels turn and the
+    others pass.  ``layout``: ``"interleaved"`` turns channels ``(2i, 2i + 1)``, ``"half"``
+    ``(i, i + R / 2)``.
+    ``positions``: the tables' row of every token, int32 or int64 ``[S]`` or ``[B, S]`` (packed: ``[T]``),
+    clamped to the tables; without them a token's row is its place in its sequence axis.
+    ``q_weight``, ``k_weight``: ``[D]`` of the tensors' type: ``x / sqrt(mean(x^2) + eps) * weight``
+    before the turn.
+
+    Everything in between is float32 and rounded once.  Gradients for ``q``, ``k`` and the
+    weights; none for the tables."""
+    fn = "rotary"
+    if layout not in _lib.ROTARY_LAYOUTS:
+        raise ValueError(f"[{fn}] layout must be 'interleaved' or 'half', got {layout!r}")
+    if q.ndim not in (3, 4):
+        raise ValueError(f"[{fn}] q must be [B, S, H, D] or packed [T, H, D], got {tuple(q.shape)}")
+    if q.dtype not in _DTYPE_CODE:
+        raise ValueError(f"[{fn}] q must be float32, float16 or bfloat16, got {q.dtype}")
+    D = q.shape[-1]
+    if D % 2 or not 0 < D <= 512:
+        raise ValueError(f"[{fn}] heads must have an even size up to 512, got {D}")
+    if k is not None and (k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != D or k.dtype != q.dtype):
+        raise ValueError(f"[{fn}] q and k must agree in type and in all axes but the heads, got {tuple(q.shape)} {q.dtype} and "
+                         f"{tuple(k.shape)} {k.dtype}")
+    if not 0 < q.shape[-2] <= 65536 or (k is not None and not 0 < k.shape[-2] <= 65536):
+        raise ValueError(f"[{fn}] q and k need between 1 and 65536 heads")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"[{fn}] cos and sin must be float32 [P, R / 2] of one shape, got {tuple(cos.shape)} {cos.dtype} and "
+                         f"{tuple(sin.shape)} {sin.dtype}")
+    if 2 * cos.shape[1] > D:
+        raise ValueError(f"[{fn}] the tables turn {2 * cos.shape[1]} channels, heads have {D}")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError(f"[{fn}] the tables have no gradient here: detach them")
+    tokens = q.shape[-3]
+    if cos.shape[0] == 0 and q.numel():
+        raise ValueError(f"[{fn}] the tables are empty")
+    if positions is None:
+        if cos.shape[0] < tokens:
+            raise ValueError(f"[{fn}] the tables have {cos.shape[0]} rows for {tokens} tokens")
+    else:
+        shapes = ((tokens,),) if q.ndim == 3 else ((tokens,), (1, tokens), (q.shape[0], tokens))
+        if tuple(positions.shape) not in shapes:
+            raise ValueError(f"[{fn}] positions must have the shape {shapes[-1]}, got {tuple(positions.shape)}")
+    for name, w, t in (("q_weight", q_weight, q), ("k_weight", k_weight, k)):
+        if w is not None and (t is None or tuple(w.shape) != (D,) or w.dtype != q.dtype):
+            raise ValueError(f"[{fn}] {name} must be a [{D}] vector of {q.dtype}" + (" and needs its tensor" if t is None else ""))
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise ValueError(f"[{fn}] eps must not be negative, got {eps!r}")
+    for name, t in (("k", k), ("cos", cos), ("sin", sin), ("positions", positions), ("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"[{fn}] `{name}` lives on {t.device}, q on {q.device}")
+    if positions is not None:
+        positions = _integers(fn, "positions", positions, q.device).reshape(-1, tokens)
+    _require_hip(fn, q, "q")
+    packed = q.ndim == 3
+    if packed:
+        q, k = q[None], None if k is None else k[None]
+    arguments = (q, k, cos, sin, positions, q_weight, k_weight, _lib.ROTARY_LAYOUTS[layout], float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        out = _RotaryFunction.apply(*arguments)
+        yq, yk = (out, None) if k is None else out
+    else:
+        yq, yk = _lib.ops().rotary(*arguments)
+    if packed:
+        yq, yk = yq[0], None if k is None else yk[0]
+    return yq if k is None else (yq, yk)
+
+
+# ---- attention ------------------------------------------------------------------------
+
+class _AttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale):
+        y, lse = _lib.ops().attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, True)
+        ctx.save_for_backward(q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths)
+        ctx.causal, ctx.scale = causal, scale
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv = _lib.ops().attention_backward(dy, q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths, ctx.causal, ctx.scale,
+                                                   need[0], need[1] or need[2])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None) + (None,) * 6
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, scale: float | None = None,
+              q_lengths: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None,
+              q_offsets: torch.Tensor | None = None, k_offsets: torch.Tensor | None = None) -> torch.Tensor:
+    """``softmax(scale * q k^T + mask) v`` with grouped heads, for batched or packed sequences
+    (``mx.fast.scaled_dot_product_attention`` in the reference).
+
+    Batched: ``q [B, Sq, H, D]``, ``k`` and ``v [B, Sk, Hkv, D]``; ``q_lengths`` and ``k_lengths`` (``[B]``
+    integers on the device, each optional) say how many queries and keys of an entry there are.
+    Packed: ``q [Tq, H, D]``, ``k`` and ``v [Tk, Hkv, D]``, sequence ``s`` having the rows ``q_offsets[s]`` to
+    ``q_offsets[s + 1]`` of ``q`` and the same of ``k_offsets`` (default: ``q_offsets``) of ``k`` and ``v``; offsets
+    must not decrease.  Lengths and offsets are read by the kernels alone, clamped to the
+    tensors: a call never waits for the device, and wrong ones never reach outside them.
+
+    float16 or bfloat16, ``D`` a multiple of 8 up to 256, ``H`` a multiple of ``Hkv`` (head ``h`` reads
+    key head ``h // (H // Hkv)``).  Any strides of rows of whole 16 bytes; others are copied first.
+    ``scale``: ``1 / sqrt(D)`` unless given; positive.
+    ``causal``: aligned to the last token, query ``i`` of ``n`` sees the first ``i + 1 + m - n`` of ``m`` keys, so one
+    query behind a cache sees all of it.  A query that sees no key gets zeros, and so does every
+    row that belongs to no sequence (padding; rows behind the last offset), in the result and
+    in the gradients.  What a query does not see never reaches it, infinities and NaN included.
+
+    Statistics and sums are float32; the probabilities (and in the backward pass the
+    scores' gradients) are rounded to the tensors' type for the second product.  The backward
+    pass makes the scores again from one saved float32 per row and head."""
+    fn = "attention"
+    packed = q_offsets is not None
+    if k_offsets is not None and not packed:
+        raise ValueError(f"[{fn}] k_offsets need q_offsets")
+    if packed and (q_lengths is not None or k_lengths is not None):
+        raise ValueError(f"[{fn}] packed sequences have offsets, batched ones lengths, not both")
+    n = 3 if packed else 4
+    if q.ndim != n or k.ndim != n or v.ndim != n:
+        raise ValueError(f"[{fn}] q, k and v must be " + ("packed [T, H, D] with offsets" if packed else "[B, S, H, D] without offsets") +
+                         f", got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.shape != v.shape or q.shape[-1] != k.shape[-1] or (not packed and q.shape[0] != k.shape[0]):
+        raise ValueError(f"[{fn}] k and v must have one shape and q's batch and head size, got {tuple(q.shape)}, {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"[{fn}] q, k and v must all be float16 or all bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    H, D = q.shape[-2:]
+    if D % 8 or not 0 < D <= 256:
+        raise ValueError(f"[{fn}] the head size must be a multiple of 8 up to 256, got {D}")
+    if not 0 < k.shape[-2] <= H or H % k.shape[-2] or H > 65536:
+        raise ValueError(f"[{fn}] {H} query heads do not share {k.shape[-2]} key heads evenly")
+    if q.shape[-3] * H > 2 ** 30 or k.shape[-3] > 2 ** 30:
+        raise ValueError(f"[{fn}] at most 2^30 queries times heads, and keys, in an entry")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if not 0 < scale <= 1e30:
+        raise ValueError(f"[{fn}] scale must be positive and finite, got {scale!r}")
+    for name, t in (("k", k), ("v", v), ("q_offsets", q_offsets), ("k_offsets", k_offsets), ("q_lengths", q_lengths), ("k_lengths", k_lengths)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"[{fn}] `{name}` lives on {t.device}, q on {q.device}")
+
+    def counts(name, t, length):
+        if t is None:
+            return None
+        if t.ndim != 1 or (length is not None and t.shape[0] != length):
+            raise ValueError(f"[{fn}] {name} must be a vector" + ("" if length is None else f" of {length} values") + f", got {tuple(t.shape)}")
+        return _integers(fn, name, t, q.device)
+
+    if packed:
+        q_offsets = counts("q_offsets", q_offsets, None)
+        if q_offsets.shape[0] < 2:
+            raise ValueError(f"[{fn}] offsets are one more than the sequences, of which there is at least one")
+        k_offsets = q_offsets if k_offsets is None else counts("k_offsets", k_offsets, q_offsets.shape[0])
+    else:
+        q_lengths, k_lengths = counts("q_lengths", q_lengths, q.shape[0]), counts("k_lengths", k_lengths, q.shape[0])
+    _require_hip(fn, q, "q")
+    arguments = (q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, bool(causal), float(scale))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _AttentionFunction.apply(*arguments)
+    return _lib.ops().attention(*arguments, False)[0]
