@@ -269,6 +269,23 @@ __device__ inline float max_halves(float v) {
   return fmaxf(h.low, h.high);
 }
 
+// sum + the operand's eight values: what the second product weighs with is what the sum divides by, rounded alike
+template <typename T>
+__device__ inline float add_sum(typename T::vec8 p, float sum) {
+  const u32x4a w = __builtin_bit_cast(u32x4a, p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::code == MFQ_BF16) {
+      typedef __bf16 pair __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, (uint32_t)w[i]), __builtin_bit_cast(pair, 0x3f803f80u), sum, false);
+    } else {
+      typedef __fp16 pair __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, (uint32_t)w[i]), __builtin_bit_cast(pair, 0x3c003c00u), sum, false);
+    }
+  }
+  return sum;
+}
+
 // acc (columns of the tile x the lane's column) += tile^T p for 16 rows of the tile, all kBlocks blocks of 32 columns
 template <typename T, int kPitch, int kBlocks>
 __device__ inline void add_columns(f32x16 (&acc)[kBlocks], const char* tile16, typename T::vec8 p, int lane) {
@@ -347,16 +364,29 @@ struct QueryState {
   // One step over kTiles x 32 keys, tiles of K and V in LDS.  `limit`: keys of the tile that the lane's query sees (may be
   // negative or beyond the tile); kMasked: whether any lane's ends inside it.  c: scale * log2(e).
   template <int kTiles, bool kMasked>
-  __device__ inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane) {
+  __device__ __attribute__((always_inline)) inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane) {
     bool one_by_one = false;
     if constexpr (kMasked) one_by_one = tile_not_finite<T, kPitch, kSteps, kTiles>(v_tile, lane);
     f32x16 s[kTiles];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      s[t] = zero16();
+    for (int t = 0; t < kTiles; ++t) s[t] = zero16();
+    // operands are read a step ahead of the matrix instructions that take them
+    vec8 a[2][kTiles];
 #pragma unroll
-      for (int e = 0; e < kSteps; ++e) s[t] = mfma32(tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, e, lane), q[e], s[t]);
+    for (int t = 0; t < kTiles; ++t) a[0][t] = tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, 0, lane);
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) {
+      if (e + 1 < kSteps) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) a[(e + 1) & 1][t] = tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, e + 1, lane);
+      }
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) s[t] = mfma32(a[e & 1][t], q[e], s[t]);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    vec8 w[2][kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(v_tile, b, lane);
     float most = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
@@ -380,22 +410,26 @@ struct QueryState {
     }
     const float shift = top == -__builtin_inff() ? 0.f : top * c;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -shift));
-        sum += s[t][i];
-      }
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int slab = 0; slab < 2; ++slab) {
+        const int n = 2 * t + slab;
+#pragma unroll
+        for (int i = 8 * slab; i < 8 * slab + 8; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -shift));
         const vec8 p = result_operand<T>(s[t], slab);
-        const char* v16 = v_tile + (t * 32 + slab * 16) * kPitch * 2;
-        if (kMasked && __builtin_expect(one_by_one, 0))
-          add_columns_one_by_one<T, kPitch, kBlocks>(o, v16, p, lane, [&](int row) { return 32 * t + 16 * slab + row < limit; });
-        else
-          add_columns<T, kPitch, kBlocks>(o, v16, p, lane);
+        sum = add_sum<T>(p, sum);
+        if (n + 1 < 2 * kTiles) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) w[(n + 1) & 1][b] = tile_columns<T, kPitch>(v_tile + (n + 1) * 16 * kPitch * 2, b, lane);
+        }
+        if (kMasked && __builtin_expect(one_by_one, 0)) {
+          add_columns_one_by_one<T, kPitch, kBlocks>(o, v_tile + n * 16 * kPitch * 2, p, lane, [&](int row) { return 16 * n + row < limit; });
+        } else {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) o[b] = mfma32(w[n & 1][b], p, o[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
   }
 };
 

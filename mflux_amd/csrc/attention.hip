@@ -49,7 +49,8 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
     const float scale = c.scale * kLog2e;
     load_k.load(k, lds_at, keys, thread);
     load_v.load(v, lds_at + kTileBytes, keys, thread);
-    for (int first = 0, buffer = 0; first < keys; first += kKeys, buffer ^= 1) {
+    // the tile of `buffer` has arrived and the next one is requested
+    auto advance = [&](int first, int buffer) __attribute__((always_inline)) {
       arrive_and_sync();
       const int next = first + kKeys;
       if (next < keys) {
@@ -57,9 +58,21 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
         load_k.load(k + (int64_t)next * c.k.token, to, keys - next, thread);
         load_v.load(v + (int64_t)next * c.v.token, to + kTileBytes, keys - next, thread);
       }
+    };
+    // Tiles that every lane sees all of come first, by pairs, so that their places in LDS are constants.  Wavefronts leave this loop at
+    // different tiles and meet the same barriers in the next one.
+    int first = 0, buffer = 0;
+    for (; first + 2 * kKeys <= least; first += 2 * kKeys) {
+      advance(first, 0);
+      state.template step<2, false>(lds, lds + kTileBytes, kKeys, scale, lane);
+      advance(first + kKeys, 1);
+      state.template step<2, false>(lds + 2 * kTileBytes, lds + 3 * kTileBytes, kKeys, scale, lane);
+    }
+#pragma unroll 1
+    for (; first < keys; first += kKeys, buffer ^= 1) {
+      advance(first, buffer);
       const char* k_tile = lds + buffer * 2 * kTileBytes;
-      if (next <= least) state.template step<2, false>(k_tile, k_tile + kTileBytes, kKeys, scale, lane);
-      else if (first < most) state.template step<2, true>(k_tile, k_tile + kTileBytes, limit - first, scale, lane);
+      if (first < most) state.template step<2, true>(k_tile, k_tile + kTileBytes, limit - first, scale, lane);
     }
   }
   if (row >= run.rows) return;
