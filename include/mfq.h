@@ -566,8 +566,11 @@ int mfq_rotary_backward(const mfq_rotary_args* args, void* workspace, size_t wor
  * Softmax and sums in float32, the probabilities rounded to dtype for the second product.  scale > 0.
  *   lse    [heads, rows] float32, rows = q_tokens or batch * q_tokens: written by the forward pass if not NULL,
  *          read by the backward pass (which needs it, y, dy, and delta of the same size to write to)
+ *   rest   as out: y before its rounding minus y, rounded; written by the forward pass if not NULL and read by
+ *          the backward pass if not NULL (sum(dy y) from the rounded y alone is off by as much as a gradient's rounding)
  *   dq, dk, dv  backward: NULL where not wanted
- * workspace: mfq_attention_workspace_bytes() of it (few queries against many keys), 16-byte aligned.
+ * workspace: mfq_attention_workspace_bytes() (few queries against many keys), for the backward pass
+ * mfq_attention_backward_workspace_bytes() of it (grouped heads), 16-byte aligned.
  */
 typedef struct mfq_attention_tensor {
   const void* p;
@@ -578,13 +581,14 @@ typedef struct mfq_attention_args {
   float scale;
   int64_t batch, heads, kv_heads, q_tokens, k_tokens;
   mfq_attention_tensor q, k, v, y, dy;
-  void *out, *dq, *dk, *dv;
+  void *out, *rest, *dq, *dk, *dv;
   float *lse, *delta;
   const int32_t *q_offsets, *k_offsets, *q_lengths, *k_lengths;
 } mfq_attention_args;
 size_t mfq_attention_workspace_bytes(const mfq_attention_args* args);
 int mfq_attention(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
-int mfq_attention_backward(const mfq_attention_args* args, void* stream);
+size_t mfq_attention_backward_workspace_bytes(const mfq_attention_args* args);
+int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -41,7 +41,7 @@ class AttentionArgs(ctypes.Structure):  # mfq_attention_args
     _fields_ = [("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("dim", ctypes.c_int32), ("scale", ctypes.c_float)] + [
         (n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_tokens", "k_tokens")] + [
         (n, AttentionTensor) for n in ("q", "k", "v", "y", "dy")] + [
-        (n, ctypes.c_void_p) for n in ("out", "dq", "dk", "dv", "lse", "delta", "q_offsets", "k_offsets", "q_lengths", "k_lengths")]
+        (n, ctypes.c_void_p) for n in ("out", "rest", "dq", "dk", "dv", "lse", "delta", "q_offsets", "k_offsets", "q_lengths", "k_lengths")]
 
 
 # every symbol include/mfq.h declares, with its ctypes signature
@@ -89,7 +89,8 @@ SIGNATURES = {
     "mfq_rotary_backward": (_INT, [ctypes.POINTER(RotaryArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
     "mfq_attention": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
-    "mfq_attention_backward": (_INT, [ctypes.POINTER(AttentionArgs), _PTR]),
+    "mfq_attention_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+    "mfq_attention_backward": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_low_rank_add": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _PTR, _INT, _PTR]),
 }
 

@@ -532,9 +532,10 @@ static int attention_call(const mfq_attention_args* a, bool backward, mfq::Atten
   }
   if (!backward && !a->out) return MFQ_ENULL;
   if (backward && (!a->lse || !a->delta || (!a->dq && !a->dk && !a->dv))) return MFQ_ENULL;
-  for (const void* p : {(const void*)a->out, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+  for (const void* p : {(const void*)a->out, (const void*)a->rest, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
     if (!mfq::aligned16(p)) return MFQ_EALIGN;
   c->out = static_cast<uint16_t*>(a->out);
+  c->rest = static_cast<uint16_t*>(a->rest);
   c->dq = static_cast<uint16_t*>(a->dq);
   c->dk = static_cast<uint16_t*>(a->dk);
   c->dv = static_cast<uint16_t*>(a->dv);
@@ -561,6 +562,12 @@ size_t mfq_attention_workspace_bytes(const mfq_attention_args* args) {
   return mfq::attention_split_bytes(c, mfq::attention_splits(c));
 }
 
+size_t mfq_attention_backward_workspace_bytes(const mfq_attention_args* args) {
+  mfq::AttentionCall c;
+  if (attention_call(args, true, &c) != MFQ_OK) return 0;
+  return mfq::attention_backward_bytes(c, mfq::attention_backward_parts(c));
+}
+
 int mfq_attention(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
   mfq::AttentionCall c;
   if (int rc = attention_call(args, false, &c)) return rc;
@@ -573,10 +580,15 @@ int mfq_attention(const mfq_attention_args* args, void* workspace, size_t worksp
   return mfq::launch_attention_split(args->dtype, c, splits, workspace, (hipStream_t)stream);
 }
 
-int mfq_attention_backward(const mfq_attention_args* args, void* stream) {
+int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
   mfq::AttentionCall c;
   if (int rc = attention_call(args, true, &c)) return rc;
-  return mfq::launch_attention_backward(args->dtype, c, (hipStream_t)stream);
+  const int parts = mfq::attention_backward_parts(c);
+  const size_t need = mfq::attention_backward_bytes(c, parts);
+  if (need && !workspace) return MFQ_ENULL;
+  if (need > workspace_bytes) return MFQ_ESCRATCH;
+  if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
+  return mfq::launch_attention_backward(args->dtype, c, parts, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

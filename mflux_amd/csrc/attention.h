@@ -32,6 +32,7 @@ struct AttentionTensor {
 
 struct AttentionCall {
   AttentionTensor q, k, v, y, dy;  // y: the result, or in the backward pass the forward's
+  uint16_t* rest = nullptr;  // y before its rounding minus y, densely packed: forward writes it where not nullptr, backward reads it
   uint16_t *out = nullptr, *dq = nullptr, *dk = nullptr, *dv = nullptr;  // densely packed, [(batch,) tokens, heads, dim]
   float* lse = nullptr;    // [heads][rows]: log2 of the sum of exp2 of the scaled scores, +inf for a row that sees nothing
   float* delta = nullptr;  // [heads][rows]: sum of dy * y
@@ -286,13 +287,6 @@ __device__ inline float add_sum(typename T::vec8 p, float sum) {
   return sum;
 }
 
-// acc (columns of the tile x the lane's column) += tile^T p for 16 rows of the tile, all kBlocks blocks of 32 columns
-template <typename T, int kPitch, int kBlocks>
-__device__ inline void add_columns(f32x16 (&acc)[kBlocks], const char* tile16, typename T::vec8 p, int lane) {
-#pragma unroll
-  for (int b = 0; b < kBlocks; ++b) acc[b] = mfma32(tile_columns<T, kPitch>(tile16, b, lane), p, acc[b]);
-}
-
 // Whether a tile of kTiles x 32 rows holds an infinity or a NaN: in a product with zeros every finite element gives zero.  Asked of
 // tiles at a mask's edge alone: a masked row's probability is zero, but zero times such an element is NaN, which the product would
 // hand to columns that never see the row.
@@ -301,7 +295,7 @@ __device__ inline bool tile_not_finite(const char* tile, int lane) {
   using vec8 = typename T::vec8;
   const vec8 none = __builtin_bit_cast(vec8, u32x4a{0u, 0u, 0u, 0u});
   f32x16 probe = zero16();
-#pragma unroll
+#pragma unroll 1
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int e = 0; e < kSteps; ++e) probe = mfma32(tile_rows<T, kPitch>(tile + t * 32 * kPitch * 2, e, lane), none, probe);
@@ -311,7 +305,19 @@ __device__ inline bool tile_not_finite(const char* tile, int lane) {
   return __any(sum != 0.f);
 }
 
-// add_columns for such a tile, row by row, each added only where it is visible.  visible(row): of the lane's column.
+template <typename T>
+__device__ inline typename T::vec8 masked(typename T::vec8 v, uint32_t mask) {
+  return __builtin_bit_cast(typename T::vec8, __builtin_bit_cast(u32x4a, v) & u32x4a{mask, mask, mask, mask});
+}
+
+// The product of a 32 x 32 tile of results with zeros: 0, or NaN if any of them is not finite
+__device__ inline float times_zero(const f32x16& s, float sum) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(s[i], 0.f, sum);
+  return sum;
+}
+
+// acc += tile^T p for 16 rows of such a tile, row by row, each added only where it is visible.  visible(row): of the lane's column.
 template <typename T, int kPitch, int kBlocks, typename Visible>
 __device__ inline void add_columns_one_by_one(f32x16 (&acc)[kBlocks], const char* tile16, typename T::vec8 p, int lane, Visible visible) {
   using vec8 = typename T::vec8;
@@ -362,11 +368,10 @@ struct QueryState {
   }
 
   // One step over kTiles x 32 keys, tiles of K and V in LDS.  `limit`: keys of the tile that the lane's query sees (may be
-  // negative or beyond the tile); kMasked: whether any lane's ends inside it.  c: scale * log2(e).
+  // negative or beyond the tile); kMasked: whether any lane's ends inside it (code of its own: a branch around these parts has the
+  // compiler copy every accumulator twice a step).  c: scale * log2(e).
   template <int kTiles, bool kMasked>
   __device__ __attribute__((always_inline)) inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane) {
-    bool one_by_one = false;
-    if constexpr (kMasked) one_by_one = tile_not_finite<T, kPitch, kSteps, kTiles>(v_tile, lane);
     f32x16 s[kTiles];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) s[t] = zero16();
@@ -387,14 +392,20 @@ struct QueryState {
     vec8 w[2][kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(v_tile, b, lane);
+    bool one_by_one = false;
+    if constexpr (kMasked) {
+      one_by_one = tile_not_finite<T, kPitch, kSteps, kTiles>(v_tile, lane);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * t + result_row(i, lane) >= limit) s[t][i] = -__builtin_inff();
+    }
     float most = -__builtin_inff();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (kMasked && 32 * t + result_row(i, lane) >= limit) s[t][i] = -__builtin_inff();
-        most = fmaxf(most, s[t][i]);
-      }
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
     most = max_halves(most);
     // The reference follows the maximum only where that has grown by more than 2^8: up to there the exponentials are at most 256,
     // which float32 sums and 16-bit probabilities hold as well as values up to 1, and the accumulators need no pass.
@@ -409,27 +420,37 @@ struct QueryState {
         for (int i = 0; i < 16; ++i) o[b][i] *= factor;
     }
     const float shift = top == -__builtin_inff() ? 0.f : top * c;
+    vec8 p[2 * kTiles];
+    if constexpr (kMasked) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+      for (int n = 0; n < 2 * kTiles; ++n) p[n] = probabilities(s[n / 2], n & 1, c, shift);
+      if (__builtin_expect(one_by_one, 0)) {
 #pragma unroll
-      for (int slab = 0; slab < 2; ++slab) {
-        const int n = 2 * t + slab;
-#pragma unroll
-        for (int i = 8 * slab; i < 8 * slab + 8; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -shift));
-        const vec8 p = result_operand<T>(s[t], slab);
-        sum = add_sum<T>(p, sum);
-        if (n + 1 < 2 * kTiles) {
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) w[(n + 1) & 1][b] = tile_columns<T, kPitch>(v_tile + (n + 1) * 16 * kPitch * 2, b, lane);
-        }
-        if (kMasked && __builtin_expect(one_by_one, 0)) {
-          add_columns_one_by_one<T, kPitch, kBlocks>(o, v_tile + n * 16 * kPitch * 2, p, lane, [&](int row) { return 16 * n + row < limit; });
-        } else {
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) o[b] = mfma32(w[n & 1][b], p, o[b]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < 2 * kTiles; ++n)
+          add_columns_one_by_one<T, kPitch, kBlocks>(o, v_tile + n * 16 * kPitch * 2, p[n], lane, [&](int row) { return 16 * n + row < limit; });
       }
+    }
+    const uint32_t keep = one_by_one ? 0u : ~0u;  // the product adds nothing where that has been done
+#pragma unroll
+    for (int n = 0; n < 2 * kTiles; ++n) {
+      if constexpr (kMasked) p[n] = masked<T>(p[n], keep);
+      else p[n] = probabilities(s[n / 2], n & 1, c, shift);
+      if (n + 1 < 2 * kTiles) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) w[(n + 1) & 1][b] = tile_columns<T, kPitch>(v_tile + (n + 1) * 16 * kPitch * 2, b, lane);
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) o[b] = mfma32(kMasked ? masked<T>(w[n & 1][b], keep) : w[n & 1][b], p[n], o[b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // exponentials of half a score tile as the second product's operand, added to the sum
+  __device__ __attribute__((always_inline)) inline vec8 probabilities(f32x16& s, int slab, float c, float shift) {
+#pragma unroll
+    for (int i = 8 * slab; i < 8 * slab + 8; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -shift));
+    const vec8 p = result_operand<T>(s, slab);
+    sum = add_sum<T>(p, sum);
+    return p;
   }
 };
 
@@ -450,17 +471,30 @@ __device__ inline int wave_max(int v) {
   return uniform(v);
 }
 
-// A column of results (kDim / 32 of them) as a row of the output: four consecutive elements a store
+// four values as 16-bit elements, and what their rounding left of them
+template <typename T>
+__device__ inline u32x2 pack4(f32x4 v) { return u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])}; }
+template <typename T>
+__device__ inline u32x2 pack4_rest(f32x4 v, u32x2 p) {
+  return u32x2{T::pack2(v[0] - lo_f32<T>(p[0]), v[1] - hi_f32<T>(p[0])), T::pack2(v[2] - lo_f32<T>(p[1]), v[3] - hi_f32<T>(p[1]))};
+}
+
+// A column of results (kDim / 32 of them) as a row of the output, zeros where it is not `seen`; `rest`: of the rounding, or nullptr.
+// Four consecutive elements a store.
 template <typename T, int kBlocks>
-__device__ inline void store_row(uint16_t* row, const f32x16 (&o)[kBlocks], float factor, int dim, int lane) {
+__device__ inline void store_row(uint16_t* row, uint16_t* rest, const f32x16 (&o)[kBlocks], bool seen, float factor, int dim, int lane) {
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int d = 32 * b + result_row(i, lane);
-      if (d < dim)
-        *reinterpret_cast<u32x2*>(row + d) = u32x2{T::pack2(o[b][i] * factor, o[b][i + 1] * factor),
-                                                   T::pack2(o[b][i + 2] * factor, o[b][i + 3] * factor)};
+      if (d >= dim) continue;
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = seen ? o[b][i + j] * factor : 0.f;
+      const u32x2 p = pack4<T>(v);
+      *reinterpret_cast<u32x2*>(row + d) = p;
+      if (rest) *reinterpret_cast<u32x2*>(rest + d) = pack4_rest<T>(v, p);
     }
 }
 
@@ -469,6 +503,9 @@ int launch_attention(int dtype, const AttentionCall& c, hipStream_t stream);
 int attention_splits(const AttentionCall& c);
 size_t attention_split_bytes(const AttentionCall& c, int splits);  // of workspace, 16-byte aligned
 int launch_attention_split(int dtype, const AttentionCall& c, int splits, void* workspace, hipStream_t stream);
-int launch_attention_backward(int dtype, const AttentionCall& c, hipStream_t stream);
+// into how many parts the query heads that share a key head are cut, each with float32 sums of its own
+int attention_backward_parts(const AttentionCall& c);
+size_t attention_backward_bytes(const AttentionCall& c, int parts);  // of workspace, 16-byte aligned
+int launch_attention_backward(int dtype, const AttentionCall& c, int parts, void* workspace, hipStream_t stream);
 
 }  // namespace mfq

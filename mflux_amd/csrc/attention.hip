@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
   const int limit = visible_keys(run, row, c.causal);
   // keys that any query of the workgroup sees: the last one's, as limits grow along the rows
   const int keys = uniform(run.tile * kQueries < run.nq ? visible_keys(run, min(run.tile * kQueries + kQueries, run.nq) - 1, c.causal) : 0);
-  const int least = wave_min(limit), most = wave_max(limit);
+  const int least = wave_min(row < run.nq ? limit : INT32_MAX), most = wave_max(limit);
 
   QueryState<T, kDim, kPitch> state;
   state.init();
@@ -59,27 +59,33 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
         load_v.load(v + (int64_t)next * c.v.token, to + kTileBytes, keys - next, thread);
       }
     };
-    // Tiles that every lane sees all of come first, by pairs, so that their places in LDS are constants.  Wavefronts leave this loop at
-    // different tiles and meet the same barriers in the next one.
+    // Tiles that every query of the workgroup sees all of (those that are there: the others' rows are not stored) come first, by pairs, so that their places in LDS are constants.
+    const int whole = uniform(c.causal ? visible_keys(run, run.tile * kQueries, 1) : run.nk);
     int first = 0, buffer = 0;
-    for (; first + 2 * kKeys <= least; first += 2 * kKeys) {
+    for (; first + 2 * kKeys <= whole; first += 2 * kKeys) {
       advance(first, 0);
       state.template step<2, false>(lds, lds + kTileBytes, kKeys, scale, lane);
       advance(first + kKeys, 1);
       state.template step<2, false>(lds + 2 * kTileBytes, lds + 3 * kTileBytes, kKeys, scale, lane);
     }
+    // the others in blocks of 32 keys, so that of a wavefront's own edge only what lies across it is masked
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
       advance(first, buffer);
-      const char* k_tile = lds + buffer * 2 * kTileBytes;
-      if (first < most) state.template step<2, true>(k_tile, k_tile + kTileBytes, limit - first, scale, lane);
+#pragma unroll 1
+      for (int at = first; at < min(first + kKeys, most); at += 32) {
+        const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
+        if (at + 32 <= least) state.template step<1, false>(k32, k32 + kTileBytes, 32, scale, lane);
+        else state.template step<1, true>(k32, k32 + kTileBytes, limit - at, scale, lane);
+      }
     }
   }
   if (row >= run.rows) return;
   const float sum = sum_halves(state.sum);
   const int64_t at = (int64_t)run.batch * c.q_tokens + run.q0 + row;  // of the densely packed result
   const bool seen = limit > 0;
-  store_row<T, kDim / 32>(c.out + (at * c.heads + head) * c.dim, state.o, seen ? 1.0f / sum : 0.f, c.dim, lane);
+  const int64_t to = (at * c.heads + head) * c.dim;
+  store_row<T, kDim / 32>(c.out + to, c.rest ? c.rest + to : nullptr, state.o, seen, 1.0f / sum, c.dim, lane);
   if (c.lse && lane < 32) {
     const int64_t rows = (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens;
     c.lse[head * rows + at] = seen ? state.top * (c.scale * kLog2e) + __builtin_amdgcn_logf(sum) : __builtin_inff();

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel
 
   const int row = run.tile * kRows + (lane & 31), token = row / group, head = kv_head * group + row % group;
   const int limit = visible_keys(run, token, c.causal);
-  const int most = wave_max(limit), least = wave_min(token < run.rows ? limit : INT32_MAX);
+  const int most = wave_max(limit), least = wave_min(token < run.nq ? limit : INT32_MAX);
   const int chunk = ((run.nk + splits - 1) / splits + kStep - 1) / kStep * kStep;
   const int begin = split * chunk, end = min(min(begin + chunk, run.nk), most);
 
@@ -122,8 +122,12 @@ __global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel
     const int64_t at = ((int64_t)run.batch * c.q_tokens + run.q0 + tok) * c.heads + kv_head * group + p % group;
     if (splits == 1) {
       const bool seen = visible_keys(run, tok, c.causal) > 0;
-      const float f = seen ? 1.0f / total : 0.f;
-      *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = u32x2{T::pack2(o[0] * f, o[1] * f), T::pack2(o[2] * f, o[3] * f)};
+      const float f = 1.0f / total;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = seen ? o[e] * f : 0.f;
+      const u32x2 packed = pack4<T>(o);
+      *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = packed;
+      if (c.rest) *reinterpret_cast<u32x2*>(c.rest + at * c.dim + d) = pack4_rest<T>(o, packed);
       if (c.lse && d == 0)
         c.lse[(at % c.heads) * rows + at / c.heads] = seen ? top * c2 + __builtin_amdgcn_logf(total) : __builtin_inff();
     } else {
@@ -161,9 +165,14 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows
   }
   // a row that sees no key has neither a maximum nor a sum (a sum that is NaN is a row's own)
   const bool empty = top == -__builtin_inff() && total == 0.f;
-  const float f = empty ? 0.f : 1.0f / total;
-  if (d < c.dim)
-    *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = u32x2{T::pack2(o[0] * f, o[1] * f), T::pack2(o[2] * f, o[3] * f)};
+  const float f = 1.0f / total;
+  if (d < c.dim) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = empty ? 0.f : o[e] * f;
+    const u32x2 packed = pack4<T>(o);
+    *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = packed;
+    if (c.rest) *reinterpret_cast<u32x2*>(c.rest + at * c.dim + d) = pack4_rest<T>(o, packed);
+  }
   if (c.lse && lane == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + __builtin_amdgcn_logf(total);
 }
 

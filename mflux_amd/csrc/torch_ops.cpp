@@ -586,27 +586,31 @@ struct AttentionOperands {
   int64_t rows() const { return (a.q_offsets ? 1 : a.batch) * a.q_tokens; }
 };
 
-// (y, log-sum-exps or an empty tensor)
-std::tuple<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+// (y, and for a backward pass what y's rounding left and the rows' log-sum-exps: empty otherwise)
+std::tuple<Tensor, Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
                                      const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
-                                     const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool want_lse) {
+                                     const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool training) {
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   AttentionOperands o("mfq::attention", q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
   Tensor y = at::empty(q.sizes(), q.options());
-  Tensor lse = want_lse ? at::empty({o.a.heads, o.rows()}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
-  if (q.numel() == 0) return {y, lse};
-  if (k.numel() == 0) return {y.zero_(), lse.fill_(std::numeric_limits<float>::infinity())};
+  Tensor rest = training ? at::empty(q.sizes(), q.options()) : at::empty({0}, q.options());
+  Tensor lse = training ? at::empty({o.a.heads, o.rows()}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {y, rest, lse};
+  if (k.numel() == 0) return {y.zero_(), rest.zero_(), lse.fill_(std::numeric_limits<float>::infinity())};
   o.a.out = y.data_ptr();
-  if (want_lse) o.a.lse = lse.data_ptr<float>();
+  if (training) {
+    o.a.rest = rest.data_ptr();
+    o.a.lse = lse.data_ptr<float>();
+  }
   const size_t bytes = mfq_attention_workspace_bytes(&o.a);
   Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
   check_status("mfq_attention", mfq_attention(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
-  return {y, lse};
+  return {y, rest, lse};
 }
 
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& dy, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& y,
-                                                      const Tensor& lse, const c10::optional<Tensor>& q_offsets,
+                                                      const Tensor& rest, const Tensor& lse, const c10::optional<Tensor>& q_offsets,
                                                       const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
                                                       const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool want_dq,
                                                       bool want_dkv) {
@@ -621,6 +625,9 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& dy, const Te
   if (q.numel() == 0 || k.numel() == 0 || (!want_dq && !want_dkv)) return {dq.zero_(), dk.zero_(), dv.zero_()};
   TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == o.a.heads * o.rows() && lse.device() == q.device(),
               "mfq::attention_backward: lse [H, rows] of the forward pass");
+  TORCH_CHECK(rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() && rest.is_contiguous() && rest.device() == q.device(),
+              "mfq::attention_backward: the rest of y's rounding as the forward pass gave it");
+  o.a.rest = rest.data_ptr();
   attention_tensor(o.keep, o.a.y, y);
   attention_tensor(o.keep, o.a.dy, dy);
   Tensor delta = at::empty_like(lse);
@@ -631,7 +638,10 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& dy, const Te
     o.a.dk = dk.data_ptr();
     o.a.dv = dv.data_ptr();
   }
-  check_status("mfq_attention_backward", mfq_attention_backward(&o.a, stream_of(q)));
+  const size_t bytes = mfq_attention_backward_workspace_bytes(&o.a);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_status("mfq_attention_backward", mfq_attention_backward(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
   return {dq, dk, dv};
 }
 
@@ -655,8 +665,8 @@ TORCH_LIBRARY(mfq, m) {
   m.def("rotary_tables(Tensor positions, float[] frequencies, int[] axis, float factor) -> (Tensor, Tensor)");
   m.def("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("rotary_backward(Tensor dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps, bool want_x, bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_lse) -> (Tensor, Tensor)");
-  m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
+  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool training) -> (Tensor, Tensor, Tensor)");
+  m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor rest, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA dispatch key

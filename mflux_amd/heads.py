@@ -227,17 +227,17 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torc
 class _AttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale):
-        y, lse = _lib.ops().attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, True)
-        ctx.save_for_backward(q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths)
+        y, rest, lse = _lib.ops().attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, True)
+        ctx.save_for_backward(q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths)
         ctx.causal, ctx.scale = causal, scale
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths = ctx.saved_tensors
+        q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _lib.ops().attention_backward(dy, q, k, v, y, lse, q_offsets, k_offsets, q_lengths, k_lengths, ctx.causal, ctx.scale,
+        dq, dk, dv = _lib.ops().attention_backward(dy, q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths, ctx.causal, ctx.scale,
                                                    need[0], need[1] or need[2])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None) + (None,) * 6
 
@@ -265,7 +265,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     Statistics and sums are float32; the probabilities (and in the backward pass the
     scores' gradients) are rounded to the tensors' type for the second product.  The backward
-    pass makes the scores again from one saved float32 per row and head."""
+    pass makes the scores again from one saved float32 per row and head, and takes ``sum(dy y)``
+    from ``y`` and what its rounding left, which the forward pass keeps when a gradient is wanted."""
     fn = "attention"
     packed = q_offsets is not None
     if k_offsets is not None and not packed:
