@@ -369,9 +369,13 @@ struct QueryState {
 
   // One step over kTiles x 32 keys, tiles of K and V in LDS.  `limit`: keys of the tile that the lane's query sees (may be
   // negative or beyond the tile); kMasked: whether any lane's ends inside it (code of its own: a branch around these parts has the
-  // compiler copy every accumulator twice a step).  c: scale * log2(e).
-  template <int kTiles, bool kMasked>
-  __device__ __attribute__((always_inline)) inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane) {
+  // compiler copy every accumulator twice a step).  c: scale * log2(e).  between(): run when K's tile has been read, before V's is.
+  struct Nothing {
+    __device__ inline void operator()() const {}
+  };
+  template <int kTiles, bool kMasked, typename Between = Nothing>
+  __device__ __attribute__((always_inline)) inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane,
+                                                             Between between = Between()) {
     f32x16 s[kTiles];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) s[t] = zero16();
@@ -389,6 +393,7 @@ struct QueryState {
       for (int t = 0; t < kTiles; ++t) s[t] = mfma32(a[e & 1][t], q[e], s[t]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    between();
     vec8 w[2][kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(v_tile, b, lane);

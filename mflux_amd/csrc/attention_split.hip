@@ -20,9 +20,9 @@ constexpr int waves_of(int dim) { return dim <= 128 ? 4 : 2; }
 
 template <typename T, int kDim>
 struct SplitShape {
-  static constexpr int kPitch = pitch_of(kDim), kWaves = waves_of(kDim), kStages = 2;
+  static constexpr int kPitch = pitch_of(kDim), kWaves = waves_of(kDim);
   static constexpr int kTile = kStep * kPitch * 2;            // bytes
-  static constexpr int kRing = kStages * 2 * kTile;           // of a wavefront: K, V of each stage
+  static constexpr int kRing = 2 * kTile > kRows * (kDim + 4) * 4 ? 2 * kTile : kRows * (kDim + 4) * 4;  // of a wavefront: K, V
   static constexpr int kPart = kRows * (kDim + 4) * 4;        // a wavefront's result on its way to the others
   static constexpr int kStats = kWaves * kRing;               // where its statistics lie
   static constexpr int kLds = kStats + kWaves * kRows * 8;
@@ -30,22 +30,22 @@ struct SplitShape {
 };
 
 template <typename T, int kDim>
-__global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel(AttentionCall c, int tiles, int splits, float* part_o,
+__global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void attention_split_kernel(AttentionCall c, int splits, int least_chunk, float* part_o,
                                                                                  float2* part_stats) {
   using S = SplitShape<T, kDim>;
   constexpr int kPitch = S::kPitch, kWaves = S::kWaves;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
-  // workgroups are dealt round-robin to the XCDs: the splits of a tile and head behind each other
-  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
-  const int kv_head = item % c.kv_heads, group = c.heads / c.kv_heads;
-  const Run run = find_run<kRows>(c, item / c.kv_heads, false, false, group);
+  // neighbours: the heads of the same tokens, which lie side by side in memory
+  const int kv_head = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
+  const int split = item % splits, group = c.heads / c.kv_heads;
+  const Run run = find_run<kRows>(c, item / splits, false, false, group);
   if (!run.valid) return;
 
   const int row = run.tile * kRows + (lane & 31), token = row / group, head = kv_head * group + row % group;
   const int limit = visible_keys(run, token, c.causal);
   const int most = wave_max(limit), least = wave_min(token < run.nq ? limit : INT32_MAX);
-  const int chunk = ((run.nk + splits - 1) / splits + kStep - 1) / kStep * kStep;
+  const int chunk = max(((run.nk + splits - 1) / splits + kStep - 1) / kStep * kStep, least_chunk);
   const int begin = split * chunk, end = min(min(begin + chunk, run.nk), most);
 
   QueryState<T, kDim, kPitch> state;
@@ -58,29 +58,43 @@ __global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel
     TileLoader<kPitch, kStep, 64> load_k, load_v;
     load_k.init(lane, c.k.token, c.dim);
     load_v.init(lane, c.v.token, c.dim);
-    char* ring = lds + wave * S::kRing;
     const uint32_t ring_at = (uint32_t)(uintptr_t)lds + wave * S::kRing;
     const float scale = c.scale * kLog2e;
-    constexpr int kRequests = 2 * TileLoader<kPitch, kStep, 64>::kLoads;
-    auto request = [&](int first, int stage) __attribute__((always_inline)) {
-      load_k.load(k + (int64_t)first * c.k.token, ring_at + stage * 2 * S::kTile, run.nk - first, lane);
-      load_v.load(v + (int64_t)first * c.v.token, ring_at + stage * 2 * S::kTile + S::kTile, run.nk - first, lane);
+    // A tile of K and one of V in LDS: the next K is requested when the scores are made, the next V behind the second product, so one
+    // of them is always in flight (and eight wavefronts share a compute unit).  A wavefront's requests arrive in order: with the later
+    // tile's still out, the earlier one is there.
+    constexpr int kRequests = TileLoader<kPitch, kStep, 64>::kLoads;
+    const char* k_tile = lds + wave * S::kRing;
+    const char* v_tile = k_tile + S::kTile;
+    auto request_k = [&](int first) __attribute__((always_inline)) {
+      load_k.load(k + (int64_t)first * c.k.token, ring_at, run.nk - first, lane);
+    };
+    auto request_v = [&](int first) __attribute__((always_inline)) {
+      load_v.load(v + (int64_t)first * c.v.token, ring_at + S::kTile, run.nk - first, lane);
     };
     const int first_tile = begin + wave * kStep;
-    if (first_tile < end) request(first_tile, 0);
-    int stage = 0;
-    for (int first = first_tile; first < end; first += kWaves * kStep, stage ^= 1) {
+    if (first_tile < end) {
+      request_k(first_tile);
+      request_v(first_tile);
+    }
+    for (int first = first_tile; first < end; first += kWaves * kStep) {
       const int next = first + kWaves * kStep;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+      auto between = [&]() __attribute__((always_inline)) {
+        if (next < end) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+          request_k(next);
+          asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+      };
+      if (first + kStep <= least) state.template step<1, false>(k_tile, v_tile, kStep, scale, lane, between);
+      else state.template step<1, true>(k_tile, v_tile, limit - first, scale, lane, between);
       if (next < end) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is overwritten
-        request(next, stage ^ 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V
+        request_v(next);
       }
-      const char* tile = ring + stage * 2 * S::kTile;
-      if (first + kStep <= least) state.template step<1, false>(tile, tile + S::kTile, kStep, scale, lane);
-      else state.template step<1, true>(tile, tile + S::kTile, limit - first, scale, lane);
     }
   }
 
@@ -132,48 +146,69 @@ __global__ __launch_bounds__(64 * waves_of(kDim), 1) void attention_split_kernel
         c.lse[(at % c.heads) * rows + at / c.heads] = seen ? top * c2 + __builtin_amdgcn_logf(total) : __builtin_inff();
     } else {
       const int64_t slot = (int64_t)split * rows * c.heads + at;
-      *reinterpret_cast<f32x4*>(part_o + slot * c.dim + d) = o;
+      if (begin < run.nk) *reinterpret_cast<f32x4*>(part_o + slot * c.dim + d) = o;
       if (d == 0) part_stats[slot] = make_float2(top, total);
     }
   }
 }
 
-// y = the partial results of a row joined: a wavefront to a row, the lanes along the head
+// y = the partial results of a row joined: a workgroup to a row, a quarter wavefront (half of one above 64 elements, a whole one
+// above 128) to every split of its own, four elements a lane
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows, int splits, const float* part_o, const float2* part_stats) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-  if (at >= rows * c.heads) return;
+  __shared__ float tops[4], sums[4];
+  __shared__ __attribute__((aligned(16))) float parts[16][256];
+  const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = thread / kWave;
+  const int64_t at = blockIdx.x, step = rows * c.heads;
   const float c2 = c.scale * kLog2e;
   float top = -__builtin_inff();
-  for (int s = lane; s < splits; s += kWave) top = fmaxf(top, part_stats[(int64_t)s * rows * c.heads + at].x);
+  for (int s = thread; s < splits; s += 256) top = fmaxf(top, part_stats[s * step + at].x);
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  const int d = lane * 4;
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int lanes = c.dim <= 64 ? 16 : c.dim <= 128 ? 32 : 64, groups = 256 / lanes;
+  const int mine = thread / lanes, d = thread % lanes * 4;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float total = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const int64_t slot = (int64_t)s * rows * c.heads + at;
-    const float2 st = part_stats[slot];
+#pragma unroll 4
+  for (int s = mine; s < splits; s += groups) {
+    const float2 st = part_stats[s * step + at];
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    if (d < c.dim && (st.y != 0.f || st.x != -__builtin_inff())) a = *reinterpret_cast<const f32x4*>(part_o + (s * step + at) * c.dim + d);
+    // a part without keys has the factor 0; where the reference is an infinity the scores' own NaN stay
     const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * c2);
     total += st.y * f;
-    if (d < c.dim) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(part_o + slot * c.dim + d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += a[e] * f;
-    }
+    for (int e = 0; e < 4; ++e) o[e] += a[e] * f;
   }
+  if (thread % lanes != 0) total = 0.f;  // one lane of a group counts
+#pragma unroll
+  for (int n = 1; n < kWave; n *= 2) total += __shfl_xor(total, n);
+  if (lane == 0) sums[wave] = total;
+  *reinterpret_cast<f32x4*>(&parts[mine][d]) = o;
+  __syncthreads();
+  if (mine) return;
+  total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   // a row that sees no key has neither a maximum nor a sum (a sum that is NaN is a row's own)
   const bool empty = top == -__builtin_inff() && total == 0.f;
   const float f = 1.0f / total;
   if (d < c.dim) {
+    for (int g = 1; g < groups; ++g) o += *reinterpret_cast<const f32x4*>(&parts[g][d]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = empty ? 0.f : o[e] * f;
     const u32x2 packed = pack4<T>(o);
     *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = packed;
     if (c.rest) *reinterpret_cast<u32x2*>(c.rest + at * c.dim + d) = pack4_rest<T>(o, packed);
   }
-  if (c.lse && lane == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + __builtin_amdgcn_logf(total);
+  if (c.lse && thread == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + __builtin_amdgcn_logf(total);
+}
+
+// keys of a call's longest sequence as the host knows it, over the splits
+int least_chunk(const AttentionCall& c, int splits) {
+  const int64_t keys = c.q_offsets ? (c.k_tokens + c.batch - 1) / c.batch : c.k_tokens;
+  return (int)(((keys + splits - 1) / splits + kStep - 1) / kStep * kStep);
 }
 
 int64_t rows_of(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens; }
@@ -191,11 +226,11 @@ int launch(const AttentionCall& c, int splits, float* workspace, hipStream_t str
   if (grid > INT32_MAX) return MFQ_ESHAPE;
   float* part_o = workspace;
   float2* part_stats = splits > 1 ? reinterpret_cast<float2*>(workspace + splits * rows * c.heads * c.dim) : nullptr;
-  hipLaunchKernelGGL((attention_split_kernel<T, kDim>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, (int)tiles, splits,
-                     part_o, part_stats);
+  hipLaunchKernelGGL((attention_split_kernel<T, kDim>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, splits,
+                     least_chunk(c, splits), part_o, part_stats);
   if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
   if (splits == 1) return MFQ_OK;
-  hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((rows * c.heads + 3) / 4)), dim3(256), 0, stream, c, rows, splits, part_o, part_stats);
+  hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(rows * c.heads)), dim3(256), 0, stream, c, rows, splits, part_o, part_stats);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
@@ -217,8 +252,11 @@ int attention_splits(const AttentionCall& c) {
   if (queries * group > kRows) return 0;
   const int64_t keys = c.q_offsets ? (c.k_tokens + c.batch - 1) / std::max(c.batch, 1) : c.k_tokens;
   const int64_t items = std::max<int64_t>(tiles_of(c) - (c.q_offsets ? 2 : 0), 1) * c.kv_heads;
-  const int64_t most = std::max<int64_t>(keys / 256, 1);  // a split has 256 keys at least
-  return (int)std::min({most, (4 * (int64_t)compute_units() + items - 1) / items, (int64_t)256});
+  // Eight workgroups for every compute unit, so that sequences of different lengths fill it evenly (32 of them, 1024 to 8192 keys, 8
+  // key heads: 132, 134, 125, 125 us with one, four, eight, sixteen), each with 256 keys at least; and at most 64 ranges, which
+  // the join reads behind each other (one sequence of 100003 keys, 4 key heads: 47, 51, 60 us with 64, 128, 256).
+  const int64_t want = (8 * (int64_t)compute_units() + items - 1) / items;
+  return (int)std::min({std::max<int64_t>(keys / 256, 1), want, (int64_t)64});
 }
 
 size_t attention_split_bytes(const AttentionCall& c, int splits) {
