@@ -76,7 +76,8 @@ __device__ inline int wave_scan(int v) {
 
 // Tile `index` of kTile rows among all sequences' tiles.  Packed calls: offsets are read clamped to the tensor (whatever they
 // hold, no row outside it is touched), the rows in front of the first and behind the last sequence count as sequences without
-// keys, and the sequences' tiles are counted by a scan over the lanes, so the host needs no sequence's length.  `by_key`: tiles
+// keys, and the sequences' tiles are counted by the lanes, one to a sequence, so the host needs no sequence's length: up to 62
+// of them by decreasing number of keys, so that the longest workgroups start first, more in their own order.  `by_key`: tiles
 // of key rows instead of query rows; `per`: rows that a token counts for.  `reverse`: the last tile first (causal: the longest
 // first).
 template <int kTile>
@@ -114,13 +115,39 @@ __device__ inline Run find_run(const AttentionCall& c, int index, bool by_key, b
     if (s < n) bounds(offsets, tokens, s, first, count);
     return (count * per + kTile - 1) / kTile;
   };
+  r.valid = false;
+  r.batch = r.q0 = r.nq = r.k0 = r.nk = r.rows = r.tile = 0;
+  if (n <= kWave) {
+    int q0 = 0, nq = 0, k0 = 0, nk = 0;
+    if (lane < n) {
+      bounds(c.q_offsets, c.q_tokens, lane, q0, nq);
+      bounds(c.k_offsets, c.k_tokens, lane, k0, nk);
+    }
+    const int rows = by_key ? nk : nq, tiles = (rows * per + kTile - 1) / kTile;
+    if (lane == 0 || lane >= n - 1) nq = nk = 0;
+    int before = 0;
+    for (int i = 0; i < n; ++i) {
+      const int keys = __builtin_amdgcn_readlane(nk, i), count = __builtin_amdgcn_readlane(tiles, i);
+      before += keys > nk || (keys == nk && i < lane) ? count : 0;
+    }
+    const uint64_t here = __ballot(lane < n && index >= before && index < before + tiles);
+    if (!here) return r;
+    const int l = __builtin_ctzll(here);
+    r.valid = true;
+    r.tile = index - __builtin_amdgcn_readlane(before, l);
+    if (reverse) r.tile = __builtin_amdgcn_readlane(tiles, l) - 1 - r.tile;
+    r.q0 = __builtin_amdgcn_readlane(q0, l);
+    r.nq = __builtin_amdgcn_readlane(nq, l);
+    r.k0 = __builtin_amdgcn_readlane(k0, l);
+    r.nk = __builtin_amdgcn_readlane(nk, l);
+    r.rows = __builtin_amdgcn_readlane(rows, l);
+    return r;
+  }
   int total = 0;
   if (reverse) {
     for (int s = 0; s < n; s += kWave) total += __shfl(wave_scan(tiles_of(s + lane)), kWave - 1);
     index = total - 1 - index;
   }
-  r.valid = false;
-  r.batch = r.q0 = r.nq = r.k0 = r.nk = r.rows = r.tile = 0;
   if (index < 0) return r;
   int before = 0;
   for (int s = 0; s < n; s += kWave) {
@@ -379,18 +406,19 @@ struct QueryState {
     f32x16 s[kTiles];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) s[t] = zero16();
-    // operands are read a step ahead of the matrix instructions that take them
-    vec8 a[2][kTiles];
+    // operands are read two steps ahead of the matrix instructions that take them
+    vec8 a[3][kTiles];
+    auto rows = [&](int e) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) a[0][t] = tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, 0, lane);
+      for (int t = 0; t < kTiles; ++t) a[e % 3][t] = tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, e, lane);
+    };
+    rows(0);
+    rows(1);
 #pragma unroll
     for (int e = 0; e < kSteps; ++e) {
-      if (e + 1 < kSteps) {
+      if (e + 2 < kSteps) rows(e + 2);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) a[(e + 1) & 1][t] = tile_rows<T, kPitch>(k_tile + t * 32 * kPitch * 2, e + 1, lane);
-      }
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) s[t] = mfma32(a[e & 1][t], q[e], s[t]);
+      for (int t = 0; t < kTiles; ++t) s[t] = mfma32(a[e % 3][t], q[e], s[t]);
       __builtin_amdgcn_sched_barrier(0);
     }
     between();

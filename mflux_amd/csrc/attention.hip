@@ -8,17 +8,18 @@
 // tiles go straight from memory into LDS (two of each, the next pair in flight while the current one is multiplied) and are
 // read by all four wavefronts.  See attention.h for the orientation of the products.
 #include "attention.h"
+#include <cstdlib>
 
 namespace mfq {
 namespace {
 
-constexpr int kQueries = 128;  // of a workgroup
-constexpr int kKeys = 64;      // of a step
+constexpr int kKeys = 64;  // of a step
 
 constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-template <typename T, int kDim>
-__global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
+template <typename T, int kDim, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
+  constexpr int kQueries = 32 * kWaves;
   constexpr int kPitch = pitch_of(kDim);
   constexpr int kTileBytes = kKeys * kPitch * 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // K, V, K, V
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
     state.load_row(state.q, c.q.p + q_at, c.dim, lane);
     const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
     const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
-    TileLoader<kPitch, kKeys, 256> load_k, load_v;
+    TileLoader<kPitch, kKeys, 64 * kWaves> load_k, load_v;
     load_k.init(thread, c.k.token, c.dim);
     load_v.init(thread, c.v.token, c.dim);
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
@@ -92,25 +93,26 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
   }
 }
 
-template <typename T, int kDim>
+template <typename T, int kDim, int kWaves>
 int launch(const AttentionCall& c, hipStream_t stream) {
+  constexpr int kQueries = 32 * kWaves;
   constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
   static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim>), kBytes)) return MFQ_ELAUNCH;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim, kWaves>), kBytes)) return MFQ_ELAUNCH;
   // packed: a tile that is not full for every sequence at most, and for the rows in front of and behind them
   const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
   if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
-  hipLaunchKernelGGL((attention_kernel<T, kDim>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+  hipLaunchKernelGGL((attention_kernel<T, kDim, kWaves>), dim3((unsigned)(tiles * c.heads)), dim3(64 * kWaves), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
 template <typename T>
 int launch_dim(const AttentionCall& c, hipStream_t stream) {
-  if (c.dim <= 64) return launch<T, 64>(c, stream);
-  if (c.dim <= 96) return launch<T, 96>(c, stream);
-  if (c.dim <= 128) return launch<T, 128>(c, stream);
-  if (c.dim <= 192) return launch<T, 192>(c, stream);
-  return launch<T, 256>(c, stream);
+  if (c.dim <= 64) return launch<T, 64, 4>(c, stream);
+  if (c.dim <= 96) return launch<T, 96, 4>(c, stream);
+  if (c.dim <= 128) return getenv("W8") ? launch<T, 128, 8>(c, stream) : launch<T, 128, 4>(c, stream);
+  if (c.dim <= 192) return launch<T, 192, 4>(c, stream);
+  return launch<T, 256, 4>(c, stream);
 }
 
 }  // namespace
