@@ -477,6 +477,81 @@ struct QueryState {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  // ---- the same over 32 keys in two halves that overlap: while the matrix pipeline makes the next block's scores, the vector pipeline
+  // takes this one's exponentials, and while it multiplies with V, the maximum over the next block's.
+  // scores of a block alone (the first one)
+  __device__ __attribute__((always_inline)) inline void scores(f32x16& s, const char* k32, int lane) {
+    s = zero16();
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) s = mfma32(tile_rows<T, kPitch>(k32, e, lane), q[e], s);
+  }
+  // the reference follows the block's maximum (see step)
+  __device__ __attribute__((always_inline)) inline void follow(float most, float c) {
+    most = max_halves(most);
+    if (__any((most - top) * c > 8.f)) {
+      const float next = fmaxf(top, most);
+      const float factor = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((top - next) * c);
+      top = next;
+      sum *= factor;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= factor;
+    }
+  }
+  __device__ __attribute__((always_inline)) static inline float maximum(const f32x16& s) {
+    float most = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+    return most;
+  }
+  // s: the block's scores; kNext: next = the scores of the block at k32
+  template <bool kNext>
+  __device__ __attribute__((always_inline)) inline void overlapped(f32x16& s, f32x16& next, const char* k32, const char* v32, float c, int lane) {
+    const float shift = top == -__builtin_inff() ? 0.f : top * c;
+    vec8 p[2], w[2][kBlocks], a[3];
+    if constexpr (kNext) {
+      next = zero16();
+      a[0] = tile_rows<T, kPitch>(k32, 0, lane);
+      a[1] = tile_rows<T, kPitch>(k32, 1, lane);
+    }
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) {
+      if constexpr (kNext) {
+        if (e + 2 < kSteps) a[(e + 2) % 3] = tile_rows<T, kPitch>(k32, e + 2, lane);
+        next = mfma32(a[e % 3], q[e], next);
+      }
+      // V's first operands, when the reads of K end
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        if (b * 2 / kBlocks + kSteps - 2 == e) w[0][b] = tile_columns<T, kPitch>(v32, b, lane);
+#pragma unroll
+      for (int i = 16 * e / kSteps; i < 16 * (e + 1) / kSteps; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -shift));
+        if ((i & 7) == 7) {
+          p[i >> 3] = result_operand<T>(s, i >> 3);
+          sum = add_sum<T>(p[i >> 3], sum);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float most[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        if (n == 0) w[1][b] = tile_columns<T, kPitch>(v32 + 16 * kPitch * 2, b, lane);
+        o[b] = mfma32(w[n][b], p[n], o[b]);
+        if constexpr (kNext) {
+          const int g = n * kBlocks + b;
+#pragma unroll
+          for (int i = 16 * g / (2 * kBlocks); i < 16 * (g + 1) / (2 * kBlocks); ++i) most[i & 3] = fmaxf(most[i & 3], next[i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (kNext) follow(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), c);
+  }
   // exponentials of half a score tile as the second product's operand, added to the sum
   __device__ __attribute__((always_inline)) inline vec8 probabilities(f32x16& s, int slab, float c, float shift) {
 #pragma unroll

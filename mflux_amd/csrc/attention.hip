@@ -8,7 +8,6 @@
 // tiles go straight from memory into LDS (two of each, the next pair in flight while the current one is multiplied) and are
 // read by all four wavefronts.  See attention.h for the orientation of the products.
 #include "attention.h"
-#include <cstdlib>
 
 namespace mfq {
 namespace {
@@ -17,9 +16,9 @@ constexpr int kKeys = 64;  // of a step
 
 constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-template <typename T, int kDim, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
-  constexpr int kQueries = 32 * kWaves;
+template <typename T, int kDim>
+__global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
+  constexpr int kQueries = 128;  // of a workgroup
   constexpr int kPitch = pitch_of(kDim);
   constexpr int kTileBytes = kKeys * kPitch * 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // K, V, K, V
@@ -43,36 +42,72 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ke
     state.load_row(state.q, c.q.p + q_at, c.dim, lane);
     const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
     const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
-    TileLoader<kPitch, kKeys, 64 * kWaves> load_k, load_v;
+    TileLoader<kPitch, kKeys, 256> load_k, load_v;
     load_k.init(thread, c.k.token, c.dim);
     load_v.init(thread, c.v.token, c.dim);
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
     const float scale = c.scale * kLog2e;
-    load_k.load(k, lds_at, keys, thread);
-    load_v.load(v, lds_at + kTileBytes, keys, thread);
+    auto request_k = [&](int first) __attribute__((always_inline)) {
+      load_k.load(k + (int64_t)first * c.k.token, lds_at + (first / kKeys & 1) * 2 * kTileBytes, keys - first, thread);
+    };
+    auto request_v = [&](int first) __attribute__((always_inline)) {
+      load_v.load(v + (int64_t)first * c.v.token, lds_at + (first / kKeys & 1) * 2 * kTileBytes + kTileBytes, keys - first, thread);
+    };
+    request_k(0);
+    request_v(0);
+    // Tiles that every query of the workgroup sees all of (those that are there: the others' rows are not stored) come first, by pairs, so
+    // that their places in LDS are constants, in blocks of 32 keys whose two halves overlap with the neighbours'.  At the first block of a
+    // tile its K has arrived (its V may be on the way), everyone is done with the K of the tile before, and the next one's is
+    // requested into its place; at the second block the same goes for V.
+    constexpr int kRequests = TileLoader<kPitch, kKeys, 256>::kLoads, kHalf = 32 * kPitch * 2;
+    const int whole = uniform(c.causal ? visible_keys(run, run.tile * kQueries, 1) : run.nk) / (2 * kKeys) * (2 * kKeys);
+    int first = 0, buffer = 0;
+    if (whole > 0) {
+      f32x16 s0, s1;
+      auto arrive_k = [&](int at) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kRequests) : "memory");
+        if (at + kKeys < keys) request_k(at + kKeys);
+      };
+      auto arrive_v = [&](int at) __attribute__((always_inline)) {
+        if (at + kKeys < keys) {
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kRequests) : "memory");
+          request_v(at + kKeys);
+        } else {
+          arrive_and_sync();
+        }
+      };
+      const char *k0 = lds, *v0 = lds + kTileBytes, *k1 = lds + 2 * kTileBytes, *v1 = lds + 3 * kTileBytes;
+      auto three_blocks = [&](int at) __attribute__((always_inline)) {
+        arrive_v(at);
+        state.template overlapped<true>(s0, s1, k0 + kHalf, v0, scale, lane);
+        arrive_k(at + kKeys);
+        state.template overlapped<true>(s1, s0, k1, v0 + kHalf, scale, lane);
+        arrive_v(at + kKeys);
+        state.template overlapped<true>(s0, s1, k1 + kHalf, v1, scale, lane);
+      };
+      arrive_k(0);
+      state.scores(s0, k0, lane);
+      state.follow(state.maximum(s0), scale);
+      three_blocks(0);
+      for (first = 2 * kKeys; first < whole; first += 2 * kKeys) {
+        arrive_k(first);
+        state.template overlapped<true>(s1, s0, k0, v1 + kHalf, scale, lane);
+        three_blocks(first);
+      }
+      state.template overlapped<false>(s1, s0, nullptr, v1 + kHalf, scale, lane);
+    }
     // the tile of `buffer` has arrived and the next one is requested
-    auto advance = [&](int first, int buffer) __attribute__((always_inline)) {
+    auto advance = [&](int at) __attribute__((always_inline)) {
       arrive_and_sync();
-      const int next = first + kKeys;
-      if (next < keys) {
-        const uint32_t to = lds_at + (buffer ^ 1) * 2 * kTileBytes;
-        load_k.load(k + (int64_t)next * c.k.token, to, keys - next, thread);
-        load_v.load(v + (int64_t)next * c.v.token, to + kTileBytes, keys - next, thread);
+      if (at + kKeys < keys) {
+        request_k(at + kKeys);
+        request_v(at + kKeys);
       }
     };
-    // Tiles that every query of the workgroup sees all of (those that are there: the others' rows are not stored) come first, by pairs, so that their places in LDS are constants.
-    const int whole = uniform(c.causal ? visible_keys(run, run.tile * kQueries, 1) : run.nk);
-    int first = 0, buffer = 0;
-    for (; first + 2 * kKeys <= whole; first += 2 * kKeys) {
-      advance(first, 0);
-      state.template step<2, false>(lds, lds + kTileBytes, kKeys, scale, lane);
-      advance(first + kKeys, 1);
-      state.template step<2, false>(lds + 2 * kTileBytes, lds + 3 * kTileBytes, kKeys, scale, lane);
-    }
     // the others in blocks of 32 keys, so that of a wavefront's own edge only what lies across it is masked
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
-      advance(first, buffer);
+      advance(first);
 #pragma unroll 1
       for (int at = first; at < min(first + kKeys, most); at += 32) {
         const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
@@ -93,26 +128,26 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ke
   }
 }
 
-template <typename T, int kDim, int kWaves>
+template <typename T, int kDim>
 int launch(const AttentionCall& c, hipStream_t stream) {
-  constexpr int kQueries = 32 * kWaves;
+  constexpr int kQueries = 128;  // of a workgroup
   constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
   static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim, kWaves>), kBytes)) return MFQ_ELAUNCH;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim>), kBytes)) return MFQ_ELAUNCH;
   // packed: a tile that is not full for every sequence at most, and for the rows in front of and behind them
   const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
   if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
-  hipLaunchKernelGGL((attention_kernel<T, kDim, kWaves>), dim3((unsigned)(tiles * c.heads)), dim3(64 * kWaves), kBytes, stream, c, (int)tiles);
+  hipLaunchKernelGGL((attention_kernel<T, kDim>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
 template <typename T>
 int launch_dim(const AttentionCall& c, hipStream_t stream) {
-  if (c.dim <= 64) return launch<T, 64, 4>(c, stream);
-  if (c.dim <= 96) return launch<T, 96, 4>(c, stream);
-  if (c.dim <= 128) return getenv("W8") ? launch<T, 128, 8>(c, stream) : launch<T, 128, 4>(c, stream);
-  if (c.dim <= 192) return launch<T, 192, 4>(c, stream);
-  return launch<T, 256, 4>(c, stream);
+  if (c.dim <= 64) return launch<T, 64>(c, stream);
+  if (c.dim <= 96) return launch<T, 96>(c, stream);
+  if (c.dim <= 128) return launch<T, 128>(c, stream);
+  if (c.dim <= 192) return launch<T, 192>(c, stream);
+  return launch<T, 256>(c, stream);
 }
 
 }  // namespace
