@@ -238,6 +238,20 @@ struct TileLoader {
   }
 };
 
+// Whether any of the workgroup's kWaves wavefronts says so; `at`: LDS that nobody reads any more.  Nothing is in flight afterwards.
+template <int kWaves>
+__device__ inline bool any_wave(bool mine, char* at) {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  int* flags = reinterpret_cast<int*>(at);
+  if ((threadIdx.x & (kWave - 1)) == 0) flags[threadIdx.x / kWave] = mine;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) any |= flags[w];
+  __syncthreads();
+  return uniform(any);
+}
+
 // this wavefront's requests have arrived, and everyone's reads so far are done
 __device__ inline void arrive_and_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -316,7 +330,8 @@ __device__ inline float add_sum(typename T::vec8 p, float sum) {
 
 // Whether a tile of kTiles x 32 rows holds an infinity or a NaN: in a product with zeros every finite element gives zero.  Asked of
 // tiles at a mask's edge alone: a masked row's probability is zero, but zero times such an element is NaN, which the product would
-// hand to columns that never see the row.
+// hand to columns that never see the row.  A workgroup (in the split form a wavefront) that met such a tile begins again and adds every
+// row by itself: code of its own, so that it costs the other calls no register.
 template <typename T, int kPitch, int kSteps, int kTiles>
 __device__ inline bool tile_not_finite(const char* tile, int lane) {
   using vec8 = typename T::vec8;
@@ -332,11 +347,6 @@ __device__ inline bool tile_not_finite(const char* tile, int lane) {
   return __any(sum != 0.f);
 }
 
-template <typename T>
-__device__ inline typename T::vec8 masked(typename T::vec8 v, uint32_t mask) {
-  return __builtin_bit_cast(typename T::vec8, __builtin_bit_cast(u32x4a, v) & u32x4a{mask, mask, mask, mask});
-}
-
 // The product of a 32 x 32 tile of results with zeros: 0, or NaN if any of them is not finite
 __device__ inline float times_zero(const f32x16& s, float sum) {
 #pragma unroll
@@ -344,7 +354,7 @@ __device__ inline float times_zero(const f32x16& s, float sum) {
   return sum;
 }
 
-// acc += tile^T p for 16 rows of such a tile, row by row, each added only where it is visible.  visible(row): of the lane's column.
+// acc += tile^T p for 16 rows of a tile, row by row, each added only where it is visible.  visible(row): of the lane's column.
 template <typename T, int kPitch, int kBlocks, typename Visible>
 __device__ inline void add_columns_one_by_one(f32x16 (&acc)[kBlocks], const char* tile16, typename T::vec8 p, int lane, Visible visible) {
   using vec8 = typename T::vec8;
@@ -397,11 +407,12 @@ struct QueryState {
   // One step over kTiles x 32 keys, tiles of K and V in LDS.  `limit`: keys of the tile that the lane's query sees (may be
   // negative or beyond the tile); kMasked: whether any lane's ends inside it (code of its own: a branch around these parts has the
   // compiler copy every accumulator twice a step).  c: scale * log2(e).  between(): run when K's tile has been read, before V's is.
+  // A masked step answers whether V's tile holds an infinity or a NaN: then its result is not to be used, and kOneByOne gives it.
   struct Nothing {
     __device__ inline void operator()() const {}
   };
-  template <int kTiles, bool kMasked, typename Between = Nothing>
-  __device__ __attribute__((always_inline)) inline void step(const char* k_tile, const char* v_tile, int limit, float c, int lane,
+  template <int kTiles, bool kMasked, bool kOneByOne = false, typename Between = Nothing>
+  __device__ __attribute__((always_inline)) inline bool step(const char* k_tile, const char* v_tile, int limit, float c, int lane,
                                                              Between between = Between()) {
     f32x16 s[kTiles];
 #pragma unroll
@@ -425,14 +436,13 @@ struct QueryState {
     vec8 w[2][kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(v_tile, b, lane);
-    bool one_by_one = false;
+    bool not_finite = false;
     if constexpr (kMasked) {
-      one_by_one = tile_not_finite<T, kPitch, kSteps, kTiles>(v_tile, lane);
+      if constexpr (!kOneByOne) not_finite = tile_not_finite<T, kPitch, kSteps, kTiles>(v_tile, lane);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * t + result_row(i, lane) >= limit) s[t][i] = -__builtin_inff();
+        for (int i = 0; i < 16; ++i) s[t][i] = 32 * t + result_row(i, lane) < limit ? s[t][i] : -__builtin_inff();
     }
     float most = -__builtin_inff();
 #pragma unroll
@@ -453,29 +463,30 @@ struct QueryState {
         for (int i = 0; i < 16; ++i) o[b][i] *= factor;
     }
     const float shift = top == -__builtin_inff() ? 0.f : top * c;
-    vec8 p[2 * kTiles];
-    if constexpr (kMasked) {
-#pragma unroll
-      for (int n = 0; n < 2 * kTiles; ++n) p[n] = probabilities(s[n / 2], n & 1, c, shift);
-      if (__builtin_expect(one_by_one, 0)) {
-#pragma unroll
-        for (int n = 0; n < 2 * kTiles; ++n)
-          add_columns_one_by_one<T, kPitch, kBlocks>(o, v_tile + n * 16 * kPitch * 2, p[n], lane, [&](int row) { return 16 * n + row < limit; });
-      }
-    }
-    const uint32_t keep = one_by_one ? 0u : ~0u;  // the product adds nothing where that has been done
 #pragma unroll
     for (int n = 0; n < 2 * kTiles; ++n) {
-      if constexpr (kMasked) p[n] = masked<T>(p[n], keep);
-      else p[n] = probabilities(s[n / 2], n & 1, c, shift);
-      if (n + 1 < 2 * kTiles) {
+      const vec8 p = probabilities(s[n / 2], n & 1, c, shift);
+      if constexpr (kOneByOne) {
+        add_columns_one_by_one<T, kPitch, kBlocks>(o, v_tile + n * 16 * kPitch * 2, p, lane, [&](int row) { return 16 * n + row < limit; });
+      } else {
+        if (n + 1 < 2 * kTiles) {
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) w[(n + 1) & 1][b] = tile_columns<T, kPitch>(v_tile + (n + 1) * 16 * kPitch * 2, b, lane);
+          for (int b = 0; b < kBlocks; ++b) w[(n + 1) & 1][b] = tile_columns<T, kPitch>(v_tile + (n + 1) * 16 * kPitch * 2, b, lane);
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] = mfma32(w[n & 1][b], p, o[b]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) o[b] = mfma32(kMasked ? masked<T>(w[n & 1][b], keep) : w[n & 1][b], p[n], o[b]);
-      __builtin_amdgcn_sched_barrier(0);
     }
+    return not_finite;
+  }
+  // exponentials of half a score tile as the second product's operand, added to the sum
+  __device__ __attribute__((always_inline)) inline vec8 probabilities(f32x16& s, int slab, float c, float shift) {
+#pragma unroll
+    for (int i = 8 * slab; i < 8 * slab + 8; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -shift));
+    const vec8 p = result_operand<T>(s, slab);
+    sum = add_sum<T>(p, sum);
+    return p;
   }
   // ---- the same over 32 keys in two halves that overlap: while the matrix pipeline makes the next block's scores, the vector pipeline
   // takes this one's exponentials, and while it multiplies with V, the maximum over the next block's.
@@ -551,14 +562,6 @@ struct QueryState {
       }
     }
     if constexpr (kNext) follow(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), c);
-  }
-  // exponentials of half a score tile as the second product's operand, added to the sum
-  __device__ __attribute__((always_inline)) inline vec8 probabilities(f32x16& s, int slab, float c, float shift) {
-#pragma unroll
-    for (int i = 8 * slab; i < 8 * slab + 8; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -shift));
-    const vec8 p = result_operand<T>(s, slab);
-    sum = add_sum<T>(p, sum);
-    return p;
   }
 };
 

@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
       }
     };
     // the others in blocks of 32 keys, so that of a wavefront's own edge only what lies across it is masked
+    bool not_finite = false;
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
       advance(first);
@@ -112,7 +113,21 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
       for (int at = first; at < min(first + kKeys, most); at += 32) {
         const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
         if (at + 32 <= least) state.template step<1, false>(k32, k32 + kTileBytes, 32, scale, lane);
-        else state.template step<1, true>(k32, k32 + kTileBytes, limit - at, scale, lane);
+        else not_finite |= state.template step<1, true>(k32, k32 + kTileBytes, limit - at, scale, lane);
+      }
+    }
+    if (whole < keys && any_wave<4>(not_finite, lds)) {
+      state.init();
+      request_k(0);
+      request_v(0);
+#pragma unroll 1
+      for (first = 0, buffer = 0; first < keys; first += kKeys, buffer ^= 1) {
+        advance(first);
+#pragma unroll 1
+        for (int at = first; at < min(first + kKeys, most); at += 32) {
+          const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
+          state.template step<1, true, true>(k32, k32 + kTileBytes, limit - at, scale, lane);
+        }
       }
     }
   }

@@ -15,6 +15,11 @@ namespace {
 
 constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+// a step over what every row sees, over what some see, and the same where a row is not finite (attention.h, tile_not_finite)
+enum { kWhole, kEdge, kRowByRow };
+template <int kMode>
+using Mode = std::integral_constant<int, kMode>;
+
 constexpr int kQueries = 128;  // of a workgroup of the first kernel
 constexpr int kKeys = 64;      // of its step
 
@@ -72,9 +77,9 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     const float scale = c.scale * kLog2e;
 
     // 32 keys
-    auto step = [&](const char* k32, const char* v32, int left, auto is_masked) __attribute__((always_inline)) {
-      constexpr bool kMasked = decltype(is_masked)::value;
-      bool one_by_one = false;
+    auto step = [&](const char* k32, const char* v32, int left, auto mode) __attribute__((always_inline)) {
+      constexpr bool kMasked = decltype(mode)::value != kWhole, kOneByOne = decltype(mode)::value == kRowByRow;
+      bool not_finite = false;
       {
         f32x16 s = zero16(), dp = zero16();
         // operands are read a step ahead of the matrix instructions that take them
@@ -93,33 +98,30 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(k32, b, lane);
         // a row of K that is not finite shows in every score of it (attention.h, tile_not_finite)
-        if constexpr (kMasked) one_by_one = __any(times_zero(s, 0.f) != 0.f);
+        if constexpr (kMasked && !kOneByOne) not_finite = __any(times_zero(s, 0.f) != 0.f);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse));
           s[i] = p * (dp[i] - delta);
-          if (kMasked && result_row(i, lane) >= left) s[i] = 0.f;
+          if constexpr (kMasked) s[i] = result_row(i, lane) < left ? s[i] : 0.f;
         }
-        if (kMasked && __builtin_expect(one_by_one, 0)) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            add_columns_one_by_one<T, kPitch, kBlocks>(dq, k32 + n * 16 * kPitch * 2, result_operand<T>(s, n), lane,
-                                                       [&](int r) { return 16 * n + r < left; });
-        }
-        const uint32_t keep = one_by_one ? 0u : ~0u;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          vec8 ds = result_operand<T>(s, n);
-          if constexpr (kMasked) ds = masked<T>(ds, keep);
-          if (n == 0) {
+          const vec8 ds = result_operand<T>(s, n);
+          if constexpr (kOneByOne) {
+            add_columns_one_by_one<T, kPitch, kBlocks>(dq, k32 + n * 16 * kPitch * 2, ds, lane, [&](int r) { return 16 * n + r < left; });
+          } else {
+            if (n == 0) {
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) w[1][b] = tile_columns<T, kPitch>(k32 + 16 * kPitch * 2, b, lane);
+              for (int b = 0; b < kBlocks; ++b) w[1][b] = tile_columns<T, kPitch>(k32 + 16 * kPitch * 2, b, lane);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) dq[b] = mfma32(w[n][b], ds, dq[b]);
+            __builtin_amdgcn_sched_barrier(0);
           }
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) dq[b] = mfma32(kMasked ? masked<T>(w[n][b], keep) : w[n][b], ds, dq[b]);
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      return not_finite;
     };
     load_k.load(k, lds_at, keys, thread);
     load_v.load(v, lds_at + kTileBytes, keys, thread);
@@ -138,20 +140,36 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     constexpr int kHalf = 32 * kPitch * 2;
     for (; first + 2 * kKeys <= whole; first += 2 * kKeys) {
       advance(first, 0);
-      step(lds, lds + kTileBytes, 32, std::false_type());
-      step(lds + kHalf, lds + kTileBytes + kHalf, 32, std::false_type());
+      step(lds, lds + kTileBytes, 32, Mode<kWhole>());
+      step(lds + kHalf, lds + kTileBytes + kHalf, 32, Mode<kWhole>());
       advance(first + kKeys, 1);
-      step(lds + 2 * kTileBytes, lds + 3 * kTileBytes, 32, std::false_type());
-      step(lds + 2 * kTileBytes + kHalf, lds + 3 * kTileBytes + kHalf, 32, std::false_type());
+      step(lds + 2 * kTileBytes, lds + 3 * kTileBytes, 32, Mode<kWhole>());
+      step(lds + 2 * kTileBytes + kHalf, lds + 3 * kTileBytes + kHalf, 32, Mode<kWhole>());
     }
+    bool not_finite = false;
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
       advance(first, buffer);
 #pragma unroll 1
       for (int at = first; at < min(first + kKeys, most); at += 32) {
         const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
-        if (at + 32 <= least) step(k32, k32 + kTileBytes, 32, std::false_type());
-        else step(k32, k32 + kTileBytes, limit - at, std::true_type());
+        if (at + 32 <= least) step(k32, k32 + kTileBytes, 32, Mode<kWhole>());
+        else not_finite |= step(k32, k32 + kTileBytes, limit - at, Mode<kEdge>());
+      }
+    }
+    if (any_wave<4>(not_finite, lds)) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) dq[b] = zero16();
+      load_k.load(k, lds_at, keys, thread);
+      load_v.load(v, lds_at + kTileBytes, keys, thread);
+#pragma unroll 1
+      for (first = 0, buffer = 0; first < keys; first += kKeys, buffer ^= 1) {
+        advance(first, buffer);
+#pragma unroll 1
+        for (int at = first; at < min(first + kKeys, most); at += 32) {
+          const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
+          step(k32, k32 + kTileBytes, limit - at, Mode<kRowByRow>());
+        }
       }
     }
   }
@@ -268,13 +286,13 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
       if (wave == 1) load_floats(delta0 + head * rows + first, to + 2 * S::kTile + 256, run.nq - first, kRows, lane);
     };
     // masked: the queries [start, left) of the wavefront's 32 are there and see the lane's key
-    auto step = [&](const char* stage, int start, int left, auto is_masked) __attribute__((always_inline)) {
-      constexpr bool kMasked = decltype(is_masked)::value;
+    auto step = [&](const char* stage, int start, int left, auto mode) __attribute__((always_inline)) {
+      constexpr bool kMasked = decltype(mode)::value != kWhole, kOneByOne = decltype(mode)::value == kRowByRow;
       const char* q32 = stage + half * 32 * kPitch * 2;
       const char* dy32 = q32 + S::kTile;
       const float* lse = reinterpret_cast<const float*>(stage + 2 * S::kTile) + half * 32;
       const float* delta = lse + 64;
-      bool one_by_one = false;
+      bool not_finite = false;
       f32x16 s = zero16(), dp = zero16();
       vec8 a[2][4];
       auto operands = [&](int e) __attribute__((always_inline)) {
@@ -292,7 +310,7 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
         dp = mfma32(a[e & 1][1], a[e & 1][2], dp);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (kMasked) one_by_one = __any(times_zero(s, times_zero(dp, 0.f)) != 0.f);
+      if constexpr (kMasked && !kOneByOne) not_finite = __any(times_zero(s, times_zero(dp, 0.f)) != 0.f);
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int r = result_row(i, lane);
@@ -305,36 +323,35 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
           dp[i + j] = see ? ds : 0.f;
         }
       }
-      if (kMasked && __builtin_expect(one_by_one, 0)) {
+      if constexpr (kOneByOne) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           auto visible = [&](int r) { return 16 * n + r >= start && 16 * n + r < left; };
           add_columns_one_by_one<T, kPitch, kBlocks>(dv, dy32 + n * 16 * kPitch * 2, result_operand<T>(s, n), lane, visible);
           add_columns_one_by_one<T, kPitch, kBlocks>(dk, q32 + n * 16 * kPitch * 2, result_operand<T>(dp, n), lane, visible);
         }
-      }
-      const uint32_t keep = one_by_one ? 0u : ~0u;
-      // four products of 16 rows each: dv, dk, dv, dk
-      vec8 w[2][kBlocks];
+      } else {
+        // four products of 16 rows each: dv, dk, dv, dk
+        vec8 w[2][kBlocks];
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(dy32, b, lane);
+        for (int b = 0; b < kBlocks; ++b) w[0][b] = tile_columns<T, kPitch>(dy32, b, lane);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (n < 3) {
+        for (int n = 0; n < 4; ++n) {
+          if (n < 3) {
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b)
-            w[(n + 1) & 1][b] = tile_columns<T, kPitch>((n & 1 ? dy32 : q32) + ((n + 1) >> 1) * 16 * kPitch * 2, b, lane);
+            for (int b = 0; b < kBlocks; ++b)
+              w[(n + 1) & 1][b] = tile_columns<T, kPitch>((n & 1 ? dy32 : q32) + ((n + 1) >> 1) * 16 * kPitch * 2, b, lane);
+          }
+          const vec8 x = result_operand<T>(n & 1 ? dp : s, n >> 1);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            if (n & 1) dk[b] = mfma32(w[n & 1][b], x, dk[b]);
+            else dv[b] = mfma32(w[n & 1][b], x, dv[b]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        vec8 x = result_operand<T>(n & 1 ? dp : s, n >> 1);
-        if constexpr (kMasked) x = masked<T>(x, keep);
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const vec8 left_operand = kMasked ? masked<T>(w[n & 1][b], keep) : w[n & 1][b];
-          if (n & 1) dk[b] = mfma32(left_operand, x, dk[b]);
-          else dv[b] = mfma32(left_operand, x, dv[b]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      return not_finite;
     };
     request(0, 0);
     if (c.dim < kDim) {
@@ -350,19 +367,31 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
     for (; i + 2 <= heads * whole; i += 2) {
       arrive_and_sync();
       request(i + 1, 1);
-      step(lds + S::kV, 0, 32, std::false_type());
+      step(lds + S::kV, 0, 32, Mode<kWhole>());
       arrive_and_sync();
       if (i + 2 < items) request(i + 2, 0);
-      step(lds + S::kV + S::kStage, 0, 32, std::false_type());
+      step(lds + S::kV + S::kStage, 0, 32, Mode<kWhole>());
     }
     int stage = 0;
+    auto edges = [&](auto mode) __attribute__((always_inline)) {
+      bool not_finite = false;
 #pragma unroll 1
-    for (; i < items; ++i, stage ^= 1) {
-      arrive_and_sync();
-      if (i + 1 < items) request(i + 1, stage ^ 1);
-      int head;
-      const int first = first_of(i, head) + 32 * half;
-      step(lds + S::kV + stage * S::kStage, mine - first, run.nq - first, std::true_type());
+      for (; i < items; ++i, stage ^= 1) {
+        arrive_and_sync();
+        if (i + 1 < items) request(i + 1, stage ^ 1);
+        int head;
+        const int first = first_of(i, head) + 32 * half;
+        not_finite |= step(lds + S::kV + stage * S::kStage, mine - first, run.nq - first, mode);
+      }
+      return not_finite;
+    };
+    const bool not_finite = edges(Mode<kEdge>());
+    if (edge > 0 && any_wave<S::kWaves>(not_finite, lds + S::kV)) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) dk[b] = dv[b] = zero16();
+      i = stage = 0;
+      request(0, 0);
+      edges(Mode<kRowByRow>());
     }
   }
   if constexpr (S::kHalves == 2) {

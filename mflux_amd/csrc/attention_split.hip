@@ -8,6 +8,7 @@
 #include "attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mfq {
 namespace {
@@ -73,28 +74,40 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
       load_v.load(v + (int64_t)first * c.v.token, ring_at + S::kTile, run.nk - first, lane);
     };
     const int first_tile = begin + wave * kStep;
-    if (first_tile < end) {
-      request_k(first_tile);
-      request_v(first_tile);
-    }
-    for (int first = first_tile; first < end; first += kWaves * kStep) {
-      const int next = first + kWaves * kStep;
-      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
-      auto between = [&]() __attribute__((always_inline)) {
-        if (next < end) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
-          request_k(next);
-          asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-      };
-      if (first + kStep <= least) state.template step<1, false>(k_tile, v_tile, kStep, scale, lane, between);
-      else state.template step<1, true>(k_tile, v_tile, limit - first, scale, lane, between);
-      if (next < end) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V
-        request_v(next);
+    auto walk = [&](auto one_by_one) __attribute__((always_inline)) {
+      constexpr bool kOneByOne = decltype(one_by_one)::value;
+      bool not_finite = false;
+      if (first_tile < end) {
+        request_k(first_tile);
+        request_v(first_tile);
       }
+#pragma unroll 1
+      for (int first = first_tile; first < end; first += kWaves * kStep) {
+        const int next = first + kWaves * kStep;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+        auto between = [&]() __attribute__((always_inline)) {
+          if (next < end) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+            request_k(next);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+          } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          }
+        };
+        if constexpr (kOneByOne) state.template step<1, true, true>(k_tile, v_tile, limit - first, scale, lane, between);
+        else if (first + kStep <= least) state.template step<1, false>(k_tile, v_tile, kStep, scale, lane, between);
+        else not_finite |= state.template step<1, true>(k_tile, v_tile, limit - first, scale, lane, between);
+        if (next < end) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V
+          request_v(next);
+        }
+      }
+      return not_finite;
+    };
+    if (walk(std::false_type())) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      state.init();
+      walk(std::true_type());
     }
   }
 
