@@ -526,7 +526,7 @@ int mfq_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, 
  * The first `rotated` channels (even) turn, pairs (i, i + rotated / 2) for MFQ_ROTARY_HALF, (2i, 2i + 1) for
  * MFQ_ROTARY_INTERLEAVED; the others pass.  cos, sin [table_rows, rotated / 2] float32; a token's row is
  * positions[b * position_batch + token], or its place in its entry without positions, clamped to the table.
- * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16; dim even, at most 512.  Any alignment of elements; 16-byte aligned
+ * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16; dim even, at most 512; fewer than 2^31 rows (token, head).  Any alignment of elements; 16-byte aligned
  * pointers and strides of whole 16 bytes load wider.  No array may overlap another that is written.
  * workspace: mfq_rotary_workspace_bytes() of it, 16-byte aligned, for the backward pass of a weight.
  */

@@ -468,6 +468,7 @@ static int check_rotary(const mfq_rotary_args* a, bool backward, bool* wide) {
   if (a->batch <= 0 || a->tokens <= 0 || a->batch > INT32_MAX || a->tokens > INT32_MAX || a->batch * a->tokens > ((int64_t)1 << 40)) return MFQ_ESHAPE;
   if (a->table_rows <= 0 || a->table_rows > INT32_MAX || a->position_batch < 0) return MFQ_ESHAPE;
   if (a->q.heads <= 0 || a->k.heads < 0 || a->q.heads > 65536 || a->k.heads > 65536) return MFQ_ESHAPE;
+  if (a->batch * a->tokens * a->q.heads >= INT32_MAX || a->batch * a->tokens * a->k.heads >= INT32_MAX) return MFQ_ESHAPE;
   if (!(a->eps >= 0.f)) return MFQ_ESHAPE;
   if (a->rotated && (!a->cos || !a->sin)) return MFQ_ENULL;
   const int64_t per16 = a->dtype == MFQ_F32 ? 4 : 8;

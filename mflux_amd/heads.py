@@ -180,6 +180,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torc
                          f"{tuple(k.shape)} {k.dtype}")
     if not 0 < q.shape[-2] <= 65536 or (k is not None and not 0 < k.shape[-2] <= 65536):
         raise ValueError(f"[{fn}] q and k need between 1 and 65536 heads")
+    if any(t is not None and t.numel() // D >= 2 ** 31 - 1 for t in (q, k)):
+        raise ValueError(f"[{fn}] fewer than 2^31 rows (token, head) fit a call")
     if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError(f"[{fn}] cos and sin must be float32 [P, R / 2] of one shape, got {tuple(cos.shape)} {cos.dtype} and "
                          f"{tuple(sin.shape)} {sin.dtype}")
