@@ -10,6 +10,8 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <limits>
@@ -645,6 +647,113 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& dy, const Te
   return {dq, dk, dv};
 }
 
+// ---- the two with their gradients: what mflux_amd.heads calls
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients of a backward pass that is itself recorded: a second derivative asks for what is not there, with an error
+variable_list once(const char* fn, variable_list gradients) {
+  if (!at::GradMode::is_enabled()) return gradients;
+  variable_list some;
+  for (const auto& g : gradients)
+    if (g.defined()) some.push_back(g);
+  variable_list marked = (*std::make_shared<torch::autograd::DelayedError>(std::string(fn) + ": trying to differentiate twice a function that has "
+                                                                           "no second derivative", (int)some.size()))(std::move(some));
+  size_t n = 0;
+  for (auto& g : gradients)
+    if (g.defined()) g = marked[n++];
+  return gradients;
+}
+
+c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+Tensor or_none(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+bool wanted(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                               const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
+                               const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [yq, yk] = rotary(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
+    ctx->save_for_backward({q, or_none(k), cos, sin, or_none(positions), or_none(q_weight), or_none(k_weight)});
+    ctx->saved_data["layout"] = layout;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["wanted"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(q_weight) << 2 | wanted(k_weight) << 3);
+    if (!k.has_value()) return {yq};
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1];
+    const int64_t want = ctx->saved_data["wanted"].toInt();
+    variable_list out(9);
+    std::tuple<Tensor, Tensor, Tensor, Tensor> g;
+    {
+      at::AutoGradMode off(false);
+      at::AutoDispatchBelowADInplaceOrView guard;
+      g = rotary_backward(dy[0], k.defined() ? c10::optional<Tensor>(dy[1]) : c10::nullopt, q, if_defined(k), saved[2], saved[3], if_defined(saved[4]),
+                          if_defined(saved[5]), if_defined(saved[6]), ctx->saved_data["layout"].toInt(), ctx->saved_data["eps"].toDouble(),
+                          want & 3, want & 4, want & 8);
+    }
+    if (want & 1) out[0] = std::get<0>(g);
+    if (want & 2) out[1] = std::get<1>(g);
+    if (want & 4) out[5] = std::get<2>(g);
+    if (want & 8) out[6] = std::get<3>(g);
+    return once("mfq::rotary", std::move(out));
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_call(const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
+                                       const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
+                                       const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
+  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(q_weight) || wanted(k_weight))) {
+    auto out = RotaryFunction::apply(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
+    return {out[0], out.size() > 1 ? out[1] : at::empty({0}, q.options())};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rotary(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
+}
+
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                        const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
+                        bool causal, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, rest, lse] = attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, true);
+    ctx->save_for_backward({q, k, v, y, rest, lse, or_none(q_offsets), or_none(k_offsets), or_none(q_lengths), or_none(k_lengths)});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["wanted"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(v) << 2);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t want = ctx->saved_data["wanted"].toInt();
+    variable_list out(9);
+    std::tuple<Tensor, Tensor, Tensor> g;
+    {
+      at::AutoGradMode off(false);
+      at::AutoDispatchBelowADInplaceOrView guard;
+      g = attention_backward(dy[0], saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], if_defined(saved[6]), if_defined(saved[7]),
+                             if_defined(saved[8]), if_defined(saved[9]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+                             want & 1, want & 6);
+    }
+    if (want & 1) out[0] = std::get<0>(g);
+    if (want & 2) out[1] = std::get<1>(g);
+    if (want & 4) out[2] = std::get<2>(g);
+    return once("mfq::attention", std::move(out));
+  }
+};
+
+Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                      const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
+                      bool causal, double scale) {
+  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v)))
+    return AttentionFunction::apply(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return std::get<0>(attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, false));
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mfq, m) {
@@ -666,6 +775,8 @@ TORCH_LIBRARY(mfq, m) {
   m.def("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("rotary_backward(Tensor dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps, bool want_x, bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool training) -> (Tensor, Tensor, Tensor)");
+  m.def("rotary_call(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
+  m.def("attention_call(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale) -> Tensor");
   m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor rest, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
 }
 
@@ -689,4 +800,11 @@ TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA d
   m.impl("rotary_backward", rotary_backward);
   m.impl("attention", attention);
   m.impl("attention_backward", attention_backward);
+  m.impl("rotary_call", rotary_call);
+  m.impl("attention_call", attention_call);
+}
+
+TORCH_LIBRARY_IMPL(mfq, AutogradCUDA, m) {  // the ops with gradients; the others are called from these and from Python functions
+  m.impl("rotary_call", rotary_call);
+  m.impl("attention_call", attention_call);
 }

@@ -124,28 +124,6 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
 
 # ---- RMS norm of the heads and rotary positions -------------------------------------
 
-class _RotaryFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, q_weight, k_weight, layout, eps):
-        yq, yk = _lib.ops().rotary(q, k, cos, sin, positions, q_weight, k_weight, layout, eps)
-        # without a weight the gradient is the gradient turned back: nothing of the input is needed but its shape
-        ctx.save_for_backward(q, k, cos, sin, positions, q_weight, k_weight)
-        ctx.layout, ctx.eps = layout, eps
-        return yq if k is None else (yq, yk)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dyq, dyk=None):
-        q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if not any(need):
-            return (None,) * 9
-        dq, dk, dwq, dwk = _lib.ops().rotary_backward(dyq, dyk, q, k, cos, sin, positions, q_weight, k_weight, ctx.layout, ctx.eps,
-                                                      need[0] or need[1], need[5], need[6])
-        return (dq if need[0] else None, dk if need[1] else None, None, None, None, dwq if need[5] else None, dwk if need[6] else None,
-                None, None)
-
-
 def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, *, layout: str = "interleaved",
            positions: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
            eps: float = 1e-6):
@@ -213,36 +191,13 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torc
     packed = q.ndim == 3
     if packed:
         q, k = q[None], None if k is None else k[None]
-    arguments = (q, k, cos, sin, positions, q_weight, k_weight, _lib.ROTARY_LAYOUTS[layout], float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        out = _RotaryFunction.apply(*arguments)
-        yq, yk = (out, None) if k is None else out
-    else:
-        yq, yk = _lib.ops().rotary(*arguments)
+    yq, yk = _lib.ops().rotary_call(q, k, cos, sin, positions, q_weight, k_weight, _lib.ROTARY_LAYOUTS[layout], eps)
     if packed:
         yq, yk = yq[0], None if k is None else yk[0]
     return yq if k is None else (yq, yk)
 
 
 # ---- attention ------------------------------------------------------------------------
-
-class _AttentionFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale):
-        y, rest, lse = _lib.ops().attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, True)
-        ctx.save_for_backward(q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths)
-        ctx.causal, ctx.scale = causal, scale
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dv = _lib.ops().attention_backward(dy, q, k, v, y, rest, lse, q_offsets, k_offsets, q_lengths, k_lengths, ctx.causal, ctx.scale,
-                                                   need[0], need[1] or need[2])
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None) + (None,) * 6
-
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, scale: float | None = None,
               q_lengths: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None,
@@ -314,7 +269,4 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     else:
         q_lengths, k_lengths = counts("q_lengths", q_lengths, q.shape[0]), counts("k_lengths", k_lengths, q.shape[0])
     _require_hip(fn, q, "q")
-    arguments = (q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, bool(causal), float(scale))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _AttentionFunction.apply(*arguments)
-    return _lib.ops().attention(*arguments, False)[0]
+    return _lib.ops().attention_call(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale)
