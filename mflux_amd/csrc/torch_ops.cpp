@@ -14,7 +14,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <limits>
+#include <memory>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -397,24 +401,47 @@ Tensor device_int32(const char* fn, const char* name, const Tensor& t, const Ten
   return t.contiguous();
 }
 
-std::tuple<Tensor, Tensor> rotary_tables(const Tensor& positions, const std::vector<double>& frequencies, const std::vector<int64_t>& axis,
-                                         double factor) {
-  TORCH_CHECK(positions.dim() == 2 && positions.scalar_type() == at::kInt && positions.is_contiguous(),
-              "mfq::rotary_tables: positions must be a contiguous int32 matrix");
-  TORCH_CHECK(frequencies.size() == axis.size() && !axis.empty() && axis.size() <= MFQ_ROTARY_MAX_PAIRS,
-              "mfq::rotary_tables: an axis for every frequency");
-  const c10::hip::HIPGuardMasqueradingAsCUDA guard(positions.device());
-  uint8_t of[MFQ_ROTARY_MAX_PAIRS];
-  for (size_t i = 0; i < axis.size(); ++i) {
-    TORCH_CHECK(axis[i] >= 0 && axis[i] < positions.size(1), "mfq::rotary_tables: no such axis");
-    of[i] = (uint8_t)axis[i];
+// The angles that a position adds, pair by pair, of `dim` channels; scaling: 0 none, 1 linear, 2 ntk, 3 yarn (mflux_amd.heads.rotary_tables)
+void rotary_frequencies(int64_t dim, double base, int64_t scaling, double factor, double length, double fast, double slow,
+                        std::vector<double>& out) {
+  const double d = (double)dim;
+  if (scaling == 2) base *= std::pow(factor, d / (d - 2));
+  auto pair_of = [&](double turns) { return d * std::log(length / (turns * 2 * M_PI)) / (2 * std::log(base)); };  // that turns so often over length
+  double low = 0, high = 0;
+  if (scaling == 3) {
+    low = std::max(std::floor(pair_of(fast)), 0.0);
+    high = std::min(std::ceil(pair_of(slow)), d - 1);
   }
-  const int64_t n = positions.size(0), pairs = (int64_t)axis.size();
-  Tensor cos = at::empty({n, pairs}, positions.options().dtype(at::kFloat)), sin = at::empty_like(cos);
+  for (int64_t i = 0; i < dim / 2; ++i) {
+    double f = std::pow(base, -2.0 * (double)i / d);
+    if (scaling == 1) f /= factor;
+    if (scaling == 3) {
+      const double stretched = std::min(std::max(((double)i - low) / std::max(high - low, 0.001), 0.0), 1.0);
+      f = f / factor * stretched + f * (1.0 - stretched);
+    }
+    out.push_back(f);
+  }
+}
+
+std::tuple<Tensor, Tensor> rotary_tables(const Tensor& positions, at::IntArrayRef dims, double base, int64_t scaling, double factor, double length,
+                                         double fast, double slow, double table_factor) {
+  TORCH_CHECK(positions.dim() == 2 && positions.scalar_type() == at::kInt && positions.size(1) == (int64_t)dims.size() && !dims.empty(),
+              "mfq::rotary_tables: positions must be an int32 matrix with a column for each dimension");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(positions.device());
+  std::vector<double> frequencies;
+  uint8_t axis[MFQ_ROTARY_MAX_PAIRS];
+  for (size_t a = 0; a < dims.size(); ++a) {
+    TORCH_CHECK(dims[a] > 0 && dims[a] % 2 == 0 && (int64_t)frequencies.size() + dims[a] / 2 <= MFQ_ROTARY_MAX_PAIRS,
+                "mfq::rotary_tables: dimensions must be even, of at most 512 channels in all");
+    for (int64_t i = 0; i < dims[a] / 2; ++i) axis[frequencies.size() + i] = (uint8_t)a;
+    rotary_frequencies(dims[a], base, scaling, factor, length, fast, slow, frequencies);
+  }
+  const Tensor p = positions.contiguous();
+  const int64_t n = p.size(0), pairs = (int64_t)frequencies.size();
+  Tensor cos = at::empty({n, pairs}, p.options().dtype(at::kFloat)), sin = at::empty_like(cos);
   if (n == 0) return {cos, sin};
-  check_status("mfq_rotary_tables",
-               mfq_rotary_tables(positions.data_ptr<int32_t>(), n, (int)positions.size(1), (int)pairs, frequencies.data(), of, (float)factor,
-                                 cos.data_ptr<float>(), sin.data_ptr<float>(), stream_of(positions)));
+  check_status("mfq_rotary_tables", mfq_rotary_tables(p.data_ptr<int32_t>(), n, (int)p.size(1), (int)pairs, frequencies.data(), axis,
+                                                      (float)table_factor, cos.data_ptr<float>(), sin.data_ptr<float>(), stream_of(p)));
   return {cos, sin};
 }
 
@@ -771,7 +798,7 @@ TORCH_LIBRARY(mfq, m) {
   m.def("low_rank_forward(Tensor x, Tensor af, int rank) -> (Tensor, Tensor)");
   m.def("low_rank_gradient(Tensor g, Tensor bf, Tensor tf, int rank, float scale, bool want_gt, bool want_db) -> (Tensor, Tensor, Tensor)");
   m.def("low_rank_up(Tensor x, Tensor tf, int rank) -> Tensor");
-  m.def("rotary_tables(Tensor positions, float[] frequencies, int[] axis, float factor) -> (Tensor, Tensor)");
+  m.def("rotary_tables(Tensor positions, int[] dims, float base, int scaling, float factor, float length, float fast, float slow, float table_factor) -> (Tensor, Tensor)");
   m.def("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("rotary_backward(Tensor dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps, bool want_x, bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool training) -> (Tensor, Tensor, Tensor)");

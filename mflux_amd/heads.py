@@ -36,49 +36,42 @@ def _is_integer(value) -> bool:
 
 # ---- tables -----------------------------------------------------------------
 
-def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:
-    """The ``dim / 2`` angles a position adds, and what the tables are multiplied
-    by (1 except for ``"yarn"``).  ``scaling`` stretches them for contexts longer than the
-    ``rotary_tables`` docstring says."""
-    if not _is_integer(dim) or dim <= 0 or dim % 2:
-        raise ValueError(f"[rotary_tables] a dimension must be a positive even number, got {dim!r}")
-    if not (base > 0 and math.isfinite(base)):
-        raise ValueError(f"[rotary_tables] base must be positive, got {base!r}")
-    plain = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+_SCALINGS = {"linear": (1, {"type", "factor"}), "ntk": (2, {"type", "factor"}),
+             "yarn": (3, {"type", "factor", "original_length", "beta_fast", "beta_slow", "attention_factor"})}
+
+
+def _number(value) -> bool:
+    return isinstance(value, (int, float)) and not isinstance(value, bool) and math.isfinite(value)
+
+
+def _scaling(scaling: dict | None, base: float, dims: tuple[int, ...]) -> tuple:
+    """``(kind, factor, original length, beta_fast, beta_slow, factor of the tables)`` as the op takes them."""
     if scaling is None:
-        return plain, 1.0
-    known = {"linear": {"type", "factor"}, "ntk": {"type", "factor"},
-             "yarn": {"type", "factor", "original_length", "beta_fast", "beta_slow", "attention_factor"}}
+        return 0, 1.0, 1.0, 32.0, 1.0, 1.0
     kind = scaling.get("type")
-    if kind not in known:
+    if kind not in _SCALINGS:
         raise ValueError(f"[rotary_tables] scaling type must be 'linear', 'ntk' or 'yarn', got {kind!r}")
-    if set(scaling) - known[kind]:
-        raise ValueError(f"[rotary_tables] unknown scaling entries for '{kind}': {sorted(set(scaling) - known[kind])}")
+    code, known = _SCALINGS[kind]
+    if set(scaling) - known:
+        raise ValueError(f"[rotary_tables] unknown scaling entries for '{kind}': {sorted(map(str, set(scaling) - known))}")
     factor = scaling.get("factor")
-    if not isinstance(factor, (int, float)) or not (factor >= 1 and math.isfinite(factor)):
+    if not _number(factor) or factor < 1:
         raise ValueError(f"[rotary_tables] scaling factor must be at least 1, got {factor!r}")
-    if kind == "linear":
-        return [f / factor for f in plain], 1.0
-    if kind == "ntk":
-        if dim == 2:
-            raise ValueError("[rotary_tables] 'ntk' needs a dimension above 2")
-        return [(base * factor ** (dim / (dim - 2))) ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
+    if kind == "ntk" and 2 in dims:
+        raise ValueError("[rotary_tables] 'ntk' needs dimensions above 2")
+    if kind != "yarn":
+        return code, factor, 1.0, 32.0, 1.0, 1.0
     length, fast, slow = scaling.get("original_length"), scaling.get("beta_fast", 32.0), scaling.get("beta_slow", 1.0)
-    if not isinstance(length, (int, float)) or length <= 0:
+    if not _number(length) or length <= 0:
         raise ValueError(f"[rotary_tables] 'yarn' needs a positive original_length, got {length!r}")
-    if not (fast >= slow > 0) or base <= 1:
+    if not (_number(fast) and _number(slow) and fast >= slow > 0) or base <= 1:
         raise ValueError("[rotary_tables] 'yarn' needs beta_fast >= beta_slow > 0 and a base above 1")
-
-    def pair_of(turns: float) -> float:
-        return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
-
-    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), dim - 1)
-    out = []
-    for i, f in enumerate(plain):
-        stretched = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
-        out.append(f / factor * stretched + f * (1.0 - stretched))
     tables = scaling.get("attention_factor")
-    return out, 0.1 * math.log(factor) + 1.0 if tables is None else float(tables)
+    if tables is None:
+        tables = 0.1 * math.log(factor) + 1.0
+    elif not _number(tables):
+        raise ValueError(f"[rotary_tables] attention_factor must be a number, got {tables!r}")
+    return code, factor, length, fast, slow, tables
 
 
 def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: float = 10000.0,
@@ -108,18 +101,16 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
         axes = tuple(dims) if isinstance(dims, (tuple, list)) else (dims,)
         if len(axes) != positions.shape[1]:
             raise ValueError(f"[{fn}] positions have {positions.shape[1]} axes, dims {len(axes)}")
-    if not all(_is_integer(d) for d in axes) or not axes:
-        raise ValueError(f"[{fn}] dims must be a number, or one for each axis, got {dims!r}")
-    frequencies, axis, factor = [], [], 1.0
-    for a, dim in enumerate(axes):
-        f, factor = rotary_frequencies(dim, base, scaling)
-        frequencies += f
-        axis += [a] * len(f)
-    if len(frequencies) > 256:
-        raise ValueError(f"[{fn}] at most 512 channels turn, got {2 * len(frequencies)}")
+    if not axes or not all(_is_integer(d) and d > 0 and d % 2 == 0 for d in axes):
+        raise ValueError(f"[{fn}] dims must be a positive even number, or one for each axis, got {dims!r}")
+    if sum(axes) > 512:
+        raise ValueError(f"[{fn}] at most 512 channels turn, got {sum(axes)}")
+    if not _number(base) or base <= 0:
+        raise ValueError(f"[{fn}] base must be positive, got {base!r}")
+    arguments = _scaling(scaling, base, axes)
     positions = _integers(fn, "positions", positions, positions.device)
     _require_hip(fn, positions, "positions")
-    return _lib.ops().rotary_tables(positions.reshape(positions.shape[0], len(axes)).contiguous(), frequencies, axis, factor)
+    return _lib.ops().rotary_tables(positions.reshape(positions.shape[0], len(axes)), axes, base, *arguments)
 
 
 # ---- RMS norm of the heads and rotary positions -------------------------------------

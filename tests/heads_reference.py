@@ -19,6 +19,28 @@ TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0, torc
 E = 2.0 ** -24
 
 
+def rotary_frequencies(dim, base, scaling):
+    """The angle a position adds to each pair, and the factor of the tables.  yarn: a pair that makes more than beta_fast turns over
+    the original length keeps its angle, one that makes less than beta_slow has it divided, with whole pairs as the ends of the ramp."""
+    kind, factor = (None, 1.0) if scaling is None else (scaling["type"], scaling["factor"])
+    if kind == "ntk":
+        base = base * factor ** (dim / (dim - 2))
+    f = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if kind == "linear":
+        f = [x / factor for x in f]
+    if kind != "yarn":
+        return f, 1.0
+    length = scaling["original_length"]
+
+    def pair(turns):  # turns = length * base^(-2 i / dim) / (2 pi), for i
+        return dim / 2 * math.log(length / (2 * math.pi * turns)) / math.log(base)
+
+    low, high = max(math.floor(pair(scaling.get("beta_fast", 32.0))), 0), min(math.ceil(pair(scaling.get("beta_slow", 1.0))), dim - 1)
+    share = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(dim // 2)]
+    tables = scaling.get("attention_factor")
+    return [x * (1 - t) + x / factor * t for x, t in zip(f, share)], 1 + 0.1 * math.log(factor) if tables is None else tables
+
+
 def visible(nq, nk, causal, device):
     if not causal:
         return torch.ones(nq, nk, dtype=torch.bool, device=device)

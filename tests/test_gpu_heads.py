@@ -37,13 +37,12 @@ def ints(values):
 ])
 def test_tables(positions, dims, base, scaling):
     import mflux_amd
-    from mflux_amd import heads
 
     p = ints(positions)
     cos, sin = mflux_amd.rotary_tables(p, dims, base, scaling)
     columns, factor = [], 1.0
     for a, d in enumerate((dims,) if isinstance(dims, int) else dims):
-        f, factor = heads.rotary_frequencies(d, base, scaling)
+        f, factor = ref.rotary_frequencies(d, base, scaling)
         columns.append((p if p.ndim == 1 else p[:, a])[:, None].double() * torch.tensor(f, dtype=torch.float64, device="cuda"))
     angle = torch.cat(columns, 1)
     for got, want in ((cos, angle.cos() * factor), (sin, angle.sin() * factor)):
