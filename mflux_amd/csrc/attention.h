@@ -275,6 +275,45 @@ __device__ inline typename T::vec8 tile_columns(const char* tile, int block, int
   return __builtin_bit_cast(typename T::vec8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The same by addresses in LDS that a lane computes once: operand e of tile_rows lies at rows[e], the two halves of block b of
+// tile_columns at columns[0][b] and [1][b], from the tile's first row on, so that a tile, a block of rows and a half of it are constants
+// in the instruction.  (Left to itself the compiler makes them again for every read, 90 vector instructions a step of 64 keys.)
+typedef __attribute__((address_space(3))) const char* LdsAddress;
+template <int kPitch, int kSteps, int kBlocks>
+struct OperandAddresses {
+  uint32_t rows[kSteps], columns[2][kBlocks];
+
+  __device__ inline void init(const char* lds, int lane) {
+    const uint32_t base = (uint32_t)(uintptr_t)lds;
+    const int row = lane & 31, i = lane & 15, first = 4 * (lane >> 5) + (i >> 2), piece = 2 * (lane >> 4 & 1) + (i >> 1 & 1);
+    const uint32_t r = row * (kPitch * 2) + 16 * ((lane >> 5) ^ swizzle<kPitch>(row));
+    const uint32_t c = first * (kPitch * 2) + 16 * (piece ^ swizzle<kPitch>(first)) + 8 * (i & 1);
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) {
+      rows[e] = base + (r ^ (32 * e));
+      asm volatile("" : "+v"(rows[e]));
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      columns[0][b] = base + (c ^ (64 * b));
+      columns[1][b] = base + (c ^ (64 * b) ^ 16) + 8 * kPitch * 2;  // eight rows on: the swizzle's low bit turns
+      asm volatile("" : "+v"(columns[0][b]), "+v"(columns[1][b]));
+    }
+  }
+  template <typename T>
+  __device__ inline typename T::vec8 row_operand(int e, int offset) const {
+    typedef __attribute__((address_space(3))) const typename T::vec8 operand;
+    return *(operand*)(LdsAddress)(uintptr_t)(rows[e] + offset);
+  }
+  template <typename T>
+  __device__ inline typename T::vec8 column_operand(int b, int offset) const {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(columns[0][b] + offset));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(columns[1][b] + offset));
+    return __builtin_bit_cast(typename T::vec8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
 __device__ inline f32x16 zero16() {
   f32x16 z;
 #pragma unroll
@@ -490,11 +529,12 @@ struct QueryState {
   }
   // ---- the same over 32 keys in two halves that overlap: while the matrix pipeline makes the next block's scores, the vector pipeline
   // takes this one's exponentials, and while it multiplies with V, the maximum over the next block's.
-  // scores of a block alone (the first one)
-  __device__ __attribute__((always_inline)) inline void scores(f32x16& s, const char* k32, int lane) {
+  using Addresses = OperandAddresses<kPitch, kSteps, kBlocks>;
+  // scores of a block alone (the first one), k32: its place in LDS
+  __device__ __attribute__((always_inline)) inline void scores(f32x16& s, const Addresses& at, int k32) {
     s = zero16();
 #pragma unroll
-    for (int e = 0; e < kSteps; ++e) s = mfma32(tile_rows<T, kPitch>(k32, e, lane), q[e], s);
+    for (int e = 0; e < kSteps; ++e) s = mfma32(at.template row_operand<T>(e, k32), q[e], s);
   }
   // the reference follows the block's maximum (see step)
   __device__ __attribute__((always_inline)) inline void follow(float most, float c) {
@@ -518,24 +558,24 @@ struct QueryState {
   }
   // s: the block's scores; kNext: next = the scores of the block at k32
   template <bool kNext>
-  __device__ __attribute__((always_inline)) inline void overlapped(f32x16& s, f32x16& next, const char* k32, const char* v32, float c, int lane) {
+  __device__ __attribute__((always_inline)) inline void overlapped(f32x16& s, f32x16& next, const Addresses& at, int k32, int v32, float c) {
     const float shift = top == -__builtin_inff() ? 0.f : top * c;
     vec8 p[2], w[2][kBlocks], a[3];
     if constexpr (kNext) {
       next = zero16();
-      a[0] = tile_rows<T, kPitch>(k32, 0, lane);
-      a[1] = tile_rows<T, kPitch>(k32, 1, lane);
+      a[0] = at.template row_operand<T>(0, k32);
+      a[1] = at.template row_operand<T>(1, k32);
     }
 #pragma unroll
     for (int e = 0; e < kSteps; ++e) {
       if constexpr (kNext) {
-        if (e + 2 < kSteps) a[(e + 2) % 3] = tile_rows<T, kPitch>(k32, e + 2, lane);
+        if (e + 2 < kSteps) a[(e + 2) % 3] = at.template row_operand<T>(e + 2, k32);
         next = mfma32(a[e % 3], q[e], next);
       }
       // V's first operands, when the reads of K end
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b)
-        if (b * 2 / kBlocks + kSteps - 2 == e) w[0][b] = tile_columns<T, kPitch>(v32, b, lane);
+        if (b * 2 / kBlocks + kSteps - 2 == e) w[0][b] = at.template column_operand<T>(b, v32);
 #pragma unroll
       for (int i = 16 * e / kSteps; i < 16 * (e + 1) / kSteps; ++i) {
         s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -shift));
@@ -551,7 +591,7 @@ struct QueryState {
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        if (n == 0) w[1][b] = tile_columns<T, kPitch>(v32 + 16 * kPitch * 2, b, lane);
+        if (n == 0) w[1][b] = at.template column_operand<T>(b, v32 + 16 * kPitch * 2);
         o[b] = mfma32(w[n][b], p[n], o[b]);
         if constexpr (kNext) {
           const int g = n * kBlocks + b;

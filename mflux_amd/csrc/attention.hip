@@ -76,25 +76,27 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
           arrive_and_sync();
         }
       };
-      const char *k0 = lds, *v0 = lds + kTileBytes, *k1 = lds + 2 * kTileBytes, *v1 = lds + 3 * kTileBytes;
+      constexpr int k0 = 0, v0 = kTileBytes, k1 = 2 * kTileBytes, v1 = 3 * kTileBytes;
+      typename QueryState<T, kDim, kPitch>::Addresses places;
+      places.init(lds, lane);
       auto three_blocks = [&](int at) __attribute__((always_inline)) {
         arrive_v(at);
-        state.template overlapped<true>(s0, s1, k0 + kHalf, v0, scale, lane);
+        state.template overlapped<true>(s0, s1, places, k0 + kHalf, v0, scale);
         arrive_k(at + kKeys);
-        state.template overlapped<true>(s1, s0, k1, v0 + kHalf, scale, lane);
+        state.template overlapped<true>(s1, s0, places, k1, v0 + kHalf, scale);
         arrive_v(at + kKeys);
-        state.template overlapped<true>(s0, s1, k1 + kHalf, v1, scale, lane);
+        state.template overlapped<true>(s0, s1, places, k1 + kHalf, v1, scale);
       };
       arrive_k(0);
-      state.scores(s0, k0, lane);
+      state.scores(s0, places, k0);
       state.follow(state.maximum(s0), scale);
       three_blocks(0);
       for (first = 2 * kKeys; first < whole; first += 2 * kKeys) {
         arrive_k(first);
-        state.template overlapped<true>(s1, s0, k0, v1 + kHalf, scale, lane);
+        state.template overlapped<true>(s1, s0, places, k0, v1 + kHalf, scale);
         three_blocks(first);
       }
-      state.template overlapped<false>(s1, s0, nullptr, v1 + kHalf, scale, lane);
+      state.template overlapped<false>(s1, s0, places, 0, v1 + kHalf, scale);
     }
     // the tile of `buffer` has arrived and the next one is requested
     auto advance = [&](int at) __attribute__((always_inline)) {

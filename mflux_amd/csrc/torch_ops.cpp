@@ -615,26 +615,42 @@ struct AttentionOperands {
   int64_t rows() const { return (a.q_offsets ? 1 : a.batch) * a.q_tokens; }
 };
 
-// (y, and for a backward pass what y's rounding left and the rows' log-sum-exps: empty otherwise)
-std::tuple<Tensor, Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
-                                     const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
-                                     const c10::optional<Tensor>& k_lengths, bool causal, double scale, bool training) {
+// y, and for a backward pass (rest and lse not nullptr) what y's rounding left and the rows' log-sum-exps
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                         const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
+                         bool causal, double scale, Tensor* rest, Tensor* lse) {
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   AttentionOperands o("mfq::attention", q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
   Tensor y = at::empty(q.sizes(), q.options());
-  Tensor rest = training ? at::empty(q.sizes(), q.options()) : at::empty({0}, q.options());
-  Tensor lse = training ? at::empty({o.a.heads, o.rows()}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
-  if (q.numel() == 0) return {y, rest, lse};
-  if (k.numel() == 0) return {y.zero_(), rest.zero_(), lse.fill_(std::numeric_limits<float>::infinity())};
+  if (rest) {
+    *rest = at::empty(q.sizes(), q.options());
+    *lse = at::empty({o.a.heads, o.rows()}, q.options().dtype(at::kFloat));
+  }
+  if (q.numel() == 0) return y;
+  if (k.numel() == 0) {
+    if (rest) {
+      rest->zero_();
+      lse->fill_(std::numeric_limits<float>::infinity());
+    }
+    return y.zero_();
+  }
   o.a.out = y.data_ptr();
-  if (training) {
-    o.a.rest = rest.data_ptr();
-    o.a.lse = lse.data_ptr<float>();
+  if (rest) {
+    o.a.rest = rest->data_ptr();
+    o.a.lse = lse->data_ptr<float>();
   }
   const size_t bytes = mfq_attention_workspace_bytes(&o.a);
   Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
   check_status("mfq_attention", mfq_attention(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  return y;
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
+                                             const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths,
+                                             const c10::optional<Tensor>& k_lengths, bool causal, double scale) {
+  Tensor rest, lse;
+  Tensor y = attention_forward(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, &rest, &lse);
   return {y, rest, lse};
 }
 
@@ -746,7 +762,7 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
                         const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
                         bool causal, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [y, rest, lse] = attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, true);
+    auto [y, rest, lse] = attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
     ctx->save_for_backward({q, k, v, y, rest, lse, or_none(q_offsets), or_none(k_offsets), or_none(q_lengths), or_none(k_lengths)});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
@@ -778,7 +794,7 @@ Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const c
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v)))
     return AttentionFunction::apply(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
   at::AutoDispatchBelowADInplaceOrView guard;
-  return std::get<0>(attention(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, false));
+  return attention_forward(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, nullptr, nullptr);
 }
 
 }  // namespace
@@ -801,7 +817,7 @@ TORCH_LIBRARY(mfq, m) {
   m.def("rotary_tables(Tensor positions, int[] dims, float base, int scaling, float factor, float length, float fast, float slow, float table_factor) -> (Tensor, Tensor)");
   m.def("rotary(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("rotary_backward(Tensor dyq, Tensor? dyk, Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps, bool want_x, bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool training) -> (Tensor, Tensor, Tensor)");
+  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale) -> (Tensor, Tensor, Tensor)");
   m.def("rotary_call(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("attention_call(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale) -> Tensor");
   m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor rest, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
