@@ -20,6 +20,52 @@ enum { kWhole, kEdge, kRowByRow };
 template <int kMode>
 using Mode = std::integral_constant<int, kMode>;
 
+// float16 has neither the range nor the small numbers for the scores' gradients of any loss (a few keys and a large dy: above 65504, many
+// keys and a small one: below 2^-24, with results that float16 holds), so they are rounded as multiples of a power of two that each
+// lane's column of sums has for itself: taken from the first gradients that are not zero, and again, with the sums, from larger ones.
+// bfloat16 has float32's range and needs none.
+template <typename T, int kBlocks>
+struct ColumnUnit {
+  float unit = 0.f;  // what values are multiplied with, 0: none yet
+
+  __device__ __attribute__((always_inline)) inline void apply(f32x16& ds, f32x16 (&sums)[kBlocks]) {
+    if constexpr (T::code == MFQ_F16) {
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, __builtin_fabsf(ds[i]));
+      most = max_halves(most);
+      const bool low = most * unit > 16384.f || (unit == 0.f && most > 0.f);
+      if (__any(low && most < 3e38f)) {
+        // 2^4 over the power of two that `most` lies above
+        const int exponent = min(max(131 + 127 - (int)(__float_as_uint(most) >> 23), 1), 254);
+        const float next = low && most < 3e38f ? __uint_as_float((uint32_t)exponent << 23) : unit;
+        const float factor = unit == 0.f ? 1.f : next / unit;
+        unit = next;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sums[b][i] *= factor;
+      }
+      const float by = unit == 0.f ? 1.f : unit;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] *= by;
+    }
+  }
+  __device__ __attribute__((always_inline)) inline void remove(f32x16 (&sums)[kBlocks]) {
+    if constexpr (T::code == MFQ_F16) {
+      const float by = unit == 0.f ? 1.f : 1.f / unit;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[b][i] *= by;
+      unit = 0.f;
+    }
+  }
+};
+// and probabilities of very many keys as multiples of 2^-8
+template <typename T>
+constexpr float kProbabilityShift = T::code == MFQ_F16 ? 8.f : 0.f;
+
 constexpr int kQueries = 128;  // of a workgroup of the first kernel
 constexpr int kKeys = 64;      // of its step
 
@@ -46,6 +92,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
   f32x16 dq[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) dq[b] = zero16();
+  ColumnUnit<T, kBlocks> unit;
   float delta = 0.f;
   if (keys > 0) {
     const int64_t inside = run.q0 + min(row, run.nq - 1);
@@ -105,6 +152,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
           s[i] = p * (dp[i] - delta);
           if constexpr (kMasked) s[i] = result_row(i, lane) < left ? s[i] : 0.f;
         }
+        unit.apply(s, dq);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const vec8 ds = result_operand<T>(s, n);
@@ -160,6 +208,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     if (any_wave<4>(not_finite, lds)) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) dq[b] = zero16();
+      unit = {};
       load_k.load(k, lds_at, keys, thread);
       load_v.load(v, lds_at + kTileBytes, keys, thread);
 #pragma unroll 1
@@ -173,6 +222,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
       }
     }
   }
+  unit.remove(dq);
   if (row >= run.rows) return;
   if (lane < 32) c.delta[head * rows + at] = delta;
   if (c.dq) store_row<T, kBlocks>(c.dq + (at * c.heads + head) * c.dim, nullptr, dq, limit > 0, c.scale, c.dim, lane);
@@ -236,6 +286,8 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
   f32x16 dk[kBlocks], dv[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) dk[b] = dv[b] = zero16();
+  ColumnUnit<T, kBlocks> unit;
+  constexpr float kShift = kProbabilityShift<T>;
   if (t3 > t0 && heads > 0) {
     const int64_t inside = run.k0 + min(row, run.nk - 1);
     vec8 k[S::kHoldK ? kSteps : 1];
@@ -317,12 +369,13 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
         const f32x4 l = *reinterpret_cast<const f32x4*>(lse + r), d = *reinterpret_cast<const f32x4*>(delta + r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + j], scale, -l[j])), ds = p * (dp[i + j] - d[j]);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + j], scale, kShift - l[j])), ds = p * (dp[i + j] - d[j]);
           const bool see = !kMasked || ((r + j >= start) & (r + j < left));
           s[i + j] = see ? p : 0.f;
           dp[i + j] = see ? ds : 0.f;
         }
       }
+      unit.apply(dp, dk);
       if constexpr (kOneByOne) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -389,11 +442,14 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
     if (edge > 0 && any_wave<S::kWaves>(not_finite, lds + S::kV)) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) dk[b] = dv[b] = zero16();
+      unit = {};
       i = stage = 0;
       request(0, 0);
       edges(Mode<kRowByRow>());
     }
   }
+  unit.remove(dk);
+  const float k_factor = c.scale * __builtin_amdgcn_exp2f(-kShift), v_factor = __builtin_amdgcn_exp2f(-kShift);
   if constexpr (S::kHalves == 2) {
     // the second half's sums to the first, one array after the other
     float* slot = reinterpret_cast<float*>(lds) + (keys_of * 32 + (lane & 31)) * S::kFloats;
@@ -426,8 +482,8 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
   const int64_t at = ((int64_t)run.batch * c.k_tokens + run.k0 + row) * c.kv_heads + kv_head;
   const bool seen = mine < run.nq;
   if (parts == 1) {
-    if (c.dk) store_row<T, kBlocks>(c.dk + at * c.dim, nullptr, dk, seen, c.scale, c.dim, lane);
-    if (c.dv) store_row<T, kBlocks>(c.dv + at * c.dim, nullptr, dv, seen, 1.f, c.dim, lane);
+    if (c.dk) store_row<T, kBlocks>(c.dk + at * c.dim, nullptr, dk, seen, k_factor, c.dim, lane);
+    if (c.dv) store_row<T, kBlocks>(c.dv + at * c.dim, nullptr, dv, seen, v_factor, c.dim, lane);
     return;
   }
   const int64_t plane = (int64_t)(c.q_offsets ? 1 : c.batch) * c.k_tokens * c.kv_heads * c.dim;
@@ -440,8 +496,8 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
       f32x4 x, y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = seen ? dk[b][i + j] * c.scale : 0.f;
-        y[j] = seen ? dv[b][i + j] : 0.f;
+        x[j] = seen ? dk[b][i + j] * k_factor : 0.f;
+        y[j] = seen ? dv[b][i + j] * v_factor : 0.f;
       }
       *reinterpret_cast<f32x4*>(part_k + part * plane + at * c.dim + d) = x;
       *reinterpret_cast<f32x4*>(part_v + part * plane + at * c.dim + d) = y;

@@ -6,8 +6,9 @@ attention   A probability p is rounded once (u p), its score is a float32 sum of
             sum |q k|, which is the same relative error of p after the exponential; the exponential and the factors add a few e more),
             and the sums over keys are float32 (at most one e an addition).  float16 also loses 2^-25 of a probability that is not
             normal there, times |v|.  Then y is rounded.
-gradients   p as above from the saved float32 log-sum-exp; dS = p (dP - delta) is rounded once, and delta = sum dy y is taken
-            from the rounded y: off by u sum |dy y|.  Then the sums and the rounding of the result.
+gradients   p as above from the saved float32 log-sum-exp; dS = p (dP - delta) is rounded once, and delta = sum dy y is as far off as
+            y is.  Then the sums and the rounding of the result.  float16 rounds multiples of its gradients: 2^8 p, so 2^-33 of a
+            probability is lost, and dS times a power of two that has a column's largest at 2^4 or above, so at most 2^-28 of that.
 """
 import math
 
@@ -87,8 +88,8 @@ def attention_sequence(q, k, v, causal, scale, dy=None):
         adelta = (dyh.abs() * (y.abs() + out["y"][1][:, h])).sum(1, keepdim=True)
         # dS before its rounding: p's relative error, dP's and delta's float32 sums, delta's rounded y
         eds = c * ds.abs() + torch.where(see, p * (E * (D + 4) * (adp + adelta) + (dyh.abs() * out["y"][1][:, h]).sum(1, keepdim=True)), 0.0)
-        eds = (eds + u * (ds.abs() + eds) + tiny * see) * 1.01
-        ep = torch.where(see, (u + c) * p * 1.01 + tiny, 0.0)
+        eds = (eds + u * (ds.abs() + eds) + (tiny > 0) * 2.0 ** -28 * ds.abs().amax() * see) * 1.01
+        ep = torch.where(see, (u + c) * p * 1.01 + tiny * 2.0 ** -8, 0.0)
         n = nq * g
         for name, value, error, first in (
                 ("dq", scale * (ds @ kh), scale * (eds @ kh.abs() + E * (nk + 4) * (ds.abs() @ kh.abs())), True),

@@ -277,6 +277,24 @@ def test_attention_growing_scores():
             ref.check("y", y[0], *want)
 
 
+@pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 6, 2.0 ** -9, 2.0 ** -15])
+@pytest.mark.parametrize("n", [3, 700])
+def test_attention_float16_gradients_of_any_size(size, n):
+    """Large and small gradients that float16 holds, through scores' gradients that it would not.  They are linear in dy: those of
+    dy are off by `size` times the bound of dy / size, whose gradients are of order one, and by what is lost in the results."""
+    import mflux_amd
+
+    q, k, v = (randn(i, 1, n, 2, 64, dtype=F16).requires_grad_() for i in range(3))
+    dy = (randn(5, 1, n, 2, 64) * size).to(F16)
+    got = torch.autograd.grad(mflux_amd.attention(q, k, v, causal=True), (q, k, v), dy)
+    want = ref.attention_sequence(q.detach()[0], k.detach()[0], v.detach()[0], True, 0.125, dy[0].double() / size)
+    for name, g in zip(("dq", "dk", "dv"), got):
+        value, bound = want[name][0] * size, want[name][1] * size
+        inside = value.abs() + bound < 65000
+        assert float(inside.float().mean()) > 0.5
+        ref.check(name, g[0][inside], value[inside], bound[inside] + 2.0 ** -25)
+
+
 @pytest.mark.parametrize("queries", [96, 2])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_masked_infinities(queries, bad):
