@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -699,7 +700,7 @@ variable_list once(const char* fn, variable_list gradients) {
   if (!at::GradMode::is_enabled()) return gradients;
   variable_list some;
   for (const auto& g : gradients)
-    if (g.defined()) some.push_back(g);
+    if (g.defined()) some.push_back(g.detach().set_requires_grad(true));
   variable_list marked = (*std::make_shared<torch::autograd::DelayedError>(std::string(fn) + ": trying to differentiate twice a function that has "
                                                                            "no second derivative", (int)some.size()))(std::move(some));
   size_t n = 0;
@@ -711,6 +712,23 @@ variable_list once(const char* fn, variable_list gradients) {
 c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 Tensor or_none(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 bool wanted(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+
+// A backward pass that is captured into a graph hands a leaf's gradient to the node that an earlier, still living graph of the leaf made for
+// it on the stream of its time.  Where that is the default stream the engine makes the capture wait for it, which HIP forbids, in a
+// thread that cannot hand the error on: the process ends.  Such a call is refused while there is nothing to lose.
+void check_capture(const char* fn, std::initializer_list<const c10::optional<Tensor>*> leaves, const Tensor& like) {
+  const auto stream = c10::hip::getCurrentHIPStream(like.get_device());
+  if (!stream.stream()) return;  // the default stream is never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const auto* t : leaves) {
+    if (!wanted(*t) || !(*t)->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(**t);
+    const auto of = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!of.has_value() || of->id() != 0, fn, ": a graph is being captured while an earlier result computed from the same leaf on the default "
+                "stream still lives; its gradient would make the capture wait for that stream.  Delete that result first.");
+  }
+}
 
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
@@ -750,6 +768,8 @@ std::tuple<Tensor, Tensor> rotary_call(const Tensor& q, const c10::optional<Tens
                                        const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
                                        const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(q_weight) || wanted(k_weight))) {
+    const c10::optional<Tensor> first(q);
+    check_capture("mfq::rotary", {&first, &k, &q_weight, &k_weight}, q);
     auto out = RotaryFunction::apply(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
     return {out[0], out.size() > 1 ? out[1] : at::empty({0}, q.options())};
   }
@@ -791,8 +811,11 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
 Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
                       const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
                       bool causal, double scale) {
-  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v)))
+  if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) {
+    const c10::optional<Tensor> a(q), b(k), c(v);
+    check_capture("mfq::attention", {&a, &b, &c}, q);
     return AttentionFunction::apply(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
+  }
   at::AutoDispatchBelowADInplaceOrView guard;
   return attention_forward(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, nullptr, nullptr);
 }

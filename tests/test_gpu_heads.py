@@ -558,3 +558,70 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outputs[0], step()))
         assert torch.equal(outputs[1], decode())
+
+
+def test_capture_next_to_a_living_graph_is_refused():
+    """An eager result of the same leaves on the default stream: its nodes would end the process when the captured backward pass
+    reaches them.  Refused before anything is captured; without it the same capture works."""
+    import mflux_amd
+
+    q = randn(1, 1, 20, 2, 64, dtype=BF16).requires_grad_()
+    cos, sin = randn(2, 20, 32).cos(), randn(2, 20, 32).sin()
+    for call in (lambda: mflux_amd.attention(q, q.detach(), q.detach()), lambda: mflux_amd.rotary(q, None, cos, sin)):
+        want = torch.autograd.grad(call(), q, torch.ones_like(q))[0]
+        held = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="graph is being captured"):
+            with torch.cuda.graph(graph):
+                call()
+        torch.cuda.synchronize()
+        del held, graph
+        graph = torch.cuda.CUDAGraph()
+        ones = torch.ones_like(q)
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call(), q, ones)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
+def test_no_second_derivative():
+    import mflux_amd
+
+    q, k, v = (randn(i, 1, 9, 2, 32, dtype=BF16).requires_grad_() for i in range(3))
+    g, = torch.autograd.grad(mflux_amd.attention(q, k, v).float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.float().sum().backward()
+    cos, sin = randn(2, 9, 16).cos(), randn(2, 9, 16).sin()
+    g, = torch.autograd.grad(mflux_amd.rotary(q, None, cos, sin).float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.float().sum().backward()
+
+
+def test_c_entry_points_agree_with_the_ops():
+    """The C ABI on the same buffers gives the ops' bits."""
+    import ctypes
+
+    import mflux_amd
+    from mflux_amd import _lib
+
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    q, k, v = randn(1, 2, 70, 4, 64, dtype=BF16), randn(2, 2, 70, 2, 64, dtype=BF16), randn(3, 2, 70, 2, 64, dtype=BF16)
+    a = _lib.AttentionArgs(dtype=_lib.BF16, causal=1, dim=64, scale=0.125, batch=2, heads=4, kv_heads=2, q_tokens=70, k_tokens=70)
+    y = torch.empty_like(q)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        setattr(a, name, _lib.AttentionTensor(t.data_ptr(), (ctypes.c_int64 * 3)(*t.stride()[:3])))
+    a.out = y.data_ptr()
+    assert lib.mfq_attention_workspace_bytes(ctypes.byref(a)) == 0
+    _lib.check("mfq_attention", lib.mfq_attention(ctypes.byref(a), None, 0, stream))
+    assert torch.equal(y, mflux_amd.attention(q, k, v, causal=True))
+    cos, sin = randn(4, 70, 32).cos(), randn(4, 70, 32).sin()
+    r = _lib.RotaryArgs(dtype=_lib.BF16, layout=1, dim=64, rotated=64, batch=2, tokens=70, table_rows=70, cos=cos.data_ptr(), sin=sin.data_ptr())
+    yq, yk = torch.empty_like(q), torch.empty_like(k)
+    for name, t, out in (("q", q, yq), ("k", k, yk)):
+        setattr(r, name, _lib.RotaryTensor(x=t.data_ptr(), out=out.data_ptr(), x_stride=(ctypes.c_int64 * 3)(*t.stride()[:3]), heads=t.shape[2]))
+    _lib.check("mfq_rotary", lib.mfq_rotary(ctypes.byref(r), stream))
+    want = mflux_amd.rotary(q, k, cos, sin, layout="half")
+    assert torch.equal(yq, want[0]) and torch.equal(yk, want[1])
