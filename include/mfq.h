@@ -586,6 +586,9 @@ typedef struct mfq_attention_args {
   const int32_t *q_offsets, *k_offsets, *q_lengths, *k_lengths;
 } mfq_attention_args;
 size_t mfq_attention_workspace_bytes(const mfq_attention_args* args);
+/* the form a call takes: 0 for tiles of 128 queries that walk all their keys, otherwise 32 (token, head of a
+ * group) rows to a workgroup and the keys in so many ranges; negative: an error code */
+int mfq_attention_ranges(const mfq_attention_args* args);
 int mfq_attention(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t mfq_attention_backward_workspace_bytes(const mfq_attention_args* args);
 int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);

@@ -88,6 +88,7 @@ SIGNATURES = {
     "mfq_rotary": (_INT, [ctypes.POINTER(RotaryArgs), _PTR]),
     "mfq_rotary_backward": (_INT, [ctypes.POINTER(RotaryArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+    "mfq_attention_ranges": (_INT, [ctypes.POINTER(AttentionArgs)]),
     "mfq_attention": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_attention_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
     "mfq_attention_backward": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),

@@ -563,6 +563,12 @@ size_t mfq_attention_workspace_bytes(const mfq_attention_args* args) {
   return mfq::attention_split_bytes(c, mfq::attention_splits(c));
 }
 
+int mfq_attention_ranges(const mfq_attention_args* args) {
+  mfq::AttentionCall c;
+  if (int rc = attention_call(args, false, &c)) return rc;
+  return mfq::attention_splits(c);
+}
+
 size_t mfq_attention_backward_workspace_bytes(const mfq_attention_args* args) {
   mfq::AttentionCall c;
   if (attention_call(args, true, &c) != MFQ_OK) return 0;

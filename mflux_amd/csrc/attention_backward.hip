@@ -66,11 +66,12 @@ struct ColumnUnit {
 template <typename T>
 constexpr float kProbabilityShift = T::code == MFQ_F16 ? 8.f : 0.f;
 
-constexpr int kQueries = 128;  // of a workgroup of the first kernel
-constexpr int kKeys = 64;      // of its step
+constexpr int kKeys = 64;  // of a step of the first kernel
 
-template <typename T, int kDim>
+// kHalves == 2: a workgroup has 64 queries, and two wavefronts the same 32, each one half of every tile's keys, joined in LDS at the end
+template <typename T, int kDim, int kHalves>
 __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(AttentionCall c, int tiles) {
+  constexpr int kQueries = 128 / kHalves;
   constexpr int kPitch = pitch_of(kDim), kSteps = kDim / 16, kBlocks = kDim / 32;
   constexpr int kTileBytes = kKeys * kPitch * 2;
   using vec8 = typename T::vec8;
@@ -82,7 +83,8 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
   const Run run = find_run<kQueries>(c, index, false, c.causal);
   if (!run.valid) return;
   const int kv_head = head / (c.heads / c.kv_heads);
-  const int row = run.tile * kQueries + wave * 32 + (lane & 31);
+  const int half = wave / (4 / kHalves);
+  const int row = run.tile * kQueries + wave % (4 / kHalves) * 32 + (lane & 31);
   const int limit = visible_keys(run, row, c.causal);
   const int keys = uniform(run.tile * kQueries < run.nq ? visible_keys(run, min(run.tile * kQueries + kQueries, run.nq) - 1, c.causal) : 0);
   const int least = wave_min(row < run.nq ? limit : INT32_MAX), most = wave_max(limit);
@@ -186,20 +188,26 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     const int whole = uniform(c.causal ? visible_keys(run, run.tile * kQueries, 1) : run.nk);
     int first = 0, buffer = 0;
     constexpr int kHalf = 32 * kPitch * 2;
+    auto whole_tile = [&](const char* k64) __attribute__((always_inline)) {
+      if constexpr (kHalves == 2) {
+        step(k64 + half * kHalf, k64 + kTileBytes + half * kHalf, 32, Mode<kWhole>());
+      } else {
+        step(k64, k64 + kTileBytes, 32, Mode<kWhole>());
+        step(k64 + kHalf, k64 + kTileBytes + kHalf, 32, Mode<kWhole>());
+      }
+    };
     for (; first + 2 * kKeys <= whole; first += 2 * kKeys) {
       advance(first, 0);
-      step(lds, lds + kTileBytes, 32, Mode<kWhole>());
-      step(lds + kHalf, lds + kTileBytes + kHalf, 32, Mode<kWhole>());
+      whole_tile(lds);
       advance(first + kKeys, 1);
-      step(lds + 2 * kTileBytes, lds + 3 * kTileBytes, 32, Mode<kWhole>());
-      step(lds + 2 * kTileBytes + kHalf, lds + 3 * kTileBytes + kHalf, 32, Mode<kWhole>());
+      whole_tile(lds + 2 * kTileBytes);
     }
     bool not_finite = false;
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
       advance(first, buffer);
 #pragma unroll 1
-      for (int at = first; at < min(first + kKeys, most); at += 32) {
+      for (int at = first + (kHalves == 2 ? 32 * half : 0); at < min(first + kKeys, most); at += 32 * kHalves) {
         const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
         if (at + 32 <= least) step(k32, k32 + kTileBytes, 32, Mode<kWhole>());
         else not_finite |= step(k32, k32 + kTileBytes, limit - at, Mode<kEdge>());
@@ -215,7 +223,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
       for (first = 0, buffer = 0; first < keys; first += kKeys, buffer ^= 1) {
         advance(first, buffer);
 #pragma unroll 1
-        for (int at = first; at < min(first + kKeys, most); at += 32) {
+        for (int at = first + (kHalves == 2 ? 32 * half : 0); at < min(first + kKeys, most); at += 32 * kHalves) {
           const char* k32 = lds + buffer * 2 * kTileBytes + (at - first) * kPitch * 2;
           step(k32, k32 + kTileBytes, limit - at, Mode<kRowByRow>());
         }
@@ -223,6 +231,28 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     }
   }
   unit.remove(dq);
+  if constexpr (kHalves == 2) {
+    constexpr int kFloats = kDim + 4;
+    float* slot = reinterpret_cast<float*>(lds) + (wave % 2 * 32 + (lane & 31)) * kFloats;
+    __syncthreads();  // (nothing is in flight, and what has been requested has been read)
+    if (half) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<f32x4*>(slot + 32 * b + result_row(i, lane)) = f32x4{dq[b][i], dq[b][i + 1], dq[b][i + 2], dq[b][i + 3]};
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 o = *reinterpret_cast<const f32x4*>(slot + 32 * b + result_row(i, lane));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dq[b][i + j] += o[j];
+      }
+  }
   if (row >= run.rows) return;
   if (lane < 32) c.delta[head * rows + at] = delta;
   if (c.dq) store_row<T, kBlocks>(c.dq + (at * c.heads + head) * c.dim, nullptr, dq, limit > 0, c.scale, c.dim, lane);
@@ -529,15 +559,24 @@ int64_t key_values(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : 
 template <typename T, int kDim>
 int launch(const AttentionCall& c, int parts, float* workspace, hipStream_t stream) {
   const int64_t more = c.q_offsets ? c.batch + 2 : 0;  // as in the forward pass
-  {
+  auto launch_dq = [&](auto kernel, int queries) {
     constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
     static PerDeviceInt configured;
-    if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dq_kernel<T, kDim>), kBytes)) return MFQ_ELAUNCH;
-    const int64_t tiles = more ? c.q_tokens / kQueries + more : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
-    if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
-    hipLaunchKernelGGL((attention_dq_kernel<T, kDim>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
-    if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
-  }
+    if (!raise_lds_limit(configured, reinterpret_cast<const void*>(kernel), kBytes)) return (int)MFQ_ELAUNCH;
+    const int64_t tiles = more ? c.q_tokens / queries + more : (int64_t)((c.q_tokens + queries - 1) / queries) * c.batch;
+    if (tiles * c.heads > INT32_MAX) return (int)MFQ_ESHAPE;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+    return (int)(hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH);
+  };
+  // 64 queries to a workgroup where 128 leave compute units idle, or (causal) the longest of them working alone: causal heads of 128,
+  // 2048 tokens x 8 heads (128 such workgroups) 49 against 60 us, 4096 x 16 (512) 131 and 156, 4608 x 24 (864) 242 and 220; not causal,
+  // 1500 x 24 (288) 90 and 71, 2048 x 24 (384) 93 and 89.
+  const int64_t groups = (more ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
+  const bool halves = 2 * groups <= (c.causal ? 4 : 1) * (int64_t)compute_units();
+  int rc;
+  if constexpr (kDim <= 128) rc = halves ? launch_dq(&attention_dq_kernel<T, kDim, 2>, 64) : launch_dq(&attention_dq_kernel<T, kDim, 1>, 128);
+  else rc = launch_dq(&attention_dq_kernel<T, kDim, 1>, 128);
+  if (rc != MFQ_OK) return rc;
   if (!c.dk && !c.dv) return MFQ_OK;
   using S = KeyShape<kDim>;
   static PerDeviceInt configured;

@@ -259,17 +259,27 @@ int launch_dim(const AttentionCall& c, int splits, float* workspace, hipStream_t
 }  // namespace
 
 int attention_splits(const AttentionCall& c) {
-  const int64_t group = c.heads / c.kv_heads;
-  // mean queries of a sequence
-  const int64_t queries = c.q_offsets ? (c.q_tokens + c.batch - 1) / std::max(c.batch, 1) : c.q_tokens;
-  if (queries * group > kRows) return 0;
-  const int64_t keys = c.q_offsets ? (c.k_tokens + c.batch - 1) / std::max(c.batch, 1) : c.k_tokens;
+  const int64_t group = c.heads / c.kv_heads, units = compute_units();
+  // mean queries and keys of a sequence
+  const int64_t queries = c.q_offsets ? (c.q_tokens + c.batch - 1) / c.batch : c.q_tokens;
+  const int64_t keys = c.q_offsets ? (c.k_tokens + c.batch - 1) / c.batch : c.k_tokens;
   const int64_t items = std::max<int64_t>(tiles_of(c) - (c.q_offsets ? 2 : 0), 1) * c.kv_heads;
-  // Eight workgroups for every compute unit, so that sequences of different lengths fill it evenly (32 of them, 1024 to 8192 keys, 8
-  // key heads: 132, 134, 125, 125 us with one, four, eight, sixteen), each with 256 keys at least; and at most 64 ranges, which
-  // the join reads behind each other (one sequence of 100003 keys, 4 key heads: 47, 51, 60 us with 64, 128, 256).
-  const int64_t want = (8 * (int64_t)compute_units() + items - 1) / items;
-  return (int)std::min({std::max<int64_t>(keys / 256, 1), want, (int64_t)64});
+  if (queries * group <= kRows) {
+    // Single tokens: eight workgroups for every compute unit, so that sequences of different lengths fill it evenly (32 of them, 1024 to
+    // 8192 keys, 8 key heads: 132, 134, 125, 125 us with one, four, eight, sixteen), each with 256 keys at least; and at most 64
+    // ranges, which the join reads behind each other (one sequence of 100003 keys, 4 key heads: 47, 51, 60 us with 64, 128, 256).
+    const int64_t want = (8 * units + items - 1) / items;
+    return (int)std::min({std::max<int64_t>(keys / 256, 1), want, (int64_t)64});
+  }
+  // A prompt whose tiles of 128 queries leave compute units idle: 32 rows to a workgroup, the keys dealt to its wavefronts, is as much
+  // work on four times the units (heads of 128, causal: 1024 tokens x 8 heads 15.8 us here, 24.8 there; 2048 x 8, 128 such tiles, 29.9
+  // and 42.1; 1024 x 24, 192, 26.2 and 26.4; 2048 x 16, 256, 45.9 and 43.0).
+  const int64_t tiles = (c.q_offsets ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
+  if (4 * tiles > 3 * units) return 0;
+  // and the keys in ranges where even those are few (128 queries x 8 heads against 32768 keys: 350, 97, 57, 49, 82 us with 1, 4, 8, 16
+  // and 32; 128 against 4096: 43, 19, 15, 16, 25), but not where the join has as many rows again (1024 x 8: 15.8 us with 1, 25.7 with 2)
+  if (2 * items > units) return 1;
+  return (int)std::max<int64_t>(std::min({keys / 512, 2 * units / items, (int64_t)64}), 1);
 }
 
 size_t attention_split_bytes(const AttentionCall& c, int splits) {

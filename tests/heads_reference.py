@@ -5,7 +5,9 @@ Bounds, with u half a step of the 16-bit type and e = 2^-24 of float32:
 attention   A probability p is rounded once (u p), its score is a float32 sum of dim products (off by dim e
             sum |q k|, which is the same relative error of p after the exponential; the exponential and the factors add a few e more),
             and the sums over keys are float32 (at most one e an addition).  float16 also loses 2^-25 of a probability that is not
-            normal there, times |v|.  Then y is rounded.
+            normal there, times |v|.  The probabilities are divided by the sum of the rounded ones, so that they add up to 1: a sum
+            that is off by u at most, which is u |y| of the result and u of every probability that the backward pass makes from the
+            saved log-sum-exp.  Then y is rounded.
 gradients   p as above from the saved float32 log-sum-exp; dS = p (dP - delta) is rounded once, and delta = sum dy y is as far off as
             y is.  Then the sums and the rounding of the result.  float16 rounds multiples of its gradients: 2^8 p, so 2^-33 of a
             probability is lost, and dS times a power of two that has a column's largest at 2^4 or above, so at most 2^-28 of that.
@@ -76,7 +78,7 @@ def attention_sequence(q, k, v, causal, scale, dy=None):
         av = p @ vh.abs()
         lost = tiny * (see.double() @ vh.abs())
         out["y"][0][:, h] = y
-        bound = (u + c) * av * 1.01 + lost
+        bound = ((u + c) * av + u * y.abs()) * 1.01 + lost
         out["y"][1][:, h] = bound + u * (y.abs() + bound) + tiny
         if dy is None:
             continue
@@ -87,9 +89,9 @@ def attention_sequence(q, k, v, causal, scale, dy=None):
         adp = dyh.abs() @ vh.abs().t().contiguous()
         adelta = (dyh.abs() * (y.abs() + out["y"][1][:, h])).sum(1, keepdim=True)
         # dS before its rounding: p's relative error, dP's and delta's float32 sums, delta's rounded y
-        eds = c * ds.abs() + torch.where(see, p * (E * (D + 4) * (adp + adelta) + (dyh.abs() * out["y"][1][:, h]).sum(1, keepdim=True)), 0.0)
+        eds = (u + c) * ds.abs() + torch.where(see, p * (E * (D + 4) * (adp + adelta) + (dyh.abs() * out["y"][1][:, h]).sum(1, keepdim=True)), 0.0)
         eds = (eds + u * (ds.abs() + eds) + (tiny > 0) * 2.0 ** -28 * ds.abs().amax() * see) * 1.01
-        ep = torch.where(see, (u + c) * p * 1.01 + tiny * 2.0 ** -8, 0.0)
+        ep = torch.where(see, (2 * u + c) * p * 1.01 + tiny * 2.0 ** -8, 0.0)
         n = nq * g
         for name, value, error, first in (
                 ("dq", scale * (ds @ kh), scale * (eds @ kh.abs() + E * (nk + 4) * (ds.abs() @ kh.abs())), True),

@@ -159,8 +159,26 @@ def test_rotary_turns_back():
 
 # ---- attention --------------------------------------------------------------------------------------------------------
 
-def run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad, scale=None, spare=0, seed=0):
-    """All sequences at once against each of them in float64; rows of no sequence must come out as zeros."""
+def ranges(q, k, packed_sequences=0):
+    """The form that a call takes here (mfq_attention_ranges): 0 for tiles of 128 queries, otherwise the ranges of its keys."""
+    import ctypes
+
+    from mflux_amd import _lib
+
+    if torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("shapes are chosen for 256 compute units")
+    a = _lib.AttentionArgs(dtype=_lib.BF16, dim=q.shape[-1], scale=1.0, batch=packed_sequences or q.shape[0], heads=q.shape[-2],
+                           kv_heads=k.shape[-2], q_tokens=q.shape[-3], k_tokens=k.shape[-3], out=256)
+    for name in ("q", "k", "v"):
+        setattr(a, name, _lib.AttentionTensor(256, (ctypes.c_int64 * 3)(8, 8, 8)))
+    if packed_sequences:
+        a.q_offsets = a.k_offsets = 256
+    return _lib.load().mfq_attention_ranges(ctypes.byref(a))
+
+
+def run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad, scale=None, spare=0, seed=0, tiles=None):
+    """All sequences at once against each of them in float64; rows of no sequence must come out as zeros.  tiles: whether the call
+    has to take the form of whole tiles of queries, or the other."""
     import mflux_amd
 
     n = len(q_lengths)
@@ -180,6 +198,8 @@ def run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad, sc
     k = randn(seed + 2, *lead_k, Hkv, D, dtype=dtype)
     v = randn(seed + 3, *lead_k, Hkv, D, dtype=dtype)
     dy = randn(seed + 4, *lead_q, H, D, dtype=dtype) if grad else None
+    if tiles is not None:
+        assert (ranges(q, k, n if form == "packed" else 0) == 0) == tiles
     # what no sequence holds must not be read into a result
     if spare:
         for t, i in ((q, 0), (k, 1), (v, 1)) + (((dy, 0),) if grad else ()):
@@ -194,6 +214,13 @@ def run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad, sc
     if grad:
         got.update(zip(("dq", "dk", "dv"), torch.autograd.grad(y, (q, k, v), dy)))
     scale = D ** -0.5 if scale is None else scale
+    if Hkv > 40:  # some of very many heads, spread over the compute units
+        some = sorted({0, 1, 7, Hkv // 3, Hkv // 2, Hkv - 2, Hkv - 1})
+        of_q = [h * (H // Hkv) + i for h in some for i in range(H // Hkv)]
+        assert all(bool(t.isfinite().all()) for t in got.values())
+        got = {name: t[..., of_q if name in ("y", "dq") else some, :] for name, t in got.items()}
+        q, k, v = q.detach()[..., of_q, :], k.detach()[..., some, :], v.detach()[..., some, :]
+        dy = None if dy is None else dy[..., of_q, :]
     for name, t in got.items():
         full_v, full_b = torch.zeros(t.shape, dtype=torch.float64, device="cuda"), torch.zeros(t.shape, dtype=torch.float64, device="cuda")
         got[name] = (t, full_v, full_b)
@@ -218,7 +245,31 @@ def run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad, sc
 def test_attention(form, causal, dtype, D, H, Hkv, q_lengths, k_lengths):
     """Forward and backward; lengths of zero and one, tiles that end inside, queries that see nothing."""
     print(f"{form} causal={causal} {dtype} D={D} H={H}/{Hkv} {q_lengths} {k_lengths}", flush=True)
-    run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad=True)
+    run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad=True, tiles=False)
+
+
+# heads enough that whole tiles of queries fill the compute units, in the backward pass as well
+@pytest.mark.parametrize("form", ["batched", "packed"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,H,Hkv,q_lengths,k_lengths", [
+    (128, 530, 530, [1], [200]), (128, 530, 265, [128], [128]), (128, 270, 90, [129, 1, 63], [129, 1, 63]), (64, 260, 260, [77, 30, 5], [77, 30, 5]),
+    (128, 260, 65, [100, 257], [300, 257]), (80, 300, 150, [65, 200], [65, 200]), (72, 520, 520, [40], [100]), (8, 520, 260, [33], [33]),
+    (96, 264, 264, [130, 600], [70, 601]), (256, 300, 150, [150], [150]), (192, 300, 300, [150], [150]), (128, 260, 260, [200, 100], [60, 0]),
+    (64, 520, 260, [0, 40], [10, 40]), (128, 200, 100, [290], [700]),
+])
+def test_attention_whole_tiles(form, causal, dtype, D, H, Hkv, q_lengths, k_lengths):
+    """The same in the form of 128 queries to a workgroup: steps of the main loop, blocks at the edges, both parities of them."""
+    print(f"{form} causal={causal} {dtype} D={D} H={H}/{Hkv} {q_lengths} {k_lengths}", flush=True)
+    if max(q_lengths) * H // Hkv <= 32:
+        q_lengths, k_lengths = q_lengths + [140], k_lengths + [150]
+    run_attention(form, dtype, D, H, Hkv, q_lengths, k_lengths, causal, grad=True, tiles=True)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_whole_tiles_leave_out_what_no_sequence_holds(causal):
+    for form in ("batched", "packed"):
+        run_attention(form, BF16, 128, 260, 130, [70, 129], [70, 140], causal, grad=True, spare=37, tiles=True)
 
 
 @pytest.mark.parametrize("form", ["batched", "packed"])
@@ -250,13 +301,16 @@ def test_attention_many_short_sequences():
 
 
 def test_attention_long():
-    run_attention("batched", BF16, 128, 2, 1, [2500], [2500], True, grad=True)
-    run_attention("batched", F16, 64, 1, 1, [300], [4000], False, grad=True)
+    run_attention("batched", BF16, 128, 2, 1, [2500], [2500], True, grad=True, tiles=False)
+    run_attention("batched", F16, 64, 1, 1, [300], [4000], False, grad=True, tiles=False)
+    run_attention("batched", BF16, 128, 14, 2, [2500], [2500], True, grad=True, tiles=True)
+    run_attention("packed", F16, 64, 20, 10, [2100, 300], [2100, 1000], False, grad=True, tiles=True)
 
 
 def test_attention_large_scores():
     """Scores of hundreds: the running reference moves far, probabilities of almost all keys vanish."""
     run_attention("batched", BF16, 128, 2, 2, [200], [200], False, grad=True, scale=3.0)
+    run_attention("batched", BF16, 128, 260, 260, [200], [400], False, grad=True, scale=3.0, tiles=True)
     run_attention("batched", BF16, 128, 8, 2, [1], [2000], False, grad=False, scale=3.0)
 
 
@@ -271,8 +325,9 @@ def test_attention_growing_scores():
         q = torch.zeros(1, 5, 1, 64, device="cuda", dtype=BF16)
         q[..., 0] = 1.0
         v = randn(1, 1, nk, 1, 64, dtype=BF16)
-        for queries in (q, q.repeat(1, 40, 1, 1)):
+        for queries in (q, q.repeat(1, 40, 1, 1), q.repeat(1, 40, 130, 1)):
             y = mflux_amd.attention(queries, k, v, scale=1.0)
+            assert (ranges(queries, k) == 0) == (queries.shape[2] > 1)
             want = ref.attention_sequence(queries[0], k[0], v[0], False, 1.0)["y"]
             ref.check("y", y[0], *want)
 
@@ -295,14 +350,15 @@ def test_attention_float16_gradients_of_any_size(size, n):
         ref.check(name, g[0][inside], value[inside], bound[inside] + 2.0 ** -25)
 
 
-@pytest.mark.parametrize("queries", [96, 2])
+@pytest.mark.parametrize("queries,H", [(96, 2), (2, 2), (96, 260)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_attention_masked_infinities(queries, bad):
+def test_attention_masked_infinities(queries, H, bad):
     """A key that a query does not see never reaches it, whatever it and its value hold."""
     import mflux_amd
 
     nk = 200
-    q, k, v = randn(1, 1, queries, 2, 128, dtype=BF16), randn(2, 1, nk, 2, 128, dtype=BF16), randn(3, 1, nk, 2, 128, dtype=BF16)
+    q, k, v = randn(1, 1, queries, H, 128, dtype=BF16), randn(2, 1, nk, H, 128, dtype=BF16), randn(3, 1, nk, H, 128, dtype=BF16)
+    assert (ranges(q, k) == 0) == (H > 2)
     want = mflux_amd.attention(q, k, v, causal=True)
     at = nk - queries // 2
     k[0, at, 0] = bad
@@ -320,12 +376,13 @@ def test_attention_masked_infinities(queries, bad):
     assert torch.equal(got2[0, 1:].view(torch.int16), got[0, 1:].view(torch.int16))
 
 
-def test_attention_backward_masked_infinities():
+@pytest.mark.parametrize("H", [1, 530])
+def test_attention_backward_masked_infinities(H):
     """Rows behind a sequence's visible part do not reach gradients either: keys that no query sees but the last."""
     import mflux_amd
 
     n = 100
-    q, k, v, dy = (randn(i, 1, n, 1, 64, dtype=BF16) for i in range(4))
+    q, k, v, dy = (randn(i, 1, n, H, 64, dtype=BF16) for i in range(4))
     cut = 70
 
     def gradients(q, k, v, dy, upto):
@@ -504,7 +561,8 @@ def test_prompt_then_tokens():
 def test_other_stream():
     import mflux_amd
 
-    q, k, v = (randn(i, 1, 500, 4, 128, dtype=BF16) for i in range(3))
+    q, k, v = (randn(i, 1, 500, 64, 128, dtype=BF16) for i in range(3))
+    assert ranges(q, k) == 0
     want = mflux_amd.attention(q, k, v, causal=True)
     token = mflux_amd.attention(q[:, -1:], k, v)
     stream = torch.cuda.Stream()
