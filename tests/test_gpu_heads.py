@@ -256,7 +256,7 @@ def test_attention(form, causal, dtype, D, H, Hkv, q_lengths, k_lengths):
     (128, 530, 530, [1], [200]), (128, 530, 265, [128], [128]), (128, 270, 90, [129, 1, 63], [129, 1, 63]), (64, 260, 260, [77, 30, 5], [77, 30, 5]),
     (128, 260, 65, [100, 257], [300, 257]), (80, 300, 150, [65, 200], [65, 200]), (72, 520, 520, [40], [100]), (8, 520, 260, [33], [33]),
     (96, 264, 264, [130, 600], [70, 601]), (256, 300, 150, [150], [150]), (192, 300, 300, [150], [150]), (128, 260, 260, [200, 100], [60, 0]),
-    (64, 520, 260, [0, 40], [10, 40]), (128, 200, 100, [290], [700]),
+    (64, 520, 260, [0, 40], [10, 40]), (128, 200, 100, [290], [700]), (256, 300, 150, [150], [420]), (192, 300, 300, [140], [390]),
 ])
 def test_attention_whole_tiles(form, causal, dtype, D, H, Hkv, q_lengths, k_lengths):
     """The same in the form of 128 queries to a workgroup: steps of the main loop, blocks at the edges, both parities of them."""
@@ -291,6 +291,20 @@ def test_attention_few_queries(form, causal, dtype, D, H, Hkv, q_lengths, k_leng
 def test_attention_leaves_out_what_no_sequence_holds(form, causal, q_lengths, k_lengths):
     """NaN in every row around the sequences: none may reach a result, and the rows' own results are zeros."""
     run_attention(form, BF16, 128, 4, 2, q_lengths, k_lengths, causal, grad=True, spare=37)
+
+
+def test_attention_empty():
+    """No queries, no keys, no entries: nothing, or zeros, in the gradients too."""
+    import mflux_amd
+
+    for q_shape, k_shape, offsets in (((2, 0, 4, 64), (2, 5, 2, 64), None), ((2, 5, 4, 64), (2, 0, 2, 64), None), ((0, 5, 4, 64), (0, 5, 2, 64), None),
+                                      ((7, 4, 64), (0, 2, 64), [0, 3]), ((0, 4, 64), (7, 2, 64), [0, 0])):
+        q, k, v = (torch.ones(shape, device="cuda", dtype=BF16, requires_grad=True) for shape in (q_shape, k_shape, k_shape))
+        keywords = {} if offsets is None else {"q_offsets": ints(offsets), "k_offsets": ints([0, 0])}
+        y = mflux_amd.attention(q, k, v, **keywords)
+        assert y.shape == q.shape and bool((y == 0).all())
+        for g, t in zip(torch.autograd.grad(y, (q, k, v), torch.ones_like(y)), (q, k, v)):
+            assert g.shape == t.shape and bool((g == 0).all())
 
 
 def test_attention_many_short_sequences():
