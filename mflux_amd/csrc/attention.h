@@ -191,12 +191,12 @@ __device__ inline void head_and_tile(int id, int heads, int tiles, int& head, in
 
 // ---- tiles in LDS -----------------------------------------------------------------------------------------
 // A tile is rows of kPitch elements (a power of two, the head's 16-byte pieces padded up to it), the pieces of a row permuted by
-// an exclusive or with the row's bits: 16 rows' pieces of the same number lie in different banks (a matrix operand's rows), and so
-// do the 32-byte pairs of eight consecutive rows (the transposing read).
+// an exclusive or with the row's bits: pieces of the same number of 16 rows lie in different banks (a matrix operand's rows), and so
+// do 64 bytes of each of four consecutive rows (what 32 lanes of the transposing read take).
 template <int kPitch>
 __device__ inline int swizzle(int row) {
-  if constexpr (kPitch == 64) return ((row >> 1 & 3) << 1) | (row >> 3 & 1);
-  return ((row & 7) << 1) | (row >> 3 & 1);
+  if constexpr (kPitch == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 1) << 1 | (row >> 3 & 1);  // (two rows to a turn of the banks)
+  return (row & 3) << 2 | (row >> 2 & 1) << 1 | (row >> 3 & 1);
 }
 
 // Loads a tile of kRows rows straight into LDS with kThreads threads, 16 bytes a lane and instruction; rows past `rows` repeat the
