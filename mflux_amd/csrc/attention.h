@@ -174,14 +174,15 @@ __device__ inline Run find_run(const AttentionCall& c, int index, bool by_key, b
 }
 
 // The (head, tile) of workgroup `id` of heads x tiles.  Workgroups are dealt round-robin to the 8 XCDs, each with an L2 of its
-// own: an XCD takes whole heads, neighbours (which share their keys and values in a grouped call) behind each other, and all its
-// workgroups in flight read the same head's keys; the heads past a multiple of 8 are spread tile by tile.
-__device__ inline void head_and_tile(int id, int heads, int tiles, int& head, int& tile) {
+// own: an XCD takes whole heads, neighbours (which share their keys and values in a grouped call), one behind the other, so that all its
+// workgroups in flight read the same head's keys; the heads past a multiple of 8 are spread tile by tile.  `uneven`: tiles of different
+// lengths, the longest first: then an XCD takes its heads' tiles in turn, or the last head's longest would start last.
+__device__ inline void head_and_tile(int id, int heads, int tiles, bool uneven, int& head, int& tile) {
   const int per_xcd = heads / 8, whole = per_xcd * 8 * tiles;
   if (id < whole) {
     const int x = id & 7, j = id >> 3;
-    head = x * per_xcd + j / tiles;
-    tile = j % tiles;
+    head = x * per_xcd + (uneven ? j % per_xcd : j / tiles);
+    tile = uneven ? j / per_xcd : j % tiles;
   } else {
     const int rest = heads - per_xcd * 8, j = id - whole;
     head = per_xcd * 8 + j % rest;

@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
   extern __shared__ __attribute__((aligned(16))) char lds[];  // K, V, K, V
   const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
   int head, index;
-  head_and_tile(blockIdx.x, c.heads, tiles, head, index);
+  head_and_tile(blockIdx.x, c.heads, tiles, c.causal || c.q_offsets, head, index);
   const Run run = find_run<kQueries>(c, index, false, c.causal);
   if (!run.valid) return;
   const int kv_head = head / (c.heads / c.kv_heads);

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
   extern __shared__ __attribute__((aligned(16))) char lds[];  // K, V, K, V
   const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
   int head, index;
-  head_and_tile(blockIdx.x, c.heads, tiles, head, index);
+  head_and_tile(blockIdx.x, c.heads, tiles, c.causal || c.q_offsets, head, index);
   const Run run = find_run<kQueries>(c, index, false, c.causal);
   if (!run.valid) return;
   const int kv_head = head / (c.heads / c.kv_heads);
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
   const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
   const int keys_of = wave & 3, half = wave >> 2;
   int which, index;
-  head_and_tile(blockIdx.x, c.kv_heads * parts, tiles, which, index);
+  head_and_tile(blockIdx.x, c.kv_heads * parts, tiles, c.causal || c.q_offsets, which, index);
   const int kv_head = which / parts, part = which - kv_head * parts;
   const Run run = find_run<kKeyRows>(c, index, true, false);  // causal: the first keys have the most queries
   if (!run.valid) return;
