@@ -5,8 +5,13 @@
 //
 // One pass over the keys with the softmax's running maximum and sum in float32; the scores never leave the registers.
 // A workgroup of four wavefronts has 128 queries of one head, 32 a wavefront, and walks the keys 64 at a time: K and V
-// tiles go straight from memory into LDS (two of each, the next pair in flight while the current one is multiplied) and are
-// read by all four wavefronts.  See attention.h for the orientation of the products.
+// tiles go straight from memory into LDS (two of each, the next in flight while the current one is multiplied) and are
+// read by all four wavefronts.  Two workgroups share a compute unit.  See attention.h for the orientation of the products.
+//
+// 4608 tokens, 24 heads of 128, bfloat16, calls behind each other: 274 us, 0.95 PFLOP/s (a large library product: 1.39); 16384
+// causal tokens, 28 / 4 heads: 1.84 ms, 1.04.  The counters show the matrix units busy in 41 % of the cycles, six vector instructions
+// to a matrix instruction and no bank conflicts; power has a part as well, on zeros the first call takes 227 us.  256 queries to a
+// workgroup, three stages of tiles, 128 keys a step and wavefront priorities were tried and were no faster.
 #include "attention.h"
 
 namespace mfq {

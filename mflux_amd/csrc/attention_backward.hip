@@ -4,7 +4,12 @@
 // the rows' sums of dy y, which the other needs), one the queries of a tile of keys (dk and dv, over all heads that share them).
 // That makes the scores twice, 14 instead of 10 operations a pair and element of a head, and no sum is made by atomics, so the
 // gradients are the same bits every time.  All sums are float32; P and dS are rounded to the inputs' type for the second products,
-// as P is in the forward pass.
+// as P is in the forward pass.  sum(dy y) is taken from y and what its rounding left: with the roundings of bfloat16 put into a
+// 64-bit calculation (1024 causal tokens, D = 128) dq is off by 2.6 10^-3 of its norm from the rounded y, by 2.4 from this one.
+//
+// 4608 tokens, 24 heads of 128: dq 380 us, 1.03 PFLOP/s of its 6 operations a pair and element; dk and dv 572 us, 0.91 of their 8;
+// causal 0.93 and 0.91.  4099 causal tokens in three sequences, 24 / 8 heads: 124 and 186 us, and 19 to join the parts; there the
+// counters show the matrix units busy in 28 and 30 % of the cycles.
 #include "attention.h"
 
 #include <algorithm>

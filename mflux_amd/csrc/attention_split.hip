@@ -5,6 +5,10 @@
 // rows = tokens x heads of a group to a workgroup), and every wavefront streams key tiles of its own through a ring in LDS
 // that no other wavefront waits for.  The wavefronts of a workgroup are joined in LDS, the workgroups of a sequence by a second
 // launch over their float32 partial results (none if the axis is not split).
+//
+// One token of 32 sequences of up to 8192 keys, 32 / 8 heads of 128: 124 us, 602 MB, 4.9 TB/s (as a large copy), 5 us of them the join;
+// 205 MB of keys and values of one sequence: 47 us, 4.4 TB/s, 6 of them the join.  Prompts too small for tiles of 128 queries come
+// here as well (attention_splits).
 #include "attention.h"
 
 #include <algorithm>

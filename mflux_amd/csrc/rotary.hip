@@ -6,8 +6,9 @@
 // gradients:  dn = the turned back dy,  dw = sum dn x r,  dx = r (w dn - x r mean(w dn x r)),  r = 1 / sqrt(mean(x^2) + eps).
 // Everything between a load and its store is float32 and rounded once; sums over rows are float32 and in a fixed order.
 //
-// Bound by HBM: every element is read and written once.  A lane holds kVec pairs of a row, as many lanes as that takes a row, and a
-// wavefront a token's rows: its cosines and sines are loaded once for all heads it walks.
+// Bound by HBM: every element is read and written once.  A lane holds kVec pairs of a row, as many lanes as that takes a row, and
+// rows (token, head) are dealt to the wavefronts.  4608 tokens, 24 + 24 heads of 128 with norms, bfloat16: 28 us, 4.1 TB/s (a large copy:
+// 4.9); backward of 4110 tokens, 16 + 4 heads, float16: 23 us, and 4 for the weights' sums.
 #include "common.h"
 
 #include <algorithm>
