@@ -207,6 +207,20 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
       advance(first + kKeys, 1);
       whole_tile(lds + 2 * kTileBytes);
     }
+    // at the largest heads what follows has offsets and rows of its own, as in the forward pass
+    auto separate = [&]() __attribute__((always_inline)) {
+      if constexpr (kDim > 192) {
+        int own = thread;
+        asm volatile("" : "+v"(own));
+        load_k.init(own, c.k.token, c.dim);
+        load_v.init(own, c.v.token, c.dim);
+        int64_t at = inside;
+        asm volatile("" : "+v"(at));
+        Row::load_row(q, c.q.p + run.batch * c.q.batch + at * c.q.token + head * c.q.head, c.dim, own & (kWave - 1));
+        Row::load_row(dy, c.dy.p + run.batch * c.dy.batch + at * c.dy.token + head * c.dy.head, c.dim, own & (kWave - 1));
+      }
+    };
+    separate();
     bool not_finite = false;
 #pragma unroll 1
     for (; first < keys; first += kKeys, buffer ^= 1) {
@@ -222,6 +236,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) dq[b] = zero16();
       unit = {};
+      separate();
       load_k.load(k, lds_at, keys, thread);
       load_v.load(v, lds_at + kTileBytes, keys, thread);
 #pragma unroll 1
@@ -473,12 +488,27 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
       }
       return not_finite;
     };
+    auto separate = [&]() __attribute__((always_inline)) {  // as in the dq kernel
+      if constexpr (kDim > 192) {
+        int own = thread;
+        asm volatile("" : "+v"(own));
+        load_q.init(own, c.q.token, c.dim);
+        load_dy.init(own, c.dy.token, c.dim);
+        if constexpr (S::kHoldK) {
+          int64_t at = inside;
+          asm volatile("" : "+v"(at));
+          Row::load_row(k, c.k.p + run.batch * c.k.batch + at * c.k.token + kv_head * c.k.head, c.dim, own & (kWave - 1));
+        }
+      }
+    };
+    separate();
     const bool not_finite = edges(Mode<kEdge>());
     if (edge > 0 && any_wave<S::kWaves>(not_finite, lds + S::kV)) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) dk[b] = dv[b] = zero16();
       unit = {};
       i = stage = 0;
+      separate();
       request(0, 0);
       edges(Mode<kRowByRow>());
     }
