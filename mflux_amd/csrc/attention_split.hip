@@ -77,41 +77,65 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
     auto request_v = [&](int first) __attribute__((always_inline)) {
       load_v.load(v + (int64_t)first * c.v.token, ring_at + S::kTile, run.nk - first, lane);
     };
-    const int first_tile = begin + wave * kStep;
-    auto walk = [&](auto one_by_one) __attribute__((always_inline)) {
-      constexpr bool kOneByOne = decltype(one_by_one)::value;
+    int first = begin + wave * kStep;
+    auto start = [&]() __attribute__((always_inline)) {
+      if (first < end) {
+        request_k(first);
+        request_v(first);
+      }
+    };
+    enum { kWhole, kEdge, kRowByRow };
+    // the tile at `first`, whose mode is one value
+    auto tile = [&](auto mode) __attribute__((always_inline)) {
+      constexpr int kMode = decltype(mode)::value;
       bool not_finite = false;
-      if (first_tile < end) {
-        request_k(first_tile);
-        request_v(first_tile);
-      }
-#pragma unroll 1
-      for (int first = first_tile; first < end; first += kWaves * kStep) {
-        const int next = first + kWaves * kStep;
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
-        auto between = [&]() __attribute__((always_inline)) {
-          if (next < end) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
-            request_k(next);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
-          } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          }
-        };
-        if constexpr (kOneByOne) state.template step<1, true, true>(k_tile, v_tile, limit - first, scale, lane, between);
-        else if (first + kStep <= least) state.template step<1, false>(k_tile, v_tile, kStep, scale, lane, between);
-        else not_finite |= state.template step<1, true>(k_tile, v_tile, limit - first, scale, lane, between);
+      const int next = first + kWaves * kStep;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+      auto between = [&]() __attribute__((always_inline)) {
         if (next < end) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V
-          request_v(next);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+          request_k(next);
+          asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kRequests) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
+      };
+      if constexpr (kMode == kWhole) state.template step<1, false>(k_tile, v_tile, kStep, scale, lane, between);
+      else not_finite = state.template step<1, true, kMode == kRowByRow>(k_tile, v_tile, limit - first, scale, lane, between);
+      if (next < end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V
+        request_v(next);
       }
+      first = next;
       return not_finite;
     };
-    if (walk(std::false_type())) {
+    // at the largest heads what follows the whole tiles has offsets and queries of its own (attention.hip has the reason)
+    auto separate = [&]() __attribute__((always_inline)) {
+      if constexpr (kDim > 192) {
+        int own = lane;
+        asm volatile("" : "+v"(own));
+        load_k.init(own, c.k.token, c.dim);
+        load_v.init(own, c.v.token, c.dim);
+        int64_t at = q_at;
+        asm volatile("" : "+v"(at));
+        state.load_row(state.q, c.q.p + at, c.dim, own);
+      }
+    };
+    start();
+#pragma unroll 1
+    while (first < end && first + kStep <= least) tile(std::integral_constant<int, kWhole>());
+    separate();
+    bool not_finite = false;
+#pragma unroll 1
+    while (first < end) not_finite |= tile(std::integral_constant<int, kEdge>());
+    if (not_finite) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       state.init();
-      walk(std::true_type());
+      separate();
+      first = begin + wave * kStep;
+      start();
+#pragma unroll 1
+      while (first < end) tile(std::integral_constant<int, kRowByRow>());
     }
   }
 
