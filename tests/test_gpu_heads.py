@@ -419,6 +419,45 @@ def test_attention_backward_masked_infinities(H):
         assert bool(a[0, 30:].isfinite().all()) and float((a[0, 30:].float() - b[0, 30:].float()).abs().max()) <= 0.05
 
 
+@pytest.mark.parametrize("H,tiles", [(1, False), (260, True)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("D", [128, 136, 192, 200, 256])
+def test_attention_masked_infinities_of_large_heads(D, bad, H, tiles):
+    """Behind whole tiles, at every size of a head: what is not finite behind a key leaves the queries in front of it what they are in
+    the shorter sequence, and in front of a query it leaves the keys behind it what they are without those queries."""
+    import mflux_amd
+
+    n, cut, some = 400, 300, [0, H - 1]
+    q, k, v, dy = (randn(i + 1, 1, n, H, D, dtype=BF16) for i in range(4))
+    assert (ranges(q, k) == 0) == tiles
+
+    def run(q, k, v, dy):
+        q, k, v = (t.detach().clone().requires_grad_() for t in (q, k, v))
+        y = mflux_amd.attention(q, k, v, causal=True)
+        return [t[0][:, some] for t in (y.detach(), *torch.autograd.grad(y, (q, k, v), dy))]
+
+    def sequence(*t):
+        return [x[0][:, some] for x in t]
+
+    k2, v2 = k.clone(), v.clone()
+    k2[0, cut + 3:] = bad
+    v2[0, cut:] = bad
+    y, dq, _, _ = run(q, k2, v2, dy)
+    a, b, c, d = sequence(q[:, :cut], k[:, :cut], v[:, :cut], dy[:, :cut])
+    want = ref.attention_sequence(a, b, c, True, D ** -0.5, d)
+    ref.check("y", y[:cut], *want["y"])
+    ref.check("dq", dq[:cut], *want["dq"])
+    assert bool((~y[cut + 3:].isfinite()).all())
+    q2, dy2 = q.clone(), dy.clone()
+    q2[0, :cut - 5] = bad
+    dy2[0, :cut] = bad
+    _, _, dk, dv = run(q2, k, v, dy2)
+    a, b, c, d = sequence(q[:, cut:], k, v, dy[:, cut:])
+    want = ref.attention_sequence(a, b, c, True, D ** -0.5, d)
+    for name, t in (("dk", dk), ("dv", dv)):
+        ref.check(name, t[cut:], want[name][0][cut:], want[name][1][cut:])
+
+
 @pytest.mark.parametrize("queries", [100, 1])
 def test_attention_strides(queries):
     """Slices of a stacked product, the [B, H, S, D] order, an odd address, an expanded batch and head: the same bits."""
