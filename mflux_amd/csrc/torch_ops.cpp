@@ -713,6 +713,13 @@ c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::op
 Tensor or_none(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 bool wanted(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
+// A forward-mode derivative is not there either, and below autograd a tangent would be dropped without a word
+void check_forward_mode(const char* fn, std::initializer_list<const c10::optional<Tensor>*> operands) {
+  for (const auto* t : operands)
+    TORCH_CHECK(!t->has_value() || !(*t)->_fw_grad(0).defined(), fn, ": trying to differentiate in forward mode a function that has no "
+                "forward-mode derivative");
+}
+
 // A backward pass that is captured into a graph hands a leaf's gradient to the node that an earlier, still living graph of the leaf made for
 // it on the stream of its time.  Where that is the default stream the engine makes the capture wait for it, which HIP forbids, in a
 // thread that cannot hand the error on: the process ends.  Such a call is refused while there is nothing to lose.
@@ -767,8 +774,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 std::tuple<Tensor, Tensor> rotary_call(const Tensor& q, const c10::optional<Tensor>& k, const Tensor& cos, const Tensor& sin,
                                        const c10::optional<Tensor>& positions, const c10::optional<Tensor>& q_weight,
                                        const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
+  const c10::optional<Tensor> first(q), c(cos), s(sin);
+  check_forward_mode("mfq::rotary", {&first, &k, &c, &s, &q_weight, &k_weight});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(q_weight) || wanted(k_weight))) {
-    const c10::optional<Tensor> first(q);
     check_capture("mfq::rotary", {&first, &k, &q_weight, &k_weight}, q);
     auto out = RotaryFunction::apply(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
     return {out[0], out.size() > 1 ? out[1] : at::empty({0}, q.options())};
@@ -811,8 +819,9 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
 Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q_offsets,
                       const c10::optional<Tensor>& k_offsets, const c10::optional<Tensor>& q_lengths, const c10::optional<Tensor>& k_lengths,
                       bool causal, double scale) {
+  const c10::optional<Tensor> a(q), b(k), c(v);
+  check_forward_mode("mfq::attention", {&a, &b, &c});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) {
-    const c10::optional<Tensor> a(q), b(k), c(v);
     check_capture("mfq::attention", {&a, &b, &c}, q);
     return AttentionFunction::apply(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale);
   }

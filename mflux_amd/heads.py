@@ -10,7 +10,8 @@ their strides: a slice of a stacked product needs no copy.
 
 The calls run on the current stream of their tensors' device and launch nothing
 anywhere else; sums are made in a fixed order, so the same inputs give the same
-bits.  All three can be captured into a graph.
+bits.  All three can be captured into a graph.  Gradients are first derivatives in
+reverse mode: a second derivative and forward mode are refused.
 """
 from __future__ import annotations
 

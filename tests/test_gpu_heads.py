@@ -711,6 +711,30 @@ def test_no_second_derivative():
         g.float().sum().backward()
 
 
+def test_no_forward_mode():
+    """A tangent is refused, not dropped, on every operand and with or without a gradient in reverse mode as well."""
+    import mflux_amd
+    from torch.autograd import forward_ad
+
+    q, k, v = (randn(i, 1, 9, 2, 32, dtype=BF16) for i in range(3))
+    w = randn(4, 32, dtype=BF16)
+    cos, sin = randn(2, 9, 16).cos(), randn(2, 9, 16).sin()
+    calls = [((q, k, v), lambda q, k, v: mflux_amd.attention(q, k, v)),
+             ((q, k, cos, sin, w, w.clone()), lambda q, k, cos, sin, a, b: mflux_amd.rotary(q, k, cos, sin, q_weight=a, k_weight=b)[0])]
+    for operands, call in calls:
+        for i, t in enumerate(operands):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call(*operands[:i], dual, *operands[i + 1:])
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                    call(*operands[:i], dual, *operands[i + 1:])
+                # a dual level alone refuses nothing
+                assert torch.equal(call(*operands), call(*operands))
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.func.jvp(lambda x: call(*operands[:i], x, *operands[i + 1:]), (t,), (torch.ones_like(t),))
+
+
 def test_c_entry_points_agree_with_the_ops():
     """The C ABI on the same buffers gives the ops' bits."""
     import ctypes
