@@ -416,6 +416,17 @@ __device__ inline void add_columns_one_by_one(f32x16 (&acc)[kBlocks], const char
   }
 }
 
+// The exponentials' reference follows a row's maximum only where that has grown by more than a factor of 2^kLag: up to there float32
+// sums and 16-bit probabilities hold them as well as values up to 1, and the accumulators need no pass.  bfloat16 has the range for any
+// lag.  float16 ends at 2^16 and loses bits below 2^-14 and everything below 2^-25, so its probabilities are multiples of 2^-kLift, and so is
+// the sum that they are divided by: at most 2^-35 of the largest is lost.  (Without it 8192 keys of weight e^-18 each beside a strong one
+// vanished together.)  A lag of 4 takes the time that one of 8 takes on scores of a standard deviation of 1 (4608 tokens x 24 heads of 128: 286
+// us), and 294 instead of 288 us at 3, where a lag of 1 with another three powers took 309 and 318.
+template <typename T>
+constexpr float kLag = T::code == MFQ_F16 ? 4.f : 8.f;
+template <typename T>
+constexpr float kLift = T::code == MFQ_F16 ? 10.f : 0.f;
+
 // ---- a lane's query as the softmax goes over its keys -----------------------------------------------------------
 // kDim: the head's size padded to a multiple of 32.  O^T accumulates in kDim / 32 results.
 template <typename T, int kDim, int kPitch>
@@ -490,9 +501,7 @@ struct QueryState {
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
     most = max_halves(most);
-    // The reference follows the maximum only where that has grown by more than 2^8: up to there the exponentials are at most 256,
-    // which float32 sums and 16-bit probabilities hold as well as values up to 1, and the accumulators need no pass.
-    if (__any((most - top) * c > 8.f)) {
+    if (__any((most - top) * c > kLag<T>)) {
       const float next = fmaxf(top, most);
       const float factor = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((top - next) * c);
       top = next;
@@ -502,7 +511,7 @@ struct QueryState {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] *= factor;
     }
-    const float shift = top == -__builtin_inff() ? 0.f : top * c;
+    const float shift = reference(c);
 #pragma unroll
     for (int n = 0; n < 2 * kTiles; ++n) {
       const vec8 p = probabilities(s[n / 2], n & 1, c, shift);
@@ -520,6 +529,10 @@ struct QueryState {
     }
     return not_finite;
   }
+  // what the scaled scores are taken against
+  __device__ __attribute__((always_inline)) inline float reference(float c) const { return top == -__builtin_inff() ? 0.f : top * c - kLift<T>; }
+  // the row's log2 of the sum of exp2 of the scaled scores; `total`: of both halves and all parts
+  __device__ static inline float log_sum(float top, float total, float c) { return top * c + (__builtin_amdgcn_logf(total) - kLift<T>); }
   // exponentials of half a score tile as the second product's operand, added to the sum
   __device__ __attribute__((always_inline)) inline vec8 probabilities(f32x16& s, int slab, float c, float shift) {
 #pragma unroll
@@ -540,7 +553,7 @@ struct QueryState {
   // the reference follows the block's maximum (see step)
   __device__ __attribute__((always_inline)) inline void follow(float most, float c) {
     most = max_halves(most);
-    if (__any((most - top) * c > 8.f)) {
+    if (__any((most - top) * c > kLag<T>)) {
       const float next = fmaxf(top, most);
       const float factor = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((top - next) * c);
       top = next;
@@ -560,7 +573,7 @@ struct QueryState {
   // s: the block's scores; kNext: next = the scores of the block at k32
   template <bool kNext>
   __device__ __attribute__((always_inline)) inline void overlapped(f32x16& s, f32x16& next, const Addresses& at, int k32, int v32, float c) {
-    const float shift = top == -__builtin_inff() ? 0.f : top * c;
+    const float shift = reference(c);
     vec8 p[2], w[2][kBlocks], a[3];
     if constexpr (kNext) {
       next = zero16();

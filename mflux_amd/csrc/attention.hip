@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
   store_row<T, kDim / 32>(c.out + to, c.rest ? c.rest + to : nullptr, state.o, seen, 1.0f / sum, c.dim, lane);
   if (c.lse && lane < 32) {
     const int64_t rows = (int64_t)(c.q_offsets ? 1 : c.batch) * c.q_tokens;
-    c.lse[head * rows + at] = seen ? state.top * (c.scale * kLog2e) + __builtin_amdgcn_logf(sum) : __builtin_inff();
+    c.lse[head * rows + at] = seen ? state.log_sum(state.top, sum, c.scale * kLog2e) : __builtin_inff();
   }
 }
 

@@ -67,9 +67,10 @@ struct ColumnUnit {
     }
   }
 };
-// and probabilities of very many keys as multiples of 2^-8
+// and probabilities as multiples of 2^-13, for those that many queries give to a key that none of them looks at in earnest (attention.h, kLift;
+// what is left to float16's 2^16 is for scores of millions, whose float32 log-sum-exp is itself off by more than 1)
 template <typename T>
-constexpr float kProbabilityShift = T::code == MFQ_F16 ? 8.f : 0.f;
+constexpr float kProbabilityShift = T::code == MFQ_F16 ? 13.f : 0.f;
 
 constexpr int kKeys = 64;  // of a step of the first kernel
 

@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
       *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = packed;
       if (c.rest) *reinterpret_cast<u32x2*>(c.rest + at * c.dim + d) = pack4_rest<T>(o, packed);
       if (c.lse && d == 0)
-        c.lse[(at % c.heads) * rows + at / c.heads] = seen ? top * c2 + __builtin_amdgcn_logf(total) : __builtin_inff();
+        c.lse[(at % c.heads) * rows + at / c.heads] = seen ? state.log_sum(top, total, c2) : __builtin_inff();
     } else {
       const int64_t slot = (int64_t)split * rows * c.heads + at;
       if (begin < run.nk) *reinterpret_cast<f32x4*>(part_o + slot * c.dim + d) = o;
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows
     *reinterpret_cast<u32x2*>(c.out + at * c.dim + d) = packed;
     if (c.rest) *reinterpret_cast<u32x2*>(c.rest + at * c.dim + d) = pack4_rest<T>(o, packed);
   }
-  if (c.lse && thread == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + __builtin_amdgcn_logf(total);
+  if (c.lse && thread == 0) c.lse[(at % c.heads) * rows + at / c.heads] = empty ? __builtin_inff() : top * c2 + (__builtin_amdgcn_logf(total) - kLift<T>);
 }
 
 // keys of a call's longest sequence as the host knows it, over the splits

@@ -9,8 +9,8 @@ attention   A probability p is rounded once (u p), its score is a float32 sum of
             that is off by u at most, which is u |y| of the result and u of every probability that the backward pass makes from the
             saved log-sum-exp.  Then y is rounded.
 gradients   p as above from the saved float32 log-sum-exp; dS = p (dP - delta) is rounded once, and delta = sum dy y is as far off as
-            y is.  Then the sums and the rounding of the result.  float16 rounds multiples of its gradients: 2^8 p, so 2^-33 of a
-            probability is lost, and dS times a power of two that has a column's largest at 2^4 or above, so at most 2^-28 of that.
+            y is.  Then the sums and the rounding of the result.  float16 rounds multiples of its gradients: 2^13 p, so less than 2^-33 of a
+            probability is lost (and of the forward pass's, multiples as well, less than 2^-25), and dS times a power of two that has a column's largest at 2^4 or above, so at most 2^-28 of that.
 """
 import math
 
@@ -50,12 +50,14 @@ def visible(nq, nk, causal, device):
     return torch.arange(nk, device=device)[None] <= torch.arange(nq, device=device)[:, None] + (nk - nq)
 
 
-def attention_sequence(q, k, v, causal, scale, dy=None):
-    """q [nq, H, D], k and v [nk, Hkv, D] of one sequence: {"y": (value, bound), and with dy "dq", "dk", "dv"}, float64."""
+def attention_sequence(q, k, v, causal, scale, dy=None, lost_p=None):
+    """q [nq, H, D], k and v [nk, Hkv, D] of one sequence: {"y": (value, bound), and with dy "dq", "dk", "dv"}, float64.
+    lost_p: what float16 may lose of a probability, in the result and in dv (default: as derived above)."""
     nq, H, D = q.shape
     nk, Hkv = k.shape[:2]
     g = H // Hkv
     u, tiny = HALF[q.dtype], TINY[q.dtype]
+    lost_y, lost_dv = (tiny, tiny * 2.0 ** -8) if lost_p is None else lost_p
     q, k, v = q.double(), k.double(), v.double()
     names = ["y"] if dy is None else ["y", "dq", "dk", "dv"]
     shapes = {"y": q, "dq": q, "dk": k, "dv": v}
@@ -76,7 +78,7 @@ def attention_sequence(q, k, v, causal, scale, dy=None):
         size = torch.where(see, scale * (qh.abs() @ kh.abs().t().contiguous()), 0.0).amax()
         c = E * (2 * (D + 8) * size + 8 * top[some].abs().amax().clamp(min=1.0) + nk + 32) if some.any() else torch.tensor(0.0).to(q)
         av = p @ vh.abs()
-        lost = tiny * (see.double() @ vh.abs())
+        lost = lost_y * (see.double() @ vh.abs())
         out["y"][0][:, h] = y
         bound = ((u + c) * av + u * y.abs()) * 1.01 + lost
         out["y"][1][:, h] = bound + u * (y.abs() + bound) + tiny
@@ -91,7 +93,7 @@ def attention_sequence(q, k, v, causal, scale, dy=None):
         # dS before its rounding: p's relative error, dP's and delta's float32 sums, delta's rounded y
         eds = (u + c) * ds.abs() + torch.where(see, p * (E * (D + 4) * (adp + adelta) + (dyh.abs() * out["y"][1][:, h]).sum(1, keepdim=True)), 0.0)
         eds = (eds + u * (ds.abs() + eds) + (tiny > 0) * 2.0 ** -28 * ds.abs().amax() * see) * 1.01
-        ep = torch.where(see, (2 * u + c) * p * 1.01 + tiny * 2.0 ** -8, 0.0)
+        ep = torch.where(see, (2 * u + c) * p * 1.01 + lost_dv, 0.0)
         n = nq * g
         for name, value, error, first in (
                 ("dq", scale * (ds @ kh), scale * (eds @ kh.abs() + E * (nk + 4) * (ds.abs() @ kh.abs())), True),

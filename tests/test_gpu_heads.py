@@ -364,6 +364,46 @@ def test_attention_float16_gradients_of_any_size(size, n):
         ref.check(name, g[0][inside], value[inside], bound[inside] + 2.0 ** -25)
 
 
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("gap", [10.0, 15.0, 17.0, 18.0, 20.0, 22.0])
+@pytest.mark.parametrize("queries,H,n", [(1, 1, 8192), (32, 2, 3000), (128, 260, 4097)])
+def test_attention_float16_small_probabilities(queries, H, n, gap, D):
+    """A strong key of small value and thousands whose probabilities are e^-gap of its own: together they are the result, and
+    their own gradients.  A probability is made as a multiple of 2^-10 of the largest's or more, so that 2^-25 lost of it is 2^-35; for dv
+    it is a multiple of 2^-13 of 1: 2^-38."""
+    import mflux_amd
+
+    lost = 2.0 ** -35, 2.0 ** -38
+    for at in (0, n // 2, n - 1):  # the strong key before, among and behind the others
+        k = randn(1, 1, n, 1, D, dtype=F16, std=0.05)
+        k[..., 0] = 0.0
+        k[0, at, 0, 0] = gap
+        v = (randn(2, 1, n, 1, D) + 1.0).to(F16)
+        v[0, at] = 0.0
+        q = randn(3, 1, queries, 1, D, dtype=F16, std=0.1)
+        q[..., 0] = 1.0
+        call = [t.expand(-1, -1, H, -1).detach().requires_grad_() for t in (q, k, v)]
+        assert (ranges(*call[:2]) == 0) == (H > 2)
+        y = mflux_amd.attention(*call, scale=1.0)
+        if gap > 20.0 or queries == 1:
+            for h in (0, H - 1):
+                ref.check("y", y[0, :, h:h + 1], *ref.attention_sequence(q[0], k[0], v[0], False, 1.0, lost_p=lost)["y"])
+            continue
+        dy = (randn(4, 1, queries, 1, D) + 1.0).to(F16)
+        dv, = torch.autograd.grad(y, call[2], dy.expand(-1, -1, H, -1))
+        want = ref.attention_sequence(q[0], k[0], v[0], False, 1.0, dy[0], lost_p=lost)
+        for h in (0, H - 1):
+            ref.check("y", y[0, :, h:h + 1], *want["y"])
+            ref.check("dv", dv[0, :, h:h + 1], *want["dv"])
+
+
+def test_attention_float16_large_scores():
+    """Scores of hundreds, in both forms of a call."""
+    run_attention("batched", F16, 128, 2, 2, [200], [200], False, grad=True, scale=3.0)
+    run_attention("batched", F16, 128, 260, 260, [200], [400], False, grad=True, scale=3.0, tiles=True)
+    run_attention("batched", F16, 128, 8, 2, [1], [2000], False, grad=False, scale=3.0)
+
+
 @pytest.mark.parametrize("queries,H", [(96, 2), (2, 2), (96, 260)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_masked_infinities(queries, H, bad):
