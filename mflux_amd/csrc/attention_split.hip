@@ -188,7 +188,8 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
     } else {
       const int64_t slot = (int64_t)split * rows * c.heads + at;
       if (begin < run.nk) *reinterpret_cast<f32x4*>(part_o + slot * c.dim + d) = o;
-      if (d == 0) part_stats[slot] = make_float2(top, total);
+      // a range in which the row sees no key has the sum -1: one in which its scores are all -infinity has the sum 0
+      if (d == 0) part_stats[slot] = make_float2(top, visible_keys(run, tok, c.causal) > begin ? total : -1.f);
     }
   }
 }
@@ -217,10 +218,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows
   for (int s = mine; s < splits; s += groups) {
     const float2 st = part_stats[s * step + at];
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    if (d < c.dim && (st.y != 0.f || st.x != -__builtin_inff())) a = *reinterpret_cast<const f32x4*>(part_o + (s * step + at) * c.dim + d);
-    // a part without keys has the factor 0; where the reference is an infinity the scores' own NaN stay
+    const bool seen = !(st.y < 0.f);  // (a sum that is NaN is a row's own)
+    if (d < c.dim && seen) a = *reinterpret_cast<const f32x4*>(part_o + (s * step + at) * c.dim + d);
+    // where the reference is an infinity the scores' own NaN stay
     const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * c2);
-    total += st.y * f;
+    total += seen ? st.y * f : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += a[e] * f;
   }
@@ -232,8 +234,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionCall c, int64_t rows
   __syncthreads();
   if (mine) return;
   total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  // a row that sees no key has neither a maximum nor a sum (a sum that is NaN is a row's own)
-  const bool empty = top == -__builtin_inff() && total == 0.f;
+  const bool empty = part_stats[at].y < 0.f;  // a row that sees any key sees the first one
   const float f = 1.0f / total;
   if (d < c.dim) {
     for (int g = 1; g < groups; ++g) o += *reinterpret_cast<const f32x4*>(&parts[g][d]);

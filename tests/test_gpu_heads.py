@@ -364,6 +364,34 @@ def test_attention_float16_gradients_of_any_size(size, n):
         ref.check(name, g[0][inside], value[inside], bound[inside] + 2.0 ** -25)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,H,nk,form", [(1, 2, 100, 1), (1, 2, 5000, 2), (4, 2, 9000, 2), (140, 90, 300, 0)])
+def test_attention_scores_of_minus_infinity(queries, H, nk, form, causal, D):
+    """Scores that are all -infinity have no softmax: NaN, in every form of a call (form 2: ranges that are joined), where a row
+    that sees no key is zeros.  Among others they weigh nothing."""
+    import mflux_amd
+
+    q = randn(1, 5, queries, H, D, dtype=BF16).abs()
+    k, v = randn(2, 5, nk, H, D, dtype=BF16), randn(3, 5, nk, H, D, dtype=BF16)
+    assert min(ranges(q, k), 2) == form
+    want = mflux_amd.attention(q, k[:, 7:8], v[:, 7:8])
+    k[:2, :, :, D // 2] = -math.inf
+    k[1, 7] = 0.0
+    k[4, 60:, :, D // 2] = -math.inf
+    y = mflux_amd.attention(q, k, v, causal=causal, k_lengths=ints([nk, nk, 0, nk, nk]))
+    last = y[:, -1] if causal else y  # (causal: earlier queries may see fewer keys)
+    assert bool(last[0].isnan().all())
+    assert torch.equal(last[1], want[1, -1] if causal else want[1])
+    assert bool((y[2] == 0).all())
+    assert bool(y[3].isfinite().all()) and bool(last[4].isfinite().all())
+    short = mflux_amd.attention(q[4:], k[4:, :60].contiguous(), v[4:, :60].contiguous())[0]
+    # (each of the two off by three roundings of at most |v|: probabilities, their sum, the result)
+    assert float((last[4].float() - (short[-1] if causal else short).float()).abs().max()) <= 6.01 * 2.0 ** -8 * float(v[4, :60].float().abs().max())
+    if causal and queries <= nk:  # every query sees keys here
+        assert bool(y[0].isnan().all())
+
+
 @pytest.mark.parametrize("D", [64, 128, 192, 256])
 @pytest.mark.parametrize("gap", [10.0, 15.0, 17.0, 18.0, 20.0, 22.0])
 @pytest.mark.parametrize("queries,H,n", [(1, 1, 8192), (32, 2, 3000), (128, 260, 4097)])
