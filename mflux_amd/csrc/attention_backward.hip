@@ -592,26 +592,27 @@ int64_t key_tiles(const AttentionCall& c) {
 }
 int64_t key_values(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : c.batch) * c.k_tokens * c.kv_heads * c.dim; }
 
+template <typename T, int kDim, int kHalves>
+int launch_dq(const AttentionCall& c, hipStream_t stream) {
+  constexpr int kQueries = 128 / kHalves, kBytes = 4 * kKeys * pitch_of(kDim) * 2;
+  static PerDeviceInt configured;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dq_kernel<T, kDim, kHalves>), kBytes)) return MFQ_ELAUNCH;
+  const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
+  if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
+  hipLaunchKernelGGL((attention_dq_kernel<T, kDim, kHalves>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+  return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+}
+
 template <typename T, int kDim>
 int launch(const AttentionCall& c, int parts, float* workspace, hipStream_t stream) {
-  const int64_t more = c.q_offsets ? c.batch + 2 : 0;  // as in the forward pass
-  auto launch_dq = [&](auto kernel, int queries) {
-    constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
-    static PerDeviceInt configured;
-    if (!raise_lds_limit(configured, reinterpret_cast<const void*>(kernel), kBytes)) return (int)MFQ_ELAUNCH;
-    const int64_t tiles = more ? c.q_tokens / queries + more : (int64_t)((c.q_tokens + queries - 1) / queries) * c.batch;
-    if (tiles * c.heads > INT32_MAX) return (int)MFQ_ESHAPE;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
-    return (int)(hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH);
-  };
   // 64 queries to a workgroup where 128 leave compute units idle, or (causal) the longest of them working alone: causal heads of 128,
   // 2048 tokens x 8 heads (128 such workgroups) 49 against 60 us, 4096 x 16 (512) 131 and 156, 4608 x 24 (864) 242 and 220; not causal,
   // 1500 x 24 (288) 90 and 71, 2048 x 24 (384) 93 and 89.
-  const int64_t groups = (more ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
+  const int64_t groups = (c.q_offsets ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
   const bool halves = 2 * groups <= (c.causal ? 4 : 1) * (int64_t)compute_units();
   int rc;
-  if constexpr (kDim <= 128) rc = halves ? launch_dq(&attention_dq_kernel<T, kDim, 2>, 64) : launch_dq(&attention_dq_kernel<T, kDim, 1>, 128);
-  else rc = launch_dq(&attention_dq_kernel<T, kDim, 1>, 128);
+  if constexpr (kDim <= 128) rc = halves ? launch_dq<T, kDim, 2>(c, stream) : launch_dq<T, kDim, 1>(c, stream);
+  else rc = launch_dq<T, kDim, 1>(c, stream);
   if (rc != MFQ_OK) return rc;
   if (!c.dk && !c.dv) return MFQ_OK;
   using S = KeyShape<kDim>;

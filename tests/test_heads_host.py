@@ -2,6 +2,7 @@
 looked for, and at the C ABI an error code before anything is launched.  No GPU."""
 import ctypes
 import os
+import re
 import subprocess
 
 import pytest
@@ -230,3 +231,15 @@ def test_structures_match_the_header(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(source), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [value for _, value in lines]
+
+
+def test_every_attention_kernel_raises_its_own_limit():
+    """A kernel's limit of dynamic LDS is raised once per device and remembered; what remembers it belongs to that kernel alone, or
+    the second of two kernels would be launched with the limit it was built with."""
+    lines = subprocess.run(["nm", "-C", os.path.join(ROOT, "mflux_amd", "csrc", "libmfq.so")], capture_output=True, text=True, check=True).stdout
+    names = [line.split(maxsplit=2)[2] for line in lines.splitlines() if len(line.split(maxsplit=2)) == 3]
+    kernels = {n for n in names if re.search(r"::attention_(split_|dq_|dkv_)?kernel<", n) and "__device_stub__" not in n}
+    flags = [n for n in names if n.endswith("::configured") and "AttentionCall" in n and "guard variable" not in n]
+    if not names:
+        pytest.skip("a library without symbols")
+    assert len(kernels) >= 40 and len(flags) == len(kernels)
