@@ -202,12 +202,15 @@ __device__ inline int swizzle(int row) {
 
 // Loads a tile of kRows rows straight into LDS with kThreads threads, 16 bytes a lane and instruction; rows past `rows` repeat the
 // last one and pieces past the head's end its last piece, so that nothing outside the tensor is read (their scores are masked,
-// and the other operand is zero there).
-template <int kPitch, int kRows, int kThreads>
+// and the other operand is zero there).  kSkip: pieces past the head's end are left alone, for a tile in which they have been cleared: an
+// infinity that the head ends with would come to a NaN in the product with zero.  Every instruction loads whole rows, so none is
+// without lanes, and a count of requests in flight holds.
+template <int kPitch, int kRows, int kThreads, bool kSkip = false>
 struct TileLoader {
   static constexpr int kPieces = kPitch / 8;  // of a row
   static constexpr int kLoads = kRows * kPieces / kThreads;
-  static_assert(kRows * kPieces % kThreads == 0, "whole instructions");
+  static constexpr uint32_t kNone = ~0u;  // no offset: 127 rows of less than 2^25 bytes and a head lie below
+  static_assert(kRows * kPieces % kThreads == 0 && kWave % kPieces == 0, "whole instructions of whole rows");
   uint32_t row_bytes;
   uint32_t offset[kLoads];
 
@@ -217,7 +220,9 @@ struct TileLoader {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int piece = (wave * kLoads + i) * kWave + lane, row = piece / kPieces, slot = piece % kPieces;
-      offset[i] = (uint32_t)row * row_bytes + 16u * (uint32_t)min(slot ^ swizzle<kPitch>(row), dim / 8 - 1);
+      const int place = slot ^ swizzle<kPitch>(row);
+      offset[i] = (uint32_t)row * row_bytes + 16u * (uint32_t)min(place, dim / 8 - 1);
+      if (kSkip && place >= dim / 8) offset[i] = kNone;
     }
   }
   // `base`: the tile's first row in memory; `lds`: the tile's address in LDS; `rows`: those that are there, at least one
@@ -232,12 +237,23 @@ struct TileLoader {
         const int row = ((wave * kLoads + i) * kWave + lane) / kPieces;
         if (row >= rows) o -= (uint32_t)(row - rows + 1) * row_bytes;
       }
+      if (kSkip && offset[i] == kNone) continue;
       // one wait state behind the write of m0, which the compiler does not see to inside a statement of assembly
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(o), "s"(base), "s"(uniform((int)(to + (uint32_t)i * kWave * 16u)))
                    : "memory", "m0");
     }
   }
 };
+
+// The pieces past the head's end of `rows` rows of a tile, up to the size it is padded to, become zero; by `threads` threads
+template <int kPitch, int kDim>
+__device__ inline void clear_padding(char* tile, int rows, int dim, int thread, int threads) {
+  const int from = dim / 8, pieces = kDim / 8 - from;
+  for (int n = thread; n < rows * pieces; n += threads) {
+    const int r = n / pieces, piece = from + n % pieces;
+    *reinterpret_cast<u32x4a*>(tile + r * kPitch * 2 + 16 * (piece ^ swizzle<kPitch>(r))) = u32x4a{0u, 0u, 0u, 0u};
+  }
+}
 
 // Whether any of the workgroup's kWaves wavefronts says so; `at`: LDS that nobody reads any more.  Nothing is in flight afterwards.
 template <int kWaves>

@@ -21,7 +21,8 @@ constexpr int kKeys = 64;  // of a step
 
 constexpr int pitch_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-template <typename T, int kDim>
+// kPadded: the head is smaller than kDim
+template <typename T, int kDim, bool kPadded>
 __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(AttentionCall c, int tiles) {
   constexpr int kQueries = 128;  // of a workgroup
   constexpr int kPitch = pitch_of(kDim);
@@ -47,7 +48,8 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
     state.load_row(state.q, c.q.p + q_at, c.dim, lane);
     const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
     const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
-    TileLoader<kPitch, kKeys, 256> load_k, load_v;
+    TileLoader<kPitch, kKeys, 256, kPadded> load_k;
+    TileLoader<kPitch, kKeys, 256> load_v;
     load_k.init(thread, c.k.token, c.dim);
     load_v.init(thread, c.v.token, c.dim);
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
@@ -58,6 +60,10 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
     auto request_v = [&](int first) __attribute__((always_inline)) {
       load_v.load(v + (int64_t)first * c.v.token, lds_at + (first / kKeys & 1) * 2 * kTileBytes + kTileBytes, keys - first, thread);
     };
+    if constexpr (kPadded) {
+      clear_padding<kPitch, kDim>(lds, kKeys, c.dim, thread, 256);
+      clear_padding<kPitch, kDim>(lds + 2 * kTileBytes, kKeys, c.dim, thread, 256);
+    }
     request_k(0);
     request_v(0);
     // Tiles that every query of the workgroup sees all of (those that are there: the others' rows are not stored) come first, by pairs, so
@@ -166,26 +172,31 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_kernel(Att
   }
 }
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kPadded>
 int launch(const AttentionCall& c, hipStream_t stream) {
   constexpr int kQueries = 128;  // of a workgroup
   constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
   static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim>), kBytes)) return MFQ_ELAUNCH;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim, kPadded>), kBytes)) return MFQ_ELAUNCH;
   // packed: a tile that is not full for every sequence at most, and for the rows in front of and behind them
   const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
   if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
-  hipLaunchKernelGGL((attention_kernel<T, kDim>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+  hipLaunchKernelGGL((attention_kernel<T, kDim, kPadded>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+}
+
+template <typename T, int kDim>
+int launch_padded(const AttentionCall& c, hipStream_t stream) {
+  return c.dim < kDim ? launch<T, kDim, true>(c, stream) : launch<T, kDim, false>(c, stream);
 }
 
 template <typename T>
 int launch_dim(const AttentionCall& c, hipStream_t stream) {
-  if (c.dim <= 64) return launch<T, 64>(c, stream);
-  if (c.dim <= 96) return launch<T, 96>(c, stream);
-  if (c.dim <= 128) return launch<T, 128>(c, stream);
-  if (c.dim <= 192) return launch<T, 192>(c, stream);
-  return launch<T, 256>(c, stream);
+  if (c.dim <= 64) return launch_padded<T, 64>(c, stream);
+  if (c.dim <= 96) return launch_padded<T, 96>(c, stream);
+  if (c.dim <= 128) return launch_padded<T, 128>(c, stream);
+  if (c.dim <= 192) return launch_padded<T, 192>(c, stream);
+  return launch_padded<T, 256>(c, stream);
 }
 
 }  // namespace

@@ -75,7 +75,7 @@ constexpr float kProbabilityShift = T::code == MFQ_F16 ? 13.f : 0.f;
 constexpr int kKeys = 64;  // of a step of the first kernel
 
 // kHalves == 2: a workgroup has 64 queries, and two wavefronts the same 32, each one half of every tile's keys, joined in LDS at the end
-template <typename T, int kDim, int kHalves>
+template <typename T, int kDim, bool kPadded, int kHalves>
 __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(AttentionCall c, int tiles) {
   constexpr int kQueries = 128 / kHalves;
   constexpr int kPitch = pitch_of(kDim), kSteps = kDim / 16, kBlocks = kDim / 32;
@@ -125,7 +125,8 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
     const float lse = c.lse[head * rows + (int64_t)run.batch * c.q_tokens + inside];
     const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
     const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
-    TileLoader<kPitch, kKeys, 256> load_k, load_v;
+    TileLoader<kPitch, kKeys, 256, kPadded> load_k;
+    TileLoader<kPitch, kKeys, 256> load_v;
     load_k.init(thread, c.k.token, c.dim);
     load_v.init(thread, c.v.token, c.dim);
     const uint32_t lds_at = (uint32_t)(uintptr_t)lds;
@@ -179,6 +180,10 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_dq_kernel(
       }
       return not_finite;
     };
+    if constexpr (kPadded) {
+      clear_padding<kPitch, kDim>(lds, kKeys, c.dim, thread, 256);
+      clear_padding<kPitch, kDim>(lds + 2 * kTileBytes, kKeys, c.dim, thread, 256);
+    }
     load_k.load(k, lds_at, keys, thread);
     load_v.load(v, lds_at + kTileBytes, keys, thread);
     auto advance = [&](int first, int buffer) __attribute__((always_inline)) {
@@ -461,11 +466,7 @@ __global__ __launch_bounds__(64 * KeyShape<kDim>::kWaves, KeyShape<kDim>::kWaves
     if (c.dim < kDim) {
       // both operands of the first products come out of LDS, where the pieces past the head's end repeat its last: one side has to be zero
       arrive_and_sync();
-      const int from_piece = c.dim / 8, pieces = kDim / 8 - from_piece;
-      for (int n = thread; n < S::kV / (kPitch * 2) * pieces; n += 64 * S::kWaves) {
-        const int r = n / pieces, piece = from_piece + n % pieces;  // K's tile lies 128 rows behind V's
-        *reinterpret_cast<u32x4a*>(lds + r * kPitch * 2 + 16 * (piece ^ swizzle<kPitch>(r))) = u32x4a{0u, 0u, 0u, 0u};
-      }
+      clear_padding<kPitch, kDim>(lds, S::kV / (kPitch * 2), c.dim, thread, 64 * S::kWaves);  // K's tile lies 128 rows behind V's
     }
     int i = 0;
     for (; i + 2 <= heads * whole; i += 2) {
@@ -592,14 +593,14 @@ int64_t key_tiles(const AttentionCall& c) {
 }
 int64_t key_values(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : c.batch) * c.k_tokens * c.kv_heads * c.dim; }
 
-template <typename T, int kDim, int kHalves>
+template <typename T, int kDim, bool kPadded, int kHalves>
 int launch_dq(const AttentionCall& c, hipStream_t stream) {
   constexpr int kQueries = 128 / kHalves, kBytes = 4 * kKeys * pitch_of(kDim) * 2;
   static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dq_kernel<T, kDim, kHalves>), kBytes)) return MFQ_ELAUNCH;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dq_kernel<T, kDim, kPadded, kHalves>), kBytes)) return MFQ_ELAUNCH;
   const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
   if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
-  hipLaunchKernelGGL((attention_dq_kernel<T, kDim, kHalves>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
+  hipLaunchKernelGGL((attention_dq_kernel<T, kDim, kPadded, kHalves>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
@@ -611,8 +612,11 @@ int launch(const AttentionCall& c, int parts, float* workspace, hipStream_t stre
   const int64_t groups = (c.q_offsets ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
   const bool halves = 2 * groups <= (c.causal ? 4 : 1) * (int64_t)compute_units();
   int rc;
-  if constexpr (kDim <= 128) rc = halves ? launch_dq<T, kDim, 2>(c, stream) : launch_dq<T, kDim, 1>(c, stream);
-  else rc = launch_dq<T, kDim, 1>(c, stream);
+  if constexpr (kDim <= 128)
+    rc = c.dim < kDim ? (halves ? launch_dq<T, kDim, true, 2>(c, stream) : launch_dq<T, kDim, true, 1>(c, stream))
+                      : (halves ? launch_dq<T, kDim, false, 2>(c, stream) : launch_dq<T, kDim, false, 1>(c, stream));
+  else
+    rc = c.dim < kDim ? launch_dq<T, kDim, true, 1>(c, stream) : launch_dq<T, kDim, false, 1>(c, stream);
   if (rc != MFQ_OK) return rc;
   if (!c.dk && !c.dv) return MFQ_OK;
   using S = KeyShape<kDim>;

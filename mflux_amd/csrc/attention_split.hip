@@ -34,7 +34,7 @@ struct SplitShape {
   static_assert(kPart <= kRing, "a wavefront's result fits its ring");
 };
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kPadded>
 __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void attention_split_kernel(AttentionCall c, int splits, int least_chunk, float* part_o,
                                                                                  float2* part_stats) {
   using S = SplitShape<T, kDim>;
@@ -60,7 +60,8 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
     state.load_row(state.q, c.q.p + q_at, c.dim, lane);
     const uint16_t* k = uniform(c.k.p + run.batch * c.k.batch + (int64_t)run.k0 * c.k.token + kv_head * c.k.head);
     const uint16_t* v = uniform(c.v.p + run.batch * c.v.batch + (int64_t)run.k0 * c.v.token + kv_head * c.v.head);
-    TileLoader<kPitch, kStep, 64> load_k, load_v;
+    TileLoader<kPitch, kStep, 64, kPadded> load_k;
+    TileLoader<kPitch, kStep, 64> load_v;
     load_k.init(lane, c.k.token, c.dim);
     load_v.init(lane, c.v.token, c.dim);
     const uint32_t ring_at = (uint32_t)(uintptr_t)lds + wave * S::kRing;
@@ -121,6 +122,7 @@ __global__ __launch_bounds__(64 * waves_of(kDim), kDim <= 128 ? 2 : 1) void atte
         state.load_row(state.q, c.q.p + at, c.dim, own);
       }
     };
+    if constexpr (kPadded) clear_padding<kPitch, kDim>(lds + wave * S::kRing, kStep, c.dim, lane, kWave);
     start();
 #pragma unroll 1
     while (first < end && first + kStep <= least) tile(std::integral_constant<int, kWhole>());
@@ -259,16 +261,16 @@ int64_t tiles_of(const AttentionCall& c) {
   return c.q_offsets ? c.q_tokens * group / kRows + c.batch + 2 : (c.q_tokens * group + kRows - 1) / kRows * c.batch;
 }
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kPadded>
 int launch(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
   using S = SplitShape<T, kDim>;
   static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_split_kernel<T, kDim>), S::kLds)) return MFQ_ELAUNCH;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_split_kernel<T, kDim, kPadded>), S::kLds)) return MFQ_ELAUNCH;
   const int64_t tiles = tiles_of(c), rows = rows_of(c), grid = tiles * c.kv_heads * splits;
   if (grid > INT32_MAX) return MFQ_ESHAPE;
   float* part_o = workspace;
   float2* part_stats = splits > 1 ? reinterpret_cast<float2*>(workspace + splits * rows * c.heads * c.dim) : nullptr;
-  hipLaunchKernelGGL((attention_split_kernel<T, kDim>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, splits,
+  hipLaunchKernelGGL((attention_split_kernel<T, kDim, kPadded>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, splits,
                      least_chunk(c, splits), part_o, part_stats);
   if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
   if (splits == 1) return MFQ_OK;
@@ -276,13 +278,18 @@ int launch(const AttentionCall& c, int splits, float* workspace, hipStream_t str
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
+template <typename T, int kDim>
+int launch_padded(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
+  return c.dim < kDim ? launch<T, kDim, true>(c, splits, workspace, stream) : launch<T, kDim, false>(c, splits, workspace, stream);
+}
+
 template <typename T>
 int launch_dim(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
-  if (c.dim <= 64) return launch<T, 64>(c, splits, workspace, stream);
-  if (c.dim <= 96) return launch<T, 96>(c, splits, workspace, stream);
-  if (c.dim <= 128) return launch<T, 128>(c, splits, workspace, stream);
-  if (c.dim <= 192) return launch<T, 192>(c, splits, workspace, stream);
-  return launch<T, 256>(c, splits, workspace, stream);
+  if (c.dim <= 64) return launch_padded<T, 64>(c, splits, workspace, stream);
+  if (c.dim <= 96) return launch_padded<T, 96>(c, splits, workspace, stream);
+  if (c.dim <= 128) return launch_padded<T, 128>(c, splits, workspace, stream);
+  if (c.dim <= 192) return launch_padded<T, 192>(c, splits, workspace, stream);
+  return launch_padded<T, 256>(c, splits, workspace, stream);
 }
 
 }  // namespace

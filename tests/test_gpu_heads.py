@@ -392,6 +392,33 @@ def test_attention_scores_of_minus_infinity(queries, H, nk, form, causal, D):
         assert bool(y[0].isnan().all())
 
 
+@pytest.mark.parametrize("D", [8, 24, 64, 72, 80, 96, 104, 128, 136, 184, 192, 200, 248, 256])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("queries,H,nk,form", [(33, 2, 230, 1), (1, 2, 4000, 2), (140, 270, 331, 0)])
+def test_attention_key_of_minus_infinity(queries, H, nk, form, dtype, D):
+    """A visible key that ends with -infinity under positive queries weighs nothing, at sizes of a head that fill the kernels' tiles and
+    that do not: the others' result and gradients are those of the keys without it (dq but in its own channel, where 0 times it is NaN)."""
+    import mflux_amd
+
+    at, some = 100, sorted({0, H - 1})
+    q, k, v = (randn(i, 1, n, H, D, dtype=dtype) for i, n in ((1, queries), (2, nk), (3, nk)))
+    dy = randn(4, 1, queries, H, D, dtype=dtype)
+    q[..., -1] = q[..., -1].abs() + 0.5
+    k[0, at, :, -1] = -math.inf
+    assert min(ranges(q, k), 2) == form
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = mflux_amd.attention(*leaves)
+    got = dict(zip(("y", "dq", "dk", "dv"), (y, *torch.autograd.grad(y, leaves, dy))))
+    got = {name: t.detach()[0][:, some] for name, t in got.items()}
+    keep = torch.arange(nk, device="cuda") != at
+    want = ref.attention_sequence(q[0][:, some], k[0, keep][:, some], v[0, keep][:, some], False, D ** -0.5, dy[0][:, some])
+    ref.check("y", got["y"], *want["y"])
+    ref.check("dq", got["dq"][..., :-1], want["dq"][0][..., :-1], want["dq"][1][..., :-1])
+    for name in ("dk", "dv"):
+        ref.check(name, got[name][keep], *want[name])
+        assert bool((got[name][at] == 0).all())
+
+
 @pytest.mark.parametrize("D", [64, 128, 192, 256])
 @pytest.mark.parametrize("gap", [10.0, 15.0, 17.0, 18.0, 20.0, 22.0])
 @pytest.mark.parametrize("queries,H,n", [(1, 1, 8192), (32, 2, 3000), (128, 260, 4097)])
