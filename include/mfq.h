@@ -508,7 +508,8 @@ int mfq_low_rank_up(const void* x, const void* tf, int dtype, int64_t M, int64_t
 /*
  * Rotary tables: cos[i][p] = factor * cos(positions[i][axis[p]] * frequencies[p]), sin the same, evaluated in
  * float64 and rounded once.  positions [n, axes] int32; frequencies and axis: `pairs` values each, HOST
- * pointers, read before the call returns; cos, sin [n, pairs] float32.  At most MFQ_ROTARY_MAX_PAIRS pairs.
+ * pointers, read before the call returns; cos, sin [n, pairs] float32.  At most MFQ_ROTARY_MAX_PAIRS pairs, frequencies
+ * of a magnitude up to 4 (angles are reduced exactly enough up to 2^33), a finite factor.
  */
 #define MFQ_ROTARY_MAX_PAIRS 256
 int mfq_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, const double* frequencies,

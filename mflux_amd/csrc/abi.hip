@@ -4,6 +4,9 @@
 #include "attention.h"
 #include "common.h"
 
+#include <cmath>
+#include <limits>
+
 namespace {
 
 int check_common(int gs, int bits) {
@@ -455,8 +458,9 @@ int mfq_rotary_tables(const int32_t* positions, int64_t n, int axes, int pairs, 
   if (n <= 0 || axes <= 0 || axes > 255 || pairs <= 0 || pairs > MFQ_ROTARY_MAX_PAIRS || n > ((int64_t)1 << 31)) return MFQ_ESHAPE;
   if (n * pairs > ((int64_t)1 << 38)) return MFQ_ESHAPE;
   if (!positions || !frequencies || !axis || !cos || !sin) return MFQ_ENULL;
+  if (!(std::fabs(factor) <= std::numeric_limits<float>::max())) return MFQ_ESHAPE;
   for (int i = 0; i < pairs; ++i)
-    if (axis[i] >= axes) return MFQ_ESHAPE;
+    if (axis[i] >= axes || !(std::fabs(frequencies[i]) <= 4.0)) return MFQ_ESHAPE;
   return mfq::launch_rotary_tables(positions, n, axes, pairs, frequencies, axis, factor, cos, sin, (hipStream_t)stream);
 }
 

@@ -318,7 +318,7 @@ struct Frequencies {
   uint8_t axis[MFQ_ROTARY_MAX_PAIRS];
 };
 
-// Sine and cosine of an angle of up to 2^33 in float64, times a factor and rounded once: less the nearest multiple of pi / 2 (whose
+// Sine and cosine of an angle of up to 2^33 (a position times a frequency of up to 4) in float64, times a factor and rounded once: less the nearest multiple of pi / 2 (whose
 // second half makes up for the first's rounding, the products being exact in an fma), then the series in up to |r| = pi / 4, cut where
 // the next term is below 2^-33.  The multiple is rounded by adding 1.5 * 2^52, which leaves it in the sum's low bits.
 __device__ inline void sine_cosine(double angle, double factor, float& s, float& c) {

@@ -41,6 +41,9 @@ _SCALINGS = {"linear": (1, {"type", "factor"}), "ntk": (2, {"type", "factor"}),
              "yarn": (3, {"type", "factor", "original_length", "beta_fast", "beta_slow", "attention_factor"})}
 
 
+_FLOAT32_MAX = torch.finfo(torch.float32).max
+
+
 def _number(value) -> bool:
     return isinstance(value, (int, float)) and not isinstance(value, bool) and math.isfinite(value)
 
@@ -70,8 +73,8 @@ def _scaling(scaling: dict | None, base: float, dims: tuple[int, ...]) -> tuple:
     tables = scaling.get("attention_factor")
     if tables is None:
         tables = 0.1 * math.log(factor) + 1.0
-    elif not _number(tables):
-        raise ValueError(f"[rotary_tables] attention_factor must be a number, got {tables!r}")
+    elif not _number(tables) or abs(tables) > _FLOAT32_MAX:
+        raise ValueError(f"[rotary_tables] attention_factor must be a number that float32 holds, got {tables!r}")
     return code, factor, length, fast, slow, tables
 
 
@@ -92,7 +95,7 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
     than ``beta_fast`` times, and multiplies the tables by ``0.1 ln f + 1``.
 
     Angles are taken in float64: a float32 product is off by thousandths at far
-    positions."""
+    positions.  ``base`` is such that a position adds at most 4 to an angle (any from 0.25 on)."""
     fn = "rotary_tables"
     if not isinstance(positions, torch.Tensor) or positions.ndim not in (1, 2):
         raise ValueError(f"[{fn}] positions must be a tensor [S] or [S, A]")
@@ -108,6 +111,8 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
         raise ValueError(f"[{fn}] at most 512 channels turn, got {sum(axes)}")
     if not _number(base) or base <= 0:
         raise ValueError(f"[{fn}] base must be positive, got {base!r}")
+    if base < 0.25 and any((1 - 2 / d) * -math.log(base) > math.log(4) for d in axes):
+        raise ValueError(f"[{fn}] base is too small: a position may add at most 4 to an angle, got {base!r}")
     arguments = _scaling(scaling, base, axes)
     positions = _integers(fn, "positions", positions, positions.device)
     _require_hip(fn, positions, "positions")

@@ -53,6 +53,19 @@ def test_tables(positions, dims, base, scaling):
     assert torch.equal(cos, mflux_amd.rotary_tables(p.long(), dims, base, scaling)[0])
 
 
+@pytest.mark.parametrize("base", [0.25, 0.5, 1.0])
+def test_tables_of_small_bases(base):
+    """Up to what is allowed: angles of almost 2^33."""
+    import mflux_amd
+
+    p = ints([2 ** 31 - 1, -2 ** 31, 1000003, -7, 0])
+    cos, sin = mflux_amd.rotary_tables(p, 64, base)
+    angle = p[:, None].double() * torch.tensor(ref.rotary_frequencies(64, base, None)[0], dtype=torch.float64, device="cuda")
+    for got, want in ((cos, angle.cos()), (sin, angle.sin())):
+        err = (got.double() - want).abs()
+        assert bool((err <= 2.0 ** -24 * want.abs() * 1.01 + angle.abs() * 2.0 ** -50).all()), float(err.max())
+
+
 # ---- rotary ------------------------------------------------------------------------------------------------------------
 
 ROTARY = [  # B, S, H, Hkv (0: no k), D, R

@@ -243,3 +243,24 @@ def test_every_attention_kernel_raises_its_own_limit():
     if not names:
         pytest.skip("a library without symbols")
     assert len(kernels) >= 40 and len(flags) == len(kernels)
+
+
+@pytest.mark.parametrize("base,dims", [(0.2, 64), (1e-12, 4), (5e-324, 128), (0.01, (2, 8))])
+def test_tables_refuse_angles_that_grow_too_fast(base, dims):
+    """Above 4 a position an angle leaves the range that its reduction holds for."""
+    positions = ints(1) if isinstance(dims, int) else ints(1, 2)[None]
+    with pytest.raises(ValueError, match="base is too small"):
+        mflux_amd.rotary_tables(positions, dims, base)
+    for base, dims in ((0.25, 64), (0.1, 2), (0.2, 4)):  # these go on to the next refusal
+        with pytest.raises(RuntimeError, match="HIP device"):
+            mflux_amd.rotary_tables(ints(1), dims, base)
+    with pytest.raises(ValueError, match="attention_factor"):
+        mflux_amd.rotary_tables(ints(1), 64, scaling={"type": "yarn", "factor": 2.0, "original_length": 100, "attention_factor": 1e39})
+
+
+def test_tables_abi_refuses_what_cannot_be_reduced():
+    lib = _lib.load()
+    axis = (ctypes.c_uint8 * 2)()
+    for frequency, factor in ((4.1, 1.0), (-4.1, 1.0), (float("nan"), 1.0), (float("inf"), 1.0), (1.0, float("inf")), (1.0, float("nan"))):
+        f = (ctypes.c_double * 2)(1.0, frequency)
+        assert lib.mfq_rotary_tables(AT, 1, 1, 2, f, axis, factor, AT, AT, None) == E["shape"]
