@@ -85,7 +85,8 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
     ``positions``: integers ``[S]`` with ``dims`` the number of channels that turn, or
     ``[S, A]`` with one such number for each of ``A`` axes, whose pairs lie side by
     side (an image token's id, row and column in the DiT blocks: ``(16, 56, 56)``).
-    Negative positions are fine.  At most 512 channels in all.
+    Negative positions are fine; int64 ones count as the nearest that int32 holds (the
+    device is not waited for to look at them).  At most 512 channels in all.
 
     ``scaling`` stretches the angles for contexts longer than a model was trained
     on: ``{"type": "linear", "factor": f}`` divides positions, ``"ntk"`` raises the base so

@@ -66,6 +66,15 @@ def test_tables_of_small_bases(base):
         assert bool((err <= 2.0 ** -24 * want.abs() * 1.01 + angle.abs() * 2.0 ** -50).all()), float(err.max())
 
 
+def test_tables_of_positions_beyond_int32():
+    """As documented: the nearest position that int32 holds."""
+    import mflux_amd
+
+    far = torch.tensor([2 ** 31, 2 ** 40, -2 ** 31 - 1, -2 ** 63, 5], dtype=torch.int64, device="cuda")
+    near = ints([2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, -2 ** 31, 5])
+    assert all(torch.equal(a, b) for a, b in zip(mflux_amd.rotary_tables(far, 64), mflux_amd.rotary_tables(near, 64)))
+
+
 # ---- rotary ------------------------------------------------------------------------------------------------------------
 
 ROTARY = [  # B, S, H, Hkv (0: no k), D, R
