@@ -184,7 +184,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torc
         if t is not None and t.device != q.device:
             raise ValueError(f"[{fn}] `{name}` lives on {t.device}, q on {q.device}")
     if positions is not None:
-        positions = _integers(fn, "positions", positions, q.device).reshape(-1, tokens)
+        positions = _integers(fn, "positions", positions, q.device)
+        positions = positions[None] if positions.ndim == 1 else positions
     _require_hip(fn, q, "q")
     packed = q.ndim == 3
     if packed:

@@ -168,6 +168,18 @@ def test_rotary_empty_and_partial_gradients():
     ref.check("dk", dk, *ref.rms_norm_rotary(k.detach(), cos[None], sin[None], "interleaved", None, 0.0, torch.ones_like(k))[1])
 
 
+@pytest.mark.parametrize("shape", [(0,), (1, 0), (2, 0)])
+def test_rotary_of_no_tokens_with_positions(shape):
+    import mflux_amd
+
+    cos, sin = randn(1, 4, 4).cos(), randn(1, 4, 4).sin()
+    q = torch.empty(2, 0, 2, 16, device="cuda", dtype=BF16, requires_grad=True)
+    y, k = mflux_amd.rotary(q, q, cos, sin, positions=torch.empty(shape, device="cuda", dtype=torch.int64))
+    assert y.shape == k.shape == q.shape and torch.autograd.grad(y, q, torch.empty_like(y))[0].shape == q.shape
+    packed = mflux_amd.rotary(q[0], None, cos, sin, positions=torch.empty(0, device="cuda", dtype=torch.int32))
+    assert packed.shape == q[0].shape
+
+
 def test_rotary_turns_back():
     """The gradient of a turn is the turn back: applied to the result it gives the input, to rounding."""
     import mflux_amd

@@ -264,3 +264,9 @@ def test_tables_abi_refuses_what_cannot_be_reduced():
     for frequency, factor in ((4.1, 1.0), (-4.1, 1.0), (float("nan"), 1.0), (float("inf"), 1.0), (1.0, float("inf")), (1.0, float("nan"))):
         f = (ctypes.c_double * 2)(1.0, frequency)
         assert lib.mfq_rotary_tables(AT, 1, 1, 2, f, axis, factor, AT, AT, None) == E["shape"]
+
+
+@pytest.mark.parametrize("shape", [(0,), (1, 0), (2, 0)])
+def test_rotary_of_no_tokens_takes_positions(shape):
+    with pytest.raises(RuntimeError, match="HIP device"):  # nothing else is wrong with the call
+        mflux_amd.rotary(z(2, 0, 4, 64), None, T, T, positions=z(*shape, dtype=torch.int32))
