@@ -478,7 +478,10 @@ static int check_rotary(const mfq_rotary_args* a, bool backward, bool* wide) {
   const int64_t per16 = a->dtype == MFQ_F32 ? 4 : 8;
   *wide = mfq::aligned16(a->cos) && mfq::aligned16(a->sin);
   for (const mfq_rotary_tensor* t : {&a->q, &a->k}) {
-    if (!t->heads) continue;
+    if (!t->heads) {
+      if (backward && t->dweight) return MFQ_ESHAPE;  // no rows to sum over
+      continue;
+    }
     if ((!backward || t->weight) && !t->x) return MFQ_ENULL;
     if (!backward && !t->out) return MFQ_ENULL;
     if (backward && !t->dy) return MFQ_ENULL;

@@ -270,3 +270,11 @@ def test_tables_abi_refuses_what_cannot_be_reduced():
 def test_rotary_of_no_tokens_takes_positions(shape):
     with pytest.raises(RuntimeError, match="HIP device"):  # nothing else is wrong with the call
         mflux_amd.rotary(z(2, 0, 4, 64), None, T, T, positions=z(*shape, dtype=torch.int32))
+
+
+def test_rotary_abi_refuses_a_weight_gradient_of_no_heads():
+    """Nothing would write the partial sums that it is made of."""
+    lib = _lib.load()
+    r = rotary_args(k_heads=0)
+    need = lib.mfq_rotary_workspace_bytes(ctypes.byref(r))
+    assert lib.mfq_rotary_backward(ctypes.byref(r), AT, need, None) == E["shape"]
