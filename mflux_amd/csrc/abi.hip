@@ -520,7 +520,7 @@ static int attention_call(const mfq_attention_args* a, bool backward, mfq::Atten
   if (a->dim <= 0 || a->dim > 256 || a->dim % 8) return MFQ_ESHAPE;
   if (a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->heads > 65536) return MFQ_ESHAPE;
   if (a->batch <= 0 || a->q_tokens <= 0 || a->k_tokens <= 0 || a->batch > (1 << 24)) return MFQ_ESHAPE;
-  if (a->q_tokens * a->heads > (1 << 30) || a->k_tokens > (1 << 30) || a->q_tokens > (1 << 30)) return MFQ_ESHAPE;
+  if (a->q_tokens > (1 << 30) || a->k_tokens > (1 << 30) || a->q_tokens * a->heads > (1 << 30)) return MFQ_ESHAPE;
   if (!(a->scale > 0.f) || a->scale > 1e30f) return MFQ_ESHAPE;
   if ((a->q_offsets == nullptr) != (a->k_offsets == nullptr)) return MFQ_ENULL;
   if (a->q_offsets && (a->q_lengths || a->k_lengths)) return MFQ_EUNSUPPORTED;

@@ -679,6 +679,9 @@ __device__ inline void store_row(uint16_t* row, uint16_t* rest, const f32x16 (&o
     }
 }
 
+// whether a launch may have so many workgroups: fewer than 2^32 threads in all
+inline bool launches(int64_t groups, int threads) { return groups <= UINT32_MAX / threads; }
+
 int launch_attention(int dtype, const AttentionCall& c, hipStream_t stream);
 // few queries against many keys: into how many ranges the key axis is cut, 0 where launch_attention is the faster
 int attention_splits(const AttentionCall& c);

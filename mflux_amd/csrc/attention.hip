@@ -176,11 +176,11 @@ template <typename T, int kDim, bool kPadded>
 int launch(const AttentionCall& c, hipStream_t stream) {
   constexpr int kQueries = 128;  // of a workgroup
   constexpr int kBytes = 4 * kKeys * pitch_of(kDim) * 2;
-  static PerDeviceInt configured;
-  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim, kPadded>), kBytes)) return MFQ_ELAUNCH;
   // packed: a tile that is not full for every sequence at most, and for the rows in front of and behind them
   const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
-  if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
+  if (!launches(tiles * c.heads, 256)) return MFQ_ESHAPE;
+  static PerDeviceInt configured;
+  if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_kernel<T, kDim, kPadded>), kBytes)) return MFQ_ELAUNCH;
   hipLaunchKernelGGL((attention_kernel<T, kDim, kPadded>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }

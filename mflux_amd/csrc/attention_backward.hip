@@ -596,16 +596,19 @@ int64_t key_values(const AttentionCall& c) { return (int64_t)(c.q_offsets ? 1 : 
 template <typename T, int kDim, bool kPadded, int kHalves>
 int launch_dq(const AttentionCall& c, hipStream_t stream) {
   constexpr int kQueries = 128 / kHalves, kBytes = 4 * kKeys * pitch_of(kDim) * 2;
+  const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
+  if (!launches(tiles * c.heads, 256)) return MFQ_ESHAPE;
   static PerDeviceInt configured;
   if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dq_kernel<T, kDim, kPadded, kHalves>), kBytes)) return MFQ_ELAUNCH;
-  const int64_t tiles = c.q_offsets ? (int64_t)c.q_tokens / kQueries + c.batch + 2 : (int64_t)((c.q_tokens + kQueries - 1) / kQueries) * c.batch;
-  if (tiles * c.heads > INT32_MAX) return MFQ_ESHAPE;
   hipLaunchKernelGGL((attention_dq_kernel<T, kDim, kPadded, kHalves>), dim3((unsigned)(tiles * c.heads)), dim3(256), kBytes, stream, c, (int)tiles);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
 template <typename T, int kDim>
 int launch(const AttentionCall& c, int parts, float* workspace, hipStream_t stream) {
+  using S = KeyShape<kDim>;
+  const int64_t tiles = key_tiles(c), n = key_values(c);
+  if ((c.dk || c.dv) && !launches(tiles * c.kv_heads * parts, 64 * S::kWaves)) return MFQ_ESHAPE;
   // 64 queries to a workgroup where 128 leave compute units idle, or (causal) the longest of them working alone: causal heads of 128,
   // 2048 tokens x 8 heads (128 such workgroups) 49 against 60 us, 4096 x 16 (512) 131 and 156, 4608 x 24 (864) 242 and 220; not causal,
   // 1500 x 24 (288) 90 and 71, 2048 x 24 (384) 93 and 89.
@@ -619,11 +622,8 @@ int launch(const AttentionCall& c, int parts, float* workspace, hipStream_t stre
     rc = c.dim < kDim ? launch_dq<T, kDim, true, 1>(c, stream) : launch_dq<T, kDim, false, 1>(c, stream);
   if (rc != MFQ_OK) return rc;
   if (!c.dk && !c.dv) return MFQ_OK;
-  using S = KeyShape<kDim>;
   static PerDeviceInt configured;
   if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_dkv_kernel<T, kDim>), S::kLds)) return MFQ_ELAUNCH;
-  const int64_t tiles = key_tiles(c), n = key_values(c);
-  if (tiles * c.kv_heads * parts > INT32_MAX) return MFQ_ESHAPE;
   float* part_v = parts > 1 ? workspace + parts * n : nullptr;
   hipLaunchKernelGGL((attention_dkv_kernel<T, kDim>), dim3((unsigned)(tiles * c.kv_heads * parts)), dim3(64 * S::kWaves), S::kLds, stream, c,
                      (int)tiles, parts, workspace, part_v);

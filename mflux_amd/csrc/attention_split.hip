@@ -264,10 +264,10 @@ int64_t tiles_of(const AttentionCall& c) {
 template <typename T, int kDim, bool kPadded>
 int launch(const AttentionCall& c, int splits, float* workspace, hipStream_t stream) {
   using S = SplitShape<T, kDim>;
+  const int64_t tiles = tiles_of(c), rows = rows_of(c), grid = tiles * c.kv_heads * splits;
+  if (!launches(grid, 64 * S::kWaves)) return MFQ_ESHAPE;
   static PerDeviceInt configured;
   if (!raise_lds_limit(configured, reinterpret_cast<const void*>(&attention_split_kernel<T, kDim, kPadded>), S::kLds)) return MFQ_ELAUNCH;
-  const int64_t tiles = tiles_of(c), rows = rows_of(c), grid = tiles * c.kv_heads * splits;
-  if (grid > INT32_MAX) return MFQ_ESHAPE;
   float* part_o = workspace;
   float2* part_stats = splits > 1 ? reinterpret_cast<float2*>(workspace + splits * rows * c.heads * c.dim) : nullptr;
   hipLaunchKernelGGL((attention_split_kernel<T, kDim, kPadded>), dim3((unsigned)grid), dim3(64 * S::kWaves), S::kLds, stream, c, splits,

@@ -278,3 +278,14 @@ def test_rotary_abi_refuses_a_weight_gradient_of_no_heads():
     r = rotary_args(k_heads=0)
     need = lib.mfq_rotary_workspace_bytes(ctypes.byref(r))
     assert lib.mfq_rotary_backward(ctypes.byref(r), AT, need, None) == E["shape"]
+
+
+@pytest.mark.parametrize("sizes", [dict(batch=1 << 24, heads=2, kv_heads=2, q_tokens=1, k_tokens=1),       # rows of single tokens
+                                   dict(batch=1 << 17, heads=256, kv_heads=256, q_tokens=128, k_tokens=1),  # tiles of 128 queries
+                                   dict(batch=1 << 22, heads=4, kv_heads=4, q_tokens=1, k_tokens=129)])
+def test_attention_abi_refuses_more_workgroups_than_a_launch_has(sizes):
+    lib = _lib.load()
+    a = attention_args(**sizes)
+    if sizes["k_tokens"] == 1:
+        assert lib.mfq_attention(ctypes.byref(a), None, 0, None) == E["shape"]
+    assert lib.mfq_attention_backward(ctypes.byref(a), AT, 1 << 62, None) == E["shape"]
