@@ -743,7 +743,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
                                const c10::optional<Tensor>& k_weight, int64_t layout, double eps) {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto [yq, yk] = rotary(q, k, cos, sin, positions, q_weight, k_weight, layout, eps);
-    ctx->save_for_backward({q, or_none(k), cos, sin, or_none(positions), or_none(q_weight), or_none(k_weight)});
+    // without a norm the turn back needs no input: it is neither kept nor held to its values
+    ctx->save_for_backward({q_weight.has_value() ? q : Tensor(), k_weight.has_value() ? or_none(k) : Tensor(), cos, sin, or_none(positions),
+                            or_none(q_weight), or_none(k_weight)});
     ctx->saved_data["layout"] = layout;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["wanted"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(q_weight) << 2 | wanted(k_weight) << 3);
@@ -752,16 +754,20 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list dy) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1];
+    const Tensor& q = saved[0].defined() ? saved[0] : dy[0];  // (for its shape alone)
+    c10::optional<Tensor> k, dyk;
+    if (dy.size() > 1) {
+      dyk = dy[1];
+      k = saved[1].defined() ? saved[1] : dy[1];
+    }
     const int64_t want = ctx->saved_data["wanted"].toInt();
     variable_list out(9);
     std::tuple<Tensor, Tensor, Tensor, Tensor> g;
     {
       at::AutoGradMode off(false);
       at::AutoDispatchBelowADInplaceOrView guard;
-      g = rotary_backward(dy[0], k.defined() ? c10::optional<Tensor>(dy[1]) : c10::nullopt, q, if_defined(k), saved[2], saved[3], if_defined(saved[4]),
-                          if_defined(saved[5]), if_defined(saved[6]), ctx->saved_data["layout"].toInt(), ctx->saved_data["eps"].toDouble(),
-                          want & 3, want & 4, want & 8);
+      g = rotary_backward(dy[0], dyk, q, k, saved[2], saved[3], if_defined(saved[4]), if_defined(saved[5]),
+                          if_defined(saved[6]), ctx->saved_data["layout"].toInt(), ctx->saved_data["eps"].toDouble(), want & 3, want & 4, want & 8);
     }
     if (want & 1) out[0] = std::get<0>(g);
     if (want & 2) out[1] = std::get<1>(g);

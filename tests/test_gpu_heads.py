@@ -168,6 +168,39 @@ def test_rotary_empty_and_partial_gradients():
     ref.check("dk", dk, *ref.rms_norm_rotary(k.detach(), cos[None], sin[None], "interleaved", None, 0.0, torch.ones_like(k))[1])
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rotary_without_a_norm_keeps_no_input(layout):
+    """The turn back needs none: inputs that are overwritten afterwards, as buffers are, leave the gradient what it is.  A tensor
+    with a norm is needed, and says so."""
+    import mflux_amd
+
+    cos, sin = randn(1, 6, 16).cos(), randn(1, 6, 16).sin()
+    q, k = randn(2, 2, 6, 3, 32, dtype=BF16).requires_grad_(), randn(3, 2, 6, 1, 32, dtype=BF16).requires_grad_()
+    w, dy = randn(4, 32, dtype=BF16), (randn(5, 2, 6, 3, 32, dtype=BF16), randn(6, 2, 6, 1, 32, dtype=BF16))
+    want = {}
+    for weights in ({}, {"q_weight": w}, {"k_weight": w}):
+        for overwritten in (None, "q", "k"):
+            a, b = q * 1, k * 1
+            out = mflux_amd.rotary(a, b, cos, sin, layout=layout, **weights)
+            if overwritten:
+                (a if overwritten == "q" else b).detach().zero_()
+            key = tuple(weights)
+            if overwritten and overwritten + "_weight" in weights:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(out, (q, k), dy)
+                continue
+            got = torch.autograd.grad(out, (q, k), dy)
+            assert all(torch.equal(x, y) for x, y in zip(got, want.setdefault(key, got)))
+    # half of the gradients, transposed ones, and one tensor alone
+    a = q * 1
+    y = mflux_amd.rotary(a, None, cos, sin, layout=layout)
+    got, = torch.autograd.grad(y, q, dy[0].transpose(1, 2).contiguous().transpose(1, 2))
+    assert torch.equal(got, want[()][0])
+    a, b = q * 1, k.detach()
+    out = mflux_amd.rotary(a, b, cos, sin, layout=layout)
+    assert torch.equal(torch.autograd.grad(out[0], q, dy[0])[0], want[()][0])
+
+
 @pytest.mark.parametrize("shape", [(0,), (1, 0), (2, 0)])
 def test_rotary_of_no_tokens_with_positions(shape):
     import mflux_amd
