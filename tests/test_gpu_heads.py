@@ -654,6 +654,46 @@ def test_attention_strides(queries):
         assert float((g - g2.float().sum(0, keepdim=True)).abs().max()) <= 2.0 ** -7 * float(g2.float().abs().sum(0).max())
 
 
+def test_attention_of_a_cache_allocated_far_beyond_its_keys():
+    """Lengths of an eighth to a thousandth of the keys that there is room for, and none; what lies behind them is NaN."""
+    import mflux_amd
+
+    nk, lengths = 20000, [2500, 1, 0, 19, 160]
+    q, k, v = randn(1, 5, 1, 8, 128, dtype=BF16), randn(2, 5, nk, 2, 128, dtype=BF16), randn(3, 5, nk, 2, 128, dtype=BF16)
+    for i, n in enumerate(lengths):
+        k[i, n:], v[i, n:] = math.nan, math.nan
+    assert ranges(q, k) > 1
+    y = mflux_amd.attention(q, k, v, causal=True, k_lengths=ints(lengths))
+    for i, n in enumerate(lengths):
+        ref.check("y", y[i], *ref.attention_sequence(q[i], k[i, :n], v[i, :n], True, 128 ** -0.5)["y"])
+
+
+@pytest.mark.parametrize("strides", [(2 ** 31 + 64, 512, 128), (2 ** 24 * 150, 2 ** 24 - 8, 128)])
+def test_offsets_beyond_32_bits(strides):
+    """Entries and tokens that lie so far apart that elements, or a tile's bytes, pass 2^31: the bits of dense tensors."""
+    import mflux_amd
+
+    n = 140
+    buffer = torch.empty((1 * strides[0] + n * strides[1] + 1024), device="cuda", dtype=BF16)
+    far = [buffer.as_strided((2, n, 2, 128), (*strides, 1), i * 256) for i in range(2)]
+    near = [randn(i, 2, n, 2, 128, dtype=BF16) for i in range(2)]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    q, dy = randn(5, 2, n, 4, 128, dtype=BF16), randn(6, 2, n, 4, 128, dtype=BF16)
+
+    def all_of(k, v):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        y = mflux_amd.attention(*leaves, causal=True)
+        single = mflux_amd.attention(q[:, -1:], k, v)
+        many = mflux_amd.attention(q.repeat(1, 1, 40, 1), k, v)
+        turned = mflux_amd.rotary(k.detach(), v.detach(), cos, sin, layout="half", q_weight=w)
+        return (y, single, many, *turned, *torch.autograd.grad(y, leaves, dy))
+
+    cos, sin, w = randn(7, n, 64).cos(), randn(8, n, 64).sin(), randn(9, 128, dtype=BF16)
+    for a, b in zip(all_of(*far), all_of(*near)):
+        assert torch.equal(a, b)
+
+
 def test_attention_same_bits_every_time():
     import mflux_amd
 
