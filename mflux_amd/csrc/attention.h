@@ -437,7 +437,7 @@ __device__ inline void add_columns_one_by_one(f32x16 (&acc)[kBlocks], const char
 // lag.  float16 ends at 2^16 and loses bits below 2^-14 and everything below 2^-25, so its probabilities are multiples of 2^-kLift, and so is
 // the sum that they are divided by: at most 2^-35 of the largest is lost.  (Without it 8192 keys of weight e^-18 each beside a strong one
 // vanished together.)  A lag of 4 takes the time that one of 8 takes on scores of a standard deviation of 1 (4608 tokens x 24 heads of 128: 286
-// us), and 294 instead of 288 us at 3, where a lag of 1 with another three powers took 309 and 318.
+// us), and 294 instead of 288 us at 3; a lag of 1 and three more powers cost 10 and 18 us.
 template <typename T>
 constexpr float kLag = T::code == MFQ_F16 ? 4.f : 8.f;
 template <typename T>

@@ -8,7 +8,7 @@
 // tiles go straight from memory into LDS (two of each, the next in flight while the current one is multiplied) and are
 // read by all four wavefronts.  Two workgroups share a compute unit.  See attention.h for the orientation of the products.
 //
-// 4608 tokens, 24 heads of 128, bfloat16, calls behind each other: 274 to 282 us on two cards, 0.93 to 0.95 PFLOP/s (a large library product: 1.39); 16384
+// 4608 tokens, 24 heads of 128, bfloat16, calls behind each other: 274 to 284 us on three cards, 0.92 to 0.95 PFLOP/s (a large library product: 1.39); 16384
 // causal tokens, 28 / 4 heads: 1.84 to 1.92 ms, 1.00 to 1.04.  The counters show the matrix units busy in 41 % of the cycles, six vector instructions
 // to a matrix instruction and no bank conflicts; power has a part as well, on zeros the first of these calls takes 227 us.  256 queries to a
 // workgroup, three stages of tiles, 128 keys a step and wavefront priorities were tried and were no faster.

@@ -7,8 +7,8 @@
 // as P is in the forward pass.  sum(dy y) is taken from y and what its rounding left: with the roundings of bfloat16 put into a
 // 64-bit calculation (1024 causal tokens, D = 128) dq is off by 2.6 10^-3 of its norm from the rounded y, by 2.4 from this one.
 //
-// 4608 tokens, 24 heads of 128: dq 380 us, 1.03 PFLOP/s of its 6 operations a pair and element; dk and dv 572 us, 0.91 of their 8;
-// causal 0.93 and 0.91.  4099 causal tokens in three sequences, 24 / 8 heads: 124 and 186 us, and 19 to join the parts; there the
+// 4608 tokens, 24 heads of 128, bfloat16: dq 374 to 391 us, 1.00 to 1.05 PFLOP/s of its 6 operations a pair and element; dk and dv 572 to
+// 593 us, 0.88 to 0.91 of their 8 (float16: 425 and 636 us); causal 0.91 to 0.93 and 0.88 to 0.91.  4099 causal tokens in three sequences, 24 / 8 heads: 124 and 186 us, and 19 to join the parts; there the
 // counters show the matrix units busy in 28 and 30 % of the cycles.
 #include "attention.h"
 

@@ -302,18 +302,20 @@ int attention_splits(const AttentionCall& c) {
   const int64_t items = std::max<int64_t>(tiles_of(c) - (c.q_offsets ? 2 : 0), 1) * c.kv_heads;
   if (queries * group <= kRows) {
     // Single tokens: eight workgroups for every compute unit, so that sequences of different lengths fill it evenly (32 of them, 1024 to
-    // 8192 keys, 8 key heads: 132, 134, 125, 125 us with one, four, eight, sixteen), each with 256 keys at least; and at most 64
-    // ranges, which the join reads behind each other (one sequence of 100003 keys, 4 key heads: 47, 51, 60 us with 64, 128, 256).
+    // 8192 keys, 8 key heads: 129, 137, 126, 125 us with one, four, eight, sixteen ranges), each with 256 keys at least; and at most 64
+    // ranges, which the join reads behind each other (one sequence of 100003 keys, 4 key heads, from a cache: 39, 43, 50 us with 64, 128, 256).
+    // The keys of a range are counted by the tensor's length where a sequence's own is shorter.
     const int64_t want = (8 * units + items - 1) / items;
     return (int)std::min({std::max<int64_t>(keys / 256, 1), want, (int64_t)64});
   }
   // A prompt whose tiles of 128 queries leave compute units idle: 32 rows to a workgroup, the keys dealt to its wavefronts, is as much
-  // work on four times the units (heads of 128, causal: 1024 tokens x 8 heads 15.8 us here, 24.8 there; 2048 x 8, 128 such tiles, 29.9
-  // and 42.1; 1024 x 24, 192, 26.2 and 26.4; 2048 x 16, 256, 45.9 and 43.0).
+  // work on four times the units (heads of 128, causal: 1024 tokens x 8 heads 15.1 us here, 25.3 there; 2048 x 8, 128 such tiles, 28.2
+  // and 42.4; 1024 x 24, 192, 25.0 and 26.8).  The limit is one for all calls and lies between theirs: at 256 tiles (2048 x 16, causal) heads of
+  // 64 take 25.7 and 32.0, of 128 42.0 and 43.6, of 256 114 and 99; without a mask 2048 x 8 heads of 128 take 31.0 and 40.6, 1024 x 24 29.2 and 25.1.
   const int64_t tiles = (c.q_offsets ? c.q_tokens / 128 + c.batch : (int64_t)((c.q_tokens + 127) / 128) * c.batch) * c.heads;
   if (4 * tiles > 3 * units) return 0;
-  // and the keys in ranges where even those are few (128 queries x 8 heads against 32768 keys: 350, 97, 57, 49, 82 us with 1, 4, 8, 16
-  // and 32; 128 against 4096: 43, 19, 15, 16, 25), but not where the join has as many rows again (1024 x 8: 15.8 us with 1, 25.7 with 2)
+  // and the keys in ranges where even those are few (128 queries x 8 heads against 32768 keys: 301, 86, 50, 43, 79 us with 1, 4, 8, 16
+  // and 32; 128 against 4096: 37, 18, 15, 16, 23), but not where the join has as many rows again (1024 x 8: 14.3 us with 1, 24 with 2)
   if (2 * items > units) return 1;
   return (int)std::max<int64_t>(std::min({keys / 512, 2 * units / items, (int64_t)64}), 1);
 }
