@@ -563,7 +563,8 @@ int mfq_rotary_backward(const mfq_rotary_args* args, void* workspace, size_t wor
  * Both are device memory: values outside the tensors are clamped to them (decreasing offsets give
  * unspecified values, never an access outside the arrays).
  * causal: query i of n sees the keys up to i + m - n of m.  A query that sees no key, and every row that no
- * sequence holds, gets zeros.  What a query does not see does not reach it, infinities and NaN included.
+ * sequence holds, gets zeros.  What a query does not see does not reach it, infinities and NaN included; a query
+ * whose visible scores are all -infinity gets NaN.
  * One call has fewer than 2^24 tiles (of 128 queries or keys, at least one an entry) times heads; backward 2^23.
  * Softmax and sums in float32, the probabilities rounded to dtype for the second product.  scale > 0.
  *   lse    [heads, rows] float32, rows = q_tokens or batch * q_tokens: written by the forward pass if not NULL,

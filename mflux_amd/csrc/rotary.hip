@@ -318,9 +318,9 @@ struct Frequencies {
   uint8_t axis[MFQ_ROTARY_MAX_PAIRS];
 };
 
-// Sine and cosine of an angle of up to 2^33 (a position times a frequency of up to 4) in float64, times a factor and rounded once: less the nearest multiple of pi / 2 (whose
-// second half makes up for the first's rounding, the products being exact in an fma), then the series in up to |r| = pi / 4, cut where
-// the next term is below 2^-33.  The multiple is rounded by adding 1.5 * 2^52, which leaves it in the sum's low bits.
+// Sine and cosine of an angle of up to 2^33 (a position times a frequency of up to 4) in float64, times a factor and rounded once: less
+// the nearest multiple of pi / 2 (whose second half makes up for the first's rounding, the products being exact in an fma), then the
+// series in up to |r| = pi / 4, cut where the next term is below 2^-33.  The multiple is rounded by adding 1.5 * 2^52, which leaves it in the sum's low bits.
 __device__ inline void sine_cosine(double angle, double factor, float& s, float& c) {
   const double shifted = __builtin_fma(angle, 0.63661977236758134308, 6755399441055744.0), quarter = shifted - 6755399441055744.0;
   const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, shifted);

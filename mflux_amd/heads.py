@@ -78,6 +78,12 @@ def _scaling(scaling: dict | None, base: float, dims: tuple[int, ...]) -> tuple:
     return code, factor, length, fast, slow, tables
 
 
+def _fastest(d: int, base: float, kind: int, factor: float) -> float:
+    """The logarithm of the angle that a position adds to the last of ``d / 2`` pairs, the fastest where ``base`` is below 1;
+    'linear' and 'ntk' both divide it."""
+    return -(1 - 2 / d) * math.log(base) - (math.log(factor) if kind in (1, 2) else 0.0)
+
+
 def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: float = 10000.0,
                   scaling: dict | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(cos, sin)`` of the rotary angles of ``positions``, float32 ``[S, R / 2]``.
@@ -112,9 +118,9 @@ def rotary_tables(positions: torch.Tensor, dims: int | tuple[int, ...], base: fl
         raise ValueError(f"[{fn}] at most 512 channels turn, got {sum(axes)}")
     if not _number(base) or base <= 0:
         raise ValueError(f"[{fn}] base must be positive, got {base!r}")
-    if base < 0.25 and any((1 - 2 / d) * -math.log(base) > math.log(4) for d in axes):
-        raise ValueError(f"[{fn}] base is too small: a position may add at most 4 to an angle, got {base!r}")
     arguments = _scaling(scaling, base, axes)
+    if base < 0.25 and any(_fastest(d, base, *arguments[:2]) > math.log(4) for d in axes):
+        raise ValueError(f"[{fn}] base is too small: a position may add at most 4 to an angle, got {base!r}")
     positions = _integers(fn, "positions", positions, positions.device)
     _require_hip(fn, positions, "positions")
     return _lib.ops().rotary_tables(positions.reshape(positions.shape[0], len(axes)), axes, base, *arguments)
@@ -217,7 +223,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     ``causal``: aligned to the last token, query ``i`` of ``n`` sees the first ``i + 1 + m - n`` of ``m`` keys, so one
     query behind a cache sees all of it.  A query that sees no key gets zeros, and so does every
     row that belongs to no sequence (padding; rows behind the last offset), in the result and
-    in the gradients.  What a query does not see never reaches it, infinities and NaN included.
+    in the gradients.  What a query does not see never reaches it, infinities and NaN included; one whose
+    visible scores are all ``-inf`` has no softmax and gets NaN.
 
     Statistics and sums are float32; the probabilities (and in the backward pass the
     scores' gradients) are rounded to the tensors' type for the second product.  The backward

@@ -251,9 +251,12 @@ def test_tables_refuse_angles_that_grow_too_fast(base, dims):
     positions = ints(1) if isinstance(dims, int) else ints(1, 2)[None]
     with pytest.raises(ValueError, match="base is too small"):
         mflux_amd.rotary_tables(positions, dims, base)
-    for base, dims in ((0.25, 64), (0.1, 2), (0.2, 4)):  # these go on to the next refusal
+    for base, dims, scaling in ((0.25, 64, None), (0.1, 2, None), (0.2, 4, None), (0.1, 64, {"type": "linear", "factor": 4.0}),
+                                (0.1, 64, {"type": "ntk", "factor": 4.0})):  # these go on to the next refusal
         with pytest.raises(RuntimeError, match="HIP device"):
-            mflux_amd.rotary_tables(ints(1), dims, base)
+            mflux_amd.rotary_tables(ints(1), dims, base, scaling)
+    with pytest.raises(ValueError, match="base is too small"):
+        mflux_amd.rotary_tables(ints(1), 64, 0.01, {"type": "ntk", "factor": 2.0})
     with pytest.raises(ValueError, match="attention_factor"):
         mflux_amd.rotary_tables(ints(1), 64, scaling={"type": "yarn", "factor": 2.0, "original_length": 100, "attention_factor": 1e39})
 
