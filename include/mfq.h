@@ -596,6 +596,65 @@ int mfq_attention(const mfq_attention_args* args, void* workspace, size_t worksp
 size_t mfq_attention_backward_workspace_bytes(const mfq_attention_args* args);
 int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * RMS norm of rows, with the residual's addition in front of it (h = h + block(x); norm(h) of a transformer block), and its
+ * gradients:
+ *   sum = round(x + residual), or x;   y = sum / sqrt(mean(sum^2) + eps) * weight
+ *   x, residual (NULL: none), dy, dsum   [rows, columns] by the stride of their rows (elements)
+ *   weight   [columns], NULL: all ones
+ *   y, sum, dx   densely packed; sum is written where there is a residual (and may be NULL without one)
+ * or the normalised row in 8 bits (mfq_int8_quantize): codes and scales instead of y, codes by code_stride.
+ * Backward: x is what was normalised (the forward pass's sum), dsum its own gradient (NULL: none), which is added to
+ * dx (NULL: not wanted; the gradient of x and of residual); dweight [columns], NULL: not wanted.
+ * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16 of all of them; sums in float32, each result rounded once.  Any alignment of elements;
+ * 16-byte aligned pointers and rows of whole 16 bytes load wider.  No array may overlap another that is written.
+ * workspace: mfq_rms_norm_workspace_bytes() of it, 16-byte aligned, for the backward pass with dweight.
+ */
+typedef struct mfq_rms_norm_args {
+  int32_t dtype;
+  float eps;
+  int64_t rows, columns;
+  const void *x, *residual, *weight, *dy, *dsum;
+  int64_t x_stride, residual_stride, dy_stride, dsum_stride, code_stride;
+  void *y, *sum, *dx, *dweight;
+  int8_t* codes;
+  float* scales;
+} mfq_rms_norm_args;
+size_t mfq_rms_norm_workspace_bytes(const mfq_rms_norm_args* args);
+int mfq_rms_norm(const mfq_rms_norm_args* args, void* stream);
+int mfq_rms_norm_backward(const mfq_rms_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows in 8 bits: codes[i] = rint(127 p[i] / max|p|), ties to even, and scale = max|p| / 127 times what p lacks of the value
+ * (p = x; in mfq_rms_norm p = sum * weight, the scale taking the root).  The codes are those of the exact quotient for
+ * 16-bit types whose products float32 holds as normal numbers.  A row of zeros has codes and scale 0, one that holds an
+ * infinity or NaN codes 0 and scale NaN.
+ *   x [rows, columns] dtype by x_stride, codes [rows, columns] by code_stride, scales [rows] float32
+ */
+int mfq_int8_quantize(const void* x, int dtype, int64_t rows, int64_t columns, int64_t x_stride, int8_t* codes, int64_t code_stride,
+                      float* scales, void* stream);
+/* out[rows, columns] = code * scale, rounded to dtype */
+int mfq_int8_dequantize(const int8_t* codes, int64_t code_stride, const float* scales, int64_t rows, int64_t columns, void* out, int dtype,
+                        void* stream);
+
+/*
+ * y[m][n] = x_scales[m] * w_scales[n] * sum_k x[m][k] w[n][k] (+ bias[n]): the product of a linear layer whose activations and
+ * weights are 8-bit integers with a scale for each token and for each output feature.  The sum is exact; it times x_scales[m],
+ * that times w_scales[n] and the bias are float32, rounded once to dtype.
+ *   x [M, K], w [N, K] int8 by the stride of their rows; K a multiple of 16 below 2^17, pointers 16-byte aligned, strides
+ *   multiples of 16 below 2^20 (rows of other lengths are padded with zeros by the caller)
+ *   y [M, N] dense, 16-byte aligned, bias [N] or NULL, both of dtype (MFQ_F32, MFQ_F16 or MFQ_BF16)
+ * workspace: mfq_int8_matmul_workspace_bytes() of it, 16-byte aligned (the sums of a K that is cut).
+ * mfq_int8_matmul_plan: the kernel that a product takes (MFQ_INT8_*, or an error code), the ranges that it cuts K into and its
+ * tile (NULL where not wanted).
+ */
+enum mfq_int8_kernel { MFQ_INT8_FEW = 1, MFQ_INT8_TILES = 2 };
+int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int* k_ranges, int* tile_rows, int* tile_columns);
+size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
+                    const void* bias, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

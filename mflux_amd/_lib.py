@@ -44,6 +44,16 @@ class AttentionArgs(ctypes.Structure):  # mfq_attention_args
         (n, ctypes.c_void_p) for n in ("out", "rest", "dq", "dk", "dv", "lse", "delta", "q_offsets", "k_offsets", "q_lengths", "k_lengths")]
 
 
+class RmsNormArgs(ctypes.Structure):  # mfq_rms_norm_args
+    _fields_ = [("dtype", ctypes.c_int32), ("eps", ctypes.c_float), ("rows", ctypes.c_int64), ("columns", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("x", "residual", "weight", "dy", "dsum")] + [
+        (n, ctypes.c_int64) for n in ("x_stride", "residual_stride", "dy_stride", "dsum_stride", "code_stride")] + [
+        (n, ctypes.c_void_p) for n in ("y", "sum", "dx", "dweight", "codes", "scales")]
+
+
+# what mfq_int8_matmul_plan answers
+INT8_FEW, INT8_TILES = 1, 2
+
 # every symbol include/mfq.h declares, with its ctypes signature
 _I64, _INT, _PTR = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
 SIGNATURES = {
@@ -92,6 +102,14 @@ SIGNATURES = {
     "mfq_attention": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_attention_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
     "mfq_attention_backward": (_INT, [ctypes.POINTER(AttentionArgs), _PTR, ctypes.c_size_t, _PTR]),
+    "mfq_rms_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RmsNormArgs)]),
+    "mfq_rms_norm": (_INT, [ctypes.POINTER(RmsNormArgs), _PTR]),
+    "mfq_rms_norm_backward": (_INT, [ctypes.POINTER(RmsNormArgs), _PTR, ctypes.c_size_t, _PTR]),
+    "mfq_int8_quantize": (_INT, [_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _PTR]),
+    "mfq_int8_dequantize": (_INT, [_PTR, _I64, _PTR, _I64, _I64, _PTR, _INT, _PTR]),
+    "mfq_int8_matmul_plan": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_INT), ctypes.POINTER(_INT), ctypes.POINTER(_INT)]),
+    "mfq_int8_matmul_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "mfq_int8_matmul": (_INT, [_PTR, _I64, _PTR, _PTR, _I64, _PTR, _PTR, _I64, _I64, _I64, _PTR, _INT, _PTR, ctypes.c_size_t, _PTR]),
     "mfq_low_rank_add": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _PTR, _INT, _PTR]),
 }
 

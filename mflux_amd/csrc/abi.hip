@@ -3,6 +3,7 @@
 // code and never a device fault.
 #include "attention.h"
 #include "common.h"
+#include "rows.h"
 
 #include <cmath>
 #include <limits>
@@ -603,6 +604,157 @@ int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size
   if (need > workspace_bytes) return MFQ_ESCRATCH;
   if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
   return mfq::launch_attention_backward(args->dtype, c, parts, workspace, (hipStream_t)stream);
+}
+
+// Rows of `count` x `columns` at `stride`, and whether a call loads them 16 bytes at a time
+static int check_rows(const void* p, int64_t stride, int64_t rows, int64_t columns, int64_t per16, bool* wide) {
+  if (!p) return MFQ_ENULL;
+  if (stride < 0 || (rows > 1 && stride > ((int64_t)1 << 40))) return MFQ_ESHAPE;
+  *wide = *wide && mfq::aligned16(p) && columns % per16 == 0 && (rows == 1 || stride % per16 == 0);
+  return MFQ_OK;
+}
+
+static int rms_norm_call(const mfq_rms_norm_args* a, bool backward, bool norm, mfq::RowsCall* c, bool* wide) {
+  if (!a) return MFQ_ENULL;
+  if (!known(a->dtype)) return MFQ_EDTYPE;
+  if (a->rows <= 0 || a->columns <= 0 || a->rows > INT32_MAX || a->columns > (1 << 28) || a->rows * a->columns > ((int64_t)1 << 46)) return MFQ_ESHAPE;
+  if (norm && !(a->eps >= 0.f && a->eps <= std::numeric_limits<float>::max())) return MFQ_ESHAPE;
+  const int64_t per16 = a->dtype == MFQ_F32 ? 4 : 8;
+  *wide = mfq::aligned16(a->weight);
+  if (int rc = check_rows(a->x, a->x_stride, a->rows, a->columns, per16, wide)) return rc;
+  if (backward) {
+    if (int rc = check_rows(a->dy, a->dy_stride, a->rows, a->columns, per16, wide)) return rc;
+    if (a->dsum)
+      if (int rc = check_rows(a->dsum, a->dsum_stride, a->rows, a->columns, per16, wide)) return rc;
+    if (!a->dx && !a->dweight) return MFQ_ENULL;
+    if (a->dweight && !a->weight) return MFQ_ENULL;
+    *wide = *wide && mfq::aligned16(a->dx);
+  } else {
+    if (a->residual) {
+      if (int rc = check_rows(a->residual, a->residual_stride, a->rows, a->columns, per16, wide)) return rc;
+      if (!a->sum) return MFQ_ENULL;
+      *wide = *wide && mfq::aligned16(a->sum);
+    }
+    if (a->codes) {
+      if (a->y) return MFQ_EUNSUPPORTED;  // one of the two
+      if (!a->scales) return MFQ_ENULL;
+      if (a->rows > 1 && a->code_stride < a->columns) return MFQ_ESHAPE;
+      *wide = *wide && reinterpret_cast<uintptr_t>(a->codes) % per16 == 0 && (a->rows == 1 || a->code_stride % per16 == 0);
+    } else {
+      if (!a->y) return MFQ_ENULL;
+      *wide = *wide && mfq::aligned16(a->y);
+    }
+  }
+  *c = {};
+  c->x = a->x;
+  c->residual = a->residual;
+  c->weight = a->weight;
+  c->dy = a->dy;
+  c->dsum = a->dsum;
+  c->y = a->y;
+  c->sum = a->sum;
+  c->dx = a->dx;
+  c->dweight = a->dweight;
+  c->codes = backward ? nullptr : a->codes;
+  c->scales = a->scales;
+  c->rows = a->rows;
+  c->columns = a->columns;
+  c->x_stride = a->x_stride;
+  c->residual_stride = a->residual_stride;
+  c->dy_stride = a->dy_stride;
+  c->dsum_stride = a->dsum_stride;
+  c->code_stride = a->code_stride;
+  c->eps = a->eps;
+  c->norm = norm;
+  return MFQ_OK;
+}
+
+size_t mfq_rms_norm_workspace_bytes(const mfq_rms_norm_args* args) {
+  if (!args || !args->dweight || args->rows <= 0 || args->columns <= 0) return 0;
+  return mfq::rows_workspace_bytes(args->rows, args->columns);
+}
+
+int mfq_rms_norm(const mfq_rms_norm_args* args, void* stream) {
+  mfq::RowsCall c;
+  bool wide = false;
+  if (int rc = rms_norm_call(args, false, true, &c, &wide)) return rc;
+  return mfq::launch_rows(args->dtype, c, wide, false, (hipStream_t)stream);
+}
+
+int mfq_rms_norm_backward(const mfq_rms_norm_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  mfq::RowsCall c;
+  bool wide = false;
+  if (int rc = rms_norm_call(args, true, true, &c, &wide)) return rc;
+  const size_t need = mfq_rms_norm_workspace_bytes(args);
+  if (need && !workspace) return MFQ_ENULL;
+  if (need > workspace_bytes) return MFQ_ESCRATCH;
+  if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
+  c.parts = need ? static_cast<float*>(workspace) : nullptr;
+  return mfq::launch_rows(args->dtype, c, wide, true, (hipStream_t)stream);
+}
+
+int mfq_int8_quantize(const void* x, int dtype, int64_t rows, int64_t columns, int64_t x_stride, int8_t* codes, int64_t code_stride,
+                      float* scales, void* stream) {
+  if (!codes) return known(dtype) ? MFQ_ENULL : MFQ_EDTYPE;
+  mfq_rms_norm_args a = {};
+  a.dtype = dtype;
+  a.rows = rows;
+  a.columns = columns;
+  a.x = x;
+  a.x_stride = x_stride;
+  a.codes = codes;
+  a.code_stride = code_stride;
+  a.scales = scales;
+  mfq::RowsCall c;
+  bool wide = false;
+  if (int rc = rms_norm_call(&a, false, false, &c, &wide)) return rc;
+  return mfq::launch_rows(dtype, c, wide, false, (hipStream_t)stream);
+}
+
+int mfq_int8_dequantize(const int8_t* codes, int64_t code_stride, const float* scales, int64_t rows, int64_t columns, void* out, int dtype,
+                        void* stream) {
+  if (!known(dtype)) return MFQ_EDTYPE;
+  if (rows <= 0 || columns <= 0 || rows > INT32_MAX || columns > (1 << 28) || rows * columns > ((int64_t)1 << 46)) return MFQ_ESHAPE;
+  if (!codes || !scales || !out) return MFQ_ENULL;
+  if (code_stride < 0 || (rows > 1 && code_stride > ((int64_t)1 << 40))) return MFQ_ESHAPE;
+  return mfq::launch_rows_values(codes, code_stride, scales, rows, columns, dtype, out, (hipStream_t)stream);
+}
+
+static int check_int8(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 16 || K >= (1 << 17) || M > (1 << 30) || N > (1 << 30)) return MFQ_ESHAPE;
+  if (M * N > ((int64_t)1 << 42)) return MFQ_ESHAPE;
+  return MFQ_OK;
+}
+
+int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int* k_ranges, int* tile_rows, int* tile_columns) {
+  if (int rc = check_int8(M, N, K)) return rc;
+  const mfq::Int8Plan p = mfq::int8_plan(M, N, K);
+  if (k_ranges) *k_ranges = p.splits;
+  if (tile_rows) *tile_rows = p.rows;
+  if (tile_columns) *tile_columns = p.columns;
+  return p.kernel;
+}
+
+size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (check_int8(M, N, K) != MFQ_OK) return 0;
+  return mfq::int8_workspace_bytes(mfq::int8_plan(M, N, K), M, N);
+}
+
+int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
+                    const void* bias, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  if (!known(dtype)) return MFQ_EDTYPE;
+  if (int rc = check_int8(M, N, K)) return rc;
+  if (!x || !x_scales || !w || !w_scales || !y) return MFQ_ENULL;
+  if (x_stride < 0 || w_stride < 0 || x_stride >= (1 << 20) || w_stride >= (1 << 20)) return MFQ_ESHAPE;
+  if (!mfq::aligned16(x) || !mfq::aligned16(w) || !mfq::aligned16(y) || x_stride % 16 || w_stride % 16) return MFQ_EALIGN;
+  const mfq::Int8Plan p = mfq::int8_plan(M, N, K);
+  const size_t need = mfq::int8_workspace_bytes(p, M, N);
+  if (need && !workspace) return MFQ_ENULL;
+  if (need > workspace_bytes) return MFQ_ESCRATCH;
+  if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
+  const mfq::Int8Call c = {x, w, x_scales, w_scales, bias, y, M, N, K, x_stride, w_stride};
+  return mfq::launch_int8_matmul(dtype, c, p, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

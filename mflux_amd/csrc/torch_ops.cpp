@@ -835,6 +835,224 @@ Tensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const c
   return attention_forward(q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, causal, scale, nullptr, nullptr);
 }
 
+// ---- rows: RMS norm, 8-bit integers (include/mfq.h, mfq_rms_norm and mfq_int8_matmul)
+// [..., K] as rows: a view where one stride serves them all, otherwise a copy; the last axis dense
+Tensor rows_of(const Tensor& t) {
+  if (t.dim() == 2 && t.stride(1) == 1) return t;
+  Tensor r = t.reshape({t.numel() / t.size(-1), t.size(-1)});
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+
+struct NormOperands {
+  mfq_rms_norm_args a = {};
+  std::vector<Tensor> keep;
+  NormOperands(const char* fn, const Tensor& x, const c10::optional<Tensor>& weight, double eps) {
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, fn, ": x [..., K] of at least one value a row");
+    a.dtype = dtype_code(x.scalar_type(), "x");
+    a.eps = (float)eps;
+    a.columns = x.size(-1);
+    a.rows = x.numel() / a.columns;
+    a.x = rows(x, a.x_stride);
+    if (weight.has_value()) {
+      TORCH_CHECK(weight->dim() == 1 && weight->size(0) == a.columns && weight->scalar_type() == x.scalar_type() && weight->device() == x.device(), fn,
+                  ": the weight must be a [K] vector of x's type");
+      keep.push_back(weight->contiguous());
+      a.weight = keep.back().data_ptr();
+    }
+  }
+  const void* rows(const Tensor& t, int64_t& stride) {
+    keep.push_back(rows_of(t));
+    stride = row_stride(keep.back());
+    return keep.back().data_ptr();
+  }
+  const void* as(const char* fn, const Tensor& t, const Tensor& x, int64_t& stride) {
+    TORCH_CHECK(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(), fn, ": a residual and gradients must be as x");
+    return rows(t, stride);
+  }
+};
+
+// (y, what is normalised: the sum with the residual, empty without one)
+std::tuple<Tensor, Tensor> rms_norm(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& residual, double eps) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  NormOperands o("mfq::rms_norm", x, weight, eps);
+  Tensor y = at::empty(x.sizes(), x.options()), sum;
+  o.a.y = y.data_ptr();
+  if (residual.has_value()) {
+    o.a.residual = o.as("mfq::rms_norm", *residual, x, o.a.residual_stride);
+    sum = at::empty(x.sizes(), x.options());
+    o.a.sum = sum.data_ptr();
+  } else {
+    sum = at::empty({0}, x.options());
+  }
+  if (x.numel()) check_status("mfq_rms_norm", mfq_rms_norm(&o.a, stream_of(x)));
+  return {y, sum};
+}
+
+// sum: what was normalised.  (dx, dweight), empty where not wanted
+std::tuple<Tensor, Tensor> rms_norm_backward(const Tensor& dy, const c10::optional<Tensor>& dsum, const Tensor& sum, const c10::optional<Tensor>& weight,
+                                             double eps, bool want_x, bool want_weight) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(sum.device());
+  TORCH_CHECK(!want_weight || weight.has_value(), "mfq::rms_norm_backward: no such weight");
+  NormOperands o("mfq::rms_norm_backward", sum, weight, eps);
+  o.a.dy = o.as("mfq::rms_norm_backward", dy, sum, o.a.dy_stride);
+  if (dsum.has_value()) o.a.dsum = o.as("mfq::rms_norm_backward", *dsum, sum, o.a.dsum_stride);
+  const Tensor none = at::empty({0}, sum.options());
+  Tensor dx = want_x ? at::empty(sum.sizes(), sum.options()) : none, dw = want_weight ? at::empty({o.a.columns}, sum.options()) : none;
+  if (!sum.numel() || (!want_x && !want_weight)) return {dx, dw.zero_()};
+  if (want_x) o.a.dx = dx.data_ptr();
+  if (want_weight) o.a.dweight = dw.data_ptr();
+  const size_t bytes = mfq_rms_norm_workspace_bytes(&o.a);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, sum.options().dtype(at::kByte));
+  check_status("mfq_rms_norm_backward", mfq_rms_norm_backward(&o.a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(sum)));
+  return {dx, dw};
+}
+
+// Codes [..., K] in rows of whole 16 bytes, which is how mfq_int8_matmul reads them
+Tensor empty_codes(const Tensor& x, int64_t& stride) {
+  const int64_t K = x.size(-1);
+  stride = (K + 15) / 16 * 16;
+  std::vector<int64_t> sizes = x.sizes().vec(), strides(sizes.size());
+  int64_t step = 1;
+  for (size_t i = sizes.size(); i-- > 0;) {
+    strides[i] = step;
+    step *= i + 1 == sizes.size() ? stride : sizes[i];
+  }
+  return at::empty({std::max<int64_t>(x.numel() / K, 1) * stride}, x.options().dtype(at::kChar)).as_strided(sizes, strides);
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_int8(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& residual,
+                                                 double eps) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  NormOperands o("mfq::rms_norm_int8", x, weight, eps);
+  Tensor codes = empty_codes(x, o.a.code_stride), scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  o.a.codes = codes.data_ptr<int8_t>();
+  o.a.scales = scales.data_ptr<float>();
+  Tensor sum = at::empty(residual.has_value() ? x.sizes() : at::IntArrayRef({0}), x.options());
+  if (residual.has_value()) {
+    o.a.residual = o.as("mfq::rms_norm_int8", *residual, x, o.a.residual_stride);
+    o.a.sum = sum.data_ptr();
+  }
+  if (x.numel()) check_status("mfq_rms_norm", mfq_rms_norm(&o.a, stream_of(x)));
+  return {codes, scales, sum};
+}
+
+std::tuple<Tensor, Tensor> int8_quantize(const Tensor& x) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "mfq::int8_quantize: x [..., K] of at least one value a row");
+  const Tensor r = rows_of(x);
+  int64_t stride;
+  Tensor codes = empty_codes(x, stride), scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  if (x.numel())
+    check_status("mfq_int8_quantize", mfq_int8_quantize(r.data_ptr(), dtype_code(x.scalar_type(), "x"), r.size(0), r.size(1), row_stride(r),
+                                                        codes.data_ptr<int8_t>(), stride, scales.data_ptr<float>(), stream_of(x)));
+  return {codes, scales};
+}
+
+Tensor int8_dequantize(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) > 0 && codes.scalar_type() == at::kChar && scales.scalar_type() == at::kFloat &&
+                  scales.device() == codes.device() && scales.sizes() == codes.sizes().slice(0, codes.dim() - 1),
+              "mfq::int8_dequantize: codes [..., K] int8 and scales [...] float32 on one device");
+  const Tensor r = rows_of(codes), s = scales.contiguous();
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  if (out.numel())
+    check_status("mfq_int8_dequantize", mfq_int8_dequantize(r.data_ptr<int8_t>(), row_stride(r), s.data_ptr<float>(), r.size(0), r.size(1),
+                                                            out.data_ptr(), dtype_code(dtype, "the result"), stream_of(codes)));
+  return out;
+}
+
+// An operand of mfq_int8_matmul: rows of `length` (K in whole 16s), aligned.  Bytes behind K are read, and have to be 0 in one operand
+// (`zeros`): what is not laid out like that, or could end before them, is copied into rows that are.
+Tensor int8_rows(const Tensor& t, int64_t length, bool zeros) {
+  const int64_t K = t.size(1), stride = row_stride(t);
+  const bool inside = t.storage_offset() + (t.size(0) - 1) * stride + length <= (int64_t)t.storage().nbytes();
+  if (!(zeros && K != length) && inside && t.stride(1) == 1 && stride % 16 == 0 && stride < (1 << 20) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
+    return t;
+  if (K == length) return t.clone(at::MemoryFormat::Contiguous);
+  Tensor padded = at::empty({t.size(0), length}, t.options());
+  padded.narrow(1, 0, K).copy_(t);
+  padded.narrow(1, K, length - K).zero_();
+  return padded;
+}
+
+Tensor int8_matmul(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const c10::optional<Tensor>& bias,
+                   at::ScalarType dtype) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && x.size(-1) > 0 && x.scalar_type() == at::kChar && w.scalar_type() == at::kChar &&
+                  w.device() == x.device(),
+              "mfq::int8_matmul: x [..., K] and w [N, K], int8 on one device");
+  TORCH_CHECK(x_scales.scalar_type() == at::kFloat && w_scales.scalar_type() == at::kFloat && x_scales.device() == x.device() &&
+                  w_scales.device() == x.device() && x_scales.sizes() == x.sizes().slice(0, x.dim() - 1) && w_scales.dim() == 1 &&
+                  w_scales.size(0) == w.size(0),
+              "mfq::int8_matmul: x_scales [...] and w_scales [N], float32 on the codes' device");
+  TORCH_CHECK(!bias.has_value() || (bias->dim() == 1 && bias->size(0) == w.size(0) && bias->scalar_type() == dtype && bias->device() == x.device()),
+              "mfq::int8_matmul: bias [N] of the result's type");
+  const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K, length = (K + 15) / 16 * 16;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = N;
+  Tensor y = at::empty(sizes, x.options().dtype(dtype));
+  if (y.numel() == 0) return y;
+  const Tensor xr = int8_rows(rows_of(x), length, true), wr = int8_rows(w, length, false);
+  const Tensor xs = x_scales.contiguous(), ws = w_scales.contiguous(), b = bias.has_value() ? bias->contiguous() : Tensor();
+  const size_t bytes = mfq_int8_matmul_workspace_bytes(M, N, length);
+  Tensor scratch;
+  if (bytes) scratch = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  check_status("mfq_int8_matmul",
+               mfq_int8_matmul(xr.data_ptr<int8_t>(), row_stride(xr), xs.data_ptr<float>(), wr.data_ptr<int8_t>(), row_stride(wr), ws.data_ptr<float>(),
+                               b.defined() ? b.data_ptr() : nullptr, M, N, length, y.data_ptr(), dtype_code(dtype, "the result"),
+                               bytes ? scratch.data_ptr() : nullptr, bytes, stream_of(x)));
+  return y;
+}
+
+struct RmsNormFunction : torch::autograd::Function<RmsNormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& residual,
+                               double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, sum] = rms_norm(x, weight, residual, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({residual.has_value() ? sum : x, or_none(weight)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["wanted"] = (int64_t)(wanted(x) | wanted(weight) << 1 | wanted(residual) << 2);
+    if (!residual.has_value()) return {y};
+    return {y, sum};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t want = ctx->saved_data["wanted"].toInt();
+    variable_list out(4);
+    const Tensor dsum = d.size() > 1 ? d[1] : Tensor();
+    {
+      at::AutoGradMode off(false);
+      at::AutoDispatchBelowADInplaceOrView guard;
+      Tensor dx, dw;
+      if (d[0].defined()) {
+        std::tie(dx, dw) = rms_norm_backward(d[0], if_defined(dsum), saved[0], if_defined(saved[1]), ctx->saved_data["eps"].toDouble(), want & 5, want & 2);
+      } else {  // the sum alone was used
+        dx = dsum;
+        if ((want & 2) && dsum.defined()) dw = at::zeros_like(saved[1]);
+      }
+      if (want & 1) out[0] = dx;
+      if (want & 2) out[1] = dw;
+      if (want & 4) out[2] = dx;
+    }
+    return once("mfq::rms_norm", std::move(out));
+  }
+};
+
+std::tuple<Tensor, Tensor> rms_norm_call(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& residual, double eps) {
+  const c10::optional<Tensor> first(x);
+  check_forward_mode("mfq::rms_norm", {&first, &weight, &residual});
+  if (at::GradMode::is_enabled() && (wanted(x) || wanted(weight) || wanted(residual))) {
+    check_capture("mfq::rms_norm", {&first, &weight, &residual}, x);
+    auto out = RmsNormFunction::apply(x, weight, residual, eps);
+    return {out[0], out.size() > 1 ? out[1] : at::empty({0}, x.options())};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rms_norm(x, weight, residual, eps);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mfq, m) {
@@ -859,6 +1077,13 @@ TORCH_LIBRARY(mfq, m) {
   m.def("rotary_call(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, Tensor? k_weight, int layout, float eps) -> (Tensor, Tensor)");
   m.def("attention_call(Tensor q, Tensor k, Tensor v, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale) -> Tensor");
   m.def("attention_backward(Tensor dy, Tensor q, Tensor k, Tensor v, Tensor y, Tensor rest, Tensor lse, Tensor? q_offsets, Tensor? k_offsets, Tensor? q_lengths, Tensor? k_lengths, bool causal, float scale, bool want_dq, bool want_dkv) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps) -> (Tensor, Tensor)");
+  m.def("rms_norm_backward(Tensor dy, Tensor? dsum, Tensor sum, Tensor? weight, float eps, bool want_x, bool want_weight) -> (Tensor, Tensor)");
+  m.def("rms_norm_call(Tensor x, Tensor? weight, Tensor? residual, float eps) -> (Tensor, Tensor)");
+  m.def("rms_norm_int8(Tensor x, Tensor? weight, Tensor? residual, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("int8_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("int8_dequantize(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
+  m.def("int8_matmul(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, Tensor? bias, ScalarType dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA dispatch key
@@ -883,9 +1108,17 @@ TORCH_LIBRARY_IMPL(mfq, CUDA, m) {  // the HIP backend answers to torch's CUDA d
   m.impl("attention_backward", attention_backward);
   m.impl("rotary_call", rotary_call);
   m.impl("attention_call", attention_call);
+  m.impl("rms_norm", rms_norm);
+  m.impl("rms_norm_backward", rms_norm_backward);
+  m.impl("rms_norm_call", rms_norm_call);
+  m.impl("rms_norm_int8", rms_norm_int8);
+  m.impl("int8_quantize", int8_quantize);
+  m.impl("int8_dequantize", int8_dequantize);
+  m.impl("int8_matmul", int8_matmul);
 }
 
 TORCH_LIBRARY_IMPL(mfq, AutogradCUDA, m) {  // the ops with gradients; the others are called from these and from Python functions
   m.impl("rotary_call", rotary_call);
   m.impl("attention_call", attention_call);
+  m.impl("rms_norm_call", rms_norm_call);
 }

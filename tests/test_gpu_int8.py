@@ -1,0 +1,279 @@
+"""rms_norm, rms_norm_int8, int8_quantize, int8_dequantize and int8_matmul against float64, element by element within the
+bounds that int8_reference derives, at the sizes, strides, types and values where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import int8_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF16, F16, F32]
+
+
+def randn(seed, *shape, dtype=F32, std=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def codes(seed, *shape, low=-128):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randint(low, 128, shape, generator=g, device="cuda", dtype=torch.int8)
+
+
+def scales(seed, *shape):
+    return randn(seed, *shape).abs() * 0.02 + 0.001
+
+
+# ---- norm ------------------------------------------------------------------------------------------------------------------
+# one value; below, at and behind a lane's, a wavefront's, a workgroup's pieces; odd; longer than the registers
+ROWS = [(1, 1), (3, 8), (5, 17), (1, 64), (7, 513), (2, 512), (300, 520), (65, 768), (9, 2048), (4, 2056), (3, 3840), (1030, 1024), (2, 8192),
+        (3, 16384), (2, 16392), (2, 40001)]
+
+
+@pytest.mark.parametrize("rows,K", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("weighted,added", [(True, True), (False, False), (True, False), (False, True)])
+def test_rms_norm(rows, K, dtype, weighted, added):
+    import mflux_amd
+
+    print(f"rows={rows} K={K} {dtype} {weighted} {added}", flush=True)
+    x = randn(1, rows, K, dtype=dtype, std=1.5).requires_grad_()
+    r = randn(2, rows, K, dtype=dtype, std=0.7).requires_grad_() if added else None
+    w = randn(3, K, dtype=dtype).requires_grad_() if weighted else None
+    out = mflux_amd.rms_norm(x, w, residual=r)
+    out = list(out) if added else [out]
+    s = ref.total(x.detach(), None if r is None else r.detach())
+    dy, dsum = randn(4, rows, K, dtype=dtype), randn(5, rows, K, dtype=dtype) if added else None
+    leaves = [t for t in (x, r, w) if t is not None]
+    got = dict(zip(map(id, leaves), torch.autograd.grad(out, leaves, [dy, dsum][:len(out)])))
+    want = ref.rms_norm(s, w, 1e-6, dy, dsum)
+    ref.check("y", out[0], *want["y"])
+    if added:
+        assert torch.equal(out[1], s)
+        assert torch.equal(got[id(r)], got[id(x)])
+    ref.check("dx", got[id(x)], *want["dx"])
+    if weighted:
+        ref.check("dw", got[id(w)], *want["dw"])
+    with torch.no_grad():  # without gradients: the same call, the same bits
+        again = mflux_amd.rms_norm(x, w, residual=r)
+    assert all(torch.equal(a, b) for a, b in zip(again if added else [again], out))
+
+
+@pytest.mark.parametrize("rows,K", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("weighted,added", [(True, True), (False, False)])
+def test_rms_norm_int8(rows, K, dtype, weighted, added):
+    import mflux_amd
+
+    print(f"rows={rows} K={K} {dtype} {weighted} {added}", flush=True)
+    x, r = randn(1, rows, K, dtype=dtype, std=1.5), randn(2, rows, K, dtype=dtype, std=0.7) if added else None
+    w = randn(3, K, dtype=dtype) if weighted else None
+    q, sc, *rest = mflux_amd.rms_norm_int8(x, w, residual=r)
+    s = ref.total(x, r)
+    want_q, want_sc = ref.codes(s, w, 1e-6)
+    assert q.dtype == torch.int8 and q.shape == x.shape and sc.dtype == F32 and sc.shape == (rows,)
+    assert torch.equal(q.double(), want_q)
+    ref.check("scales", sc, want_sc, want_sc * ref.scale_bound(K, True))
+    if added:
+        assert torch.equal(rest[0], s)
+    q2, sc2 = mflux_amd.int8_quantize(s)
+    want_q, want_sc = ref.codes(s)
+    assert torch.equal(q2.double(), want_q)
+    ref.check("scales", sc2, want_sc, want_sc * ref.scale_bound(K, False))
+    for out in TYPES:
+        back = mflux_amd.int8_dequantize(q2, sc2, out)
+        value = q2.double() * sc2.double()[:, None]
+        ref.check("values", back, value, value.abs() * (ref.HALF[out] + 2 * ref.E) + ref.TINY[out])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_codes_next_to_a_border(dtype):
+    """Rows whose quotients lie on a border between two codes, or one step of the type beside it."""
+    import mflux_amd
+
+    top = torch.tensor([127.0, 1.0, 254.0, 0.3, 100.0, 3.0], device="cuda").to(dtype)
+    half = torch.arange(-126, 127, device="cuda").double() + 0.5
+    on = (half[None, :-1] * top.double()[:, None] / 127).to(dtype)
+    bits = on.view(torch.int32 if dtype == F32 else torch.int16)
+    rows = torch.cat([top[:, None], on, (bits + 1).view(dtype), (bits - 1).view(dtype)], dim=1)
+    for t in (rows, rows[:, :760], rows[:, :1]):  # 16-byte pieces, and one by one
+        q, _ = mflux_amd.int8_quantize(t)
+        assert torch.equal(q.double(), ref.codes(t)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [64, 67, 2048])
+def test_rows_of_zeros_infinities_and_extremes(dtype, K):
+    import mflux_amd
+
+    info = torch.finfo(dtype)
+    rows = randn(1, 8, K, dtype=dtype)
+    rows[1] = 0
+    rows[2, 5], rows[3, 5], rows[4, 5] = math.inf, -math.inf, math.nan
+    rows[5] = torch.where(rows[5] > 0, info.max, info.min).to(dtype)
+    rows[6] = rows[6] * info.tiny  # and below it
+    rows[7] = 0
+    rows[7, K - 1] = info.smallest_normal
+    q, sc = mflux_amd.int8_quantize(rows)
+    fine = [0, 1, 5, 6, 7]
+    want_q, want_sc = ref.codes(rows[fine])
+    assert torch.equal(q[fine].double(), want_q)
+    assert bool(((sc[fine].double() - want_sc).abs() <= want_sc * 2 * ref.E + 2.0 ** -149).all())
+    assert bool(sc[2:5].isnan().all()) and not q[2:5].any()
+    q, sc = mflux_amd.rms_norm_int8(rows, torch.ones(K, device="cuda", dtype=dtype))
+    assert bool(sc[2:5].isnan().all()) and not q[2:5].any() and float(sc[1]) == 0
+    y = mflux_amd.rms_norm(rows)
+    assert bool(y[4].isnan().all()) and not y[1].any() and bool(y[2, 5].isnan())
+    ref.check("y", y[[0, 1, 7]], *ref.rms_norm(rows[[0, 1, 7]], None, 1e-6)["y"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_strides_and_shapes(dtype):
+    """Slices of a stacked product, transposed and expanded rows, odd addresses, leading axes, no rows."""
+    import mflux_amd
+
+    big = randn(1, 2, 9, 3 * 256 + 8, dtype=dtype)
+    w = randn(2, 256, dtype=dtype)
+    flat = torch.empty(10 * 256 + 3, device="cuda", dtype=dtype)
+    flat.copy_(randn(3, 10 * 256 + 3))
+    cases = [big[:, :, 256:512], big[:, :, 3:259], big.transpose(0, 1)[:, :, :256], big[:, :1, :256].expand(2, 9, 256), big[0, 0, :256],
+             flat[3:3 + 2560].view(10, 256), big[:, :, ::3][:, :, :256], big[:0, :, :256]]
+    for t in cases:
+        x = t.detach().requires_grad_()
+        y, s = mflux_amd.rms_norm(x, w, residual=t)
+        want = ref.rms_norm(ref.total(t, t), w, 1e-6, torch.ones_like(t), torch.ones_like(t))
+        ref.check("y", y, *want["y"])
+        assert y.is_contiguous() and y.shape == t.shape and torch.equal(s, ref.total(t, t))
+        one = torch.ones((), device="cuda", dtype=dtype).expand(t.shape)
+        ref.check("dx", torch.autograd.grad((y, s), x, (one, one))[0], *want["dx"])
+        q, sc = mflux_amd.int8_quantize(t)
+        assert torch.equal(q.double(), ref.codes(t)[0]) and sc.shape == t.shape[:-1]
+        assert torch.equal(mflux_amd.int8_dequantize(q, sc, F32), q.float() * sc[..., None])
+
+
+def test_norm_partial_gradients():
+    """One of the two results, one of the inputs, the same tensor twice; a second derivative is refused."""
+    import mflux_amd
+
+    x, r, w = randn(1, 5, 264).requires_grad_(), randn(2, 5, 264).requires_grad_(), randn(3, 264).requires_grad_()
+    dy = randn(4, 5, 264)
+    want = ref.rms_norm(ref.total(x.detach(), r.detach()), w, 1e-6, dy, None)
+    y, s = mflux_amd.rms_norm(x, w, residual=r)
+    ref.check("dx", torch.autograd.grad(y, x, dy, retain_graph=True)[0], *want["dx"])
+    ref.check("dw", torch.autograd.grad(y, w, dy, retain_graph=True)[0], *want["dw"])
+    assert torch.equal(torch.autograd.grad(s, r, dy, retain_graph=True)[0], dy)
+    dw, = torch.autograd.grad(s, w, dy, retain_graph=True)
+    assert not dw.any()
+    y2, _ = mflux_amd.rms_norm(x.detach(), w, residual=r.detach())
+    ref.check("dw", torch.autograd.grad(y2, w, dy)[0], *want["dw"])
+    y2, _ = mflux_amd.rms_norm(x.detach(), w.detach(), residual=r)
+    ref.check("dr", torch.autograd.grad(y2, r, dy)[0], *want["dx"])
+    y, s = mflux_amd.rms_norm(x, w, residual=x)
+    want = ref.rms_norm(ref.total(x.detach(), x.detach()), w, 1e-6, dy, dy)
+    value, bound = want["dx"]
+    ref.check("dx", torch.autograd.grad((y, s), x, (dy, dy))[0], 2 * value, 2 * bound)
+    g, = torch.autograd.grad(mflux_amd.rms_norm(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative|differentiate twice"):
+        g.sum().backward()
+    # .grad of both leaves, which share one gradient, stay apart
+    x, r = randn(1, 4, 64).requires_grad_(), randn(2, 4, 64).requires_grad_()
+    mflux_amd.rms_norm(x, residual=r)[0].sum().backward()
+    before = r.grad.clone()
+    x.grad.add_(1)
+    assert torch.equal(r.grad, before)
+
+
+def test_norm_gradient_against_differences():
+    import mflux_amd
+
+    x, w, dy = randn(1, 3, 40), randn(2, 40), randn(3, 3, 40)
+    leaf = x.clone().requires_grad_()
+    got, = torch.autograd.grad(mflux_amd.rms_norm(leaf, w), leaf, dy)
+    step = 2.0 ** -10
+    for i in range(0, 120, 7):
+        d = torch.zeros(120, device="cuda", dtype=torch.float64)
+        d[i] = step
+        d = d.view(3, 40)
+        slope = (along(x.double() + d, w, dy) - along(x.double() - d, w, dy)) / (2 * step)
+        # the third derivative of a normalised row of this size is some tens: step^2 / 6 of that
+        assert abs(float(got.reshape(-1)[i]) - float(slope)) < 1e-4 * (1 + abs(float(slope)))
+
+
+def along(v, w, dy):
+    return (v / (v.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double() * dy.double()).sum()
+
+
+# ---- product ---------------------------------------------------------------------------------------------------------------
+PRODUCTS = [(1, 1, 1), (1, 16, 16), (1, 17, 100), (3, 40, 128), (8, 129, 144), (9, 16, 4096), (16, 1000, 1040), (5, 3840, 3840), (17, 64, 64),
+            (17, 1, 2048), (32, 300, 272), (33, 127, 4112), (64, 512, 1000), (65, 129, 129), (128, 128, 112), (200, 1023, 640), (333, 1152, 2500),
+            (130, 8, 16384), (257, 5000, 16), (3300, 3900, 272), (3329, 4001, 131), (4100, 12300, 128)]
+
+
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+@pytest.mark.parametrize("dtype,biased", [(BF16, True), (F16, False), (F32, True), (F32, False)])
+def test_int8_matmul(M, N, K, dtype, biased):
+    import mflux_amd
+
+    print(f"M={M} N={N} K={K} {dtype} {biased}", flush=True)
+    x, w = codes(1, M, K), codes(2, N, K)
+    x[0], w[N - 1] = -128, -128  # the largest sum there is
+    xs, ws = scales(3, M), scales(4, N)
+    b = randn(5, N, dtype=dtype) if biased else None
+    y = mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype)
+    assert y.dtype == dtype and y.is_contiguous()
+    ref.check("y", y, *ref.product(x, xs, w, ws, b, dtype))
+    if dtype == F32 and not biased:  # the integers themselves
+        one = torch.ones_like
+        sums = mflux_amd.int8_matmul(x, one(xs), w, one(ws), dtype=F32)
+        assert torch.equal(sums, torch.mm(x.double(), w.double().t().contiguous()).float())
+
+
+def test_int8_matmul_of_the_longest_rows():
+    import mflux_amd
+
+    K = (1 << 17) - 16
+    for M, N in ((1, 20), (40, 70), (130, 140)):
+        x, w = torch.full((M, K), -128, device="cuda", dtype=torch.int8), torch.full((N, K), -128, device="cuda", dtype=torch.int8)
+        one = torch.ones(max(M, N), device="cuda")
+        y = mflux_amd.int8_matmul(x, one[:M], w, one[:N], dtype=F32)
+        assert bool((y == float(K * 16384)).all())
+
+
+@pytest.mark.parametrize("M", [1, 12, 30, 60, 140])
+def test_int8_matmul_strides(M):
+    """Rows apart, of odd lengths and addresses, repeated, transposed; leading axes; codes that int8_quantize laid out."""
+    import mflux_amd
+
+    N, K = 200, 160
+    big_x, big_w = codes(1, M, 2 * K + 5), codes(2, N, 2 * K + 5)
+    xs, ws = scales(3, M), scales(4, N)
+    for x, w in ((big_x[:, :K], big_w[:, :K]), (big_x[:, 1:1 + K], big_w[:, 16:16 + K]), (big_x[:1, :K].expand(M, K), big_w[:1, :K].expand(N, K)),
+                 (codes(5, K, M).t(), codes(6, K, N).t()), (big_x[:, ::2][:, :K], big_w[:, ::2][:, :K]), (big_x[:, :77], big_w[:, :77])):
+        y = mflux_amd.int8_matmul(x, xs, w, ws, dtype=F32)
+        ref.check("y", y, *ref.product(x, xs, w, ws, None, F32))
+    x = codes(7, 2, 3, M, K)
+    y = mflux_amd.int8_matmul(x, scales(8, 2, 3, M), big_w[:, :K], ws)
+    ref.check("y", y, *ref.product(x, scales(8, 2, 3, M), big_w[:, :K], ws, None, BF16))
+    for odd in (1, 15, 17, 100, 1001):
+        q, s = mflux_amd.int8_quantize(randn(9, 2, M, odd))
+        p, t = mflux_amd.int8_quantize(randn(10, N, odd))
+        ref.check("y", mflux_amd.int8_matmul(q, s, p, t, dtype=F32), *ref.product(q, s, p, t, None, F32))
+    assert mflux_amd.int8_matmul(x[:, :0], scales(8, 2, 3, M)[:, :0], big_w[:, :K], ws).shape == (2, 0, M, N)
+    assert mflux_amd.int8_matmul(x, scales(8, 2, 3, M), big_w[:0, :K], ws[:0]).shape == (2, 3, M, 0)
+
+
+def test_int8_matmul_scales_that_are_not_finite():
+    """The scale of a row that held an infinity makes its products NaN, and no others."""
+    import mflux_amd
+
+    for M in (4, 40, 140):
+        x = randn(1, M, 256)
+        x[2, 7] = math.inf
+        q, s = mflux_amd.int8_quantize(x)
+        w, t = mflux_amd.int8_quantize(randn(2, 64, 256))
+        y = mflux_amd.int8_matmul(q, s, w, t)
+        assert bool(y[2].isnan().all()) and not bool(y[[0, 1, 3]].isnan().any())
