@@ -649,8 +649,8 @@ int mfq_int8_dequantize(const int8_t* codes, int64_t code_stride, const float* s
  * tile (NULL where not wanted).
  */
 enum mfq_int8_kernel { MFQ_INT8_FEW = 1, MFQ_INT8_TILES = 2 };
-int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int* k_ranges, int* tile_rows, int* tile_columns);
-size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int dtype, int* k_ranges, int* tile_rows, int* tile_columns);
+size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
                     const void* bias, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace, size_t workspace_bytes,
                     void* stream);

@@ -50,6 +50,9 @@ ASM_LDS_LOAD_SOURCES = ("qmm_frag.hip", "qmm_frag_f32.hip", "qmm_slice.hip", "at
                         "attention_backward.hip", "int8_matmul.hip")
 # Kernels that use every register there is, whose k loops must not wait for one that was put away: as above.
 FULL_REGISTER_KERNELS = {"qmm_wide.hip": "qmm_wide_kernel"}
+# Kernels whose loads into LDS take an address that the compiler computes for a statement of assembly, which must not keep
+# registers in scratch memory at all: {source: substring of the kernels' mangled names}.
+NO_SCRATCH_KERNELS = {"int8_matmul.hip": "int8_tile_kernel"}
 
 
 def _parse_blocks(body: str):
@@ -265,11 +268,69 @@ def check_loop_spills(text: str, kernel_substring: str, where: str = "listing") 
     return checked
 
 
+def check_no_scratch(text: str, kernel_substring: str, where: str = "listing") -> int:
+    """Checks every kernel of the assembly listing `text` whose name contains
+    `kernel_substring`: no instruction may touch scratch memory (spilled registers),
+    and no load into LDS may take its scalar base from a register that a vector
+    instruction (v_readlane, v_readfirstlane, a comparison) has written fewer than
+    five wait states before, which the compiler sees to for its own loads but not
+    inside a statement of assembly.  Returns the number of kernels; raises
+    RuntimeError on a finding."""
+    import re
+
+    checked = 0
+    for m in re.finditer(r"^(\S*%s\S*):" % re.escape(kernel_substring), text, re.M):
+        name, blocks = m.group(1), _parse_blocks(text[m.end():text.index(".Lfunc_end", m.end())])
+        before = {}  # label -> blocks that control comes from
+        index = {label: i for i, (label, _) in enumerate(blocks) if label}
+        for b in range(len(blocks)):
+            for nb in _successors(blocks, index, b):
+                before.setdefault(nb, []).append(b)
+
+        def writes(s, registers):
+            to = re.match(r"(?:v_readlane_b32|v_readfirstlane_b32|v_cmp\S*)\s+(s\[?[\d:]+\]?)", s)
+            if not to:
+                return False
+            lo, _, hi = to.group(1).strip("s[]").partition(":")
+            return bool(registers & set(range(int(lo), int(hi or lo) + 1)))
+
+        def look_back(b, i, budget, registers, seen):
+            ins = blocks[b][1]
+            while budget > 0:
+                i -= 1
+                if i < 0:
+                    for pb in before.get(b, ()):
+                        if seen.get(pb, 0) < budget:
+                            seen[pb] = budget
+                            look_back(pb, len(blocks[pb][1]), budget, registers, seen)
+                    return
+                if writes(ins[i], registers):
+                    raise RuntimeError(f"{where}: {name} loads into LDS from a base that a vector instruction has just written ({ins[i]})")
+                budget -= _wait_states(ins[i])
+
+        loads = 0
+        for b, (_, ins) in enumerate(blocks):
+            for i, s in enumerate(ins):
+                if s.startswith("scratch_"):
+                    raise RuntimeError(f"{where}: {name} keeps registers in scratch memory ({s})")
+                base = re.match(r"global_load_lds_\S+ v\d+, s\[(\d+):(\d+)\]", s)
+                if base:
+                    loads += 1
+                    look_back(b, i, 5, set(range(int(base.group(1)), int(base.group(2)) + 1)), {})
+        if not loads:
+            raise RuntimeError(f"{where}: {name} holds no load into LDS; the check does not see the kernel")
+        checked += 1
+    if not checked:
+        raise RuntimeError(f"{where}: no kernel named *{kernel_substring}* found")
+    return checked
+
+
 def check_generated_code(src: str) -> int:
     """Compiles `src` to assembly (device side) and runs check_lds_loads (for
     ASM_LDS_LOAD_SOURCES), check_listing (over the kernels named in
-    ASM_MFMA_KERNELS) and check_loop_spills (those in FULL_REGISTER_KERNELS).
-    Returns the number of kernels the last two checked; raises on a finding."""
+    ASM_MFMA_KERNELS), check_loop_spills (those in FULL_REGISTER_KERNELS) and
+    check_no_scratch (those in NO_SCRATCH_KERNELS).  Returns the number of kernels
+    the last three checked; raises on a finding."""
     import tempfile
 
     with tempfile.TemporaryDirectory() as tmp:
@@ -282,7 +343,8 @@ def check_generated_code(src: str) -> int:
     if src in ASM_LDS_LOAD_SOURCES:
         check_lds_loads(text, src)
     checked = check_listing(text, ASM_MFMA_KERNELS[src], src) if src in ASM_MFMA_KERNELS else 0
-    return checked + (check_loop_spills(text, FULL_REGISTER_KERNELS[src], src) if src in FULL_REGISTER_KERNELS else 0)
+    checked += check_loop_spills(text, FULL_REGISTER_KERNELS[src], src) if src in FULL_REGISTER_KERNELS else 0
+    return checked + (check_no_scratch(text, NO_SCRATCH_KERNELS[src], src) if src in NO_SCRATCH_KERNELS else 0)
 
 
 def build_library(verbose: bool = False) -> str:

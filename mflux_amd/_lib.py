@@ -107,8 +107,8 @@ SIGNATURES = {
     "mfq_rms_norm_backward": (_INT, [ctypes.POINTER(RmsNormArgs), _PTR, ctypes.c_size_t, _PTR]),
     "mfq_int8_quantize": (_INT, [_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _PTR]),
     "mfq_int8_dequantize": (_INT, [_PTR, _I64, _PTR, _I64, _I64, _PTR, _INT, _PTR]),
-    "mfq_int8_matmul_plan": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_INT), ctypes.POINTER(_INT), ctypes.POINTER(_INT)]),
-    "mfq_int8_matmul_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "mfq_int8_matmul_plan": (_INT, [_I64, _I64, _I64, _INT, ctypes.POINTER(_INT), ctypes.POINTER(_INT), ctypes.POINTER(_INT)]),
+    "mfq_int8_matmul_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _INT]),
     "mfq_int8_matmul": (_INT, [_PTR, _I64, _PTR, _PTR, _I64, _PTR, _PTR, _I64, _I64, _I64, _PTR, _INT, _PTR, ctypes.c_size_t, _PTR]),
     "mfq_low_rank_add": (_INT, [_PTR, _PTR, _INT, _I64, _I64, _I64, _PTR, _INT, _PTR]),
 }

@@ -726,18 +726,19 @@ static int check_int8(int64_t M, int64_t N, int64_t K) {
   return MFQ_OK;
 }
 
-int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int* k_ranges, int* tile_rows, int* tile_columns) {
+int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int dtype, int* k_ranges, int* tile_rows, int* tile_columns) {
+  if (!known(dtype)) return MFQ_EDTYPE;
   if (int rc = check_int8(M, N, K)) return rc;
-  const mfq::Int8Plan p = mfq::int8_plan(M, N, K);
+  const mfq::Int8Plan p = mfq::int8_plan(dtype, M, N, K);
   if (k_ranges) *k_ranges = p.splits;
   if (tile_rows) *tile_rows = p.rows;
   if (tile_columns) *tile_columns = p.columns;
   return p.kernel;
 }
 
-size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (check_int8(M, N, K) != MFQ_OK) return 0;
-  return mfq::int8_workspace_bytes(mfq::int8_plan(M, N, K), M, N);
+size_t mfq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (!known(dtype) || check_int8(M, N, K) != MFQ_OK) return 0;
+  return mfq::int8_workspace_bytes(mfq::int8_plan(dtype, M, N, K), M, N);
 }
 
 int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
@@ -748,7 +749,7 @@ int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, co
   if (!x || !x_scales || !w || !w_scales || !y) return MFQ_ENULL;
   if (x_stride < 0 || w_stride < 0 || x_stride >= (1 << 20) || w_stride >= (1 << 20)) return MFQ_ESHAPE;
   if (!mfq::aligned16(x) || !mfq::aligned16(w) || !mfq::aligned16(y) || x_stride % 16 || w_stride % 16) return MFQ_EALIGN;
-  const mfq::Int8Plan p = mfq::int8_plan(M, N, K);
+  const mfq::Int8Plan p = mfq::int8_plan(dtype, M, N, K);
   const size_t need = mfq::int8_workspace_bytes(p, M, N);
   if (need && !workspace) return MFQ_ENULL;
   if (need > workspace_bytes) return MFQ_ESCRATCH;

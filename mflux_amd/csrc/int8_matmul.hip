@@ -25,209 +25,295 @@ struct I32 {  // a range's sums as they are, for the kernel that joins them
 __device__ inline float value_of(int sum, float xs, float ws, float add) { return (float)sum * xs * ws + add; }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------
-// A workgroup of four wavefronts computes kM x kN outputs, a wavefront kWM x kWN of them on v_mfma_i32_32x32x32_i8 with w as
-// the first operand (a lane's registers are four neighbouring columns of y each, of one row).
-//   - x and w go from memory straight into LDS, 128 bytes of a row at a time: kStages steps of both, the 16-byte column of a row
-//     XORed with (row / 2) % 8, so that the 32 rows of a fragment spread over the banks;
-//   - the fragments of a quarter step (32 k) are read while the one before them is multiplied, across the end of a step too:
-//     the one barrier of a step lies in front of its last quarter, where the fragments of that quarter are in registers (the
-//     step's LDS is free for the step kStages later) and the next step's LDS has arrived.
-template <int kM_, int kN_, int kWM_, int kWN_, int kStages_>
+// A workgroup of four wavefronts computes kM x kN outputs, a wavefront kWM x kWN of them on v_mfma_i32_16x16x64_i8 with w as
+// the first operand (a lane's registers are four neighbouring columns of y, of one row).
+//   - x and w go from memory straight into LDS, a step's 128 bytes of a row at a time, into a ring of units (a step of x, then
+//     a step of w, in turn), the 16-byte column of a row XORed with swz_mask(row);
+//   - the fragments of half a step (64 k) are read while the half before them is multiplied, across the end of a step too: the
+//     one barrier of a step lies in front of its second half, where the fragments of that half are in registers (the step's two
+//     units are free) and the next step's units have arrived;
+//   - workgroups stay and walk tiles; the ring runs on over a tile's end, and results go from the registers to memory.
+// Large products are bound by power: matrix instructions alone, on operands that stay in registers (codes of a normal
+// distribution), reach 4.0 PFLOP/s where the second operand stays from one instruction to the next, 3.4 where the first one
+// does, 3.0 where both change (32x32x32: 3.4; zeros, bound by issue: 4.2, 32x32x32 4.9).
+template <int kM_, int kN_, int kWM_, int kWN_, int kUnits_>
 struct Tile {
-  static constexpr int kM = kM_, kN = kN_, kWM = kWM_, kWN = kWN_, kStages = kStages_;
+  static constexpr int kM = kM_, kN = kN_, kWM = kWM_, kWN = kWN_, kUnits = kUnits_;
   static constexpr int kAcross = kM / kWM, kWaves = kAcross * (kN / kWN), kThreads = kWaves * kWave;
-  static constexpr int kI = kWM / 32, kJ = kWN / 32;
-  static constexpr int kStageBytes = (kM + kN) * BK;
-  static constexpr int kLoads = (kM + kN) / 8 / kWaves;  // of a wavefront, a KiB each
-  static constexpr int kOutStride = kWN * 4 + 16;        // a staged row of results, of 32-bit types
-  static constexpr int kOutBytes = kWaves * (32 * kOutStride + 2 * kWN * 4);  // and w's scales and the bias of a wavefront's columns
-  static constexpr int kLds = kStages * kStageBytes > kOutBytes ? kStages * kStageBytes : kOutBytes;
-  static constexpr int kXLoads = kM / 8 / kWaves;
-  static_assert(kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && kLds <= kMaxLds, "");
+  static constexpr int kI = kWM / 16, kJ = kWN / 16;
+  static constexpr int kXLoads = kM / 8 / kWaves, kWLoads = kN / 8 / kWaves;  // of a wavefront for a unit, a KiB each
+  static constexpr int kUnitBytes = (kM > kN ? kM : kN) * BK;
+  static constexpr int kLds = kUnits * kUnitBytes;
+  static constexpr int loads(int unit) { return unit % 2 ? kWLoads : kXLoads; }
+  // loads of the units from `from` to the last one requested, before the next request (of units kUnits, kUnits + 1)
+  static constexpr int behind(int from) {
+    int n = 0;
+    for (int u = from; u < kUnits; ++u) n += loads(u);
+    return n;
+  }
+  static_assert(kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && kLds <= kMaxLds && kUnits >= 4 && behind(2) < 64, "");
 };
 
-template <typename S, typename T>
-__global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int tiles_m, int tiles_n, int splits, void* out) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kI = S::kI, kJ = S::kJ, kLoads = S::kLoads;
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
-  const int r = lane & 31, h = lane >> 5;
+// The 16-byte column of a 128-byte row of LDS is XORed with this, so that the rows of a fragment that are read together (columns
+// 2 (lane / 16) + half) spread over the banks: see qmm_frag.hip
+__device__ inline int swz_mask(int row) {
+  const int i = (row >> 1) & 7;
+  return (i & 4) | ((i & 1) << 1) | ((i >> 2) ^ ((i >> 1) & 1));
+}
 
-  // Work item = (range of K, tile); an XCD walks a contiguous run of the tiles, in bands of four tile rows
-  const int n_tiles = tiles_m * tiles_n;
-  const int split = __builtin_amdgcn_readfirstlane((int)blockIdx.x / n_tiles);
-  int tile = (int)blockIdx.x - split * n_tiles;
+// An item's part of the product: a tile and a range of K
+struct Item {
+  int64_t m0, n0;
+  int split, first, steps;
+};
+
+template <typename S>
+__device__ inline Item item_of(int item, int tiles_m, int tiles_n, int splits, int all_steps) {
+  const int n_tiles = tiles_m * tiles_n, split = item / n_tiles;
+  int tile = item - split * n_tiles;
+  // an XCD (every eighth workgroup) walks a contiguous run of the tiles, in bands of four tile rows
   const int per_xcd = n_tiles / 8;
   if (tile < per_xcd * 8) tile = (tile & 7) * per_xcd + (tile >> 3);
   constexpr int kBand = 4;
   const int band = tile / (kBand * tiles_n), band_rows = min(tiles_m - band * kBand, kBand), in_band = tile - band * kBand * tiles_n;
-  const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * kBand + in_band % band_rows) * S::kM;
-  const int64_t n0 = (int64_t)__builtin_amdgcn_readfirstlane(in_band / band_rows) * S::kN;
+  Item it;
+  it.m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * kBand + in_band % band_rows) * S::kM;
+  it.n0 = (int64_t)__builtin_amdgcn_readfirstlane(in_band / band_rows) * S::kN;
+  it.split = __builtin_amdgcn_readfirstlane(split);
+  it.first = __builtin_amdgcn_readfirstlane(all_steps * split / splits);  // of at most 1024 steps and 64 ranges
+  it.steps = __builtin_amdgcn_readfirstlane(all_steps * (split + 1) / splits) - it.first;
+  return it;
+}
 
-  const int all_steps = ((int)c.K + BK - 1) / BK;  // at most 1024, of at most 1024 ranges
-  const int first = __builtin_amdgcn_readfirstlane(all_steps * split / splits);
-  const int steps = __builtin_amdgcn_readfirstlane(all_steps * (split + 1) / splits) - first;
+template <typename S, typename T>
+__global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int tiles_m, int tiles_n, int splits, void* out) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kI = S::kI, kJ = S::kJ;
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int r = lane & 15, q4 = lane >> 4;
+  const int items = tiles_m * tiles_n * splits, all_steps = ((int)c.K + BK - 1) / BK;
+  auto item_at = [&](int item) __attribute__((always_inline)) { return item_of<S>(item, tiles_m, tiles_n, splits, all_steps); };
 
-  // ---- what the wavefront loads: eight rows x 128 bytes an instruction, the tile's rows of x dealt to the wavefronts in
-  // turn, then those of w
+  // ---- requests: eight rows x 128 bytes an instruction, a unit's rows dealt to the wavefronts in turn.  x and w have a
+  // place of their own in the sequence of (item, step).  Behind the last item they stay where they are.
   const int own_row = wave * 8 + (lane >> 3);
-  const int last_x = (int)min(c.M - m0, (int64_t)S::kM) - 1, last_w = (int)min(c.N - n0, (int64_t)S::kN) - 1;
-  uint32_t row_at[kLoads];
-#pragma unroll
-  for (int l = 0; l < kLoads; ++l)
-    row_at[l] = l < S::kXLoads ? (uint32_t)min(own_row + 8 * S::kWaves * l, last_x) * (uint32_t)c.x_stride
-                               : (uint32_t)min(own_row + 8 * S::kWaves * (l - S::kXLoads), last_w) * (uint32_t)c.w_stride;
-  const int8_t *x0 = c.x + m0 * c.x_stride, *w0 = c.w + n0 * c.w_stride;
-  const uint32_t column = 16 * ((lane & 7) ^ ((own_row >> 1) & 7));  // of a row, that goes to the lane's place
+  const uint32_t column = 16 * ((lane & 7) ^ swz_mask(own_row));  // of a row, that goes to the lane's place
+  const uint32_t tail = (uint32_t)((c.K - 1) & (BK - 1)) + 1;        // bytes of a row in the last step of all
+  const uint32_t last_column = min(column, tail - 16);                // the bytes past the end of K repeat others; x's are cleared below
   const uint32_t lds_addr = (uint32_t)(uintptr_t)lds + (uint32_t)(wave * 8 * BK);
-  const uint32_t tail = (uint32_t)((c.K - 1) & (BK - 1)) + 1;  // bytes of a row in the last step of all
-  // Step q of the item into its stage.  The bytes of the last step past the end of K repeat others; x's are cleared below.
-  auto load = [&](int q, int stage) __attribute__((always_inline)) {
-    const int at = first + q;
-    const uint32_t col = min(column, at == all_steps - 1 ? tail - 16 : (uint32_t)BK - 16);
-    const uint32_t to = lds_addr + (uint32_t)(stage * S::kStageBytes);
-#pragma unroll
-    for (int l = 0; l < kLoads; ++l)
-      asm volatile("s_add_i32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                   ::"v"(row_at[l] + col), "s"((l < S::kXLoads ? x0 : w0) + (int64_t)at * BK), "s"(to), "i"(l * S::kWaves * 1024)
-                   : "memory", "m0", "scc");
+  struct Place {
+    int item, at, left;  // step of K, steps left of the item
+    const int8_t* p;
   };
-  // x past the end of K, once it has arrived
-  auto clear_tail = [&](int stage) __attribute__((always_inline)) {
-    if (column < tail) return;
+  Place px, pw;
+  uint32_t x_row[S::kXLoads], w_row[S::kWLoads];
+  auto begin = [&](auto is_x, Place& to, uint32_t* rows, int item) __attribute__((always_inline)) {
+    const Item it = item_at(item);
+    const int64_t from = is_x ? it.m0 : it.n0, stride = is_x ? c.x_stride : c.w_stride;
+    const int last = (int)min((is_x ? c.M : c.N) - from, (int64_t)(is_x ? S::kM : S::kN)) - 1;
 #pragma unroll
-    for (int l = 0; l < S::kXLoads; ++l)
-      *reinterpret_cast<u32x4*>(lds + stage * S::kStageBytes + (wave + l * S::kWaves) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+    for (int l = 0; l < (is_x ? S::kXLoads : S::kWLoads); ++l) rows[l] = (uint32_t)min(own_row + 8 * S::kWaves * l, last) * (uint32_t)stride;
+    to.item = item;
+    to.at = it.first;
+    to.left = it.steps;
+    to.p = (is_x ? c.x : c.w) + from * stride + (int64_t)it.first * BK;
+  };
+  auto advance = [&](auto is_x, Place& to, uint32_t* rows) __attribute__((always_inline)) {
+    if (--to.left) {
+      to.p += BK;
+      ++to.at;
+    } else if (to.item + (int)gridDim.x < items) {
+      begin(is_x, to, rows, to.item + (int)gridDim.x);
+    } else {
+      to.left = 1;
+    }
+  };
+  constexpr std::true_type kX{};
+  constexpr std::false_type kW{};
+  auto request = [&](auto is_x, int l, int slot) __attribute__((always_inline)) {
+    const Place& from = is_x ? px : pw;
+    const uint32_t off = (is_x ? x_row : w_row)[l] + (from.at == all_steps - 1 ? last_column : column);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr + (uint32_t)(slot * S::kUnitBytes));
+    asm volatile("s_add_i32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 ::"v"(off), "s"(from.p), "s"(to), "i"(l * S::kWaves * 1024) : "memory", "m0", "scc");
+  };
+  // the slots of the ring, a step's x and w: (slot, slot + 1)
+  auto next_slot = [](int slot, int by) __attribute__((always_inline)) { return slot + by >= S::kUnits ? slot + by - S::kUnits : slot + by; };
+  // x past the end of K, once it has arrived
+  auto clear_tail = [&](int slot) __attribute__((always_inline)) {
+    if (column >= tail) {
+#pragma unroll
+      for (int l = 0; l < S::kXLoads; ++l)
+        *reinterpret_cast<u32x4*>(lds + slot * S::kUnitBytes + (wave + l * S::kWaves) * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
 
-  // ---- fragments
+  // ---- fragments.  Lane (r, q4) has 16 bytes of row r, those of column 2 q4 + half of a step.
   const int wm = wave % S::kAcross * S::kWM, wn = wave / S::kAcross * S::kWN;
   i32x4 xf[2][kI], wf[2][kJ];
-  const int swz = (r >> 1) & 7;
-  auto read = [&](int set, int stage, int quarter) __attribute__((always_inline)) {
-    const char* p = lds + stage * S::kStageBytes + r * BK + (((2 * quarter + h) ^ swz) << 4);
-#pragma unroll
-    for (int j = 0; j < kJ; ++j) wf[set][j] = *reinterpret_cast<const i32x4*>(p + (S::kM + wn + 32 * j) * BK);
-#pragma unroll
-    for (int i = 0; i < kI; ++i) xf[set][i] = *reinterpret_cast<const i32x4*>(p + (wm + 32 * i) * BK);
+  const int x_at = (wm + r) * BK, w_at = (wn + r) * BK, swz = swz_mask(r);
+  // fragment f of a half, in the order of their use: the first of x, those of w, the others of x
+  auto read = [&](int set, int slot, int half, int f) __attribute__((always_inline)) {
+    const int at = ((2 * q4 + half) ^ swz) << 4;
+    if (f >= 1 && f <= kJ) wf[set][f - 1] = *reinterpret_cast<const i32x4*>(lds + next_slot(slot, 1) * S::kUnitBytes + at + w_at + (f - 1) * 16 * BK);
+    else xf[set][f ? f - kJ : 0] = *reinterpret_cast<const i32x4*>(lds + slot * S::kUnitBytes + at + x_at + (f ? f - kJ : 0) * 16 * BK);
   };
-  i32x16 acc[kI][kJ];
+  i32x4 acc[kI][kJ];
+  // Multiplies half a step's fragments (`fresh`: the first of an item); in between, reads those of (slot, next) into the other set
+  // and requests a unit.  Reads and requests are dealt out over the first three quarters of the instructions.
+  constexpr int kOneX = 1, kOneW = 2;
+  auto half_step = [&](auto fresh_c, auto set_c, auto unit_c, int slot, int next, int to) __attribute__((always_inline)) {
+    constexpr int set = decltype(set_c)::value, unit = decltype(unit_c)::value;
+    constexpr int kInstr = kI * kJ, kSpan = kInstr >= 16 ? kInstr * 3 / 4 : kInstr, kReads = kI + kJ;
+    constexpr int kRequests = unit == kOneX ? S::kXLoads : S::kWLoads;
 #pragma unroll
-  for (int i = 0; i < kI; ++i)
+    for (int n = 0; n < kInstr; ++n) {
+      const int i = n / kJ, j = n % kJ;
+      acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[set][j], xf[set][i], decltype(fresh_c)::value ? i32x4{0, 0, 0, 0} : acc[i][j], 0, 0, 0);
+      if (n < kSpan) {
 #pragma unroll
-    for (int j = 0; j < kJ; ++j)
+        for (int f = kReads * n / kSpan; f < kReads * (n + 1) / kSpan; ++f) read(set ^ 1, slot, next, f);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-  auto multiply = [&](int set) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < kJ; ++j)
-#pragma unroll
-      for (int i = 0; i < kI; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[set][j], xf[set][i], acc[i][j], 0, 0, 0);
-  };
-  // own loads of the next step have arrived (and everything the wavefront has read from LDS is in registers), for all wavefronts
-  auto arrive = [&](int q) __attribute__((always_inline)) {  // q: the step that must be there
-    if (S::kStages > 2 && q + S::kStages - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::kStages - 2) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    if (tail < BK && first + q == all_steps - 1) {
-      clear_tail(q % S::kStages);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_barrier" ::: "memory");
-  };
-
-  if (steps > 0) {
-#pragma unroll
-    for (int q = 0; q < S::kStages; ++q)
-      if (q < steps) load(q, q);
-    if (S::kStages > 1 && steps >= S::kStages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S::kStages - 1) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (tail < BK && first == all_steps - 1) {
-      clear_tail(0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_barrier" ::: "memory");
-    read(0, 0, 0);
-    int stage = 0;
-    for (int q = 0; q < steps; ++q) {
-      const int after = stage + 1 == S::kStages ? 0 : stage + 1;
-      read(1, stage, 1);
-      multiply(0);
-      read(0, stage, 2);
-      multiply(1);
-      read(1, stage, 3);
-      multiply(0);
-      if (q + 1 < steps) {
-        arrive(q + 1);
-        if (q + S::kStages < steps) load(q + S::kStages, stage);
-        read(0, after, 0);
+        for (int l = kRequests * n / kSpan; l < kRequests * (n + 1) / kSpan; ++l) {
+          if constexpr (unit == kOneX) request(kX, l, to);
+          else request(kW, l, to);
+        }
       }
-      multiply(1);
-      stage = after;
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // LDS is free for the results
+    if constexpr (unit == kOneX) advance(kX, px, x_row);
+    else advance(kW, pw, w_row);
+  };
+#define MFQ_C(v) std::integral_constant<int, v>{}
 
-  // ---- results: strips of 32 rows through a private region of LDS, so that whole row segments are written
-  // register e of acc[i][j] is row wm + 32 i + r, column wn + 32 j + 8 (e / 4) + 4 h + e % 4
+  // ---- results.  Element e of acc[i][j] is row wm + 16 i + r, column wn + 16 j + 4 q4 + e.  16-bit types: two neighbouring
+  // blocks of 16 columns exchange quads, so that a lane has eight columns of one of them.
   using E = typename T::storage;
   constexpr bool kRaw = std::is_same_v<T, I32>;
-  constexpr int kEach = 16 / (int)sizeof(E);               // values of a 16-byte piece
-  constexpr int kStride = S::kWN * (int)sizeof(E) + 16;
-  constexpr int kPieces = S::kWN / kEach, kRowsAtOnce = kWave / kPieces;
-  char* strip = lds + wave * 32 * S::kOutStride;
-  E* y = static_cast<E*>(out) + (kRaw ? (int64_t)split * c.M * c.N : 0);
-  const E* bias = static_cast<const E*>(c.bias);
-  const bool whole = c.N % kEach == 0;
-  float* w_scales = reinterpret_cast<float*>(lds + S::kWaves * 32 * S::kOutStride) + wave * 2 * S::kWN;
-  if constexpr (!kRaw) {
+  auto store = [&](const Item& it) __attribute__((always_inline)) {
+    constexpr int kEach = 16 / (int)sizeof(E);
+    const bool whole = c.N % kEach == 0;
+    const int64_t n0 = it.n0 + wn, m0 = it.m0 + wm + r;
+    char* y = static_cast<char*>(out) + ((kRaw ? (int64_t)it.split * c.M : 0) + m0) * c.N * (int64_t)sizeof(E);
+    float xs[kI];
 #pragma unroll
-    for (int k = lane; k < S::kWN; k += kWave) {
-      const int64_t n = min(n0 + wn + k, c.N - 1);
-      w_scales[k] = c.w_scales[n];
-      w_scales[S::kWN + k] = bias ? T::to_f32(bias[n]) : 0.f;
-    }
-  }
+    for (int i = 0; i < kI; ++i) xs[i] = kRaw ? 0.f : c.x_scales[min(m0 + 16 * i, c.M - 1)];
+    constexpr int kPair = sizeof(E) == 2 ? 2 : 1;  // blocks of columns at a time
 #pragma unroll
-  for (int i = 0; i < kI; ++i) {
-    const int64_t m = m0 + wm + 32 * i + r;
-    float xs = 0.f;
-    if constexpr (!kRaw) xs = c.x_scales[min(m, c.M - 1)];
+    for (int j = 0; j < kJ; j += kPair) {
+      if (n0 + 16 * j >= c.N) continue;
+      float ws[kPair][4], add[kPair][4];
+      if constexpr (!kRaw) {
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) {
+        for (int p = 0; p < kPair; ++p)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int col = 32 * j + 8 * b + 4 * h;
-        if constexpr (kRaw) {
-          *reinterpret_cast<i32x4*>(strip + r * kStride + col * 4) =
-              i32x4{acc[i][j][4 * b], acc[i][j][4 * b + 1], acc[i][j][4 * b + 2], acc[i][j][4 * b + 3]};
+          for (int e = 0; e < 4; ++e) {
+            const int64_t n = min(n0 + 16 * (j + p) + 4 * q4 + e, c.N - 1);
+            ws[p][e] = c.w_scales[n];
+            add[p][e] = 0.f;
+            if (c.bias) add[p][e] = T::to_f32(static_cast<const E*>(c.bias)[n]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        E* row = reinterpret_cast<E*>(y + (int64_t)(16 * i) * c.N * (int64_t)sizeof(E));
+        const bool inside = m0 + 16 * i < c.M;
+#pragma unroll
+        for (int p = 0; p < kPair; ++p) asm volatile("" : "+a"(acc[i][j + p]));  // (or all of acc is moved to vector registers at the loop's end)
+        if constexpr (sizeof(E) == 2) {
+          uint32_t a[2], b[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            a[k] = T::pack2(value_of(acc[i][j][2 * k], xs[i], ws[0][2 * k], add[0][2 * k]),
+                            value_of(acc[i][j][2 * k + 1], xs[i], ws[0][2 * k + 1], add[0][2 * k + 1]));
+            b[k] = T::pack2(value_of(acc[i][j + 1][2 * k], xs[i], ws[1][2 * k], add[1][2 * k]),
+                            value_of(acc[i][j + 1][2 * k + 1], xs[i], ws[1][2 * k + 1], add[1][2 * k + 1]));
+            // a of odd q4 and b of even q4 change places: lane q4 has the quads q4 & ~1 and q4 | 1 of block j + q4 % 2
+            const auto s = __builtin_amdgcn_permlane16_swap(a[k], b[k], false, false);
+            a[k] = s[0];
+            b[k] = s[1];
+          }
+          const int64_t n = n0 + 16 * (j + (q4 & 1)) + 8 * (q4 >> 1);
+          if (!inside) continue;
+          if (whole) {
+            if (n < c.N) *reinterpret_cast<u32x4*>(row + n) = u32x4{a[0], a[1], b[0], b[1]};
+          } else {
+            const uint64_t low = a[0] | (uint64_t)a[1] << 32, high = b[0] | (uint64_t)b[1] << 32;
+#pragma unroll 1
+            for (int k = 0; k < 8 && n + k < c.N; ++k) row[n + k] = (E)((k < 4 ? low : high) >> (16 * (k & 3)));
+          }
         } else {
-          const f32x4 ws = *reinterpret_cast<const f32x4*>(w_scales + col), add = *reinterpret_cast<const f32x4*>(w_scales + S::kWN + col);
-          float v[4];
+          E q[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = value_of(acc[i][j][4 * b + e], xs, ws[e], add[e]);
-          if constexpr (sizeof(E) == 2) *reinterpret_cast<u32x2*>(strip + r * kStride + col * 2) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-          else *reinterpret_cast<f32x4*>(strip + r * kStride + col * 4) = f32x4{v[0], v[1], v[2], v[3]};
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (kRaw) q[k] = acc[i][j][k];
+            else q[k] = value_of(acc[i][j][k], xs[i], ws[0][k], add[0][k]);
+          }
+          const int64_t n = n0 + 16 * j + 4 * q4;
+          if (!inside) continue;
+          typedef E quad __attribute__((ext_vector_type(4)));
+          if (whole) {
+            if (n < c.N) *reinterpret_cast<quad*>(row + n) = quad{q[0], q[1], q[2], q[3]};
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (n + k < c.N) row[n + k] = q[k];
+          }
         }
       }
     }
-    const int piece = lane % kPieces;
-    const int64_t n = n0 + wn + piece * kEach;
+  };
+
+  // ---- the walk
+  int item = blockIdx.x;
+  Item it = item_at(item);
+  begin(kX, px, x_row, item);
+  begin(kW, pw, w_row, item);
 #pragma unroll
-    for (int k = 0; k < 32 / kRowsAtOnce; ++k) {
-      const int row = k * kRowsAtOnce + lane / kPieces;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(strip + row * kStride + piece * 16);
-      const int64_t at = m0 + wm + 32 * i + row;
-      if (at >= c.M) continue;
-      if (whole) {
-        if (n < c.N) *reinterpret_cast<u32x4*>(y + at * c.N + n) = v;
-      } else {
-        const E* e = reinterpret_cast<const E*>(&v);
+  for (int u = 0; u < S::kUnits - 1; ++u) {
+    if (u % 2 == 0) {
 #pragma unroll
-        for (int k2 = 0; k2 < kEach; ++k2)
-          if (n + k2 < c.N) y[at * c.N + n + k2] = e[k2];
-      }
+      for (int l = 0; l < S::kXLoads; ++l) request(kX, l, u);
+      advance(kX, px, x_row);
+    } else {
+#pragma unroll
+      for (int l = 0; l < S::kWLoads; ++l) request(kW, l, u);
+      advance(kW, pw, w_row);
     }
   }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::behind(2) - S::loads(S::kUnits - 1)) : "memory");
+  if (tail < BK && it.first == all_steps - 1) clear_tail(0);
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int f = 0; f < kI + kJ; ++f) read(0, 0, 0, f);
+  // The units requested in a step: the one that takes the place of its x, in its second half, and the one that takes that of its
+  // w, in the next step's first
+  constexpr int kFirst = S::kUnits % 2 ? kOneW : kOneX, kSecond = S::kUnits % 2 ? kOneX : kOneW;
+  int slot = 0, pending = S::kUnits - 1;
+  auto step = [&](auto fresh, int next_at) __attribute__((always_inline)) {  // next_at: step of K of the one after
+    half_step(fresh, MFQ_C(0), MFQ_C(kSecond), slot, 1, pending);
+    // everything read is in registers, the next step's units have arrived: for all wavefronts, behind the barrier.  (Behind the
+    // last step of all the ring goes round as well: what is requested and read there is not used.)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(S::behind(4)) : "memory");
+    const int after = next_slot(slot, 2);
+    if (tail < BK && next_at == all_steps - 1) clear_tail(after);
+    asm volatile("s_barrier" ::: "memory");
+    half_step(std::false_type{}, MFQ_C(1), MFQ_C(kFirst), after, 0, slot);
+    pending = next_slot(slot, 1);
+    slot = after;
+  };
+  for (;;) {
+    const int next_first = item + (int)gridDim.x < items ? item_at(item + (int)gridDim.x).first : 0;
+    step(std::true_type{}, it.steps > 1 ? it.first + 1 : next_first);
+    for (int q = 1; q < it.steps; ++q) step(std::false_type{}, q + 1 < it.steps ? it.first + q + 1 : next_first);
+    store(it);
+    item += (int)gridDim.x;
+    if (item >= items) break;
+    it = item_at(item);
+  }
+#undef MFQ_C
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // requests on their way into LDS
 }
 
 // ---- few rows of x --------------------------------------------------------------------------------------------------------
@@ -335,10 +421,10 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Call c, const int* p
   else *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-using Tile32 = Tile<32, 128, 32, 32, 4>;
-using Tile64 = Tile<64, 64, 32, 32, 4>;
-using Tile128 = Tile<128, 128, 64, 64, 2>;
-using Tile256 = Tile<256, 256, 128, 128, 2>;
+using Tile32 = Tile<32, 128, 32, 32, 5>;
+using Tile64 = Tile<64, 64, 32, 32, 10>;
+using Tile128 = Tile<128, 128, 64, 64, 5>;
+using Tile256 = Tile<256, 256, 128, 128, 5>;
 
 template <typename S, typename T>
 int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
@@ -346,8 +432,9 @@ int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(&int8_tile_kernel<S, T>);
   if (!raise_lds_limit(limit, kernel, S::kLds)) return MFQ_ELAUNCH;
   const int64_t tiles_m = (c.M + S::kM - 1) / S::kM, tiles_n = (c.N + S::kN - 1) / S::kN;
-  hipLaunchKernelGGL((int8_tile_kernel<S, T>), dim3((unsigned)(tiles_m * tiles_n * splits)), dim3(S::kThreads), S::kLds, stream, c, (int)tiles_m,
-                     (int)tiles_n, splits, out);
+  const int64_t items = tiles_m * tiles_n * splits, places = (int64_t)compute_units() * (kMaxLds / S::kLds);
+  hipLaunchKernelGGL((int8_tile_kernel<S, T>), dim3((unsigned)(items < places ? items : places)), dim3(S::kThreads), S::kLds, stream, c,
+                     (int)tiles_m, (int)tiles_n, splits, out);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 
@@ -356,7 +443,10 @@ int launch_tiles_of(const Int8Call& c, const Int8Plan& p, void* out, hipStream_t
   if (p.rows == 32) return launch_tiles<Tile32, T>(c, p.splits, out, stream);
   if (p.rows == 64) return launch_tiles<Tile64, T>(c, p.splits, out, stream);
   if (p.rows == 128) return launch_tiles<Tile128, T>(c, p.splits, out, stream);
-  return launch_tiles<Tile256, T>(c, p.splits, out, stream);
+  if constexpr (sizeof(typename T::storage) == 2) {
+    if (p.rows == 256) return launch_tiles<Tile256, T>(c, p.splits, out, stream);
+  }
+  return MFQ_EUNSUPPORTED;
 }
 
 template <typename T>
@@ -379,13 +469,13 @@ int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t st
 
 }  // namespace
 
-Int8Plan int8_plan(int64_t M, int64_t N, int64_t K) {
+Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K) {
   if (M <= 16) return {MFQ_INT8_FEW, 1, (int)M, 16};
   const int64_t units = compute_units(), steps = (K + BK - 1) / BK;
   Int8Plan p = {MFQ_INT8_TILES, 1, 256, 256};
   if (M <= 32) p.rows = 32, p.columns = 128;
   else if (M <= 64) p.rows = p.columns = 64;
-  else if (((M + 255) / 256) * ((N + 255) / 256) < units * 3 / 4) p.rows = p.columns = 128;
+  else if (dtype == MFQ_F32 || ((M + 255) / 256) * ((N + 255) / 256) < units * 3 / 4) p.rows = p.columns = 128;
   const int64_t tiles = ((M + p.rows - 1) / p.rows) * ((N + p.columns - 1) / p.columns);
   const int64_t places = p.rows == 256 ? units : 2 * units;
   if (tiles * 2 <= places) {

@@ -41,7 +41,7 @@ struct Int8Plan {
   int splits;   // ranges of K
   int rows, columns;  // of a workgroup's tile
 };
-Int8Plan int8_plan(int64_t M, int64_t N, int64_t K);
+Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K);
 size_t int8_workspace_bytes(const Int8Plan& p, int64_t M, int64_t N);
 int launch_int8_matmul(int dtype, const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t stream);
 

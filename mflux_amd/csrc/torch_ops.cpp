@@ -996,7 +996,7 @@ Tensor int8_matmul(const Tensor& x, const Tensor& x_scales, const Tensor& w, con
   if (y.numel() == 0) return y;
   const Tensor xr = int8_rows(rows_of(x), length, true), wr = int8_rows(w, length, false);
   const Tensor xs = x_scales.contiguous(), ws = w_scales.contiguous(), b = bias.has_value() ? bias->contiguous() : Tensor();
-  const size_t bytes = mfq_int8_matmul_workspace_bytes(M, N, length);
+  const size_t bytes = mfq_int8_matmul_workspace_bytes(M, N, length, dtype_code(dtype, "the result"));
   Tensor scratch;
   if (bytes) scratch = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
   check_status("mfq_int8_matmul",
