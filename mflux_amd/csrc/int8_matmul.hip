@@ -317,76 +317,126 @@ __global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int 
 }
 
 // ---- few rows of x --------------------------------------------------------------------------------------------------------
-// Up to 16 rows of x: bound by the bytes of w, which go from memory straight into registers.  On v_mfma_i32_16x16x64_i8 lane
-// (j, q) = (lane % 16, lane / 16) supplies 16 bytes of row j of either operand.  One load instruction of w takes eight rows x
+// Bound by the bytes of w, which go from memory straight into registers, kRing KiB of a wavefront ahead.  On v_mfma_i32_16x16x64_i8
+// lane (j, q) = (lane % 16, lane / 16) supplies 16 bytes of row j of either operand.  One load instruction of w takes eight rows x
 // 128 bytes, whole cache lines: operand row j is row j / 2, bytes 64 (j % 2) + 16 q.  x enters as eight rows x 128 bytes as
 // well, operand row j being row j % 8, bytes 64 (j / 8) + 16 q.  Of the 16 x 16 results those belong together whose halves are the
-// same (row 8 h + token, column 2 row + h); the others are dropped.  The wavefronts of a workgroup take a range of K each of
-// the same 16 rows of w, and their sums meet in LDS.
-template <int kTokens, int kWaves, typename T>
-__global__ __launch_bounds__(kWaves* kWave) void int8_few_kernel(Int8Call c) {
+// same (row 8 h + token, column 2 row + h); the others are dropped.
+// A workgroup walks a run of blocks of eight rows of w, its wavefronts have a range of K each; a lane keeps its share of x in
+// LDS (nothing is exchanged before the end), and the wavefronts' sums meet there behind the last block.
+constexpr int kFewMaxWaves = 16;
+
+// LDS of a workgroup: x, and a block's sums
+__host__ __device__ inline int few_image(int tokens8, int steps, int waves) { return tokens8 * 1024 * steps * waves; }
+__host__ __device__ inline int few_sums(int tokens8, int waves) { return tokens8 * 512 * waves; }
+
+template <int kX, int kRing, typename T>
+__global__ __launch_bounds__(kFewMaxWaves* kWave) void int8_few_kernel(Int8Call c, int waves, int steps, int per_group, int groups) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
   using E = typename T::storage;
-  constexpr int kX = kTokens / 8, kW = 2, kAhead = 4;
   const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int j = lane & 15, q = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int all_steps = (int)((c.K + BK - 1) / BK), tail = (int)((c.K - 1) & (BK - 1)) + 1;
-  const int first = (int)((int64_t)all_steps * wave / kWaves), end = (int)((int64_t)all_steps * (wave + 1) / kWaves);
-  const int w_column = 64 * (j & 1) + 16 * q, x_column = 64 * (j >> 3) + 16 * q;
-  const int8_t *wp[kW], *xp[kX];
-#pragma unroll
-  for (int b = 0; b < kW; ++b) wp[b] = c.w + min(n0 + 8 * b + (j >> 1), c.N - 1) * c.w_stride;
-#pragma unroll
-  for (int b = 0; b < kX; ++b) xp[b] = c.x + min((int64_t)(8 * b + (j & 7)), c.M - 1) * c.x_stride;
-  i32x4 w[kAhead][kW], x[kAhead][kX], acc[kW][kX];
-#pragma unroll
-  for (int b = 0; b < kW; ++b)
-#pragma unroll
-    for (int a = 0; a < kX; ++a) acc[b][a] = i32x4{0, 0, 0, 0};
-  // steps past the wavefront's end repeat its last one and are never multiplied; bytes past the end of K repeat others, x's are 0
-  auto load = [&](int s, int slot) __attribute__((always_inline)) {
-    const int at = max(min(s, end - 1), 0), most = at == all_steps - 1 ? tail - 16 : BK - 16;
-    const bool past = x_column > most;
-#pragma unroll
-    for (int b = 0; b < kW; ++b) w[slot][b] = *reinterpret_cast<const i32x4*>(wp[b] + (int64_t)at * BK + min(w_column, most));
-#pragma unroll
-    for (int a = 0; a < kX; ++a) {
-      x[slot][a] = *reinterpret_cast<const i32x4*>(xp[a] + (int64_t)at * BK + min(x_column, most));
-      if (past) x[slot][a] = i32x4{0, 0, 0, 0};
+  // the workgroups of a run of w are eight apart, on one XCD: all but the first find w in a cache
+  const int eight = (int)blockIdx.x >> 3, run = eight / groups * 8 + ((int)blockIdx.x & 7), token0 = eight % groups * 8 * kX;
+  const int64_t all_blocks = (c.N + 7) / 8, first_block = (int64_t)run * per_group;
+  const int blocks = (int)max(min(all_blocks - first_block, (int64_t)per_group), (int64_t)0);
+  const int all_steps = ((int)c.K + BK - 1) / BK, tail = (int)((c.K - 1) & (BK - 1)) + 1;
+  const int first = min(wave * steps, all_steps), mine = min(first + steps, all_steps) - first;  // the wavefront's steps
+
+  // ---- w: position p of the wavefront is step p % mine of block p / mine; positions behind the last repeat it
+  const int column = 64 * (j & 1) + 16 * q, last_column = min(column, tail - 16);
+  int ahead_block = 0, ahead_step = 0;
+  i32x4 w[kRing];
+  auto load = [&](int u) __attribute__((always_inline)) {
+    const int64_t row0 = (first_block + ahead_block) * 8;
+    const int row = (int)min((int64_t)(j >> 1), c.N - 1 - row0), at = first + ahead_step;
+    const int8_t* p = c.w + row0 * c.w_stride + (int64_t)at * BK;
+    w[u] = *reinterpret_cast<const i32x4*>(p + (row * (uint32_t)c.w_stride + (uint32_t)(at == all_steps - 1 ? last_column : column)));
+    if (ahead_step + 1 < mine) {
+      ++ahead_step;
+    } else if (ahead_block + 1 < blocks) {
+      ++ahead_block;
+      ahead_step = 0;
     }
   };
+  char* x = lds + wave * few_image(kX, steps, 1) + lane * 16;
+  int* sums = reinterpret_cast<int*>(lds + few_image(kX, steps, waves)) + wave * (few_sums(kX, 1) / 4);
+  const int block_ints = few_sums(kX, waves) / 4;
+  if (mine > 0 && blocks > 0) {
+    // x is requested before w, four steps at a time
+    const int x_column = 64 * (j >> 3) + 16 * q;
+    constexpr int kAtOnce = 4;
+    i32x4 v[kAtOnce][kX];
+    auto load_x = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-  for (int s = 0; s < kAhead; ++s) load(first + s, s);
-  for (int s = first; s < end; s += kAhead) {
+      for (int s = 0; s < kAtOnce; ++s) {
+        const int at = first + min(from + s, mine - 1), most = at == all_steps - 1 ? tail - 16 : BK - 16;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (s + u < end) {
-#pragma unroll
-        for (int b = 0; b < kW; ++b)
-#pragma unroll
-          for (int a = 0; a < kX; ++a) acc[b][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[u][a], w[u][b], acc[b][a], 0, 0, 0);
+        for (int a = 0; a < kX; ++a) {
+          v[s][a] = *reinterpret_cast<const i32x4*>(c.x + min((int64_t)(token0 + 8 * a + (j & 7)), c.M - 1) * c.x_stride + (int64_t)at * BK + min(x_column, most));
+          if (x_column > most) v[s][a] = i32x4{0, 0, 0, 0};
+        }
       }
-      load(s + u + kAhead, u);
-    }
-  }
-  // register e of a lane: operand row 4 q + e (half q / 2, token 4 (q % 2) + e), column j (row j / 2 of w, half j % 2)
-  __shared__ int sums[2 * kWaves][kTokens][kW * 8];
-  if ((j & 1) == (q >> 1)) {
+    };
+    auto keep_x = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < kW; ++b)
+      for (int s = 0; s < kAtOnce; ++s)
+        if (from + s < mine) {
+#pragma unroll
+          for (int a = 0; a < kX; ++a) *reinterpret_cast<i32x4*>(x + ((from + s) * kX + a) * 1024) = v[s][a];
+        }
+    };
+    load_x(0);
+#pragma unroll
+    for (int u = 0; u < kRing; ++u) load(u);
+    keep_x(0);
+    for (int s = kAtOnce; s < mine; s += kAtOnce) {
+      load_x(s);
+      keep_x(s);
+    }
+    i32x4 acc[kX];
+#pragma unroll
+    for (int a = 0; a < kX; ++a) acc[a] = i32x4{0, 0, 0, 0};
+    int step = 0;
+    auto multiply = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < kX; ++a)
+        acc[a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(x + (step * kX + a) * 1024), w[u], acc[a], 0, 0, 0);
+      if (++step < mine) return;
+      // the end of a block.  Register e of a lane: operand row 4 q + e (half q / 2, token 4 (q % 2) + e), column j (row j / 2 of w, half j % 2)
+      if ((j & 1) == (q >> 1)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sums[2 * wave + (j & 1)][8 * a + 4 * (q & 1) + e][8 * b + (j >> 1)] = acc[b][a][e];
+        for (int a = 0; a < kX; ++a) *reinterpret_cast<i32x4*>(sums + a * 128 + (j & 1) * 64 + (j >> 1) * 8 + 4 * (q & 1)) = acc[a];
+      }
+#pragma unroll
+      for (int a = 0; a < kX; ++a) acc[a] = i32x4{0, 0, 0, 0};
+      sums += block_ints;
+      step = 0;
+    };
+    int left = blocks * mine;
+    for (; left > kRing; left -= kRing) {
+#pragma unroll
+      for (int u = 0; u < kRing; ++u) {
+        multiply(u);
+        load(u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRing; ++u)
+      if (u < left) multiply(u);
+  } else {
+    for (int b = 0; b < blocks; ++b)
+      for (int k = lane; k < kX * 128; k += kWave) sums[b * block_ints + k] = 0;
   }
   __syncthreads();
-  for (int o = t; o < kTokens * kW * 8; o += kWaves * kWave) {
-    const int token = o / (kW * 8), row = o % (kW * 8);
-    const int64_t n = n0 + row;
+  const int* all = reinterpret_cast<const int*>(lds + few_image(kX, steps, waves));
+  for (int o = t; o < blocks * kX * 64; o += waves * kWave) {
+    const int row = o & 7, token = token0 + (o >> 3) % (8 * kX), block = o / (64 * kX), in_group = token - token0;
+    const int64_t n = (first_block + block) * 8 + row;
     if (token >= c.M || n >= c.N) continue;
+    const int* s = all + block * block_ints + (in_group >> 3) * 128 + row * 8 + (in_group & 7);
     int sum = 0;
-#pragma unroll
-    for (int k = 0; k < 2 * kWaves; ++k) sum += sums[k][token][row];
+    for (int k = 0; k < waves; ++k) sum += s[k * kX * 128] + s[k * kX * 128 + 64];
     const float v = value_of(sum, c.x_scales[token], c.w_scales[n], c.bias ? T::to_f32(static_cast<const E*>(c.bias)[n]) : 0.f);
     static_cast<E*>(c.y)[token * c.N + n] = T::from_f32(v);
   }
@@ -421,10 +471,14 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Call c, const int* p
   else *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-using Tile32 = Tile<32, 128, 32, 32, 5>;
-using Tile64 = Tile<64, 64, 32, 32, 10>;
-using Tile128 = Tile<128, 128, 64, 64, 5>;
-using Tile256 = Tile<256, 256, 128, 128, 5>;
+// The tiles.  The small ones, whose steps are bound by latency, keep more steps on their way.
+using Tile32x64 = Tile<32, 64, 16, 32, 20>;
+using Tile64x64 = Tile<64, 64, 32, 32, 20>;
+using Tile64x128 = Tile<64, 128, 32, 64, 10>;
+using Tile128x128 = Tile<128, 128, 64, 64, 10>;
+using Tile128x128Two = Tile<128, 128, 64, 64, 5>;  // two workgroups to a compute unit
+using Tile128x192 = Tile<128, 192, 64, 96, 6>;
+using Tile256x256 = Tile<256, 256, 128, 128, 5>;
 
 template <typename S, typename T>
 int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
@@ -433,6 +487,7 @@ int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
   if (!raise_lds_limit(limit, kernel, S::kLds)) return MFQ_ELAUNCH;
   const int64_t tiles_m = (c.M + S::kM - 1) / S::kM, tiles_n = (c.N + S::kN - 1) / S::kN;
   const int64_t items = tiles_m * tiles_n * splits, places = (int64_t)compute_units() * (kMaxLds / S::kLds);
+  if (items + places > INT32_MAX) return MFQ_ESHAPE;
   hipLaunchKernelGGL((int8_tile_kernel<S, T>), dim3((unsigned)(items < places ? items : places)), dim3(S::kThreads), S::kLds, stream, c,
                      (int)tiles_m, (int)tiles_n, splits, out);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
@@ -440,22 +495,63 @@ int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
 
 template <typename T>
 int launch_tiles_of(const Int8Call& c, const Int8Plan& p, void* out, hipStream_t stream) {
-  if (p.rows == 32) return launch_tiles<Tile32, T>(c, p.splits, out, stream);
-  if (p.rows == 64) return launch_tiles<Tile64, T>(c, p.splits, out, stream);
-  if (p.rows == 128) return launch_tiles<Tile128, T>(c, p.splits, out, stream);
-  if constexpr (sizeof(typename T::storage) == 2) {
-    if (p.rows == 256) return launch_tiles<Tile256, T>(c, p.splits, out, stream);
+  switch (p.rows * 1000 + p.columns) {
+    case 32064: return launch_tiles<Tile32x64, T>(c, p.splits, out, stream);
+    case 64064: return launch_tiles<Tile64x64, T>(c, p.splits, out, stream);
+    case 64128: return launch_tiles<Tile64x128, T>(c, p.splits, out, stream);
+    case 128128: return p.places == 2 ? launch_tiles<Tile128x128Two, T>(c, p.splits, out, stream) : launch_tiles<Tile128x128, T>(c, p.splits, out, stream);
+    case 128192: return launch_tiles<Tile128x192, T>(c, p.splits, out, stream);
+    default:
+      if constexpr (sizeof(typename T::storage) == 2) return launch_tiles<Tile256x256, T>(c, p.splits, out, stream);
+      else return MFQ_EUNSUPPORTED;  // the plan has none
   }
-  return MFQ_EUNSUPPORTED;
+}
+
+// Wavefronts of a workgroup and steps of a wavefront: the fewest steps left over, of 8 to 16 wavefronts
+void few_shape(int64_t K, int& waves, int& steps) {
+  const int all = (int)((K + BK - 1) / BK);
+  waves = all < 8 ? all : 8;
+  steps = (all + 7) / 8;
+  for (int w = 9; w <= kFewMaxWaves; ++w) {
+    const int each = (all + w - 1) / w;
+    if (each * w < steps * waves) waves = w, steps = each;
+  }
+}
+struct Few {
+  int waves, steps, per_group, groups, grid;
+};
+
+template <int kX, int kRing, typename T>
+int launch_few_of(const Int8Call& c, const Few& f, hipStream_t stream) {
+  static PerDeviceInt limit;
+  if (!raise_lds_limit(limit, reinterpret_cast<const void*>(&int8_few_kernel<kX, kRing, T>), kMaxLds)) return MFQ_ELAUNCH;
+  const int lds = few_image(kX, f.steps, f.waves) + f.per_group * few_sums(kX, f.waves);
+  hipLaunchKernelGGL((int8_few_kernel<kX, kRing, T>), dim3((unsigned)f.grid), dim3(f.waves * kWave), lds, stream, c, f.waves, f.steps, f.per_group,
+                     f.groups);
+  return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+}
+
+template <int kX, typename T>
+int launch_few(const Int8Call& c, hipStream_t stream) {
+  int waves, steps;
+  few_shape(c.K, waves, steps);
+  // One workgroup to a compute unit (two or three, each with fewer blocks, take 15 us where one takes 12: 10240 x 3840), in as many
+  // equal rounds as the room for sums asks for
+  const int64_t most = (kMaxLds - few_image(kX, steps, waves)) / few_sums(kX, waves), places = compute_units();
+  const int64_t blocks = (c.N + 7) / 8, groups = (c.M + 8 * kX - 1) / (8 * kX);
+  const int64_t rounds = (blocks * groups + places * most - 1) / (places * most);
+  const int64_t per_group = (blocks * groups + places * rounds - 1) / (places * rounds), runs = (blocks + per_group - 1) / per_group;
+  const Few f = {waves, steps, (int)per_group, (int)groups, (int)((runs + 7) / 8 * 8 * groups)};
+  const int64_t positions = per_group * steps;  // requests of a wavefront: those behind the last are in vain
+  if (positions <= 2) return launch_few_of<kX, 2, T>(c, f, stream);
+  return positions <= 5 ? launch_few_of<kX, 4, T>(c, f, stream) : launch_few_of<kX, 8, T>(c, f, stream);
 }
 
 template <typename T>
 int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t stream) {
   if (p.kernel == MFQ_INT8_FEW) {
-    const dim3 grid((unsigned)((c.N + 15) / 16));
-    if (c.M <= 8) hipLaunchKernelGGL((int8_few_kernel<8, 8, T>), grid, dim3(8 * kWave), 0, stream, c);
-    else hipLaunchKernelGGL((int8_few_kernel<16, 8, T>), grid, dim3(8 * kWave), 0, stream, c);
-    return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
+    if (p.rows == 8) return launch_few<1, T>(c, stream);
+    return launch_few<2, T>(c, stream);
   }
   if (p.splits == 1) return launch_tiles_of<T>(c, p, c.y, stream);
   if (int rc = launch_tiles_of<I32>(c, p, workspace, stream)) return rc;
@@ -469,22 +565,45 @@ int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t st
 
 }  // namespace
 
+// What a call is estimated to take, in us, and the tile of the least: launch and first bytes 3, a round of workgroups as many steps as
+// its range of K has at the tile's time each, a cut K 4 for the second launch and its planes at 3 TB/s written and read; no call is faster
+// than its bytes.  Times of a step measured with all compute units busy (30 and 80 steps, 120 to 1360 tiles): they follow the tile's
+// bytes through LDS and a latency, not its matrix instructions, but for the largest.
 Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K) {
-  if (M <= 16) return {MFQ_INT8_FEW, 1, (int)M, 16};
-  const int64_t units = compute_units(), steps = (K + BK - 1) / BK;
-  Int8Plan p = {MFQ_INT8_TILES, 1, 256, 256};
-  if (M <= 32) p.rows = 32, p.columns = 128;
-  else if (M <= 64) p.rows = p.columns = 64;
-  else if (dtype == MFQ_F32 || ((M + 255) / 256) * ((N + 255) / 256) < units * 3 / 4) p.rows = p.columns = 128;
-  const int64_t tiles = ((M + p.rows - 1) / p.rows) * ((N + p.columns - 1) / p.columns);
-  const int64_t places = p.rows == 256 ? units : 2 * units;
-  if (tiles * 2 <= places) {
-    int64_t s = places / tiles, most = steps / 4;
-    if (s > most) s = most;
-    if (s > 16) s = 16;
-    if (s >= 2) p.splits = (int)s;
+  if (M <= 16) {  // rows of x that a workgroup keeps in LDS, some blocks' sums beside them
+    int waves, steps;
+    few_shape(K, waves, steps);
+    const int tokens8 = M <= 8 ? 1 : 2;
+    if (few_image(tokens8, steps, waves) + 2 * few_sums(tokens8, waves) <= kMaxLds) return {MFQ_INT8_FEW, 1, 8 * tokens8, 8, 1};
   }
-  return p;
+  struct Choice {
+    int rows, columns, places;
+    float step;
+  };
+  static constexpr Choice kChoices[] = {{32, 64, 1, 0.30f},   {64, 64, 1, 0.40f},   {64, 128, 1, 0.47f},  {128, 128, 1, 0.66f},
+                                        {128, 128, 2, 1.12f}, {128, 192, 1, 0.84f}, {256, 256, 1, 1.58f}};
+  const int64_t units = compute_units(), steps = (K + BK - 1) / BK;
+  Int8Plan best = {};
+  float least = 1e30f;
+  for (const Choice& o : kChoices) {
+    if (o.rows == 256 && dtype == MFQ_F32) continue;
+    const int64_t tiles = ((M + o.rows - 1) / o.rows) * ((N + o.columns - 1) / o.columns), places = units * o.places;
+    int64_t splits = o.rows == 256 ? 1 : places / tiles;
+    if (splits > steps / 4) splits = steps / 4;
+    if (splits > 16) splits = 16;
+    for (int cut = 0; cut < 2; ++cut) {
+      const int64_t s = cut ? splits : 1;
+      if (cut && s < 2) break;
+      const float rounds = (float)((tiles * s + places - 1) / places);
+      float t = 3.f + rounds * (float)((steps + s - 1) / s) * o.step;
+      if (s > 1) t += 4.f + (float)(s * M * N) * 4.f / 3e6f;
+      if (t < least) {
+        least = t;
+        best = {MFQ_INT8_TILES, (int)s, o.rows, o.columns, o.places};
+      }
+    }
+  }
+  return best;
 }
 
 size_t int8_workspace_bytes(const Int8Plan& p, int64_t M, int64_t N) { return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0; }

@@ -40,6 +40,7 @@ struct Int8Plan {
   int kernel;   // MFQ_INT8_*
   int splits;   // ranges of K
   int rows, columns;  // of a workgroup's tile
+  int places;         // of workgroups on a compute unit
 };
 Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K);
 size_t int8_workspace_bytes(const Int8Plan& p, int64_t M, int64_t N);
