@@ -5,9 +5,8 @@
 //   dx = r (w dy - s r^2 mean(w dy s)) + ds,  dw = sum over the rows of dy s r
 // All of it is bound by memory: a row is read once, into registers, and written once.  A row takes one wavefront or one
 // workgroup of four, whichever has it in at most eight 16-byte pieces a lane; the weight stays in registers from row to row.
-// A code does not depend on r, so it is decided by the products p alone, and exactly: where the float32 quotient is within
-// 2^-13 of a border between two codes (its own error is below 2^-14), the sign of 254 |p| - (2 l + 1) max|p| in float64
-// decides, where both products are exact for the 16-bit types.
+// A code does not depend on r, so it is decided by the products p alone, and exactly: where the float32 quotient is next to a
+// border between two codes it is taken again in float64, which tells 16-bit types' products apart.
 // Sums are float32 (eight to some hundred terms a lane, then a tree), in an order that the row's length alone fixes.
 #include <type_traits>
 
@@ -19,9 +18,7 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kMaxChunks = 8;
+constexpr int kThreads = 256;  // of the kernels that are not a row's lanes wide
 
 template <int kCtrl, typename V>
 __device__ inline V dpp(V v) {
@@ -49,13 +46,14 @@ __device__ inline V over_wave(V v) {
     return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
   }
 }
-// the same over a row's lanes: a wavefront, or the workgroup's four, which meet in LDS (two sets of slots in turn, so that
-// one barrier is enough)
+// the same over a row's lanes: a wavefront, or a workgroup's, which meet in LDS (two sets of slots in turn, so that one barrier is
+// enough)
 template <int kLanes, typename A, typename B>
 __device__ inline void over_row(A& a, B& b, int turn) {
   a = over_wave(a);
   b = over_wave(b);
   if constexpr (kLanes > kWave) {
+    constexpr int kWaves = kLanes / kWave;
     __shared__ A sa[2][kWaves];
     __shared__ B sb[2][kWaves];
     const int wave = threadIdx.x / kWave, set = turn & 1;
@@ -64,17 +62,28 @@ __device__ inline void over_row(A& a, B& b, int turn) {
       sb[set][wave] = b;
     }
     __syncthreads();
-    a = join(join(sa[set][0], sa[set][1]), join(sa[set][2], sa[set][3]));
-    b = join(join(sb[set][0], sb[set][1]), join(sb[set][2], sb[set][3]));
+    a = sa[set][0];
+    b = sb[set][0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+      a = join(a, sa[set][i]);
+      b = join(b, sb[set][i]);
+    }
   }
 }
 
 template <typename T>
 constexpr int kVecOf = 16 / (int)sizeof(typename T::storage);
 
-template <typename T>
-__device__ inline void unpack(u32x4 raw, float (&v)[kVecOf<T>]) {
-  if constexpr (sizeof(typename T::storage) == 2) {
+// A unit of a row: 16 bytes, or one element where rows are not whole and aligned 16 bytes
+template <typename T, int V>
+using Unit = std::conditional_t<V == 1, typename T::storage, u32x4>;
+
+template <typename T, int V>
+__device__ inline void unpack(const Unit<T, V>& raw, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = T::to_f32(raw);
+  } else if constexpr (sizeof(typename T::storage) == 2) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = lo_f32<T>(raw[i]);
@@ -85,92 +94,101 @@ __device__ inline void unpack(u32x4 raw, float (&v)[kVecOf<T>]) {
     for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(raw[i]);
   }
 }
-template <typename T>
-__device__ inline u32x4 pack(const float (&v)[kVecOf<T>]) {
-  u32x4 raw;
+template <typename T, int V>
+__device__ inline Unit<T, V> pack(const float (&v)[V]) {
+  if constexpr (V == 1) {
+    return T::from_f32(v[0]);
+  } else {
+    u32x4 raw;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(typename T::storage) == 2) raw[i] = T::pack2(v[2 * i], v[2 * i + 1]);
-    else raw[i] = __float_as_uint(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(typename T::storage) == 2) raw[i] = T::pack2(v[2 * i], v[2 * i + 1]);
+      else raw[i] = __float_as_uint(v[i]);
+    }
+    return raw;
   }
-  return raw;
 }
-template <typename T>
-__device__ inline u32x4 add(u32x4 a, u32x4 b) {
-  float x[kVecOf<T>], y[kVecOf<T>];
-  unpack<T>(a, x);
-  unpack<T>(b, y);
+template <typename T, int V>
+__device__ inline Unit<T, V> add(const Unit<T, V>& a, const Unit<T, V>& b) {
+  float x[V], y[V];
+  unpack<T, V>(a, x);
+  unpack<T, V>(b, y);
 #pragma unroll
-  for (int i = 0; i < kVecOf<T>; ++i) x[i] += y[i];
-  return pack<T>(x);
+  for (int i = 0; i < V; ++i) x[i] += y[i];
+  return pack<T, V>(x);
 }
 
 // ---- codes.  The product p of a value and its weight: exact in float32 for the 16-bit types, in float64 for float32.
-template <typename T>
-using Product = std::conditional_t<sizeof(typename T::storage) == 2, float, double>;
-template <typename T>
-using Bits = std::conditional_t<sizeof(typename T::storage) == 2, uint32_t, uint64_t>;
+template <typename T, bool kWeighted>
+using Product = std::conditional_t<kWeighted && sizeof(typename T::storage) == 4, double, float>;
+template <typename P>
+using Bits = std::conditional_t<sizeof(P) == 8, uint64_t, uint32_t>;
 
 // |p| as an unsigned: its order is that of the magnitudes, with infinity above all numbers and NaN above that
-template <typename T>
-__device__ inline Bits<T> magnitude(Product<T> p) {
-  return __builtin_bit_cast(Bits<T>, p) & (~(Bits<T>)0 >> 1);
+template <typename P>
+__device__ inline Bits<P> magnitude(P p) {
+  return __builtin_bit_cast(Bits<P>, p) & (~(Bits<P>)0 >> 1);
 }
 
 // What the codes of a row are made with
-template <typename T>
+template <typename P>
 struct Coder {
-  Product<T> top;
+  P top;
   float inverse;
-  bool finite, some, tiny;
-  __device__ inline Coder(Bits<T> largest) {
-    top = __builtin_bit_cast(Product<T>, largest);
-    finite = top < (Product<T>)__builtin_inff();
+  bool finite, some, far;
+  __device__ inline Coder(Bits<P> largest) {
+    top = __builtin_bit_cast(P, largest);
+    finite = top < (P)__builtin_inff();
     some = finite && largest;
-    tiny = top < (Product<T>)0x1p-100f;  // its inverse may be no float32
+    far = top < (P)0x1p-100f || top > (P)0x1p120f;  // its inverse may be no normal float32
     inverse = 127.0f / (float)top;
   }
   // the scale of p's row, p being what it is times `factor`
-  __device__ inline float scale(float factor) const { return finite ? (float)top * factor / 127.0f : __builtin_nanf(""); }
-  __device__ inline int code(Product<T> p) const {
+  __device__ inline float scale(float factor) const { return finite ? (float)(top * (P)factor / (P)127) : __builtin_nanf(""); }
+  // The codes of N products, in the low bytes, the first lowest.  Adding 1.5 2^23 rounds a quotient to a whole number, ties to even,
+  // and leaves it in the sum's low bits; what the sum lost is how far the quotient is from it.  p * inverse is off by at most
+  // 127 * 4 * 2^-24 < 2^-14 (the inverse, the product, and for float32 the rounding of p and max|p|).
+  template <int N>
+  __device__ inline uint32_t codes(const P (&p)[N]) const {
     if (!some) return 0;
-    const Product<T> m = __builtin_bit_cast(Product<T>, magnitude<T>(p));
-    const float t = tiny ? (float)((double)m * (127.0 / (double)top)) : (float)m * inverse;
-    const float low = __builtin_floorf(t), rest = t - low;
-    bool up = rest > 0.5f;
-    if (__builtin_fabsf(rest - 0.5f) < 0x1p-13f) {
-      const double d = __builtin_fma(254.0, (double)m, -((2.0 * (double)low + 1.0) * (double)top));
-      up = d > 0.0 || (d == 0.0 && ((int)low & 1));
+    float sum[N], off = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float v = (float)p[i];
+      sum[i] = __builtin_fmaf(v, inverse, 12582912.0f);
+      off = __builtin_fmaxf(off, __builtin_fabsf(__builtin_fmaf(v, inverse, 12582912.0f - sum[i])));
     }
-    const int c = min((int)low + (up ? 1 : 0), 127);
-    return p < 0 ? -c : c;
+    if (far || off > 0.5f - 0x1p-14f) {  // one of them is next to a border
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] = 12582912.0f + (float)__builtin_rint(127.0 * (double)p[i] / (double)top);
+    }
+    if constexpr (N == 1) return __float_as_uint(sum[0]);
+    const uint32_t low = __builtin_amdgcn_perm(__float_as_uint(sum[1 % N]), __float_as_uint(sum[0]), 0x0c0c0400u);
+    return low | __builtin_amdgcn_perm(__float_as_uint(sum[3 % N]), __float_as_uint(sum[2 % N]), 0x04000c0cu);
   }
 };
 
-template <typename T>
-__device__ inline Product<T> product(float s, float w) {
-  return (Product<T>)s * (Product<T>)w;
-}
+enum Result { kNormalised, kCodes, kWeightedCodes };
 
-__device__ inline uint32_t pack_codes(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
-
-// kLanes lanes to a row, each kChunks of its 16-byte pieces
-template <typename T, int kLanes, int kChunks, bool kCodes>
-__global__ __launch_bounds__(kThreads) void rows_kernel(RowsCall c) {
+// kLanes lanes to a row, each kChunks of its units of V elements; up to 256 threads, workgroups of several rows
+template <typename T, int V, int kLanes, int kChunks, int kResult>
+__global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kernel(RowsCall c) {
   using E = typename T::storage;
-  constexpr int V = kVecOf<T>, kRows = kThreads / kLanes;
+  using U = Unit<T, V>;
+  constexpr bool kCoded = kResult != kNormalised;
+  using P = Product<T, kResult == kWeightedCodes>;
+  constexpr int kRows = kLanes > kWave ? 1 : kThreads / kWave;
   const int lane = threadIdx.x % kLanes, units = (int)(c.columns / V);
-  u32x4 w[kChunks];
+  const bool weighted = kCoded ? kResult == kWeightedCodes : c.weight != nullptr;
+  U w[kChunks];
 #pragma unroll
   for (int u = 0; u < kChunks; ++u)
-    if (c.weight && lane + u * kLanes < units) w[u] = static_cast<const u32x4*>(c.weight)[lane + u * kLanes];
+    if (weighted && lane + u * kLanes < units) w[u] = static_cast<const U*>(c.weight)[lane + u * kLanes];
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows, ++turn) {
-    const u32x4* x = reinterpret_cast<const u32x4*>(static_cast<const E*>(c.x) + row * c.x_stride);
-    const u32x4* residual = reinterpret_cast<const u32x4*>(static_cast<const E*>(c.residual) + row * c.residual_stride);
-    u32x4 s[kChunks], r[kChunks];
+    const U* x = reinterpret_cast<const U*>(static_cast<const E*>(c.x) + row * c.x_stride);
+    const U* residual = reinterpret_cast<const U*>(static_cast<const E*>(c.residual) + row * c.residual_stride);
+    U s[kChunks], r[kChunks];
 #pragma unroll
     for (int u = 0; u < kChunks; ++u)
       if (lane + u * kLanes < units) s[u] = x[lane + u * kLanes];
@@ -179,63 +197,81 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(RowsCall c) {
       for (int u = 0; u < kChunks; ++u)
         if (lane + u * kLanes < units) r[u] = residual[lane + u * kLanes];
     }
+    auto products = [&](int u, P (&p)[V]) __attribute__((always_inline)) {
+      float v[V], g[V];
+      unpack<T, V>(s[u], v);
+      if constexpr (kResult == kWeightedCodes) unpack<T, V>(w[u], g);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if constexpr (kResult == kWeightedCodes) p[i] = (P)v[i] * (P)g[i];
+        else p[i] = v[i];
+      }
+    };
     float squares = 0.f;
-    Bits<T> largest = 0;
+    Bits<P> largest = 0;
 #pragma unroll
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
       if (c.residual) {
-        s[u] = add<T>(s[u], r[u]);
-        reinterpret_cast<u32x4*>(static_cast<E*>(c.sum) + row * c.columns)[lane + u * kLanes] = s[u];
+        s[u] = add<T, V>(s[u], r[u]);
+        reinterpret_cast<U*>(static_cast<E*>(c.sum) + row * c.columns)[lane + u * kLanes] = s[u];
       }
-      float v[V], g[V];
-      unpack<T>(s[u], v);
-      if (kCodes && c.weight) unpack<T>(w[u], g);
+      float v[V];
+      unpack<T, V>(s[u], v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        squares = __builtin_fmaf(v[i], v[i], squares);
-        if constexpr (kCodes) largest = join(largest, magnitude<T>(c.weight ? product<T>(v[i], g[i]) : (Product<T>)v[i]));
+      for (int i = 0; i < V; ++i) squares = __builtin_fmaf(v[i], v[i], squares);
+      if constexpr (kCoded) {
+        P p[V];
+        products(u, p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) largest = join(largest, magnitude(p[i]));
       }
     }
     over_row<kLanes>(squares, largest, turn);
     const float rstd = c.norm ? 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps) : 1.0f;
-    const Coder<T> coder(largest);
+    const Coder<P> coder(largest);
 #pragma unroll
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
-      float v[V], g[V];
-      unpack<T>(s[u], v);
-      if (c.weight) unpack<T>(w[u], g);
-      if constexpr (kCodes) {
-        uint32_t packed[V / 4];
-#pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-          int k[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) k[e] = coder.code(c.weight ? product<T>(v[4 * i + e], g[4 * i + e]) : (Product<T>)v[4 * i + e]);
-          packed[i] = pack_codes(k[0], k[1], k[2], k[3]);
-        }
+      if constexpr (kCoded) {
+        P p[V];
+        products(u, p);
         int8_t* to = c.codes + row * c.code_stride + (int64_t)(lane + u * kLanes) * V;
-        if constexpr (V == 8) *reinterpret_cast<u32x2*>(to) = u32x2{packed[0], packed[1]};
-        else *reinterpret_cast<uint32_t*>(to) = packed[0];
+        if constexpr (V == 1) {
+          *to = (int8_t)coder.codes(p);
+        } else {
+          uint32_t packed[V / 4];
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) {
+            const P four[4] = {p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
+            packed[i] = coder.codes(four);
+          }
+          if constexpr (V == 8) *reinterpret_cast<u32x2*>(to) = u32x2{packed[0], packed[1]};
+          else *reinterpret_cast<uint32_t*>(to) = packed[0];
+        }
       } else {
+        float v[V], g[V];
+        unpack<T, V>(s[u], v);
+        if (weighted) unpack<T, V>(w[u], g);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           v[i] *= rstd;
-          if (c.weight) v[i] *= g[i];
+          if (weighted) v[i] *= g[i];
         }
-        reinterpret_cast<u32x4*>(static_cast<E*>(c.y) + row * c.columns)[lane + u * kLanes] = pack<T>(v);
+        reinterpret_cast<U*>(static_cast<E*>(c.y) + row * c.columns)[lane + u * kLanes] = pack<T, V>(v);
       }
     }
-    if (kCodes && lane == 0) c.scales[row] = coder.scale(rstd);
+    if (kCoded && lane == 0) c.scales[row] = coder.scale(rstd);
   }
 }
 
-// Rows of any length, alignment and stride: a workgroup to a row, element by element, which is read again (from a cache,
-// where it fits one) for the results.
-template <typename T, bool kCodes>
+// Rows that no registers hold: a workgroup to a row, element by element, which is read again (from a cache, where it fits one) for
+// the results.
+template <typename T, int kResult>
 __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
   using E = typename T::storage;
+  constexpr bool kCoded = kResult != kNormalised;
+  using P = Product<T, kResult == kWeightedCodes>;
   const E* weight = static_cast<const E*>(c.weight);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < c.rows; row += gridDim.x, ++turn) {
@@ -244,42 +280,48 @@ __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
     auto value = [&](int64_t k) __attribute__((always_inline)) {
       return c.residual ? T::to_f32(T::from_f32(T::to_f32(x[k]) + T::to_f32(residual[k]))) : T::to_f32(x[k]);
     };
+    auto product = [&](float s, int64_t k) __attribute__((always_inline)) {
+      if constexpr (kResult == kWeightedCodes) return (P)s * (P)T::to_f32(weight[k]);
+      else return (P)s;
+    };
     float squares = 0.f;
-    Bits<T> largest = 0;
+    Bits<P> largest = 0;
     for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
       const float s = value(k);
       if (c.residual) static_cast<E*>(c.sum)[row * c.columns + k] = T::from_f32(s);
       squares = __builtin_fmaf(s, s, squares);
-      if constexpr (kCodes) largest = join(largest, magnitude<T>(weight ? product<T>(s, T::to_f32(weight[k])) : (Product<T>)s));
+      if constexpr (kCoded) largest = join(largest, magnitude(product(s, k)));
     }
     over_row<kThreads>(squares, largest, turn);
     const float rstd = c.norm ? 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps) : 1.0f;
-    const Coder<T> coder(largest);
+    const Coder<P> coder(largest);
     for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
       float s = value(k);
-      if constexpr (kCodes) {
-        c.codes[row * c.code_stride + k] = (int8_t)coder.code(weight ? product<T>(s, T::to_f32(weight[k])) : (Product<T>)s);
+      if constexpr (kCoded) {
+        const P p[1] = {product(s, k)};
+        c.codes[row * c.code_stride + k] = (int8_t)coder.codes(p);
       } else {
         s *= rstd;
         if (weight) s *= T::to_f32(weight[k]);
         static_cast<E*>(c.y)[row * c.columns + k] = T::from_f32(s);
       }
     }
-    if (kCodes && threadIdx.x == 0) c.scales[row] = coder.scale(rstd);
+    if (kCoded && threadIdx.x == 0) c.scales[row] = coder.scale(rstd);
   }
 }
 
 // ---- gradients
-template <typename T, int kLanes, int kChunks, bool kWeight>
-__global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
+template <typename T, int V, int kLanes, int kChunks, bool kWeight>
+__global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backward_kernel(RowsCall c) {
   using E = typename T::storage;
-  constexpr int V = kVecOf<T>, kRows = kThreads / kLanes;
+  using U = Unit<T, V>;
+  constexpr int kRows = kLanes > kWave ? 1 : kThreads / kWave;
   const int lane = threadIdx.x % kLanes, units = (int)(c.columns / V);
-  u32x4 w[kChunks];
+  U w[kChunks];
   float dw[kWeight ? kChunks : 1][V];
 #pragma unroll
   for (int u = 0; u < kChunks; ++u) {
-    if (c.weight && lane + u * kLanes < units) w[u] = static_cast<const u32x4*>(c.weight)[lane + u * kLanes];
+    if (c.weight && lane + u * kLanes < units) w[u] = static_cast<const U*>(c.weight)[lane + u * kLanes];
     if constexpr (kWeight) {
 #pragma unroll
       for (int i = 0; i < V; ++i) dw[u][i] = 0.f;
@@ -287,10 +329,10 @@ __global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
   }
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows, ++turn) {
-    const u32x4* x = reinterpret_cast<const u32x4*>(static_cast<const E*>(c.x) + row * c.x_stride);
-    const u32x4* dy = reinterpret_cast<const u32x4*>(static_cast<const E*>(c.dy) + row * c.dy_stride);
-    const u32x4* dsum = reinterpret_cast<const u32x4*>(static_cast<const E*>(c.dsum) + row * c.dsum_stride);
-    u32x4 s[kChunks], g[kChunks], d[kChunks];
+    const U* x = reinterpret_cast<const U*>(static_cast<const E*>(c.x) + row * c.x_stride);
+    const U* dy = reinterpret_cast<const U*>(static_cast<const E*>(c.dy) + row * c.dy_stride);
+    const U* dsum = reinterpret_cast<const U*>(static_cast<const E*>(c.dsum) + row * c.dsum_stride);
+    U s[kChunks], g[kChunks], d[kChunks];
 #pragma unroll
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
@@ -303,9 +345,9 @@ __global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
       float v[V], a[V], b[V];
-      unpack<T>(s[u], v);
-      unpack<T>(g[u], a);
-      if (c.weight) unpack<T>(w[u], b);
+      unpack<T, V>(s[u], v);
+      unpack<T, V>(g[u], a);
+      if (c.weight) unpack<T, V>(w[u], b);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         squares = __builtin_fmaf(v[i], v[i], squares);
@@ -318,9 +360,9 @@ __global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
       float v[V], a[V], b[V];
-      unpack<T>(s[u], v);
-      unpack<T>(g[u], a);
-      if (c.weight) unpack<T>(w[u], b);
+      unpack<T, V>(s[u], v);
+      unpack<T, V>(g[u], a);
+      if (c.weight) unpack<T, V>(w[u], b);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float n = v[i] * rstd;
@@ -329,31 +371,26 @@ __global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
       }
       if (!c.dx) continue;
       if (c.dsum) {
-        unpack<T>(d[u], b);
+        unpack<T, V>(d[u], b);
 #pragma unroll
         for (int i = 0; i < V; ++i) a[i] += b[i];
       }
-      reinterpret_cast<u32x4*>(static_cast<E*>(c.dx) + row * c.columns)[lane + u * kLanes] = pack<T>(a);
+      reinterpret_cast<U*>(static_cast<E*>(c.dx) + row * c.columns)[lane + u * kLanes] = pack<T, V>(a);
     }
   }
   if constexpr (kWeight) {  // the workgroup's sums: one row of the partial sums
     float* parts = c.parts + (int64_t)blockIdx.x * c.columns;
-    if constexpr (kRows == 1) {
+    __shared__ float sums[kRows > 1 ? kRows : 1][kRows > 1 ? kLanes * kChunks * V : 1];
 #pragma unroll
-      for (int u = 0; u < kChunks; ++u) {
-        if (lane + u * kLanes >= units) continue;
+    for (int u = 0; u < kChunks; ++u) {
+      if (lane + u * kLanes >= units) continue;
 #pragma unroll
-        for (int i = 0; i < V; i += 4)
-          *reinterpret_cast<f32x4*>(parts + (int64_t)(lane + u * kLanes) * V + i) = f32x4{dw[u][i], dw[u][i + 1], dw[u][i + 2], dw[u][i + 3]};
+      for (int i = 0; i < V; ++i) {
+        if constexpr (kRows > 1) sums[threadIdx.x / kLanes][(lane + u * kLanes) * V + i] = dw[u][i];
+        else parts[(int64_t)(lane + u * kLanes) * V + i] = dw[u][i];
       }
-    } else {
-      __shared__ float sums[kRows][kLanes * kChunks * V];
-#pragma unroll
-      for (int u = 0; u < kChunks; ++u) {
-        if (lane + u * kLanes >= units) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sums[threadIdx.x / kLanes][(lane + u * kLanes) * V + i] = dw[u][i];
-      }
+    }
+    if constexpr (kRows > 1) {
       __syncthreads();
       for (int k = threadIdx.x; k < (int)c.columns; k += kThreads) {
         float v = sums[0][k];
@@ -365,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void rows_backward_kernel(RowsCall c) {
   }
 }
 
-// of any length, alignment and stride; a workgroup adds its rows' shares of the weight's gradient up in its own row of `parts`
+// rows that no registers hold; a workgroup adds its rows' shares of the weight's gradient up in its own row of `parts`
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c) {
   using E = typename T::storage;
@@ -434,7 +471,7 @@ __global__ __launch_bounds__(kThreads) void rows_values_kernel(const int8_t* cod
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = (float)(int8_t)(raw[(p * V + e) / 4] >> (8 * (e & 3))) * scale;
-        reinterpret_cast<u32x4*>(to)[p] = pack<T>(v);
+        reinterpret_cast<u32x4*>(to)[p] = pack<T, V>(v);
       }
     } else {
       *to = T::from_f32((float)codes[row * stride + k] * scale);
@@ -442,58 +479,87 @@ __global__ __launch_bounds__(kThreads) void rows_values_kernel(const int8_t* cod
   }
 }
 
-// lanes of a row and 16-byte pieces of a lane; false: the row does not fit the registers
-bool form_of(int64_t units, int& lanes, int& chunks) {
-  lanes = units <= 4 * kWave ? kWave : kThreads;
-  const int64_t each = (units + lanes - 1) / lanes;
-  chunks = 1;
-  while (chunks < each) chunks *= 2;
-  return chunks <= kMaxChunks;
-}
-
 constexpr int kBackwardGroups = 2;  // workgroups of a backward pass to a compute unit: rows of partial sums
 
+// as many rows to every workgroup
 int64_t groups_of(int64_t rows, int per_group, int64_t most) {
   const int64_t groups = (rows + per_group - 1) / per_group, each = (groups + most - 1) / most;
   return (groups + each - 1) / each;
 }
 
-template <typename T, int kLanes, int kChunks>
-void launch_form(const RowsCall& c, bool backward, int64_t groups, hipStream_t stream) {
-  const dim3 grid((unsigned)groups), block(kThreads);
-  if (backward) {
-    if (c.parts) hipLaunchKernelGGL((rows_backward_kernel<T, kLanes, kChunks, true>), grid, block, 0, stream, c);
-    else hipLaunchKernelGGL((rows_backward_kernel<T, kLanes, kChunks, false>), grid, block, 0, stream, c);
-  } else if (c.codes) {
-    hipLaunchKernelGGL((rows_kernel<T, kLanes, kChunks, true>), grid, block, 0, stream, c);
+template <typename T, int V, int kLanes, int kChunks>
+int64_t forward_form(const RowsCall& c, hipStream_t stream) {
+  constexpr int kBlock = kLanes > kWave ? kLanes : kThreads;
+  const int64_t groups = groups_of(c.rows, kBlock / kLanes, 2048 / kBlock * (int64_t)compute_units());
+  const dim3 grid((unsigned)groups), block(kBlock);
+  if (!c.codes) hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kNormalised>), grid, block, 0, stream, c);
+  else if (c.weight) hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kWeightedCodes>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kCodes>), grid, block, 0, stream, c);
+  return groups;
+}
+
+template <typename T, int V, int kLanes, int kChunks>
+int64_t backward_form(const RowsCall& c, hipStream_t stream) {
+  constexpr int kBlock = kLanes > kWave ? kLanes : kThreads;
+  const int64_t groups = groups_of(c.rows, kBlock / kLanes, kBackwardGroups * (int64_t)compute_units());
+  const dim3 grid((unsigned)groups), block(kBlock);
+  if (c.parts) hipLaunchKernelGGL((rows_backward_kernel<T, V, kLanes, kChunks, true>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((rows_backward_kernel<T, V, kLanes, kChunks, false>), grid, block, 0, stream, c);
+  return groups;
+}
+
+// The form of a row: as many lanes as hold it in two units each, which leaves registers for many rows on their way to a compute unit
+// (4352 x 3840 bfloat16: 256 lanes of two 25 us and 24 with codes, 128 lanes of four 34 and 34); a backward pass, whose workgroups each
+// cost a row of partial sums, in fewer workgroups with more of a row to a lane.
+template <typename T>
+int64_t launch_forward(const RowsCall& c, bool wide, hipStream_t stream) {
+  constexpr int V = kVecOf<T>;
+  const int64_t units = wide ? c.columns / V : c.columns;
+  if (wide) {
+    if (units <= 64) return forward_form<T, V, 64, 1>(c, stream);
+    if (units <= 128) return forward_form<T, V, 64, 2>(c, stream);
+    if (units <= 256) return forward_form<T, V, 128, 2>(c, stream);
+    if (units <= 512) return forward_form<T, V, 256, 2>(c, stream);
+    if (units <= 1024) return forward_form<T, V, 512, 2>(c, stream);
+    if (units <= 2048) return forward_form<T, V, 1024, 2>(c, stream);
+    if (units <= 4096) return forward_form<T, V, 1024, 4>(c, stream);
   } else {
-    hipLaunchKernelGGL((rows_kernel<T, kLanes, kChunks, false>), grid, block, 0, stream, c);
+    if (units <= 512) return forward_form<T, 1, 64, 8>(c, stream);
+    if (units <= 1024) return forward_form<T, 1, 256, 4>(c, stream);
+    if (units <= 4096) return forward_form<T, 1, 256, 16>(c, stream);
   }
+  const int64_t groups = groups_of(c.rows, 1, 8 * (int64_t)compute_units());
+  const dim3 grid((unsigned)groups), block(kThreads);
+  if (!c.codes) hipLaunchKernelGGL((rows_any_kernel<T, kNormalised>), grid, block, 0, stream, c);
+  else if (c.weight) hipLaunchKernelGGL((rows_any_kernel<T, kWeightedCodes>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((rows_any_kernel<T, kCodes>), grid, block, 0, stream, c);
+  return groups;
+}
+
+template <typename T>
+int64_t launch_backward(const RowsCall& c, bool wide, hipStream_t stream) {
+  constexpr int V = kVecOf<T>;
+  const int64_t units = wide ? c.columns / V : c.columns;
+  if (wide) {
+    if (units <= 64) return backward_form<T, V, 64, 1>(c, stream);
+    if (units <= 128) return backward_form<T, V, 64, 2>(c, stream);
+    if (units <= 256) return backward_form<T, V, 64, 4>(c, stream);
+    if (units <= 512) return backward_form<T, V, 256, 2>(c, stream);
+    if (units <= 1024) return backward_form<T, V, 256, 4>(c, stream);
+    if (units <= 2048) return backward_form<T, V, 512, 4>(c, stream);
+  } else {
+    if (units <= 512) return backward_form<T, 1, 64, 8>(c, stream);
+    if (units <= 1024) return backward_form<T, 1, 256, 4>(c, stream);
+    if (units <= 4096) return backward_form<T, 1, 256, 16>(c, stream);
+  }
+  const int64_t groups = groups_of(c.rows, 1, kBackwardGroups * (int64_t)compute_units());
+  hipLaunchKernelGGL((rows_backward_any_kernel<T>), dim3((unsigned)groups), dim3(kThreads), 0, stream, c);
+  return groups;
 }
 
 template <typename T>
 int launch(const RowsCall& c, bool wide, bool backward, hipStream_t stream) {
-  int lanes, chunks;
-  const bool fits = wide && form_of(c.columns / kVecOf<T>, lanes, chunks);
-  int64_t groups;
-  if (!fits) {
-    groups = groups_of(c.rows, 1, (backward ? kBackwardGroups : 8) * (int64_t)compute_units());
-    const dim3 grid((unsigned)groups), block(kThreads);
-    if (backward) hipLaunchKernelGGL((rows_backward_any_kernel<T>), grid, block, 0, stream, c);
-    else if (c.codes) hipLaunchKernelGGL((rows_any_kernel<T, true>), grid, block, 0, stream, c);
-    else hipLaunchKernelGGL((rows_any_kernel<T, false>), grid, block, 0, stream, c);
-  } else {
-    groups = groups_of(c.rows, kThreads / lanes, (backward ? kBackwardGroups : 8) * (int64_t)compute_units());
-    if (lanes == kWave) {
-      if (chunks == 1) launch_form<T, kWave, 1>(c, backward, groups, stream);
-      else if (chunks == 2) launch_form<T, kWave, 2>(c, backward, groups, stream);
-      else launch_form<T, kWave, 4>(c, backward, groups, stream);
-    } else {
-      if (chunks <= 2) launch_form<T, kThreads, 2>(c, backward, groups, stream);
-      else if (chunks == 4) launch_form<T, kThreads, 4>(c, backward, groups, stream);
-      else launch_form<T, kThreads, 8>(c, backward, groups, stream);
-    }
-  }
+  const int64_t groups = backward ? launch_backward<T>(c, wide, stream) : launch_forward<T>(c, wide, stream);
   if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
   if (!backward || !c.parts) return MFQ_OK;
   hipLaunchKernelGGL(rows_weight_kernel<T>, dim3((unsigned)((c.columns + 15) / 16)), dim3(1024), 0, stream, c.parts, (int)groups, c.columns,
