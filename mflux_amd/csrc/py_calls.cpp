@@ -251,11 +251,165 @@ PyObject* epilogue_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rows: the ordinary calls of mflux_amd.int8
+bool intercepted() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() || torch::jit::tracer::isTracing();
+}
+
+// An operand without a derivative to take: undefined, or plain with no gradient wanted and no tangent
+bool constant(const Tensor& t) {
+  return !t.defined() || (plain(t) && !(c10::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined());
+}
+
+int float_code(at::ScalarType t) { return t == at::kBFloat16 ? MFQ_BF16 : t == at::kHalf ? MFQ_F16 : t == at::kFloat ? MFQ_F32 : -1; }
+
+// x, weight or None, residual or None, eps of a norm; `ok` false: the general route
+struct Rows {
+  Tensor x, weight, residual;
+  double eps = 0;
+  mfq_rms_norm_args a = {};
+
+  bool parse(PyObject* const* args) {
+    if (!tensor_arg(args[0], &x) || !tensor_arg(args[1], &weight) || !tensor_arg(args[2], &residual) || !PyFloat_CheckExact(args[3])) return false;
+    eps = PyFloat_AS_DOUBLE(args[3]);
+    if (!x.defined() || intercepted() || !constant(x) || !constant(weight) || !constant(residual)) return false;
+    a.dtype = float_code(x.scalar_type());
+    if (a.dtype < 0 || x.dim() < 1 || x.numel() == 0 || !(eps >= 0 && eps <= 1e30)) return false;
+    a.eps = (float)eps;
+    a.columns = x.size(-1);
+    a.rows = x.numel() / a.columns;
+    a.x = x.const_data_ptr();
+    a.x_stride = a.columns;
+    if (weight.defined()) {
+      if (weight.scalar_type() != x.scalar_type() || weight.device() != x.device() || weight.dim() != 1 || weight.size(0) != a.columns) return false;
+      a.weight = weight.const_data_ptr();
+    }
+    if (residual.defined()) {
+      if (residual.scalar_type() != x.scalar_type() || residual.device() != x.device() || residual.sizes() != x.sizes()) return false;
+      a.residual = residual.const_data_ptr();
+      a.residual_stride = a.columns;
+    }
+    return true;
+  }
+  Tensor like() const { return at::empty(x.sizes(), x.options().requires_grad(false)); }
+  std::vector<c10::IValue> inputs() const { return {x, weight, residual, eps}; }
+};
+
+PyObject* pack(std::initializer_list<const Tensor*> tensors) {
+  PyObject* out = PyTuple_New((Py_ssize_t)tensors.size());
+  Py_ssize_t i = 0;
+  for (const Tensor* t : tensors) {
+    PyObject* o = out ? THPVariable_Wrap(*t) : nullptr;
+    if (!o) {
+      Py_XDECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, o);
+  }
+  return out;
+}
+
+// rms_norm(x, weight or None, residual or None, eps) -> y, (y, sum) or None
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Rows p;
+  if (n != 4 || !p.parse(args)) Py_RETURN_NONE;
+  RECORD_FUNCTION("mfq::rms_norm", p.inputs());
+  const c10::hip::HIPGuardMasqueradingAsCUDA on_device(p.x.device());
+  Tensor y = p.like(), sum;
+  p.a.y = y.data_ptr();
+  if (p.residual.defined()) {
+    sum = p.like();
+    p.a.sum = sum.data_ptr();
+  }
+  void* stream = c10::hip::getCurrentHIPStream(p.x.get_device()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mfq_rms_norm(&p.a, stream);
+  Py_END_ALLOW_THREADS
+  TORCH_CHECK(rc != MFQ_ELAUNCH, "mfq_rms_norm failed: ", mfq_strerror(rc), " (status ", rc, ")");
+  if (rc != MFQ_OK) Py_RETURN_NONE;
+  return sum.defined() ? pack({&y, &sum}) : THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_rows(x, weight or None, residual or None, eps, norm) -> (codes, scales), (codes, scales, sum) or None
+PyObject* int8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Rows p;
+  if (n != 5 || !p.parse(args) || p.a.columns % 16) Py_RETURN_NONE;
+  const bool norm = args[4] == Py_True;
+  RECORD_FUNCTION(norm ? "mfq::rms_norm_int8" : "mfq::int8_quantize", p.inputs());
+  const c10::hip::HIPGuardMasqueradingAsCUDA on_device(p.x.device());
+  const auto options = p.x.options().requires_grad(false);
+  Tensor codes = at::empty(p.x.sizes(), options.dtype(at::kChar)), scales = at::empty(p.x.sizes().slice(0, p.x.dim() - 1), options.dtype(at::kFloat)), sum;
+  p.a.codes = codes.data_ptr<int8_t>();
+  p.a.code_stride = p.a.columns;
+  p.a.scales = scales.data_ptr<float>();
+  if (p.residual.defined()) {
+    sum = p.like();
+    p.a.sum = sum.data_ptr();
+  }
+  void* stream = c10::hip::getCurrentHIPStream(p.x.get_device()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = norm ? mfq_rms_norm(&p.a, stream)
+            : mfq_int8_quantize(p.a.x, p.a.dtype, p.a.rows, p.a.columns, p.a.x_stride, p.a.codes, p.a.code_stride, p.a.scales, stream);
+  Py_END_ALLOW_THREADS
+  TORCH_CHECK(rc != MFQ_ELAUNCH, "mfq_rms_norm, mfq_int8_quantize failed: ", mfq_strerror(rc), " (status ", rc, ")");
+  if (rc != MFQ_OK) Py_RETURN_NONE;
+  return sum.defined() ? pack({&codes, &scales, &sum}) : pack({&codes, &scales});
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_matmul(x, x_scales, w, w_scales, bias or None, code of the result's type) -> y or None
+PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, xs, w, ws, bias;
+  int64_t code = 0;
+  if (n != 6 || !tensor_arg(args[0], &x) || !tensor_arg(args[1], &xs) || !tensor_arg(args[2], &w) || !tensor_arg(args[3], &ws) ||
+      !tensor_arg(args[4], &bias) || !int_arg(args[5], &code) || intercepted())
+    Py_RETURN_NONE;
+  for (const Tensor* t : {&x, &xs, &w, &ws})
+    if (!t->defined() || !constant(*t) || t->device() != x.device()) Py_RETURN_NONE;
+  if (!constant(bias) || x.scalar_type() != at::kChar || w.scalar_type() != at::kChar || xs.scalar_type() != at::kFloat || ws.scalar_type() != at::kFloat)
+    Py_RETURN_NONE;
+  if (x.dim() < 1 || w.dim() != 2 || ws.dim() != 1 || x.size(-1) != w.size(1) || ws.size(0) != w.size(0) ||
+      xs.sizes() != x.sizes().slice(0, x.dim() - 1))
+    Py_RETURN_NONE;
+  const at::ScalarType type = code == MFQ_BF16 ? at::kBFloat16 : code == MFQ_F16 ? at::kHalf : at::kFloat;
+  const int64_t K = w.size(1), N = w.size(0);
+  if (K == 0 || K % 16 || N == 0 || x.numel() == 0 || (code != MFQ_BF16 && code != MFQ_F16 && code != MFQ_F32)) Py_RETURN_NONE;
+  if (bias.defined() && (bias.scalar_type() != type || bias.dim() != 1 || bias.size(0) != N || bias.device() != x.device())) Py_RETURN_NONE;
+  RECORD_FUNCTION("mfq::int8_matmul", std::vector<c10::IValue>({x, xs, w, ws, bias}));
+  const c10::hip::HIPGuardMasqueradingAsCUDA on_device(x.device());
+  const int64_t M = x.numel() / K;
+  c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  Tensor y = at::empty(shape, x.options().dtype(type)), scratch;
+  const size_t bytes = mfq_int8_matmul_workspace_bytes(M, N, K, (int)code);
+  if (bytes) scratch = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  const auto* x_p = static_cast<const int8_t*>(x.const_data_ptr());
+  const auto* w_p = static_cast<const int8_t*>(w.const_data_ptr());
+  const auto *xs_p = static_cast<const float*>(xs.const_data_ptr()), *ws_p = static_cast<const float*>(ws.const_data_ptr());
+  const void* b_p = bias.defined() ? bias.const_data_ptr() : nullptr;
+  void *y_p = y.data_ptr(), *s_p = bytes ? scratch.data_ptr() : nullptr, *stream = c10::hip::getCurrentHIPStream(x.get_device()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mfq_int8_matmul(x_p, K, xs_p, w_p, K, ws_p, b_p, M, N, K, y_p, (int)code, s_p, bytes, stream);
+  Py_END_ALLOW_THREADS
+  return result("mfq_int8_matmul", rc, y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, "x @ dequantize(w).T (+ bias), or None"},
     {"linear_float32", (PyCFunction)(void*)linear_float32, METH_FASTCALL, "the same of a float32 x, or None"},
     {"silu_linear", (PyCFunction)(void*)silu_linear, METH_FASTCALL, "silu(x) @ dequantize(w).T (+ bias), or None"},
     {"epilogue_linear", (PyCFunction)(void*)epilogue_linear, METH_FASTCALL, "a linear with its epilogue, or None"},
+    {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "RMS norm of rows, with the residual's addition, or None"},
+    {"int8_rows", (PyCFunction)(void*)int8_rows, METH_FASTCALL, "rows as 8-bit codes with a scale each, or None"},
+    {"int8_matmul", (PyCFunction)(void*)int8_matmul, METH_FASTCALL, "the product of two matrices of codes, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libmfq_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

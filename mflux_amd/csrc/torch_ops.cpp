@@ -1053,6 +1053,38 @@ std::tuple<Tensor, Tensor> rms_norm_call(const Tensor& x, const c10::optional<Te
   return rms_norm(x, weight, residual, eps);
 }
 
+// The ops without a derivative: an operand that wants one is refused here, not passed by without a word
+void check_constant(const char* fn, std::initializer_list<const c10::optional<Tensor>*> operands) {
+  check_forward_mode(fn, operands);
+  for (const auto* t : operands) TORCH_CHECK(!at::GradMode::is_enabled() || !wanted(*t), fn, ": codes have no gradient");
+}
+std::tuple<Tensor, Tensor, Tensor> rms_norm_int8_constant(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& residual,
+                                                          double eps) {
+  const c10::optional<Tensor> first(x);
+  check_constant("mfq::rms_norm_int8", {&first, &weight, &residual});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rms_norm_int8(x, weight, residual, eps);
+}
+std::tuple<Tensor, Tensor> int8_quantize_constant(const Tensor& x) {
+  const c10::optional<Tensor> first(x);
+  check_constant("mfq::int8_quantize", {&first});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return int8_quantize(x);
+}
+Tensor int8_dequantize_constant(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  const c10::optional<Tensor> second(scales);
+  check_constant("mfq::int8_dequantize", {&second});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return int8_dequantize(codes, scales, dtype);
+}
+Tensor int8_matmul_constant(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const c10::optional<Tensor>& bias,
+                            at::ScalarType dtype) {
+  const c10::optional<Tensor> a(x_scales), b(w_scales);
+  check_constant("mfq::int8_matmul", {&a, &b, &bias});
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return int8_matmul(x, x_scales, w, w_scales, bias, dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mfq, m) {
@@ -1121,4 +1153,8 @@ TORCH_LIBRARY_IMPL(mfq, AutogradCUDA, m) {  // the ops with gradients; the other
   m.impl("rotary_call", rotary_call);
   m.impl("attention_call", attention_call);
   m.impl("rms_norm_call", rms_norm_call);
+  m.impl("rms_norm_int8", rms_norm_int8_constant);
+  m.impl("int8_quantize", int8_quantize_constant);
+  m.impl("int8_dequantize", int8_dequantize_constant);
+  m.impl("int8_matmul", int8_matmul_constant);
 }

@@ -64,6 +64,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     float32 and rounded once.  Results are densely packed.
 
     Gradients for ``x``, ``residual`` (the same one) and ``weight``, through both results."""
+    y = _lib.native().rms_norm(x, weight, residual, eps)
+    if y is not None:
+        return y
     _check_norm("rms_norm", x, weight, residual, eps)
     y, total = _lib.ops().rms_norm_call(x, weight, residual, eps)
     return y if residual is None else (y, total)
@@ -75,6 +78,9 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, *, residu
 
     A code is ``rint(127 p / max|p|)`` of the row's products ``p = sum * weight``, ties to even, decided by
     the exact quotient (the root is a factor of the scale alone).  No gradients."""
+    rows = _lib.native().int8_rows(x, weight, residual, eps, True)
+    if rows is not None:
+        return rows
     fn = "rms_norm_int8"
     _check_norm(fn, x, weight, residual, eps)
     _refuse_gradients(fn, x, weight, residual)
@@ -90,6 +96,9 @@ def int8_quantize(x: torch.Tensor):
     A row of zeros has codes and scale 0; one that holds an infinity or NaN has the scale NaN (and
     codes 0), so that its products are NaN.  Rows of codes begin at whole 16 bytes: where ``K`` is no
     multiple of 16 the codes are a view with a stride between rows.  No gradients."""
+    rows = _lib.native().int8_rows(x, None, None, 0.0, False)
+    if rows is not None:
+        return rows
     fn = "int8_quantize"
     _check_rows(fn, x)
     _refuse_gradients(fn, x)
@@ -129,6 +138,9 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scal
     sum with ``bias`` ``[N]`` of ``dtype`` are float32, rounded once to ``dtype`` (float32, float16 or bfloat16).
     Any values from -128 to 127, any strides; rows that are not whole 16 bytes apart are copied,
     and so is an ``x`` whose ``K`` is no multiple of 16.  No gradients."""
+    y = _lib.native().int8_matmul(x, x_scales, w, w_scales, bias, _DTYPE_CODE.get(dtype))
+    if y is not None:
+        return y
     fn = "int8_matmul"
     _check_codes(fn, "x", x, x_scales)
     _check_codes(fn, "w", w, w_scales)

@@ -22,7 +22,7 @@ import math
 import torch
 
 from . import _lib, core
-from .nn import Linear, QuantizedLinear
+from .nn import Int8Linear, Linear, QuantizedLinear
 
 _RANK_STEP = 16  # the kernels take the low rank in steps of 16
 
@@ -30,6 +30,8 @@ _RANK_STEP = 16  # the kernels take the low rank in steps of 16
 class LoRALinear(torch.nn.Module):
     @staticmethod
     def from_linear(linear: torch.nn.Module, r: int = 16, scale: float = 1.0) -> "LoRALinear":
+        if isinstance(linear, Int8Linear):
+            raise ValueError("[LoRALinear] an Int8Linear has no gradient to train an adapter with: wrap the float or the quantized layer")
         output_dims, input_dims = linear.weight.shape
         if isinstance(linear, QuantizedLinear):
             # packed words -> elements (the reference multiplies by 32 // bits, which is only right for 4 and 8 bits)

@@ -1,5 +1,5 @@
 """Module-level API: ``quantize``, ``QuantizedLinear``, ``Linear``,
-``QuantizedEmbedding``, ``Embedding``.
+``QuantizedEmbedding``, ``Embedding``, ``RMSNorm``, ``Int8Linear``.
 
 Mirrors the part of ``mlx.nn`` that mflux uses to quantize a model and to run
 it: ``nn.quantize(model, class_predicate=..., bits=...)`` at
@@ -19,7 +19,7 @@ from typing import Callable
 
 import torch
 
-from . import core
+from . import core, int8
 
 
 def _defaults(group_size: int | None, bits: int | None) -> tuple[int, int]:
@@ -376,6 +376,113 @@ class Linear(torch.nn.Linear):
 
     def to_quantized(self, group_size: int | None = None, bits: int | None = None, mode: str = "affine"):
         return QuantizedLinear.from_linear(self, group_size, bits, mode)
+
+    def to_int8(self) -> "Int8Linear":
+        return Int8Linear.from_linear(self)
+
+
+class RMSNorm(torch.nn.Module):
+    """MLX's ``nn.RMSNorm(dims, eps)``, the norm of the text encoders' and Z-Image's
+    blocks (src/mflux/models/z_image/model/z_image_transformer/transformer_block.py), with
+    the residual's addition in the same pass (``mflux_amd.rms_norm``): ``norm(x)``, or
+    ``y, h = norm(x, residual=h)`` for ``h = h + x; y = norm(h)``.  ``int8`` gives the normalised
+    rows as codes and scales for an :class:`Int8Linear`."""
+
+    def __init__(self, dims: int, eps: float = 1e-5, *, device=None, dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        self.eps = eps
+        self.weight = torch.nn.Parameter(torch.ones((dims,), dtype=dtype, device=device))
+
+    def extra_repr(self) -> str:
+        return f"{self.weight.shape[0]}, eps={self.eps}"
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        return int8.rms_norm(x, self.weight, residual=residual, eps=self.eps)
+
+    def int8(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """``(codes, scales)`` of the normalised rows, with ``residual`` ``(codes, scales, h)``; no gradients (the
+        weight counts as a constant)."""
+        return int8.rms_norm_int8(x, self.weight.detach(), residual=residual, eps=self.eps)
+
+
+class Int8Linear(torch.nn.Module):
+    """``y = x W^T (+ bias)`` with 8-bit integers on both sides: a scale for each row of the weight (an
+    output feature) and for each row of ``x`` (a token), the latter taken in the call.
+
+    ``weight`` int8 ``[N, K]``, ``scales`` float32 ``[N]``, optional ``bias`` ``[N]``: frozen buffers.  ``x`` is a float
+    tensor ``[..., K]``, whose type the result has, or the ``(codes, scales)`` of ``RMSNorm.int8`` or
+    ``mflux_amd.int8_quantize``, taken once for several layers; the result then has the type
+    that the layer was made from.  Beside :class:`QuantizedLinear`, which keeps the activations
+    in 16 bits: the matrix cores multiply codes at twice the rate.  Inference only: an ``x``
+    that wants a gradient is refused."""
+
+    def __init__(self, input_dims: int, output_dims: int, bias: bool = True, *, device=None, dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        self.dtype = dtype
+        device = torch.device("cpu" if device is None else device)
+        if device.type == "cuda":
+            bound = math.sqrt(1.0 / input_dims)
+            w, scales = int8.int8_quantize(torch.empty((output_dims, input_dims), device=device, dtype=torch.float32).uniform_(-bound, bound))
+        else:  # placeholders of the right shape, to be filled by load_state_dict
+            w = torch.zeros((output_dims, input_dims), dtype=torch.int8, device=device)
+            scales = torch.zeros((output_dims,), dtype=torch.float32, device=device)
+        self.register_buffer("weight", w)
+        self.register_buffer("scales", scales)
+        if bias:
+            self.register_buffer("bias", torch.zeros((output_dims,), dtype=dtype, device=device))
+        else:
+            self.bias = None
+
+    @property
+    def input_dims(self) -> int:
+        return self.weight.shape[1]
+
+    @property
+    def output_dims(self) -> int:
+        return self.weight.shape[0]
+
+    def extra_repr(self) -> str:
+        return f"input_dims={self.input_dims}, output_dims={self.output_dims}, bias={self.bias is not None}"
+
+    def _apply(self, fn, *args, **kwargs):
+        # .half() and the like cast floating point buffers: the scales stay float32, the type of results follows
+        scales, probe = self.scales, fn(torch.empty((0,), dtype=self.dtype, device=self.scales.device))
+        super()._apply(fn, *args, **kwargs)
+        if probe.dtype in core._DTYPE_CODE:
+            self.dtype = probe.dtype
+        if self.scales.dtype != torch.float32:
+            self._buffers["scales"] = scales.to(self.scales.device)
+        return self
+
+    def forward(self, x) -> torch.Tensor:
+        if isinstance(x, tuple):
+            codes, scales = x
+            dtype = self.dtype
+        else:
+            codes, scales = int8.int8_quantize(x)
+            dtype = x.dtype
+        bias = self.bias
+        if bias is not None and bias.dtype != dtype:
+            bias = bias.to(dtype)
+        return int8.int8_matmul(codes, scales, self.weight, self.scales, bias=bias, dtype=dtype)
+
+    @classmethod
+    def from_linear(cls, linear_layer: torch.nn.Module) -> "Int8Linear":
+        weight = linear_layer.weight.detach()
+        if weight.dtype not in core._DTYPE_CODE or weight.ndim != 2:
+            raise ValueError(f"[Int8Linear] expected a linear layer with a floating point weight [N, K], got {tuple(weight.shape)} {weight.dtype}")
+        layer = cls.__new__(cls)
+        torch.nn.Module.__init__(layer)
+        layer.dtype = weight.dtype
+        codes, scales = int8.int8_quantize(weight)
+        layer.register_buffer("weight", codes)
+        layer.register_buffer("scales", scales)
+        bias = getattr(linear_layer, "bias", None)
+        if bias is not None:
+            layer.register_buffer("bias", bias.detach())
+        else:
+            layer.bias = None
+        return layer
 
 
 class QuantizedEmbedding(torch.nn.Module):

@@ -277,3 +277,268 @@ def test_int8_matmul_scales_that_are_not_finite():
         w, t = mflux_amd.int8_quantize(randn(2, 64, 256))
         y = mflux_amd.int8_matmul(q, s, w, t)
         assert bool(y[2].isnan().all()) and not bool(y[[0, 1, 3]].isnan().any())
+
+
+def plan(M, N, K, dtype=0):
+    import ctypes
+
+    from mflux_amd import _lib
+
+    if torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("shapes are chosen for 256 compute units")
+    ranges, rows, columns = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    kernel = _lib.load().mfq_int8_matmul_plan(M, N, K, dtype, ctypes.byref(ranges), ctypes.byref(rows), ctypes.byref(columns))
+    return kernel, rows.value, columns.value, ranges.value > 1
+
+
+@pytest.mark.parametrize("M,N,K,want", [
+    (3, 3840, 3840, (1, 8, 8, False)), (16, 2056, 1040, (1, 16, 8, False)), (1, 40, 131056, (2, 32, 64, True)), (30, 10000, 3840, (2, 32, 64, False)),
+    (24, 600, 8208, (2, 32, 64, True)), (60, 3840, 3856, (2, 64, 64, True)), (200, 3840, 3856, (2, 64, 64, False)), (500, 3850, 1040, (2, 64, 128, False)),
+    (1000, 3840, 1152, (2, 128, 128, False)), (2048, 3840, 1040, (2, 128, 128, False)), (130, 1000, 16400, (2, 64, 128, True)),
+    (200, 3840, 8208, (2, 128, 128, True)), (333, 3840, 8208, (2, 128, 192, True)),
+    (500, 10240, 656, (2, 128, 192, False)), (4352, 3840, 1168, (2, 256, 256, False)), (4352, 12300, 272, (2, 256, 256, False)),
+])
+def test_int8_matmul_on_every_kernel(M, N, K, want):
+    """Each tile, with and without a cut K, against the integers: the last tile of either axis partly empty, K no whole step."""
+    import mflux_amd
+
+    print(f"M={M} N={N} K={K}", flush=True)
+    assert plan(M, N, K, 2) == want
+    x, w, xs, ws = codes(1, M, K), codes(2, N, K), scales(3, M), scales(4, N)
+    for dtype in (BF16, F16):
+        b = randn(5, N, dtype=dtype)
+        y = mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype)
+        ref.check("y", y, *ref.product(x, xs, w, ws, b, dtype))
+        assert torch.equal(y, mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype))
+
+
+def test_rows_behind_others_are_left_alone():
+    """A call writes its own results: what lies in front of and behind them in memory stays."""
+    from mflux_amd import _lib
+
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for M, N, K in ((3, 24, 64), (30, 72, 256), (140, 136, 256), (3300, 3864, 128)):
+        x, w, xs, ws = codes(1, M, K), codes(2, N, K), scales(3, M), scales(4, N)
+        room = torch.full((M + 4, N), 7.0, device="cuda", dtype=BF16)
+        need = lib.mfq_int8_matmul_workspace_bytes(M, N, K, _lib.BF16)
+        work = torch.empty(max(need, 16), device="cuda", dtype=torch.uint8)
+        y = room[2:2 + M]
+        _lib.check("mfq_int8_matmul", lib.mfq_int8_matmul(x.data_ptr(), K, xs.data_ptr(), w.data_ptr(), K, ws.data_ptr(), None, M, N, K, y.data_ptr(),
+                                                          _lib.BF16, work.data_ptr(), need, stream))
+        ref.check("y", y, *ref.product(x, xs, w, ws, None, BF16))
+        assert bool((room[:2] == 7).all()) and bool((room[2 + M:] == 7).all())
+
+
+# ---- streams, graphs, layers -----------------------------------------------------------------------------------------------
+
+def chain(x, h, norm, up, down):
+    """A feed-forward in 8 bits: the residual's addition and the norm, gate and up, down."""
+    import mflux_amd
+
+    q, s, h = norm.int8(x, residual=h)
+    gate, value = up((q, s)).chunk(2, dim=-1)
+    return down(torch.nn.functional.silu(gate) * value), h
+
+
+def layers(K=512, inner=768, dtype=BF16):
+    from mflux_amd import nn
+
+    norm = nn.RMSNorm(K, 1e-6, device="cuda", dtype=dtype)
+    up, down = nn.Linear(K, 2 * inner, bias=False, device="cuda", dtype=dtype), nn.Linear(inner, K, bias=True, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        norm.weight.copy_(1 + randn(11, K) * 0.1)
+        up.weight.copy_(randn(12, 2 * inner, K) * 0.05)
+        down.weight.copy_(randn(13, K, inner) * 0.05)
+        down.bias.copy_(randn(14, K))
+    return norm, up, down
+
+
+@pytest.mark.parametrize("tokens", [1, 77, 600])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_layers_together(tokens, dtype):
+    """Every layer against float64 on what it was given, and the whole near the float layers."""
+    norm, up, down = layers(dtype=dtype)
+    up8, down8 = up.to_int8(), down.to_int8()
+    x, h = randn(1, 2, tokens, 512, dtype=dtype), randn(2, 2, tokens, 512, dtype=dtype)
+    with torch.no_grad():
+        y, total = chain(x, h, norm, up8, down8)
+        assert torch.equal(total, ref.total(x, h))
+        q, s, _ = norm.int8(x, residual=h)
+        want_q, want_s = ref.codes(total, norm.weight, 1e-6)
+        assert torch.equal(q.double(), want_q)
+        ref.check("scales", s, want_s, want_s * ref.scale_bound(512, True))
+        u = up8((q, s))
+        assert u.dtype == dtype
+        ref.check("up", u, *ref.product(q, s, up8.weight, up8.scales, None, dtype))
+        gate, value = u.chunk(2, dim=-1)
+        a = torch.nn.functional.silu(gate) * value
+        qa, sa = (t.float() for t in ref.codes(a))
+        ref.check("down", down8(a), *ref.product(qa.to(torch.int8), (ref.codes(a)[1]).float(), down8.weight, down8.scales, down8.bias, dtype))
+        assert torch.equal(down8(a), y)
+        exact, _ = norm(x, residual=h)
+        gate, value = up(exact).chunk(2, dim=-1)
+        exact = down(torch.nn.functional.silu(gate) * value)
+    # rounding to 8 bits: a step is at most max|row| / 127, some 1/35 of a row's root mean square at these lengths, off by its root
+    # mean square of 0.29; four such operands (two rows, two weights) on the way to y, whose bias has no such error
+    assert float((y - exact).float().norm() / exact.float().norm()) < 0.29 / 35 * 4
+    assert up8((q[:, :0], s[:, :0])).shape == (2, 0, 1536)
+
+
+def test_layers_refuse_gradients_and_load():
+    import mflux_amd
+    from mflux_amd import nn
+
+    norm, up, _ = layers()
+    up8 = up.to_int8()
+    x = randn(1, 3, 512, dtype=BF16).requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        up8(x)
+    with pytest.raises(ValueError, match="no gradient"):
+        norm.int8(x)
+    other = nn.Int8Linear(512, 1536, bias=False, device="cuda")
+    other.load_state_dict(up8.state_dict())
+    assert torch.equal(other(x.detach()), up8(x.detach()))
+    odd = torch.nn.Linear(77, 40, device="cuda", dtype=F32)
+    odd8 = nn.Int8Linear.from_linear(odd)
+    fresh = nn.Int8Linear(77, 40, device="cuda", dtype=F32)
+    fresh.load_state_dict(odd8.state_dict())
+    t = randn(2, 5, 77)
+    assert torch.equal(fresh(t), odd8(t))
+    q, s = mflux_amd.int8_quantize(t)
+    ref.check("y", odd8(t), *ref.product(q, s, odd8.weight, odd8.scales, odd8.bias.detach(), F32))
+    # trained through the norm
+    leaf = randn(3, 3, 512, dtype=BF16).requires_grad_()
+    y, h = norm(leaf, residual=x)
+    (y.float().sum() + h.float().sum()).backward()
+    assert leaf.grad.shape == leaf.shape and norm.weight.grad.shape == (512,) and torch.equal(leaf.grad, x.grad)
+
+
+def test_int8_other_stream():
+    norm, up, down = layers()
+    up8, down8 = up.to_int8(), down.to_int8()
+    x, h = randn(1, 40, 512, dtype=BF16), randn(2, 40, 512, dtype=BF16)
+    want = chain(x, h, norm, up8, down8)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = chain(x, h, norm, up8, down8)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_int8_captured_and_replayed():
+    """Two graphs (a chain of layers whose products cut K, a training step of the norm) and eager calls in between."""
+    import mflux_amd
+
+    norm, up, down = layers(K=2048, inner=8192)
+    up8, down8 = up.to_int8(), down.to_int8()
+    assert plan(40, 2048, 8192, 2)[3]  # down's K is cut: planes, and a second kernel
+    x, h = randn(1, 40, 2048, dtype=BF16), randn(2, 40, 2048, dtype=BF16)
+    t, w = randn(3, 300, 264).requires_grad_(), randn(4, 264).requires_grad_()
+    dy, dh = randn(5, 300, 264), randn(6, 300, 264)
+
+    def step():
+        y, s = mflux_amd.rms_norm(t, w, residual=dh)
+        return (y, s, *torch.autograd.grad((y, s), (t, w), (dy, dh)))
+
+    def work():
+        with torch.no_grad():
+            return chain(x, h, norm, up8, down8)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), work()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outputs = [], []
+    for f in (step, work):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outputs.append(f())
+        graphs.append(g)
+    for i in range(4):
+        with torch.no_grad():
+            t.copy_(randn(20 + i, 300, 264))
+            x.copy_(randn(30 + i, 40, 2048, dtype=BF16))
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outputs[0], step()))
+        assert all(torch.equal(a, b) for a, b in zip(outputs[1], work()))
+
+
+def test_norm_capture_next_to_a_living_graph_is_refused():
+    """An eager result of the same leaf on the default stream: its nodes would end the process when the captured backward pass
+    reaches them.  Refused before anything is captured; without it the same capture works."""
+    import mflux_amd
+
+    t = randn(1, 20, 64).requires_grad_()
+    ones = torch.ones_like(t)
+    want = torch.autograd.grad(mflux_amd.rms_norm(t), t, ones)[0]
+    held = mflux_amd.rms_norm(t)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="graph is being captured"):
+        with torch.cuda.graph(graph):
+            mflux_amd.rms_norm(t)
+    torch.cuda.synchronize()
+    del held, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(mflux_amd.rms_norm(t), t, ones)[0]
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_int8_no_forward_mode():
+    """A tangent is refused, not dropped."""
+    import mflux_amd
+    from torch.autograd import forward_ad
+
+    x, w, q = randn(1, 3, 64), randn(2, 64), codes(3, 3, 64)
+    s = scales(4, 3)
+    calls = [((x, w, x.clone()), lambda x, w, r: mflux_amd.rms_norm(x, w, residual=r)[0]),
+             ((x, w, x.clone()), lambda x, w, r: mflux_amd.rms_norm_int8(x, w, residual=r)[1]),
+             ((x,), lambda x: mflux_amd.int8_quantize(x)[1]), ((s,), lambda s: mflux_amd.int8_dequantize(q, s, F32)),
+             ((s, s.clone(), randn(5, 3)), lambda a, b, c: mflux_amd.int8_matmul(q, a, q, b, bias=c, dtype=F32))]
+    for operands, call in calls:
+        for i, t in enumerate(operands):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call(*operands[:i], dual, *operands[i + 1:])
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                    call(*operands[:i], dual, *operands[i + 1:])
+                assert torch.equal(call(*operands), call(*operands))
+
+
+def test_int8_routes_agree():
+    """The ops, the C functions that the ordinary call takes, and the C ABI give the same bits."""
+    import ctypes
+
+    from mflux_amd import _lib
+
+    lib, ops, native, stream = _lib.load(), _lib.ops(), _lib.native(), torch.cuda.current_stream().cuda_stream
+    x, r, w = randn(1, 2, 9, 256, dtype=BF16), randn(2, 2, 9, 256, dtype=BF16), randn(3, 256, dtype=BF16)
+    y, s = ops.rms_norm(x, w, r, 1e-6)
+    got = native.rms_norm(x, w, r, 1e-6)
+    assert torch.equal(got[0], y) and torch.equal(got[1], s)
+    a = _lib.RmsNormArgs(dtype=_lib.BF16, eps=1e-6, rows=18, columns=256, x=x.data_ptr(), residual=r.data_ptr(), weight=w.data_ptr(), x_stride=256,
+                         residual_stride=256)
+    y2, s2 = torch.empty_like(y), torch.empty_like(s)
+    a.y, a.sum = y2.data_ptr(), s2.data_ptr()
+    _lib.check("mfq_rms_norm", lib.mfq_rms_norm(ctypes.byref(a), stream))
+    assert torch.equal(y2, y) and torch.equal(s2, s)
+    for norm in (True, False):
+        q = ops.rms_norm_int8(x, w, r, 1e-6)[:2] if norm else ops.int8_quantize(x)
+        got = native.int8_rows(x, w if norm else None, r if norm else None, 1e-6, norm)
+        assert torch.equal(got[0], q[0]) and torch.equal(got[1], q[1])
+    p, t = ops.int8_quantize(randn(4, 70, 256, dtype=BF16))
+    b = randn(5, 70, dtype=BF16)
+    assert torch.equal(native.int8_matmul(*q, p, t, b, _lib.BF16), ops.int8_matmul(*q, p, t, b, BF16))
+    # what the C functions leave to the ops
+    assert native.rms_norm(x[:, :, 1:], None, None, 1e-6) is None and native.rms_norm(x, w, r, -1.0) is None
+    assert native.rms_norm(x.clone().requires_grad_(), w, r, 1e-6) is None and native.int8_rows(x[..., :40], None, None, 0.0, False) is None
+    assert native.int8_matmul(q[0].cpu(), q[1], p, t, None, 2) is None and native.int8_matmul(*q, p, t, b, _lib.F16) is None
