@@ -731,8 +731,8 @@ int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int dtype, int* k_rang
   if (int rc = check_int8(M, N, K)) return rc;
   const mfq::Int8Plan p = mfq::int8_plan(dtype, M, N, K);
   if (k_ranges) *k_ranges = p.splits;
-  if (tile_rows) *tile_rows = p.rows;
-  if (tile_columns) *tile_columns = p.columns;
+  if (tile_rows) *tile_rows = p.tiles.rows;
+  if (tile_columns) *tile_columns = p.tiles.columns;
   return p.kernel;
 }
 
@@ -754,7 +754,7 @@ int mfq_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales, co
   if (need && !workspace) return MFQ_ENULL;
   if (need > workspace_bytes) return MFQ_ESCRATCH;
   if (need && !mfq::aligned16(workspace)) return MFQ_EALIGN;
-  const mfq::Int8Call c = {x, w, x_scales, w_scales, bias, y, M, N, K, x_stride, w_stride};
+  const mfq::Int8Call c = {x, w, x_scales, w_scales, bias, y, M, N, K, N, x_stride, w_stride};
   return mfq::launch_int8_matmul(dtype, c, p, workspace, (hipStream_t)stream);
 }
 

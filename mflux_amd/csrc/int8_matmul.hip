@@ -193,9 +193,10 @@ __global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int 
   constexpr bool kRaw = std::is_same_v<T, I32>;
   auto store = [&](const Item& it) __attribute__((always_inline)) {
     constexpr int kEach = 16 / (int)sizeof(E);
-    const bool whole = c.N % kEach == 0;
+    const int64_t stride = kRaw ? c.N : c.y_stride;
+    const bool whole = c.N % kEach == 0 && stride % kEach == 0;
     const int64_t n0 = it.n0 + wn, m0 = it.m0 + wm + r;
-    char* y = static_cast<char*>(out) + ((kRaw ? (int64_t)it.split * c.M : 0) + m0) * c.N * (int64_t)sizeof(E);
+    char* y = static_cast<char*>(out) + ((kRaw ? (int64_t)it.split * c.M : 0) + m0) * stride * (int64_t)sizeof(E);
     float xs[kI];
 #pragma unroll
     for (int i = 0; i < kI; ++i) xs[i] = kRaw ? 0.f : c.x_scales[min(m0 + 16 * i, c.M - 1)];
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int 
       }
 #pragma unroll
       for (int i = 0; i < kI; ++i) {
-        E* row = reinterpret_cast<E*>(y + (int64_t)(16 * i) * c.N * (int64_t)sizeof(E));
+        E* row = reinterpret_cast<E*>(y + (int64_t)(16 * i) * stride * (int64_t)sizeof(E));
         const bool inside = m0 + 16 * i < c.M;
 #pragma unroll
         for (int p = 0; p < kPair; ++p) asm volatile("" : "+a"(acc[i][j + p]));  // (or all of acc is moved to vector registers at the loop's end)
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(kFewMaxWaves* kWave) void int8_few_kernel(Int8Call 
     int sum = 0;
     for (int k = 0; k < waves; ++k) sum += s[k * kX * 128] + s[k * kX * 128 + 64];
     const float v = value_of(sum, c.x_scales[token], c.w_scales[n], c.bias ? T::to_f32(static_cast<const E*>(c.bias)[n]) : 0.f);
-    static_cast<E*>(c.y)[token * c.N + n] = T::from_f32(v);
+    static_cast<E*>(c.y)[token * c.y_stride + n] = T::from_f32(v);
   }
 }
 
@@ -494,15 +495,15 @@ int launch_tiles(const Int8Call& c, int splits, void* out, hipStream_t stream) {
 }
 
 template <typename T>
-int launch_tiles_of(const Int8Call& c, const Int8Plan& p, void* out, hipStream_t stream) {
-  switch (p.rows * 1000 + p.columns) {
-    case 32064: return launch_tiles<Tile32x64, T>(c, p.splits, out, stream);
-    case 64064: return launch_tiles<Tile64x64, T>(c, p.splits, out, stream);
-    case 64128: return launch_tiles<Tile64x128, T>(c, p.splits, out, stream);
-    case 128128: return p.places == 2 ? launch_tiles<Tile128x128Two, T>(c, p.splits, out, stream) : launch_tiles<Tile128x128, T>(c, p.splits, out, stream);
-    case 128192: return launch_tiles<Tile128x192, T>(c, p.splits, out, stream);
+int launch_tiles_of(const Int8Call& c, const Int8Tiles& t, int splits, void* out, hipStream_t stream) {
+  switch (t.rows * 1000 + t.columns) {
+    case 32064: return launch_tiles<Tile32x64, T>(c, splits, out, stream);
+    case 64064: return launch_tiles<Tile64x64, T>(c, splits, out, stream);
+    case 64128: return launch_tiles<Tile64x128, T>(c, splits, out, stream);
+    case 128128: return t.places == 2 ? launch_tiles<Tile128x128Two, T>(c, splits, out, stream) : launch_tiles<Tile128x128, T>(c, splits, out, stream);
+    case 128192: return launch_tiles<Tile128x192, T>(c, splits, out, stream);
     default:
-      if constexpr (sizeof(typename T::storage) == 2) return launch_tiles<Tile256x256, T>(c, p.splits, out, stream);
+      if constexpr (sizeof(typename T::storage) == 2) return launch_tiles<Tile256x256, T>(c, splits, out, stream);
       else return MFQ_EUNSUPPORTED;  // the plan has none
   }
 }
@@ -550,11 +551,23 @@ int launch_few(const Int8Call& c, hipStream_t stream) {
 template <typename T>
 int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t stream) {
   if (p.kernel == MFQ_INT8_FEW) {
-    if (p.rows == 8) return launch_few<1, T>(c, stream);
+    if (p.tiles.rows == 8) return launch_few<1, T>(c, stream);
     return launch_few<2, T>(c, stream);
   }
-  if (p.splits == 1) return launch_tiles_of<T>(c, p, c.y, stream);
-  if (int rc = launch_tiles_of<I32>(c, p, workspace, stream)) return rc;
+  if (p.first) {  // two products side by side, of columns that fill whole rounds of workgroups and of the others
+    using E = typename T::storage;
+    Int8Call part = c;
+    part.N = p.first;
+    if (int rc = launch_tiles_of<T>(part, p.tiles, 1, part.y, stream)) return rc;
+    part.N = c.N - p.first;
+    part.w += p.first * c.w_stride;
+    part.w_scales += p.first;
+    if (part.bias) part.bias = static_cast<const E*>(c.bias) + p.first;
+    part.y = static_cast<E*>(c.y) + p.first;
+    return launch_tiles_of<T>(part, p.rest, 1, part.y, stream);
+  }
+  if (p.splits == 1) return launch_tiles_of<T>(c, p.tiles, 1, c.y, stream);
+  if (int rc = launch_tiles_of<I32>(c, p.tiles, p.splits, workspace, stream)) return rc;
   const bool wide = c.N % 4 == 0;
   const int64_t threads = c.M * c.N / (wide ? 4 : 1);
   const dim3 grid((unsigned)((threads + 255) / 256));
@@ -565,45 +578,69 @@ int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t st
 
 }  // namespace
 
-// What a call is estimated to take, in us, and the tile of the least: launch and first bytes 3, a round of workgroups as many steps as
-// its range of K has at the tile's time each, a cut K 4 for the second launch and its planes at 3 TB/s written and read; no call is faster
-// than its bytes.  Times of a step measured with all compute units busy (30 and 80 steps, 120 to 1360 tiles): they follow the tile's
-// bytes through LDS and a latency, not its matrix instructions, but for the largest.
+// What a product is estimated to take, in us, and the tile of the least: launch and first bytes 3, a round of workgroups as many steps
+// as its range of K has at the tile's time each, a cut K 4 for the second launch and its planes at 3 TB/s written and read.  Times of a
+// step measured with all compute units busy (30 and 80 steps, 120 to 1360 tiles): they follow the tile's bytes through LDS and a
+// latency, not its matrix instructions, but for the largest.
+struct Choice {
+  Int8Tiles tiles;
+  float step;
+};
+constexpr Choice kChoices[] = {{{32, 64, 1}, 0.30f},   {{64, 64, 1}, 0.40f},   {{64, 128, 1}, 0.47f},  {{128, 128, 1}, 0.66f},
+                               {{128, 128, 2}, 1.12f}, {{128, 192, 1}, 0.84f}, {{256, 256, 1}, 1.58f}};
+
+float least_time(int dtype, int64_t M, int64_t N, int64_t steps, bool cut_k, Int8Tiles& tiles, int& splits) {
+  float least = 1e30f;
+  for (const Choice& o : kChoices) {
+    if (o.tiles.rows == 256 && dtype == MFQ_F32) continue;
+    const int64_t n = ((M + o.tiles.rows - 1) / o.tiles.rows) * ((N + o.tiles.columns - 1) / o.tiles.columns);
+    const int64_t places = (int64_t)compute_units() * o.tiles.places;
+    int64_t most = o.tiles.rows == 256 || !cut_k ? 1 : places / n;
+    if (most > steps / 4) most = steps / 4;
+    if (most > 16) most = 16;
+    for (int cut = 0; cut < 2; ++cut) {
+      const int64_t s = cut ? most : 1;
+      if (cut && s < 2) break;
+      float t = 3.f + (float)((n * s + places - 1) / places) * (float)((steps + s - 1) / s) * o.step;
+      if (s > 1) t += 4.f + (float)(s * M * N) * 4.f / 3e6f;
+      if (t < least) {
+        least = t;
+        tiles = o.tiles;
+        splits = (int)s;
+      }
+    }
+  }
+  return least;
+}
+
 Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K) {
+  Int8Plan p = {MFQ_INT8_TILES, 1, {}, 0, {}};
   if (M <= 16) {  // rows of x that a workgroup keeps in LDS, some blocks' sums beside them
     int waves, steps;
     few_shape(K, waves, steps);
     const int tokens8 = M <= 8 ? 1 : 2;
-    if (few_image(tokens8, steps, waves) + 2 * few_sums(tokens8, waves) <= kMaxLds) return {MFQ_INT8_FEW, 1, 8 * tokens8, 8, 1};
-  }
-  struct Choice {
-    int rows, columns, places;
-    float step;
-  };
-  static constexpr Choice kChoices[] = {{32, 64, 1, 0.30f},   {64, 64, 1, 0.40f},   {64, 128, 1, 0.47f},  {128, 128, 1, 0.66f},
-                                        {128, 128, 2, 1.12f}, {128, 192, 1, 0.84f}, {256, 256, 1, 1.58f}};
-  const int64_t units = compute_units(), steps = (K + BK - 1) / BK;
-  Int8Plan best = {};
-  float least = 1e30f;
-  for (const Choice& o : kChoices) {
-    if (o.rows == 256 && dtype == MFQ_F32) continue;
-    const int64_t tiles = ((M + o.rows - 1) / o.rows) * ((N + o.columns - 1) / o.columns), places = units * o.places;
-    int64_t splits = o.rows == 256 ? 1 : places / tiles;
-    if (splits > steps / 4) splits = steps / 4;
-    if (splits > 16) splits = 16;
-    for (int cut = 0; cut < 2; ++cut) {
-      const int64_t s = cut ? splits : 1;
-      if (cut && s < 2) break;
-      const float rounds = (float)((tiles * s + places - 1) / places);
-      float t = 3.f + rounds * (float)((steps + s - 1) / s) * o.step;
-      if (s > 1) t += 4.f + (float)(s * M * N) * 4.f / 3e6f;
-      if (t < least) {
-        least = t;
-        best = {MFQ_INT8_TILES, (int)s, o.rows, o.columns, o.places};
-      }
+    if (few_image(tokens8, steps, waves) + 2 * few_sums(tokens8, waves) <= kMaxLds) {
+      p.kernel = MFQ_INT8_FEW;
+      p.tiles = {8 * tokens8, 8, 1};
+      return p;
     }
   }
-  return best;
+  const int64_t steps = (K + BK - 1) / BK;
+  const float whole = least_time(dtype, M, N, steps, true, p.tiles, p.splits);
+  if (p.tiles.rows != 256) return p;
+  // The largest tiles' last round may leave most compute units idle: whole rounds of them, and smaller tiles for the columns behind
+  // (one launch -> two: 2000 x 10240 x 3840 96 -> 81 us, 5000 x 3840 x 10240 212 -> 175, 4352 x 12288 x 4096 201 -> 193,
+  // 4352 x 20480 x 3840, five rounds and a third, 305 -> 302, and 2 % slower at most, 3000 x 20480 x 3840)
+  const int64_t units = compute_units(), down = (M + 255) / 256, across = (N + 255) / 256, columns = down * across / units * units / down;
+  if (columns == 0 || columns >= across) return p;
+  int one;
+  Int8Tiles rest;
+  const float behind = least_time(dtype, M, N - 256 * columns, steps, false, rest, one);
+  if (3.f + (float)((down * columns + units - 1) / units) * (float)steps * 1.58f + behind < whole) {
+    p.first = 256 * columns;
+    p.rest = rest;
+  }
+  return p;
 }
 
 size_t int8_workspace_bytes(const Int8Plan& p, int64_t M, int64_t N) { return p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0; }

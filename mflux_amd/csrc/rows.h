@@ -30,17 +30,22 @@ struct Int8Call {
   const int8_t *x, *w;
   const float *x_scales, *w_scales;
   const void* bias;  // of y's type, or nullptr
-  void* y;           // [M, N], dense
-  int64_t M, N, K;
+  void* y;           // [M, N], rows of y_stride
+  int64_t M, N, K, y_stride;
   int64_t x_stride, w_stride;  // of rows, whole 16 bytes
 };
 
 // The kernel a call takes and how it is cut
+struct Int8Tiles {
+  int rows, columns;  // of a workgroup's tile
+  int places;         // of workgroups on a compute unit
+};
 struct Int8Plan {
   int kernel;   // MFQ_INT8_*
   int splits;   // ranges of K
-  int rows, columns;  // of a workgroup's tile
-  int places;         // of workgroups on a compute unit
+  Int8Tiles tiles;
+  int64_t first;   // columns of y that these tiles have, 0: all
+  Int8Tiles rest;  // of the others
 };
 Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K);
 size_t int8_workspace_bytes(const Int8Plan& p, int64_t M, int64_t N);

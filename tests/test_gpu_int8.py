@@ -312,6 +312,23 @@ def test_int8_matmul_on_every_kernel(M, N, K, want):
         assert torch.equal(y, mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype))
 
 
+@pytest.mark.parametrize("M,N,K,first", [(2000, 10250, 1040, 8192), (2000, 10240, 1152, 8192), (2000, 10251, 1040, 8192)])
+def test_int8_matmul_of_columns_in_two_launches(M, N, K, first):
+    """Where the largest tiles would leave a last round mostly idle: the same bits as of each columns' own product, to the last column."""
+    import mflux_amd
+
+    print(f"M={M} N={N} K={K}", flush=True)
+    assert plan(M, N, K, 2) == (2, 256, 256, False)
+    x, w, xs, ws = codes(1, M, K), codes(2, N, K), scales(3, M), scales(4, N)
+    for dtype in (BF16, F16):
+        b = randn(5, N, dtype=dtype)
+        y = mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype)
+        ref.check("y", y, *ref.product(x, xs, w, ws, b, dtype))
+        for part in (slice(0, first), slice(first, N)):
+            assert torch.equal(y[:, part], mflux_amd.int8_matmul(x, xs, w[part], ws[part], bias=b[part], dtype=dtype))
+        assert torch.equal(mflux_amd.int8_matmul(x, xs, w, ws, dtype=dtype), mflux_amd.int8_matmul(x, xs, w, ws, bias=torch.zeros_like(b), dtype=dtype))
+
+
 def test_rows_behind_others_are_left_alone():
     """A call writes its own results: what lies in front of and behind them in memory stays."""
     from mflux_amd import _lib
