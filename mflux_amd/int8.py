@@ -77,7 +77,9 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, *, residu
     ``(codes, scales)``, with ``residual`` ``(codes, scales, sum)``.
 
     A code is ``rint(127 p / max|p|)`` of the row's products ``p = sum * weight``, ties to even, decided by
-    the exact quotient (the root is a factor of the scale alone).  No gradients."""
+    the exact quotient (the root is a factor of the scale alone).  Products of 16-bit types are taken in
+    float32: one beyond its range makes the row's scale NaN, as an infinity or NaN in the row does.
+    No gradients."""
     rows = _lib.native().int8_rows(x, weight, residual, eps, True)
     if rows is not None:
         return rows
