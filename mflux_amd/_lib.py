@@ -169,14 +169,14 @@ class _NotBuilt:
     general route, which words argument errors first and then says what is missing."""
 
     linear = linear_float32 = silu_linear = epilogue_linear = staticmethod(lambda *args: None)
-    rms_norm = int8_rows = int8_matmul = staticmethod(lambda *args: None)
+    rms_norm = int8_rows = int8_dequantize = int8_matmul = staticmethod(lambda *args: None)
 
 
 def native():
     """The Python C functions of csrc/py_calls.cpp, which live in the same library
     as the ops: ``linear``, ``linear_float32``, ``silu_linear`` and
     ``epilogue_linear`` take the ordinary call of a quantized linear straight to
-    the C ABI, ``rms_norm``, ``int8_rows`` and ``int8_matmul`` those of int8.py, and return
+    the C ABI, ``rms_norm``, ``int8_rows``, ``int8_dequantize`` and ``int8_matmul`` those of int8.py, and return
     None for anything else."""
     global _native
     if _native is None:

@@ -362,6 +362,31 @@ PyObject* int8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// int8_dequantize(codes, scales, code of the result's type) -> values or None
+PyObject* int8_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor codes, scales;
+  int64_t code = 0;
+  if (n != 3 || !tensor_arg(args[0], &codes) || !tensor_arg(args[1], &scales) || !int_arg(args[2], &code) || intercepted()) Py_RETURN_NONE;
+  if (!codes.defined() || !scales.defined() || !constant(codes) || !constant(scales) || scales.device() != codes.device()) Py_RETURN_NONE;
+  if (codes.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat || codes.dim() < 1 || codes.numel() == 0 ||
+      scales.sizes() != codes.sizes().slice(0, codes.dim() - 1) || (code != MFQ_BF16 && code != MFQ_F16 && code != MFQ_F32))
+    Py_RETURN_NONE;
+  RECORD_FUNCTION("mfq::int8_dequantize", std::vector<c10::IValue>({codes, scales}));
+  const c10::hip::HIPGuardMasqueradingAsCUDA on_device(codes.device());
+  const int64_t columns = codes.size(-1), rows = codes.numel() / columns;
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(code == MFQ_BF16 ? at::kBFloat16 : code == MFQ_F16 ? at::kHalf : at::kFloat));
+  const auto* p = static_cast<const int8_t*>(codes.const_data_ptr());
+  const auto* s = static_cast<const float*>(scales.const_data_ptr());
+  void *to = out.data_ptr(), *stream = c10::hip::getCurrentHIPStream(codes.get_device()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mfq_int8_dequantize(p, columns, s, rows, columns, to, (int)code, stream);
+  Py_END_ALLOW_THREADS
+  return result("mfq_int8_dequantize", rc, out);
+  END_HANDLE_TH_ERRORS
+}
+
 // int8_matmul(x, x_scales, w, w_scales, bias or None, code of the result's type) -> y or None
 PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -409,6 +434,7 @@ PyMethodDef kMethods[] = {
     {"epilogue_linear", (PyCFunction)(void*)epilogue_linear, METH_FASTCALL, "a linear with its epilogue, or None"},
     {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, "RMS norm of rows, with the residual's addition, or None"},
     {"int8_rows", (PyCFunction)(void*)int8_rows, METH_FASTCALL, "rows as 8-bit codes with a scale each, or None"},
+    {"int8_dequantize", (PyCFunction)(void*)int8_dequantize, METH_FASTCALL, "codes times their row's scale, or None"},
     {"int8_matmul", (PyCFunction)(void*)int8_matmul, METH_FASTCALL, "the product of two matrices of codes, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "libmfq_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

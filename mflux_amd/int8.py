@@ -118,7 +118,10 @@ def _check_codes(fn: str, name: str, codes: torch.Tensor, scales: torch.Tensor) 
 
 
 def int8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``codes * scales[..., None]`` in ``dtype``, rounded once."""
+    """``codes * scales[..., None]`` in ``dtype``, rounded once.  No gradients."""
+    values = _lib.native().int8_dequantize(codes, scales, _DTYPE_CODE.get(dtype))
+    if values is not None:
+        return values
     fn = "int8_dequantize"
     _check_codes(fn, "codes", codes, scales)
     if dtype not in _DTYPE_CODE:

@@ -249,3 +249,21 @@ def test_int8_layers_copied_and_moved():
         half = copy.deepcopy(layer).half()
         assert half.scales.dtype == F32 and torch.equal(half.scales, layer.scales) and half.dtype == F16
         assert half(x.half()).dtype == F16
+
+
+def test_int8_dequantize_routes_agree():
+    from mflux_amd import _lib
+
+    native, ops = _lib.native(), _lib.ops()
+    for dtype, code in ((BF16, _lib.BF16), (F16, _lib.F16), (F32, _lib.F32)):
+        for shape in ((3, 77), (2, 5, 256), (64,), (1, 1)):
+            q, s = codes(1, *shape), scales(2, *shape[:-1], 1)[..., 0].contiguous()
+            got = native.int8_dequantize(q, s, code)
+            assert got.dtype == dtype and torch.equal(got, ops.int8_dequantize(q, s, dtype))
+            assert torch.equal(got, (q.float() * s[..., None]).to(dtype))
+    q, s = codes(1, 3, 80), scales(2, 3)
+    # what the C function leaves to the op, or to the checks
+    assert native.int8_dequantize(q[:, 1:], s, _lib.BF16) is None and native.int8_dequantize(q[:0], s[:0], _lib.BF16) is None
+    assert native.int8_dequantize(q, s[:2], _lib.BF16) is None and native.int8_dequantize(q, s, None) is None
+    assert native.int8_dequantize(q, s.double(), _lib.BF16) is None and native.int8_dequantize(q, s, 7) is None
+    assert native.int8_dequantize(q, s.clone().requires_grad_(), _lib.BF16) is None
