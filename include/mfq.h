@@ -646,7 +646,7 @@ int mfq_int8_dequantize(const int8_t* codes, int64_t code_stride, const float* s
  *   y [M, N] dense, 16-byte aligned, bias [N] or NULL, both of dtype (MFQ_F32, MFQ_F16 or MFQ_BF16)
  * workspace: mfq_int8_matmul_workspace_bytes() of it, 16-byte aligned (the sums of a K that is cut).
  * mfq_int8_matmul_plan: the kernel that a product takes (MFQ_INT8_*, or an error code), the ranges that it cuts K into and its
- * tile (NULL where not wanted).
+ * tile (NULL where not wanted).  Columns behind the last whole round of the largest tiles may run on smaller ones.
  */
 enum mfq_int8_kernel { MFQ_INT8_FEW = 1, MFQ_INT8_TILES = 2 };
 int mfq_int8_matmul_plan(int64_t M, int64_t N, int64_t K, int dtype, int* k_ranges, int* tile_rows, int* tile_columns);

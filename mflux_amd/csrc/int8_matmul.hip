@@ -35,7 +35,10 @@ __device__ inline float value_of(int sum, float xs, float ws, float add) { retur
 //   - workgroups stay and walk tiles; the ring runs on over a tile's end, and results go from the registers to memory.
 // Large products are bound by power: matrix instructions alone, on operands that stay in registers (codes of a normal
 // distribution), reach 4.0 PFLOP/s where the second operand stays from one instruction to the next, 3.4 where the first one
-// does, 3.0 where both change (32x32x32: 3.4; zeros, bound by issue: 4.2, 32x32x32 4.9).
+// does, 3.0 where both change (32x32x32: 3.4; zeros, bound by issue: 4.2, 32x32x32 4.9).  8192^3 takes 395 us (2.78 PFLOP/s),
+// 16384 x 4096 x 12288 580, 4352 x 20480 x 3840 298 (2.30; 19200 columns of it in five whole rounds, the others on 128 x 192).
+// Below some 2000 rows it is the way into LDS, about 50 bytes a ns and compute unit whatever the tile: 512 x 3840 x 3840 16.7 us,
+// 333 x 11520 x 3840 25 (a quarter of the matrix units' time), 24 x 3840 x 10240 9 and 3 for its join.
 template <int kM_, int kN_, int kWM_, int kWN_, int kUnits_>
 struct Tile {
   static constexpr int kM = kM_, kN = kN_, kWM = kWM_, kWN = kWN_, kUnits = kUnits_;
@@ -325,6 +328,7 @@ __global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int 
 // same (row 8 h + token, column 2 row + h); the others are dropped.
 // A workgroup walks a run of blocks of eight rows of w, its wavefronts have a range of K each; a lane keeps its share of x in
 // LDS (nothing is exchanged before the end), and the wavefronts' sums meet there behind the last block.
+// 1 x 10240 x 3840: 8.5 us with w in the last cache, 10 without (3.9 TB/s); 1 x 3840 x 10240 11.9; 1 x 2048 x 1024 3.6.
 constexpr int kFewMaxWaves = 16;
 
 // LDS of a workgroup: x, and a block's sums
@@ -443,7 +447,8 @@ __global__ __launch_bounds__(kFewMaxWaves* kWave) void int8_few_kernel(Int8Call 
   }
 }
 
-// ---- the ranges of a cut K joined: four outputs to a thread where rows are whole fours
+// ---- the ranges of a cut K joined: four outputs to a thread where rows are whole fours.  Bound by the launch and its first bytes
+// (24 x 3840 of eight ranges 3 us, 3 MB).
 template <typename T, bool kWide>
 __global__ __launch_bounds__(256) void int8_join_kernel(Int8Call c, const int* planes, int splits) {
   using E = typename T::storage;

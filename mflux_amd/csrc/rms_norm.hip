@@ -3,11 +3,11 @@
 //   y = round(s r w),  r = 1 / sqrt(mean(s^2) + eps)
 //   codes = rint(127 p / max|p|), scale = r max|p| / 127,  p = s w   (without a norm p = x and r = 1)
 //   dx = r (w dy - s r^2 mean(w dy s)) + ds,  dw = sum over the rows of dy s r
-// All of it is bound by memory: a row is read once, into registers, and written once.  A row takes one wavefront or one
-// workgroup of four, whichever has it in at most eight 16-byte pieces a lane; the weight stays in registers from row to row.
+// All of it is bound by memory: a row is read once, into registers, and written once.  A row takes a wavefront or a workgroup of 2 to
+// 16, by its length; the weight stays in registers from row to row.
 // A code does not depend on r, so it is decided by the products p alone, and exactly: where the float32 quotient is next to a
 // border between two codes it is taken again in float64, which tells 16-bit types' products apart.
-// Sums are float32 (eight to some hundred terms a lane, then a tree), in an order that the row's length alone fixes.
+// Sums are float32 (eight to some hundred terms a lane, then a tree), in an order that the row's length and alignment alone fix.
 #include <type_traits>
 
 #include "rows.h"
@@ -170,7 +170,9 @@ struct Coder {
 
 enum Result { kNormalised, kCodes, kWeightedCodes };
 
-// kLanes lanes to a row, each kChunks of its units of V elements; up to 256 threads, workgroups of several rows
+// kLanes lanes to a row, each kChunks of its units of V elements; up to 256 threads, workgroups of several rows.  4352 x 3840
+// bfloat16 with a residual 25 us (5.3 TB/s), with codes 24; 10240 x 3840 into codes without a norm 29; a few rows 4, a launch and
+// one trip to memory each way.
 template <typename T, int V, int kLanes, int kChunks, int kResult>
 __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kernel(RowsCall c) {
   using E = typename T::storage;
@@ -310,7 +312,8 @@ __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
   }
 }
 
-// ---- gradients
+// ---- gradients.  A row's two sums are taken again from what was normalised (one more read instead of one more array), so a pass
+// reads three arrays and writes one: 4352 x 3840 bfloat16 26.5 us (5.0 TB/s), and 4 to 5 for the partial sums' own kernel.
 template <typename T, int V, int kLanes, int kChunks, bool kWeight>
 __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backward_kernel(RowsCall c) {
   using E = typename T::storage;
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(1024) void rows_weight_kernel(const float* parts, i
   static_cast<typename T::storage*>(dw)[column] = T::from_f32(v);
 }
 
-// ---- codes times their row's scale
+// ---- codes times their row's scale: 4352 x 3840 to bfloat16 10.8 us (4.6 TB/s)
 template <typename T, bool kWide>
 __global__ __launch_bounds__(kThreads) void rows_values_kernel(const int8_t* codes, int64_t stride, const float* scales, int64_t rows,
                                                                int64_t columns, void* out) {
