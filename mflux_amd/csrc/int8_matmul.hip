@@ -328,6 +328,7 @@ __global__ __launch_bounds__(S::kThreads) void int8_tile_kernel(Int8Call c, int 
 // same (row 8 h + token, column 2 row + h); the others are dropped.
 // A workgroup walks a run of blocks of eight rows of w, its wavefronts have a range of K each; a lane keeps its share of x in
 // LDS (nothing is exchanged before the end), and the wavefronts' sums meet there behind the last block.
+// Up to 32 rows of x go through a workgroup, and up to four workgroups share a run of w.
 // 1 x 10240 x 3840: 8.5 us with w in the last cache, 10 without (3.9 TB/s); 1 x 3840 x 10240 11.9; 1 x 2048 x 1024 3.6.
 constexpr int kFewMaxWaves = 16;
 
@@ -368,9 +369,9 @@ __global__ __launch_bounds__(kFewMaxWaves* kWave) void int8_few_kernel(Int8Call 
   int* sums = reinterpret_cast<int*>(lds + few_image(kX, steps, waves)) + wave * (few_sums(kX, 1) / 4);
   const int block_ints = few_sums(kX, waves) / 4;
   if (mine > 0 && blocks > 0) {
-    // x is requested before w, four steps at a time
+    // x is requested before w, some steps at a time
     const int x_column = 64 * (j >> 3) + 16 * q;
-    constexpr int kAtOnce = 4;
+    constexpr int kAtOnce = kX > 2 ? 2 : 4;
     i32x4 v[kAtOnce][kX];
     auto load_x = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
@@ -524,8 +525,25 @@ void few_shape(int64_t K, int& waves, int& steps) {
   }
 }
 struct Few {
-  int waves, steps, per_group, groups, grid;
+  int waves, steps, per_group, groups, rounds;
+  int64_t grid;
 };
+// A product of groups of 8 tokens8 rows of x; false: x does not fit
+bool few_of(int64_t M, int64_t N, int64_t K, int tokens8, Few& f) {
+  few_shape(K, f.waves, f.steps);
+  // One workgroup to a compute unit (two or three, each with fewer blocks, take 15 us where one takes 12: 10240 x 3840), in as many
+  // equal rounds as the room for sums asks for
+  const int64_t most = (kMaxLds - few_image(tokens8, f.steps, f.waves)) / few_sums(tokens8, f.waves), places = compute_units();
+  if (most < 2) return false;
+  const int64_t blocks = (N + 7) / 8, groups = (M + 8 * tokens8 - 1) / (8 * tokens8);
+  const int64_t rounds = (blocks * groups + places * most - 1) / (places * most);
+  const int64_t per_group = (blocks * groups + places * rounds - 1) / (places * rounds), runs = (blocks + per_group - 1) / per_group;
+  f.per_group = (int)per_group;
+  f.groups = (int)groups;
+  f.rounds = (int)rounds;
+  f.grid = (runs + 7) / 8 * 8 * groups;
+  return true;
+}
 
 template <int kX, int kRing, typename T>
 int launch_few_of(const Int8Call& c, const Few& f, hipStream_t stream) {
@@ -539,16 +557,9 @@ int launch_few_of(const Int8Call& c, const Few& f, hipStream_t stream) {
 
 template <int kX, typename T>
 int launch_few(const Int8Call& c, hipStream_t stream) {
-  int waves, steps;
-  few_shape(c.K, waves, steps);
-  // One workgroup to a compute unit (two or three, each with fewer blocks, take 15 us where one takes 12: 10240 x 3840), in as many
-  // equal rounds as the room for sums asks for
-  const int64_t most = (kMaxLds - few_image(kX, steps, waves)) / few_sums(kX, waves), places = compute_units();
-  const int64_t blocks = (c.N + 7) / 8, groups = (c.M + 8 * kX - 1) / (8 * kX);
-  const int64_t rounds = (blocks * groups + places * most - 1) / (places * most);
-  const int64_t per_group = (blocks * groups + places * rounds - 1) / (places * rounds), runs = (blocks + per_group - 1) / per_group;
-  const Few f = {waves, steps, (int)per_group, (int)groups, (int)((runs + 7) / 8 * 8 * groups)};
-  const int64_t positions = per_group * steps;  // requests of a wavefront: those behind the last are in vain
+  Few f;
+  if (!few_of(c.M, c.N, c.K, kX, f)) return MFQ_EUNSUPPORTED;  // the plan has none
+  const int64_t positions = (int64_t)f.per_group * f.steps;  // requests of a wavefront: those behind the last are in vain
   if (positions <= 2) return launch_few_of<kX, 2, T>(c, f, stream);
   return positions <= 5 ? launch_few_of<kX, 4, T>(c, f, stream) : launch_few_of<kX, 8, T>(c, f, stream);
 }
@@ -556,8 +567,12 @@ int launch_few(const Int8Call& c, hipStream_t stream) {
 template <typename T>
 int launch(const Int8Call& c, const Int8Plan& p, void* workspace, hipStream_t stream) {
   if (p.kernel == MFQ_INT8_FEW) {
-    if (p.tiles.rows == 8) return launch_few<1, T>(c, stream);
-    return launch_few<2, T>(c, stream);
+    switch (p.tiles.rows) {
+      case 8: return launch_few<1, T>(c, stream);
+      case 16: return launch_few<2, T>(c, stream);
+      case 24: return launch_few<3, T>(c, stream);
+      default: return launch_few<4, T>(c, stream);
+    }
   }
   if (p.first) {  // two products side by side, of columns that fill whole rounds of workgroups and of the others
     using E = typename T::storage;
@@ -620,18 +635,28 @@ float least_time(int dtype, int64_t M, int64_t N, int64_t steps, bool cut_k, Int
 
 Int8Plan int8_plan(int dtype, int64_t M, int64_t N, int64_t K) {
   Int8Plan p = {MFQ_INT8_TILES, 1, {}, 0, {}};
-  if (M <= 16) {  // rows of x that a workgroup keeps in LDS, some blocks' sums beside them
-    int waves, steps;
-    few_shape(K, waves, steps);
-    const int tokens8 = M <= 8 ? 1 : 2;
-    if (few_image(tokens8, steps, waves) + 2 * few_sums(tokens8, waves) <= kMaxLds) {
+  const int64_t steps = (K + BK - 1) / BK;
+  const int groups = (int)((M + 31) / 32), tokens8 = M <= 128 ? (int)((M + 8 * groups - 1) / (8 * groups)) : 0;
+  Few f;
+  const bool few = tokens8 && few_of(M, N, K, tokens8, f);
+  if (few && M <= 16) {
+    p.kernel = MFQ_INT8_FEW;
+    p.tiles = {8 * tokens8, 8, 1};
+    return p;
+  }
+  const float whole = least_time(dtype, M, N, steps, true, p.tiles, p.splits);
+  // Few rows: always up to 16, where w's bytes bound it.  Above, by an estimate: a workgroup's x (KiB of LDS, once a round) and its
+  // blocks of w at 33 bytes a ns, and 0.7 us a block.  24 x 2048 x 1024 6.2 -> 4.2 us, 24 x 3840 x 3840 10.0 -> 8.1, 128 x 512 x 2048
+  // 7.5 -> 5.3 (four groups), but 24 x 10240 x 3840 would take 20 instead of 15.
+  if (few) {
+    const float kib = (float)(few_image(tokens8, f.steps, f.waves) + 8 * f.per_group * K) / 1024.f;
+    if (1.8f + (float)f.rounds * (0.03f * kib + 0.7f * (float)f.per_group) < whole) {
       p.kernel = MFQ_INT8_FEW;
+      p.splits = 1;
       p.tiles = {8 * tokens8, 8, 1};
       return p;
     }
   }
-  const int64_t steps = (K + BK - 1) / BK;
-  const float whole = least_time(dtype, M, N, steps, true, p.tiles, p.splits);
   if (p.tiles.rows != 256) return p;
   // The largest tiles' last round may leave most compute units idle: whole rounds of them, and smaller tiles for the columns behind
   // (one launch -> two: 2000 x 10240 x 3840 96 -> 81 us, 5000 x 3840 x 10240 212 -> 175, 4352 x 12288 x 4096 201 -> 193,

@@ -267,3 +267,52 @@ def test_int8_dequantize_routes_agree():
     assert native.int8_dequantize(q, s[:2], _lib.BF16) is None and native.int8_dequantize(q, s, None) is None
     assert native.int8_dequantize(q, s.double(), _lib.BF16) is None and native.int8_dequantize(q, s, 7) is None
     assert native.int8_dequantize(q, s.clone().requires_grad_(), _lib.BF16) is None
+
+
+@pytest.mark.parametrize("M,N,K,want", [
+    (17, 40, 1040, (1, 24, 8, False)), (24, 2051, 528, (1, 24, 8, False)), (31, 2048, 1024, (1, 32, 8, False)), (32, 77, 16, (1, 32, 8, False)),
+    (33, 512, 2064, (1, 24, 8, False)), (47, 100, 1296, (1, 24, 8, False)), (63, 300, 144, (1, 32, 8, False)), (65, 256, 4096, (1, 24, 8, False)),
+    (90, 513, 768, (1, 32, 8, False)), (100, 9, 112, (1, 32, 8, False)), (127, 512, 2048, (1, 32, 8, False)), (128, 1000, 400, (1, 32, 8, False)),
+    (24, 3843, 3840, (1, 24, 8, False)), (129, 512, 2048, (2, 32, 64, False)),
+])
+def test_int8_matmul_of_small_weights(M, N, K, want):
+    """17 to 128 rows through the kernel of few rows, in one to four groups, the last token, row of w and step partly there."""
+    import mflux_amd
+
+    print(f"M={M} N={N} K={K}", flush=True)
+    assert plan(M, N, K, 2) == want
+    x, w, xs, ws = codes(1, M, K), codes(2, N, K), scales(3, M), scales(4, N)
+    for dtype in (BF16, F16, F32):
+        b = randn(5, N, dtype=dtype)
+        y = mflux_amd.int8_matmul(x, xs, w, ws, bias=b, dtype=dtype)
+        ref.check("y", y, *ref.product(x, xs, w, ws, b, dtype))
+        # each row as by itself
+        for m in (0, M // 2, M - 1):
+            assert torch.equal(y[m], mflux_amd.int8_matmul(x[m], xs[m], w, ws, bias=b, dtype=dtype))
+
+
+@pytest.mark.parametrize("M", [18, 50, 129, 200])
+def test_int8_matmul_strides_above_sixteen_rows(M):
+    """The same layouts through both kernels: rows apart, at odd addresses, repeated, transposed, of an odd length; nothing behind y is written."""
+    import mflux_amd
+
+    N, K = 120, 160
+    big_x, big_w = codes(1, M, 2 * K + 5), codes(2, N, 2 * K + 5)
+    xs, ws = scales(3, M), scales(4, N)
+    for x, w in ((big_x[:, :K], big_w[:, :K]), (big_x[:, 1:1 + K], big_w[:, 16:16 + K]), (big_x[:1, :K].expand(M, K), big_w[:1, :K].expand(N, K)),
+                 (codes(5, K, M).t(), codes(6, K, N).t()), (big_x[:, ::2][:, :K], big_w[:, ::2][:, :K]), (big_x[:, :77], big_w[:, :77])):
+        y = mflux_amd.int8_matmul(x, xs, w, ws, dtype=F32)
+        ref.check("y", y, *ref.product(x, xs, w, ws, None, F32))
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 70, 256), (50, 70, 256), (100, 9, 256), (129, 70, 256)])
+def test_int8_matmul_writes_no_further(M, N, K):
+    from mflux_amd import _lib
+
+    lib = _lib.load()
+    x, w, xs, ws = codes(1, M, K), codes(2, N, K), scales(3, M), scales(4, N)
+    y = torch.full((M * N + 4096,), 7.0, device="cuda")
+    _lib.check("mfq_int8_matmul", lib.mfq_int8_matmul(x.data_ptr(), K, xs.data_ptr(), w.data_ptr(), K, ws.data_ptr(), None, M, N, K, y.data_ptr(), _lib.F32,
+                                                      None, 0, torch.cuda.current_stream().cuda_stream))
+    ref.check("y", y[:M * N].view(M, N), *ref.product(x, xs, w, ws, None, F32))
+    assert bool((y[M * N:] == 7).all())
