@@ -21,7 +21,7 @@ import math
 
 import torch
 
-from . import _lib, core
+from . import _lib, core, int8
 from .nn import Int8Linear, Linear, QuantizedLinear
 
 _RANK_STEP = 16  # the kernels take the low rank in steps of 16
@@ -292,6 +292,12 @@ def _bake(base: torch.nn.Module, loras: list[LoRALinear], requantize: bool) -> N
         deltas.append(delta)
     if not deltas:
         return
+    if isinstance(base, Int8Linear):
+        # codes of the sum with all adapters: a delta is in the units of the weight, not of its codes
+        full = int8.int8_dequantize(base.weight, base.scales, torch.float32)
+        for old, new in zip((base.weight, base.scales), int8.int8_quantize(full + sum(deltas).to(full.device))):
+            old.copy_(new)
+        return
     if quantized:
         # all adapters at once, so that the weight is requantized a single time
         full = core.dequantize(base.weight, base.scales, base.biases, base.group_size, base.bits)
@@ -306,6 +312,24 @@ def _bake(base: torch.nn.Module, loras: list[LoRALinear], requantize: bool) -> N
             base.weight.add_(delta.to(device=base.weight.device, dtype=base.weight.dtype))
 
 
+def _wrapped(obj: torch.nn.Module):
+    """(base layer, its adapters) of a wrapper, else None."""
+    if isinstance(obj, FusedLoRALinear):
+        return obj.base_linear, [lora for lora in obj.loras if isinstance(lora, LoRALinear)]
+    return (obj.linear, [obj]) if isinstance(obj, LoRALinear) else None
+
+
+def _check_bases(module: torch.nn.Module, path: str = "") -> None:
+    wrapped = _wrapped(module)
+    if wrapped:
+        module, loras = wrapped
+        if isinstance(module, Int8Linear) and loras:
+            raise ValueError(f"[bake_and_strip_lora] '{path}' has adapters on an Int8Linear, whose codes cannot take them as they are: "
+                             "pass requantize=True, or take the adapters off")
+    for name, child in module.named_children():
+        _check_bases(child, f"{path}.{name}" if path else name)
+
+
 def bake_and_strip_lora(module: torch.nn.Module, requantize: bool = False) -> torch.nn.Module:
     """Replaces every ``LoRALinear`` / ``FusedLoRALinear`` below ``module`` by its
     base layer with the adapters added into the weight, as
@@ -316,18 +340,20 @@ def bake_and_strip_lora(module: torch.nn.Module, requantize: bool = False) -> to
     strips the wrapper without baking (``:75-77``), and so does this function
     by default; ``requantize=True`` instead dequantizes the base, adds the
     adapters in float32, rounds to the 16-bit type and quantizes again with the
-    layer's group size and bits (lossy by one requantization).  Returns
+    layer's group size and bits (lossy by one requantization).  An ``Int8Linear``
+    goes the same way with ``requantize=True``, on the device; without it a tree
+    with adapters on one is refused before anything is baked.  Returns
     ``module`` (the base layer when ``module`` itself is a wrapper)."""
-    def strip(obj: torch.nn.Module) -> torch.nn.Module:
-        if isinstance(obj, FusedLoRALinear):
-            _bake(obj.base_linear, [lora for lora in obj.loras if isinstance(lora, LoRALinear)], requantize)
-            return obj.base_linear
-        if isinstance(obj, LoRALinear):
-            _bake(obj.linear, [obj], requantize)
-            return obj.linear
-        return obj
+    if not requantize:
+        _check_bases(module)
+    return _bake_and_strip(module, requantize)
 
-    module = strip(module)
+
+def _bake_and_strip(module: torch.nn.Module, requantize: bool) -> torch.nn.Module:
+    wrapped = _wrapped(module)
+    if wrapped:
+        module, loras = wrapped
+        _bake(module, loras, requantize)
     for name, child in list(module.named_children()):
-        module._modules[name] = bake_and_strip_lora(child, requantize)
+        module._modules[name] = _bake_and_strip(child, requantize)
     return module
