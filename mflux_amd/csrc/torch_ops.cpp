@@ -1016,6 +1016,7 @@ struct RmsNormFunction : torch::autograd::Function<RmsNormFunction> {
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["wanted"] = (int64_t)(wanted(x) | wanted(weight) << 1 | wanted(residual) << 2);
     if (!residual.has_value()) return {y};
+    if (!wanted(x) && !wanted(residual)) ctx->mark_non_differentiable({sum});  // it does not depend on the weight
     return {y, sum};
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
