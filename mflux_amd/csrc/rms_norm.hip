@@ -435,24 +435,29 @@ __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c)
   }
 }
 
-// dw = sum of the workgroups' partial sums: a workgroup to 16 columns, 64 threads to a column
+// dw = sum of the workgroups' partial sums: a workgroup to 16 columns, 64 threads to a column, and on to other columns where there are
+// more than a launch has (fewer than 2^32 threads: rows of up to 2^28 values would ask for 2^34)
 template <typename T>
 __global__ __launch_bounds__(1024) void rows_weight_kernel(const float* parts, int n, int64_t columns, void* dw) {
-  const int64_t column = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-  const int part = threadIdx.x >> 4;
-  float v = 0.f;
-  if (column < columns) {
-#pragma unroll 8
-    for (int i = part; i < n; i += 64) v += parts[i * columns + column];
-  }
+  const int own = threadIdx.x & 15, part = threadIdx.x >> 4;
   __shared__ float sums[64][17];
-  sums[part][threadIdx.x & 15] = v;
-  __syncthreads();
-  if (part || column >= columns) return;
-  v = 0.f;
+  for (int64_t first = (int64_t)blockIdx.x * 16; first < columns; first += (int64_t)gridDim.x * 16) {
+    const int64_t column = first + own;
+    float v = 0.f;
+    if (column < columns) {
+#pragma unroll 8
+      for (int i = part; i < n; i += 64) v += parts[i * columns + column];
+    }
+    sums[part][own] = v;
+    __syncthreads();
+    if (part == 0 && column < columns) {
+      v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) v += sums[i][threadIdx.x & 15];
-  static_cast<typename T::storage*>(dw)[column] = T::from_f32(v);
+      for (int i = 0; i < 64; ++i) v += sums[i][own];
+      static_cast<typename T::storage*>(dw)[column] = T::from_f32(v);
+    }
+    __syncthreads();
+  }
 }
 
 // ---- codes times their row's scale: 4352 x 3840 to bfloat16 10.8 us (4.6 TB/s)
@@ -565,8 +570,9 @@ int launch(const RowsCall& c, bool wide, bool backward, hipStream_t stream) {
   const int64_t groups = backward ? launch_backward<T>(c, wide, stream) : launch_forward<T>(c, wide, stream);
   if (hipGetLastError() != hipSuccess) return MFQ_ELAUNCH;
   if (!backward || !c.parts) return MFQ_OK;
-  hipLaunchKernelGGL(rows_weight_kernel<T>, dim3((unsigned)((c.columns + 15) / 16)), dim3(1024), 0, stream, c.parts, (int)groups, c.columns,
-                     c.dweight);
+  const int64_t sixteens = (c.columns + 15) / 16, most = 8 * (int64_t)compute_units();
+  hipLaunchKernelGGL(rows_weight_kernel<T>, dim3((unsigned)(sixteens < most ? sixteens : most)), dim3(1024), 0, stream, c.parts, (int)groups,
+                     c.columns, c.dweight);
   return hipGetLastError() == hipSuccess ? MFQ_OK : MFQ_ELAUNCH;
 }
 

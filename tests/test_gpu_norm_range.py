@@ -3,9 +3,30 @@ import pytest
 import torch
 
 import int8_reference as ref
-from test_gpu_int8 import F32, randn
+from test_gpu_int8 import BF16, F32, randn
+from test_gpu_int8_calls import room
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- long rows -------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("K,dtype", [((1 << 26) - 15, F32), (1 << 26, F32), (1 << 26, BF16), (1 << 28, BF16)])
+def test_weight_gradient_of_the_longest_rows(K, dtype):
+    """More columns than one launch has sixteens for, up to the longest row there is.  Values of 1 and -1, whose sums are exact."""
+    import mflux_amd
+
+    room(30)
+    print(f"K={K} {dtype}", flush=True)
+    sign = torch.ones(K, device="cuda", dtype=dtype)
+    sign[::3] = -1
+    x, w = sign[None], torch.full((K,), 0.5, device="cuda", dtype=dtype).requires_grad_()
+    dy = torch.full((K,), 0.25, device="cuda", dtype=dtype)
+    dy[5::7] = -2
+    y = mflux_amd.rms_norm(x, w, eps=0.0)
+    assert torch.equal(y.detach(), x * 0.5)
+    dw, = torch.autograd.grad(y, w, dy[None])
+    assert torch.equal(dw, sign * dy)
 
 
 # ---- what the sum's gradient is --------------------------------------------------------------------------------------------------
