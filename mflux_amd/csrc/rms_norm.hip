@@ -435,26 +435,29 @@ __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c)
   }
 }
 
-// dw = sum of the workgroups' partial sums: a workgroup to 16 columns, 64 threads to a column, and on to other columns where there are
-// more than a launch has (fewer than 2^32 threads: rows of up to 2^28 values would ask for 2^34)
+// dw = sum of the workgroups' partial sums, in float64: rounded once, whatever their number.  A workgroup to 16 columns, 64 threads to a
+// column, and on to other columns where there are more than a launch has (fewer than 2^32 threads: rows of up to 2^28 values would ask
+// for 2^34).
 template <typename T>
 __global__ __launch_bounds__(1024) void rows_weight_kernel(const float* parts, int n, int64_t columns, void* dw) {
-  const int own = threadIdx.x & 15, part = threadIdx.x >> 4;
-  __shared__ float sums[64][17];
+  constexpr int kWaves = 1024 / kWave;
+  const int own = threadIdx.x & 15, part = threadIdx.x >> 4, wave = threadIdx.x / kWave;
+  __shared__ double sums[kWaves][16];
   for (int64_t first = (int64_t)blockIdx.x * 16; first < columns; first += (int64_t)gridDim.x * 16) {
     const int64_t column = first + own;
-    float v = 0.f;
+    double v = 0.;
     if (column < columns) {
 #pragma unroll 8
-      for (int i = part; i < n; i += 64) v += parts[i * columns + column];
+      for (int i = part; i < n; i += 64) v += (double)parts[i * columns + column];
     }
-    sums[part][own] = v;
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    if ((threadIdx.x & (kWave - 1)) < 16) sums[wave][own] = v;
     __syncthreads();
     if (part == 0 && column < columns) {
-      v = 0.f;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) v += sums[i][own];
-      static_cast<typename T::storage*>(dw)[column] = T::from_f32(v);
+      for (int i = 1; i < kWaves; ++i) v += sums[i][own];
+      static_cast<typename T::storage*>(dw)[column] = T::from_f32((float)v);
     }
     __syncthreads();
   }

@@ -7,6 +7,38 @@ from test_gpu_int8 import BF16, F32, randn
 from test_gpu_int8_calls import room
 
 pytestmark = pytest.mark.gpu
+E = ref.E
+
+
+def close(name, got, value, relative, scale=None):
+    """|got - value| <= relative * scale (|value| where there is none) + the result's rounding."""
+    err = (got.double() - value).abs()
+    bound = (value.abs() if scale is None else scale) * relative + value.abs() * ref.HALF[got.dtype] * (1 + 2 * relative) + ref.TINY[got.dtype]
+    assert bool((err <= bound).all()), f"{name}: {float((err / bound).max())} of what it may be off"
+
+
+def drifting(rows, K):
+    """[rows, K] of numbers that a float32 sum drifts away from where they are the same again and again, and of others."""
+    dy = randn(1, rows, K)
+    dy[:, :K // 2] = torch.tensor([1 / 3, 0.7, 0.1, 0.9, 0.55], device="cuda").repeat(K)[:K // 2]
+    return dy
+
+
+# ---- the weight's gradient -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,K,sums", [(512, 4096, 0), (300, 8192, 0), (512, 1000, 3), (512, 4097, 0), (512, 40001, 0)])
+def test_weight_gradient_is_rounded_once(rows, K, sums):
+    """Rows of 1 and -1, whose normalised values are these: dw is the sum of dy.  A workgroup has a row of its own (or four, three float32
+    additions); what it hands on is added up without any other rounding than the result's (float64: 512 of 2^-53)."""
+    import mflux_amd
+
+    print(f"rows={rows} K={K}", flush=True)
+    x = torch.ones(rows, K, device="cuda")
+    x[:, ::2] = -1
+    w, dy = torch.ones(K, device="cuda").requires_grad_(), drifting(rows, K)
+    dw, = torch.autograd.grad(mflux_amd.rms_norm(x, w, eps=0.0), w, dy)
+    terms = dy.double() * x.double()
+    close("dw", dw, terms.sum(0), sums * E + 2.0 ** -43, terms.abs().sum(0))
 
 
 # ---- long rows -------------------------------------------------------------------------------------------------------------------
