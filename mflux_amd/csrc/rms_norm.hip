@@ -490,7 +490,13 @@ __global__ __launch_bounds__(kThreads) void rows_values_kernel(const int8_t* cod
   }
 }
 
-constexpr int kBackwardGroups = 2;  // workgroups of a backward pass to a compute unit: rows of partial sums
+// Workgroups of a backward pass, each of them a row of partial sums: two to a compute unit, and more of them where a lane would add up more
+// than 128 rows in float32 (equal terms drift: 2048 of them some 300 roundings away, 128 of them 8 to 19)
+constexpr int kBackwardGroups = 2, kBackwardRows = 128;
+int64_t most_backward_groups(int64_t rows, int per_group) {
+  const int64_t few = kBackwardGroups * (int64_t)compute_units(), each = kBackwardRows * per_group, many = (rows + each - 1) / each;
+  return many < few ? few : many < (1 << 22) ? many : 1 << 22;  // (of up to 512 threads: fewer than 2^32)
+}
 
 // as many rows to every workgroup
 int64_t groups_of(int64_t rows, int per_group, int64_t most) {
@@ -512,7 +518,8 @@ int64_t forward_form(const RowsCall& c, hipStream_t stream) {
 template <typename T, int V, int kLanes, int kChunks>
 int64_t backward_form(const RowsCall& c, hipStream_t stream) {
   constexpr int kBlock = kLanes > kWave ? kLanes : kThreads;
-  const int64_t groups = groups_of(c.rows, kBlock / kLanes, kBackwardGroups * (int64_t)compute_units());
+  constexpr int kRows = kBlock / kLanes;
+  const int64_t groups = groups_of(c.rows, kRows, most_backward_groups(c.rows, kRows));
   const dim3 grid((unsigned)groups), block(kBlock);
   if (c.parts) hipLaunchKernelGGL((rows_backward_kernel<T, V, kLanes, kChunks, true>), grid, block, 0, stream, c);
   else hipLaunchKernelGGL((rows_backward_kernel<T, V, kLanes, kChunks, false>), grid, block, 0, stream, c);
@@ -563,7 +570,7 @@ int64_t launch_backward(const RowsCall& c, bool wide, hipStream_t stream) {
     if (units <= 1024) return backward_form<T, 1, 256, 4>(c, stream);
     if (units <= 4096) return backward_form<T, 1, 256, 16>(c, stream);
   }
-  const int64_t groups = groups_of(c.rows, 1, kBackwardGroups * (int64_t)compute_units());
+  const int64_t groups = groups_of(c.rows, 1, most_backward_groups(c.rows, 1));
   hipLaunchKernelGGL((rows_backward_any_kernel<T>), dim3((unsigned)groups), dim3(kThreads), 0, stream, c);
   return groups;
 }
@@ -582,7 +589,7 @@ int launch(const RowsCall& c, bool wide, bool backward, hipStream_t stream) {
 }  // namespace
 
 size_t rows_workspace_bytes(int64_t rows, int64_t columns) {
-  const int64_t most = kBackwardGroups * (int64_t)compute_units();
+  const int64_t most = most_backward_groups(rows, 1);  // as many as any form of a row has
   return (size_t)(rows < most ? rows : most) * (size_t)columns * 4;
 }
 

@@ -41,6 +41,24 @@ def test_weight_gradient_is_rounded_once(rows, K, sums):
     close("dw", dw, terms.sum(0), sums * E + 2.0 ** -43, terms.abs().sum(0))
 
 
+@pytest.mark.parametrize("rows,K,sums", [(1 << 22, 64, 130), (1 << 21, 500, 130), (1 << 19, 1030, 127), (1 << 17, 4100, 127), (150_000, 4097, 127),
+                                         (140_000, 2048, 127)])
+def test_weight_gradient_of_many_rows(rows, K, sums):
+    """As above: a lane adds up 128 rows at most (and a workgroup its four wavefronts') in float32."""
+    import mflux_amd
+
+    room(40)
+    print(f"rows={rows} K={K}", flush=True)
+    x = torch.ones(rows, K, device="cuda")
+    x[:, ::2] = -1
+    w, dy, n = torch.ones(K, device="cuda").requires_grad_(), drifting(500, K), -(-rows // 500)
+    dw, = torch.autograd.grad(mflux_amd.rms_norm(x, w, eps=0.0), w, dy.repeat(n, 1)[:rows])
+    terms = dy.double() * x[:500].double()
+    rest = terms[:rows - (n - 1) * 500]
+    spread = (n - 1) * terms.abs().sum(0) + rest.abs().sum(0)
+    close("dw", dw, (n - 1) * terms.sum(0) + rest.sum(0), sums * E + 2.0 ** -37, spread)
+
+
 # ---- long rows -------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("K,dtype", [((1 << 26) - 15, F32), (1 << 26, F32), (1 << 26, BF16), (1 << 28, BF16)])
