@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import int8_reference as ref
-from test_gpu_int8 import BF16, F32, randn
+from test_gpu_int8 import BF16, F16, F32, randn
 from test_gpu_int8_calls import room
 
 pytestmark = pytest.mark.gpu
@@ -60,6 +60,32 @@ def test_weight_gradient_of_many_rows(rows, K, sums):
 
 
 # ---- long rows -------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("K", [(1 << 22) + 4, (1 << 23) + 12])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_norm_of_rows_of_millions(K, dtype):
+    """Equal values, whose squares no short sum of float32 adds up without a drift; the bound does not grow with the row."""
+    import mflux_amd
+
+    print(f"K={K} {dtype}", flush=True)
+    x = torch.stack([torch.full((K,), 0.7, device="cuda"), torch.full((K,), -0.1, device="cuda"), randn(1, K)]).to(dtype).requires_grad_()
+    w = (1 + 0.1 * randn(2, K)).to(dtype).requires_grad_()
+    dy = torch.where(torch.arange(K, device="cuda") % 3 == 0, 0.9, 0.3).to(dtype).expand(3, K)
+    y = mflux_amd.rms_norm(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    v, g, d = x.detach().double(), w.detach().double(), dy.double()
+    root = 1 / (v.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    close("y", y.detach(), v * root * g, 4 * E)
+    n, a = v * root, d * g
+    mean = (a * n).mean(1, keepdim=True)
+    # the two terms of dx: each to its factors' roundings
+    close("dx", dx, root * (a - n * mean), 8 * E, root * (a.abs() + n.abs() * mean.abs()))
+    close("dw", dw, (d * n).sum(0), 8 * E, (d * n).abs().sum(0))
+    q, s = mflux_amd.rms_norm_int8(x.detach(), w.detach())
+    want_q, want_s = ref.codes(x, w, 1e-6)
+    assert torch.equal(q.double(), want_q)
+    assert bool(((s.double() - want_s).abs() <= want_s * 5 * E).all())
+
 
 @pytest.mark.parametrize("K,dtype", [((1 << 26) - 15, F32), (1 << 26, F32), (1 << 26, BF16), (1 << 28, BF16)])
 def test_weight_gradient_of_the_longest_rows(K, dtype):
