@@ -58,7 +58,7 @@ __device__ inline V over_wave(V v) {
   return join(join(lane_of(v, 0), lane_of(v, 16)), join(lane_of(v, 32), lane_of(v, 48)));
 }
 // the same over a row's lanes: a wavefront, or a workgroup's, which meet in LDS (two sets of slots in turn, so that one barrier is
-// enough)
+// enough: `turn` counts the calls)
 template <int kLanes, typename A, typename B>
 __device__ inline void over_row(A& a, B& b, int turn) {
   a = over_wave(a);
@@ -129,6 +129,26 @@ __device__ inline Unit<T, V> add(const Unit<T, V>& a, const Unit<T, V>& b) {
   return pack<T, V>(x);
 }
 
+// ---- rows whose sum of squares float32 does not hold: it overflows for values above some 10^17, and squares below its normal numbers count
+// for values below 10^-19 with as small an eps.  The values of such a row are multiplied by a power of two, in the registers that hold
+// them, and its sums are taken again.  A branch for all of the row's lanes, and nothing else in the way of other rows.
+template <typename T>
+constexpr bool kFarValues = !std::is_same_v<T, F16>;  // float16 has no such values
+// of a sum that all of the row's lanes have, and its mean with eps
+__device__ inline bool far_row(float squares, float size) {
+  return __builtin_amdgcn_readfirstlane((int)!(squares <= 0x1.fffffep127f && size >= 0x1p-120f));
+}
+// the power of two: 2^15 values below 2^128, or values down to 2^-149, whose squares float32 then adds up
+__device__ inline float lift_of(float squares) { return squares <= 0x1.fffffep127f ? 0x1p100f : 0x1p-73f; }
+template <typename T, int V>
+__device__ inline Unit<T, V> lifted(const Unit<T, V>& raw, float lift) {
+  float v[V];
+  unpack<T, V>(raw, v);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] *= lift;
+  return pack<T, V>(v);
+}
+
 // ---- codes.  The product p of a value and its weight: exact in float32 for the 16-bit types, in float64 for float32.
 template <typename T, bool kWeighted>
 using Product = std::conditional_t<kWeighted && sizeof(typename T::storage) == 4, double, float>;
@@ -156,6 +176,7 @@ struct Coder {
   }
   // the scale of p's row, p being what it is times `factor`
   __device__ inline float scale(float factor) const { return finite ? (float)(top * (P)factor / (P)127) : __builtin_nanf(""); }
+  __device__ inline float scale(double factor) const { return finite ? (float)((double)top * factor / 127.0) : __builtin_nanf(""); }
   // The codes of N products, in the low bytes, the first lowest.  Adding 1.5 2^23 rounds a quotient to a whole number, ties to even,
   // and leaves it in the sum's low bits; what the sum lost is how far the quotient is from it.  p * inverse is off by at most
   // 127 * 4 * 2^-24 < 2^-14 (the inverse, the product, and for float32 the rounding of p and max|p|).
@@ -179,7 +200,7 @@ struct Coder {
   }
 };
 
-enum Result { kNormalised, kCodes, kWeightedCodes };
+enum Result { kNormalised, kCodes, kNormalisedCodes, kWeightedCodes };  // kCodes: of the values as they are, without a norm
 
 // kLanes lanes to a row, each kChunks of its units of V elements; up to 256 threads, workgroups of several rows.  4352 x 3840
 // bfloat16 with a residual 25 us (5.3 TB/s), with codes 24; 10240 x 3840 into codes without a norm 29; a few rows 4, a launch and
@@ -188,7 +209,7 @@ template <typename T, int V, int kLanes, int kChunks, int kResult>
 __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kernel(RowsCall c) {
   using E = typename T::storage;
   using U = Unit<T, V>;
-  constexpr bool kCoded = kResult != kNormalised;
+  constexpr bool kCoded = kResult != kNormalised, kNorm = kResult != kCodes;
   using P = Product<T, kResult == kWeightedCodes>;
   constexpr int kRows = kLanes > kWave ? 1 : kThreads / kWave;
   const int lane = threadIdx.x % kLanes, units = (int)(c.columns / V);
@@ -198,7 +219,7 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kerne
   for (int u = 0; u < kChunks; ++u)
     if (weighted && lane + u * kLanes < units) w[u] = static_cast<const U*>(c.weight)[lane + u * kLanes];
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows, ++turn) {
+  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows) {
     const U* x = reinterpret_cast<const U*>(static_cast<const E*>(c.x) + row * c.x_stride);
     const U* residual = reinterpret_cast<const U*>(static_cast<const E*>(c.residual) + row * c.residual_stride);
     U s[kChunks], r[kChunks];
@@ -232,7 +253,7 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kerne
       float v[V];
       unpack<T, V>(s[u], v);
 #pragma unroll
-      for (int i = 0; i < V; ++i) squares = __builtin_fmaf(v[i], v[i], squares);
+      for (int i = 0; kNorm && i < V; ++i) squares = __builtin_fmaf(v[i], v[i], squares);
       if constexpr (kCoded) {
         P p[V];
         products(u, p);
@@ -240,9 +261,29 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kerne
         for (int i = 0; i < V; ++i) largest = join(largest, magnitude(p[i]));
       }
     }
-    over_row<kLanes>(squares, largest, turn);
-    const float rstd = c.norm ? 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps) : 1.0f;
+    over_row<kLanes>(squares, largest, turn++);
+    const float size = squares / (float)c.columns + c.eps;
+    float rstd = kNorm ? 1.0f / __builtin_sqrtf(size) : 1.0f;
     const Coder<P> coder(largest);
+    float scale = kCoded ? coder.scale(rstd) : 0.f;
+    if (kFarValues<T> && kNorm && far_row(squares, size)) {
+      const float lift = lift_of(squares);
+      squares = 0.f;
+      Bits<P> none = 0;
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u) {
+        if (lane + u * kLanes >= units) continue;
+        const U t = lifted<T, V>(s[u], lift);
+        float v[V];
+        unpack<T, V>(t, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) squares = __builtin_fmaf(v[i], v[i], squares);
+        if constexpr (!kCoded) s[u] = t;
+      }
+      over_row<kLanes>(squares, none, turn++);
+      rstd = 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps * lift * lift);
+      if constexpr (kCoded) scale = coder.scale((double)rstd * (double)lift);
+    }
 #pragma unroll
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
@@ -274,19 +315,16 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_kerne
         reinterpret_cast<U*>(static_cast<E*>(c.y) + row * c.columns)[lane + u * kLanes] = pack<T, V>(v);
       }
     }
-    if (kCoded && lane == 0) c.scales[row] = coder.scale(rstd);
+    if (kCoded && lane == 0) c.scales[row] = scale;
   }
 }
 
 // Rows that no registers hold: a workgroup to a row, element by element, which is read again (from a cache, where it fits one) for
-// the results.  A thread's sum has up to 2^20 terms: 32 at a time in float32 (equal values of a row of 2^22 would drift 10^-4 away in one
-// float32 sum), these in float64.
-constexpr int kAtATime = 32;
-
+// the results.  A thread's sum has up to 2^20 terms and is float64 (equal values of a row of 2^22 would drift 10^-4 away in float32).
 template <typename T, int kResult>
 __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
   using E = typename T::storage;
-  constexpr bool kCoded = kResult != kNormalised;
+  constexpr bool kCoded = kResult != kNormalised, kNorm = kResult != kCodes;
   using P = Product<T, kResult == kWeightedCodes>;
   const E* weight = static_cast<const E*>(c.weight);
   const double share = 1.0 / (double)c.columns;
@@ -303,19 +341,17 @@ __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
     };
     double squares = 0.;
     Bits<P> largest = 0;
-    for (int64_t from = threadIdx.x; from < c.columns; from += kAtATime * kThreads) {
-      const int64_t to = min(from + kAtATime * kThreads, c.columns);
-      float some = 0.f;
-      for (int64_t k = from; k < to; k += kThreads) {
-        const float s = value(k);
-        if (c.residual) static_cast<E*>(c.sum)[row * c.columns + k] = T::from_f32(s);
-        some = __builtin_fmaf(s, s, some);
-        if constexpr (kCoded) largest = join(largest, magnitude(product(s, k)));
-      }
-      squares += (double)some;
+    for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
+      const float s = value(k);
+      if (c.residual) static_cast<E*>(c.sum)[row * c.columns + k] = T::from_f32(s);
+      if (kNorm) squares = __builtin_fma((double)s, (double)s, squares);
+      if constexpr (kCoded) largest = join(largest, magnitude(product(s, k)));
     }
     over_row<kThreads>(squares, largest, turn);
-    const float rstd = c.norm ? (float)(1.0 / __builtin_sqrt(squares * share + (double)c.eps)) : 1.0f;
+    const double root = kNorm ? 1.0 / __builtin_sqrt(squares * share + (double)c.eps) : 1.0;
+    // the root as two factors where float32 may not hold it, in the order whose first product stays inside
+    const float lift = !kFarValues<T> ? 1.f : root < 0x1p-60 ? 0x1p-84f : root > 0x1p60 ? 0x1p100f : 1.f, rstd = (float)(root / (double)lift);
+    const float first = lift > 1.f ? lift : rstd, second = lift > 1.f ? rstd : lift;
     const Coder<P> coder(largest);
     for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
       float s = value(k);
@@ -323,12 +359,12 @@ __global__ __launch_bounds__(kThreads) void rows_any_kernel(RowsCall c) {
         const P p[1] = {product(s, k)};
         c.codes[row * c.code_stride + k] = (int8_t)coder.codes(p);
       } else {
-        s *= rstd;
+        s = s * first * second;
         if (weight) s *= T::to_f32(weight[k]);
         static_cast<E*>(c.y)[row * c.columns + k] = T::from_f32(s);
       }
     }
-    if (kCoded && threadIdx.x == 0) c.scales[row] = coder.scale(rstd);
+    if (kCoded && threadIdx.x == 0) c.scales[row] = kNorm ? coder.scale(root) : coder.scale(1.f);
   }
 }
 
@@ -351,7 +387,7 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backw
     }
   }
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows, ++turn) {
+  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < c.rows; row += (int64_t)gridDim.x * kRows) {
     const U* x = reinterpret_cast<const U*>(static_cast<const E*>(c.x) + row * c.x_stride);
     const U* dy = reinterpret_cast<const U*>(static_cast<const E*>(c.dy) + row * c.dy_stride);
     const U* dsum = reinterpret_cast<const U*>(static_cast<const E*>(c.dsum) + row * c.dsum_stride);
@@ -377,8 +413,31 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backw
         dot = __builtin_fmaf(c.weight ? a[i] * b[i] : a[i], v[i], dot);
       }
     }
-    over_row<kLanes>(squares, dot, turn);
-    const float rstd = 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps), mean = rstd * dot / (float)c.columns;
+    over_row<kLanes>(squares, dot, turn++);
+    const float size = squares / (float)c.columns + c.eps;
+    float rstd = 1.0f / __builtin_sqrtf(size), slope = rstd;  // r of what is in registers, and r
+    if (kFarValues<T> && far_row(squares, size)) {
+      const float lift = lift_of(squares);
+      squares = dot = 0.f;
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u) {
+        if (lane + u * kLanes >= units) continue;
+        s[u] = lifted<T, V>(s[u], lift);
+        float v[V], a[V], b[V];
+        unpack<T, V>(s[u], v);
+        unpack<T, V>(g[u], a);
+        if (c.weight) unpack<T, V>(w[u], b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          squares = __builtin_fmaf(v[i], v[i], squares);
+          dot = __builtin_fmaf(c.weight ? a[i] * b[i] : a[i], v[i], dot);
+        }
+      }
+      over_row<kLanes>(squares, dot, turn++);
+      rstd = 1.0f / __builtin_sqrtf(squares / (float)c.columns + c.eps * lift * lift);
+      slope = rstd * lift;
+    }
+    const float mean = rstd * dot / (float)c.columns;
 #pragma unroll
     for (int u = 0; u < kChunks; ++u) {
       if (lane + u * kLanes >= units) continue;
@@ -390,7 +449,7 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backw
       for (int i = 0; i < V; ++i) {
         const float n = v[i] * rstd;
         if constexpr (kWeight) dw[u][i] = __builtin_fmaf(a[i], n, dw[u][i]);
-        a[i] = rstd * __builtin_fmaf(-mean, n, c.weight ? a[i] * b[i] : a[i]);
+        a[i] = slope * __builtin_fmaf(-mean, n, c.weight ? a[i] * b[i] : a[i]);
       }
       if (!c.dx) continue;
       if (c.dsum) {
@@ -425,6 +484,8 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backw
   }
 }
 
+constexpr int kAtATime = 32;
+
 // rows that no registers hold; a workgroup adds its rows' shares of the weight's gradient up in its own row of `parts`
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c) {
@@ -433,7 +494,8 @@ __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c)
   float* parts = c.parts ? c.parts + (int64_t)blockIdx.x * c.columns : nullptr;
   const double share = 1.0 / (double)c.columns;
   int turn = 0;
-  for (int64_t row = blockIdx.x; row < c.rows; row += gridDim.x, ++turn) {
+  bool added = false;
+  for (int64_t row = blockIdx.x; row < c.rows; row += gridDim.x) {
     const E* x = static_cast<const E*>(c.x) + row * c.x_stride;
     const E* dy = static_cast<const E*>(c.dy) + row * c.dy_stride;
     const E* dsum = static_cast<const E*>(c.dsum) + row * c.dsum_stride;
@@ -449,17 +511,32 @@ __global__ __launch_bounds__(kThreads) void rows_backward_any_kernel(RowsCall c)
       squares += (double)some;
       dot += (double)some_dot;
     }
-    over_row<kThreads>(squares, dot, turn);
-    const double root = 1.0 / __builtin_sqrt(squares * share + (double)c.eps);
-    const float rstd = (float)root, mean = (float)(root * dot * share);
+    over_row<kThreads>(squares, dot, turn++);
+    double size = squares * share + (double)c.eps;
+    float lift = 1.f;
+    if (kFarValues<T> && far_row((float)squares, (float)size)) {
+      lift = lift_of((float)squares);
+      squares = dot = 0.;
+#pragma unroll 1
+      for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
+        const double s = T::to_f32(x[k]) * lift, a = T::to_f32(dy[k]);
+        squares = __builtin_fma(s, s, squares);
+        dot = __builtin_fma(weight ? a * (double)T::to_f32(weight[k]) : a, s, dot);
+      }
+      over_row<kThreads>(squares, dot, turn++);
+      size = squares * share + (double)c.eps * (double)lift * (double)lift;
+    }
+    const double root = 1.0 / __builtin_sqrt(size);
+    const float rstd = (float)root, mean = (float)(root * dot * share), slope = rstd * lift;
     for (int64_t k = threadIdx.x; k < c.columns; k += kThreads) {
-      const float n = T::to_f32(x[k]) * rstd, a = T::to_f32(dy[k]);
-      if (parts) parts[k] = turn ? __builtin_fmaf(a, n, parts[k]) : a * n;
+      const float n = T::to_f32(x[k]) * lift * rstd, a = T::to_f32(dy[k]);
+      if (parts) parts[k] = added ? __builtin_fmaf(a, n, parts[k]) : a * n;
       if (!c.dx) continue;
-      float d = rstd * __builtin_fmaf(-mean, n, weight ? a * T::to_f32(weight[k]) : a);
+      float d = slope * __builtin_fmaf(-mean, n, weight ? a * T::to_f32(weight[k]) : a);
       if (c.dsum) d += T::to_f32(dsum[k]);
       static_cast<E*>(c.dx)[row * c.columns + k] = T::from_f32(d);
     }
+    added = true;
   }
 }
 
@@ -538,8 +615,9 @@ int64_t forward_form(const RowsCall& c, hipStream_t stream) {
   const int64_t groups = groups_of(c.rows, kBlock / kLanes, 2048 / kBlock * (int64_t)compute_units());
   const dim3 grid((unsigned)groups), block(kBlock);
   if (!c.codes) hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kNormalised>), grid, block, 0, stream, c);
+  else if (!c.norm) hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kCodes>), grid, block, 0, stream, c);
   else if (c.weight) hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kWeightedCodes>), grid, block, 0, stream, c);
-  else hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kCodes>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((rows_kernel<T, V, kLanes, kChunks, kNormalisedCodes>), grid, block, 0, stream, c);
   return groups;
 }
 
@@ -577,8 +655,9 @@ int64_t launch_forward(const RowsCall& c, bool wide, hipStream_t stream) {
   const int64_t groups = groups_of(c.rows, 1, 8 * (int64_t)compute_units());
   const dim3 grid((unsigned)groups), block(kThreads);
   if (!c.codes) hipLaunchKernelGGL((rows_any_kernel<T, kNormalised>), grid, block, 0, stream, c);
+  else if (!c.norm) hipLaunchKernelGGL((rows_any_kernel<T, kCodes>), grid, block, 0, stream, c);
   else if (c.weight) hipLaunchKernelGGL((rows_any_kernel<T, kWeightedCodes>), grid, block, 0, stream, c);
-  else hipLaunchKernelGGL((rows_any_kernel<T, kCodes>), grid, block, 0, stream, c);
+  else hipLaunchKernelGGL((rows_any_kernel<T, kNormalisedCodes>), grid, block, 0, stream, c);
   return groups;
 }
 

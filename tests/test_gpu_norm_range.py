@@ -105,6 +105,84 @@ def test_weight_gradient_of_the_longest_rows(K, dtype):
     assert torch.equal(dw, sign * dy)
 
 
+# ---- values whose squares leave float32 --------------------------------------------------------------------------------------
+
+SIZES = [1e18, 3e25, 1e38]
+
+
+@pytest.mark.parametrize("K", [1, 64, 67, 1024, 1100, 3840, 5000, 16384, 16400, 40001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_of_large_values(K, dtype):
+    """Finite rows whose sum of squares is beyond float32's range: normalised like any others, among others."""
+    import mflux_amd
+
+    print(f"K={K} {dtype}", flush=True)
+    unit = randn(1, 6, K).clamp(-3, 3)
+    size = torch.tensor([1.0, *SIZES, 1e-3, 1e19], device="cuda")[:, None]
+    x = (unit * size).to(dtype)
+    x[3, K // 2] = torch.finfo(dtype).max
+    x[4, 0] = 1e30  # alone in a row of small ones
+    x, r = x.requires_grad_(), (randn(2, 6, K).clamp(-3, 3) * size * 0.01).to(dtype)
+    r[3] = 0
+    w = (1 + 0.1 * randn(3, K)).to(dtype).requires_grad_()
+    dy, ds = randn(4, 6, K, dtype=dtype), randn(5, 6, K, dtype=dtype) * 1e-20
+    for residual, dsum in ((None, None), (r, ds)):
+        s = ref.total(x.detach(), residual)
+        assert bool(s.isfinite().all())
+        out = mflux_amd.rms_norm(x, w, residual=residual)
+        y = out if residual is None else out[0]
+        want = ref.rms_norm(s, w, 1e-6, dy, dsum)
+        ref.check("y", y, *want["y"])
+        dx, dw = torch.autograd.grad(out, (x, w), dy if residual is None else (dy, dsum))
+        ref.check("dx", dx, *want["dx"])
+        ref.check("dw", dw, *want["dw"])
+        q, sc, *_ = mflux_amd.rms_norm_int8(x.detach(), None, residual=residual)
+        want_q, want_s = ref.codes(s, None, 1e-6)
+        assert torch.equal(q.double(), want_q)
+        ref.check("scales", sc, want_s, want_s * ref.scale_bound(K, True))
+
+
+@pytest.mark.parametrize("K", [1, 64, 67, 1100, 3840, 16384, 40001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("eps", [0.0, 1e-42])
+def test_norm_of_tiny_values(K, dtype, eps):
+    """Rows whose squares vanish in float32, with an eps that leaves them their size."""
+    import mflux_amd
+
+    print(f"K={K} {dtype} {eps}", flush=True)
+    unit = randn(1, 4, K)
+    unit[:, 0] = 1
+    x = (unit * torch.tensor([1.0, 1e-18, 1e-21, 1e-30], device="cuda")[:, None]).to(dtype).requires_grad_()
+    w = (1 + 0.1 * randn(2, K)).to(dtype).requires_grad_()
+    dy = randn(3, 4, K, dtype=dtype) * 1e-6
+    y = mflux_amd.rms_norm(x, w, eps=eps)
+    held = torch.tensor(eps, dtype=F32).double().item()  # as the call holds it
+    want = ref.rms_norm(x, w, held, dy)
+    ref.check("y", y, *want["y"])
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    ref.check("dx", dx, *want["dx"])
+    ref.check("dw", dw, *want["dw"])
+    q, sc = mflux_amd.rms_norm_int8(x.detach(), None, eps=eps)
+    want_q, want_s = ref.codes(x, None, held)
+    assert torch.equal(q.double(), want_q)
+    ref.check("scales", sc, want_s, want_s * ref.scale_bound(K, True) + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("K", [64, 67, 3840, 40001])
+def test_norm_of_the_largest_values_bfloat16_has(K):
+    """Rows of nothing but the largest number and its negative: a norm of one."""
+    import mflux_amd
+
+    top = torch.finfo(BF16).max
+    x = torch.where(randn(1, 3, K) > 0, top, -top).to(BF16)
+    y = mflux_amd.rms_norm(x)
+    ref.check("y", y, *ref.rms_norm(x, None, 1e-6)["y"])
+    assert bool((y.abs() == 1).all())
+    q, s = mflux_amd.rms_norm_int8(x)
+    assert bool((q.abs() == 127).all())
+    close("values", mflux_amd.int8_dequantize(q, s, F32), x.double().sign(), (ref.scale_bound(K, True) / E + 2) * E)
+
+
 # ---- what the sum's gradient is --------------------------------------------------------------------------------------------------
 
 def test_the_sum_wants_no_gradient_of_a_weight():
