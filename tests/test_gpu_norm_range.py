@@ -1,4 +1,8 @@
-"""rms_norm and the codes behind it at the ends of what they take, and what its results' gradients are."""
+"""rms_norm and the codes behind it at the ends of what they take: rows of millions of values, millions of rows, values whose squares
+leave float32, more rows than workgroups in every form of a row, and what its results' gradients are.
+
+Bounds, with E = 2^-24: where a row's sum is right to E or better, a norm is off by the root's rounding, two products and the result's
+(int8_reference has those of the shorter rows, which grow with a row's length)."""
 import pytest
 import torch
 
@@ -181,6 +185,31 @@ def test_norm_of_the_largest_values_bfloat16_has(K):
     q, s = mflux_amd.rms_norm_int8(x)
     assert bool((q.abs() == 127).all())
     close("values", mflux_amd.int8_dequantize(q, s, F32), x.double().sign(), (ref.scale_bound(K, True) / E + 2) * E)
+
+
+# ---- more rows than workgroups -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("K", [1, 17, 513, 1025, 4099, 16392, 33001])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_norm_of_more_rows_than_workgroups(K, dtype):
+    """A workgroup's second row and those after it, in the forms of odd, of long and of short rows."""
+    import mflux_amd
+
+    rows = 2100 if K > 4096 else 20000 if K < 600 else 9000
+    print(f"rows={rows} K={K} {dtype}", flush=True)
+    x, r, w = randn(1, rows, K, dtype=dtype).requires_grad_(), randn(2, rows, K, dtype=dtype), randn(3, K, dtype=dtype).requires_grad_()
+    dy, ds = randn(4, rows, K, dtype=dtype), randn(5, rows, K, dtype=dtype)
+    y, s = mflux_amd.rms_norm(x, w, residual=r)
+    want = ref.rms_norm(ref.total(x.detach(), r), w, 1e-6, dy, ds)
+    ref.check("y", y, *want["y"])
+    dx, dw = torch.autograd.grad((y, s), (x, w), (dy, ds))
+    ref.check("dx", dx, *want["dx"])
+    ref.check("dw", dw, *want["dw"])
+    del want, dx, dw, y
+    q, sc, _ = mflux_amd.rms_norm_int8(x.detach(), w.detach(), residual=r)
+    want_q, want_s = ref.codes(s.detach(), w, 1e-6)
+    assert torch.equal(q.double(), want_q)
+    ref.check("scales", sc, want_s, want_s * ref.scale_bound(K, True))
 
 
 # ---- what the sum's gradient is --------------------------------------------------------------------------------------------------
