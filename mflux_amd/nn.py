@@ -405,11 +405,25 @@ class RMSNorm(torch.nn.Module):
         return int8.rms_norm_int8(x, self.weight.detach(), residual=residual, eps=self.eps)
 
 
+def _rows_of_16(codes: torch.Tensor) -> torch.Tensor:
+    """Codes ``[N, K]`` in rows of whole 16 bytes, which ``int8_matmul`` reads where they are: as ``int8_quantize``
+    lays them out, and as a copy, a move or a load of a row's ``K`` alone does not."""
+    if codes.dtype != torch.int8 or codes.ndim != 2 or codes.shape[1] % 16 == 0:
+        return codes
+    (N, K), stride = codes.shape, codes.stride(0)
+    length = (K + 15) // 16 * 16
+    if codes.stride(1) == 1 and stride % 16 == 0 and codes.storage_offset() % 16 == 0 \
+            and codes.storage_offset() + (N - 1) * stride + length <= codes.untyped_storage().nbytes():
+        return codes
+    rows = torch.zeros((N, length), dtype=torch.int8, device=codes.device)[:, :K]
+    return rows.copy_(codes)
+
+
 class Int8Linear(torch.nn.Module):
     """``y = x W^T (+ bias)`` with 8-bit integers on both sides: a scale for each row of the weight (an
     output feature) and for each row of ``x`` (a token), the latter taken in the call.
 
-    ``weight`` int8 ``[N, K]``, ``scales`` float32 ``[N]``, optional ``bias`` ``[N]``: frozen buffers.  ``x`` is a float
+    ``weight`` int8 ``[N, K]`` in rows of whole 16 bytes, ``scales`` float32 ``[N]``, optional ``bias`` ``[N]``: frozen buffers.  ``x`` is a float
     tensor ``[..., K]``, whose type the result has, or the ``(codes, scales)`` of ``RMSNorm.int8`` or
     ``mflux_amd.int8_quantize``, taken once for several layers; the result then has the type
     that the layer was made from.  Beside :class:`QuantizedLinear`, which keeps the activations
@@ -424,7 +438,7 @@ class Int8Linear(torch.nn.Module):
             bound = math.sqrt(1.0 / input_dims)
             w, scales = int8.int8_quantize(torch.empty((output_dims, input_dims), device=device, dtype=torch.float32).uniform_(-bound, bound))
         else:  # placeholders of the right shape, to be filled by load_state_dict
-            w = torch.zeros((output_dims, input_dims), dtype=torch.int8, device=device)
+            w = _rows_of_16(torch.zeros((output_dims, input_dims), dtype=torch.int8, device=device))
             scales = torch.zeros((output_dims,), dtype=torch.float32, device=device)
         self.register_buffer("weight", w)
         self.register_buffer("scales", scales)
@@ -452,7 +466,12 @@ class Int8Linear(torch.nn.Module):
             self.dtype = probe.dtype
         if self.scales.dtype != torch.float32:
             self._buffers["scales"] = scales.to(self.scales.device)
+        self._buffers["weight"] = _rows_of_16(self.weight)
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._buffers["weight"] = _rows_of_16(self.weight)
 
     def forward(self, x) -> torch.Tensor:
         if isinstance(x, tuple):

@@ -43,3 +43,32 @@ def test_adapters_are_baked_into_codes(K, N):
     terms = x.double().abs() @ (full.abs() + sum(abs(l.scale) * l.lora_A.detach().abs().float() @ l.lora_B.detach().abs().float() for l in loras).t()).double().t()
     bound = bound + x.double().abs().amax(1, keepdim=True) / 254 * (deltas.abs().sum(1).double() + step.double() * K) + terms * 8 * ref.HALF[BF16] + 8 * ref.HALF[BF16] * linear.bias.detach().double().abs()
     assert bool(((after.double() - before.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("how", ["move", "load", "assign", "copy"])
+def test_a_moved_layer_multiplies_its_weight_where_it_is(how):
+    """An input length that is no multiple of 16: a call allocates its x, its result and scratch, no second weight."""
+    import copy
+
+    from mflux_amd import nn
+
+    K, N = 1001, 20000
+    torch.manual_seed(1)
+    layer = nn.Linear(K, N, bias=False, device="cuda", dtype=BF16).to_int8()
+    x = randn(1, 2, K, dtype=BF16)
+    want = layer(x)
+    other = nn.Int8Linear(K, N, bias=False)
+    state = {k: v.contiguous() for k, v in layer.state_dict().items()}
+    if how == "move":
+        other = layer.cpu().cuda()
+    elif how == "copy":
+        other = copy.deepcopy(layer)
+    else:
+        other.load_state_dict(state, assign=how == "assign")
+        other = other.cuda()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = other(x)
+    assert torch.cuda.max_memory_allocated() - before < N * K // 8
+    assert torch.equal(y, want)

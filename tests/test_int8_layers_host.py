@@ -59,3 +59,40 @@ def test_an_int8_layer_without_adapters_is_stripped():
     weight = lin.weight.detach().clone()
     assert bake_and_strip_lora(FusedLoRALinear(lin, [carrier])) is lin
     assert torch.equal(lin.weight, weight + 0.5) and torch.equal(base.weight, before)
+
+
+def padded(weight):
+    """Rows of whole 16 bytes, to the last one's end."""
+    N, K = weight.shape
+    length = -(-K // 16) * 16
+    return weight.stride(1) == 1 and weight.stride(0) % 16 == 0 and \
+        weight.storage_offset() + (N - 1) * weight.stride(0) + length <= weight.untyped_storage().nbytes()
+
+
+@pytest.mark.parametrize("K,N", [(77, 5), (1, 3), (100, 1), (64, 6)])
+def test_a_weight_keeps_rows_of_whole_16_bytes(K, N):
+    """However the layer came about: int8_matmul copies a weight that lies otherwise in every call."""
+    import copy
+    import io
+
+    base = layer(K, N)
+    assert padded(base.weight) and base.weight.shape == (N, K) and not base.weight.requires_grad
+    codes = base.weight.clone().contiguous()
+    state = {k: v.contiguous() for k, v in base.state_dict().items()}
+    loaded, assigned = nn.Int8Linear(K, N, bias=False), nn.Int8Linear(K, N, bias=False)
+    loaded.load_state_dict(state)
+    assigned.load_state_dict(state, assign=True)
+    file = io.BytesIO()
+    torch.save(base, file)
+    file.seek(0)
+    meta = nn.Int8Linear(K, N, bias=False, device="meta").to_empty(device="cpu")
+    meta.load_state_dict(state)
+    for other in (loaded, assigned, copy.deepcopy(base), torch.load(file, weights_only=False), base.half(), base.to(torch.float32), meta,
+                  copy.deepcopy(loaded).to(torch.bfloat16)):
+        assert padded(other.weight) and other.weight.dtype == torch.int8 and torch.equal(other.weight, codes)
+        assert torch.equal(other.scales, state["scales"])
+    from mflux_amd.weights import update_module
+
+    fresh = nn.Int8Linear(K, N, bias=False)
+    update_module(fresh, state)
+    assert padded(fresh.weight) and torch.equal(fresh.weight, codes)
