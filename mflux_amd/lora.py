@@ -319,7 +319,8 @@ def _wrapped(obj: torch.nn.Module):
     return (obj.linear, [obj]) if isinstance(obj, LoRALinear) else None
 
 
-def _check_bases(module: torch.nn.Module, path: str = "") -> None:
+def check_bases(module: torch.nn.Module, path: str = "") -> None:
+    """Refuses a tree with adapters on an ``Int8Linear``, as ``bake_and_strip_lora`` without ``requantize`` does."""
     wrapped = _wrapped(module)
     if wrapped:
         module, loras = wrapped
@@ -327,7 +328,7 @@ def _check_bases(module: torch.nn.Module, path: str = "") -> None:
             raise ValueError(f"[bake_and_strip_lora] '{path}' has adapters on an Int8Linear, whose codes cannot take them as they are: "
                              "pass requantize=True, or take the adapters off")
     for name, child in module.named_children():
-        _check_bases(child, f"{path}.{name}" if path else name)
+        check_bases(child, f"{path}.{name}" if path else name)
 
 
 def bake_and_strip_lora(module: torch.nn.Module, requantize: bool = False) -> torch.nn.Module:
@@ -345,7 +346,7 @@ def bake_and_strip_lora(module: torch.nn.Module, requantize: bool = False) -> to
     with adapters on one is refused before anything is baked.  Returns
     ``module`` (the base layer when ``module`` itself is a wrapper)."""
     if not requantize:
-        _check_bases(module)
+        check_bases(module)
     return _bake_and_strip(module, requantize)
 
 

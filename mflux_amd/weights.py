@@ -310,11 +310,16 @@ def save_model(model: Any, bits: int | None, base_path: str | Path, weight_defin
     ``ModelSaver.save_model`` does
     (src/mflux/models/common/weights/saving/model_saver.py:38-41), LoRA wrappers
     are baked into their base layers and stripped first (in place: the model
-    keeps the baked layers), so that the saved keys are the base model's."""
-    from .lora import bake_and_strip_lora
+    keeps the baked layers), so that the saved keys are the base model's.
+    Adapters on an ``Int8Linear`` are refused (``bake_and_strip_lora`` with
+    ``requantize=True`` bakes them)."""
+    from .lora import bake_and_strip_lora, check_bases
 
-    for c in weight_definition.get_components():
-        attr = c.model_attr or c.name
+    components = [(c, c.model_attr or c.name) for c in weight_definition.get_components()]
+    for _, attr in components:  # refused before any component is baked or written
+        if getattr(model, attr, None) is not None:
+            check_bases(getattr(model, attr), attr)
+    for c, attr in components:
         component = getattr(model, attr, None)
         if component is not None:
             stripped = bake_and_strip_lora(component)

@@ -96,3 +96,23 @@ def test_a_weight_keeps_rows_of_whole_16_bytes(K, N):
     fresh = nn.Int8Linear(K, N, bias=False)
     update_module(fresh, state)
     assert padded(fresh.weight) and torch.equal(fresh.weight, codes)
+
+
+def test_a_model_with_adapters_on_codes_is_not_saved_in_part(tmp_path):
+    """The refusal comes before the first component is baked or written."""
+    from mflux_amd import weights as W
+
+    class Definition:
+        @staticmethod
+        def get_components():
+            return [W.ComponentDefinition("first", "first"), W.ComponentDefinition("second", "second")]
+
+    class Model:
+        pass
+
+    model, base = Model(), layer()
+    model.first, model.second = Block(torch.nn.Identity()), Block(FusedLoRALinear(base, [adapter(base)]))
+    before = model.first.first.linear.weight.detach().clone()
+    with pytest.raises(ValueError, match="second.inner.0"):
+        W.save_model(model, None, tmp_path, Definition)
+    assert isinstance(model.first.first, LoRALinear) and torch.equal(model.first.first.linear.weight, before) and not list(tmp_path.iterdir())
