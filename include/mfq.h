@@ -606,8 +606,10 @@ int mfq_attention_backward(const mfq_attention_args* args, void* workspace, size
  * or the normalised row in 8 bits (mfq_int8_quantize): codes and scales instead of y, codes by code_stride.
  * Backward: x is what was normalised (the forward pass's sum), dsum its own gradient (NULL: none), which is added to
  * dx (NULL: not wanted; the gradient of x and of residual); dweight [columns], NULL: not wanted.
- * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16 of all of them; sums in float32, each result rounded once.  Any alignment of elements;
- * 16-byte aligned pointers and rows of whole 16 bytes load wider.  No array may overlap another that is written.
+ * dtype: MFQ_F32, MFQ_F16 or MFQ_BF16 of all of them; arithmetic in float32, each result rounded once.  A row's sums are float32
+ * where registers hold the row and float64 where they do not, dweight's float32 for up to 128 rows and float64 beyond them.  Rows whose
+ * squares leave float32's range are normalised like any others; products dy * weight * x have to stay inside it.
+ * Any alignment of elements; 16-byte aligned pointers and rows of whole 16 bytes load wider.  No array may overlap another that is written.
  * workspace: mfq_rms_norm_workspace_bytes() of it, 16-byte aligned, for the backward pass with dweight.
  */
 typedef struct mfq_rms_norm_args {

@@ -61,9 +61,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     ``x``: ``[..., K]`` of float32, float16 or bfloat16, any strides (a last axis that is not
     dense, or rows without one stride, are copied); ``weight`` ``[K]`` and ``residual`` of its type.  The sum is
     rounded to the type, and what is normalised is the rounded sum; everything else is
-    float32 and rounded once.  Results are densely packed.
+    float32 and rounded once, of any finite row (also one whose squares float32 does not hold).  Results are densely packed.
 
-    Gradients for ``x``, ``residual`` (the same one) and ``weight``, through both results."""
+    Gradients for ``x``, ``residual`` (the same one) and ``weight``, through both results (the sum has none where
+    the weight alone wants one)."""
     y = _lib.native().rms_norm(x, weight, residual, eps)
     if y is not None:
         return y
@@ -76,8 +77,10 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor | None = None, *, residu
     """``int8_quantize(rms_norm(x, weight, residual=residual))`` without the 16-bit rounding in between:
     ``(codes, scales)``, with ``residual`` ``(codes, scales, sum)``.
 
-    A code is ``rint(127 p / max|p|)`` of the row's products ``p = sum * weight``, ties to even, decided by
-    the exact quotient (the root is a factor of the scale alone).  Products of 16-bit types are taken in
+    A code is ``rint(127 p / max|p|)`` of the row's products ``p = sum * weight``, ties to even (the root is a
+    factor of the scale alone).  It is decided by the exact quotient for 16-bit types whose products float32 holds as
+    normal numbers, and for float32 without a weight; float32 products and their quotient are float64, which may
+    decide otherwise within 2^-45 of a border.  Products of 16-bit types are taken in
     float32: one beyond its range makes the row's scale NaN, as an infinity or NaN in the row does.
     No gradients."""
     rows = _lib.native().int8_rows(x, weight, residual, eps, True)

@@ -386,7 +386,8 @@ class RMSNorm(torch.nn.Module):
     blocks (src/mflux/models/z_image/model/z_image_transformer/transformer_block.py), with
     the residual's addition in the same pass (``mflux_amd.rms_norm``): ``norm(x)``, or
     ``y, h = norm(x, residual=h)`` for ``h = h + x; y = norm(h)``.  ``int8`` gives the normalised
-    rows as codes and scales for an :class:`Int8Linear`."""
+    rows as codes and scales for an :class:`Int8Linear`.  ``x`` is of the weight's type (MLX's promotes
+    the two): ``norm.to(x.dtype)`` or ``x.to(norm.weight.dtype)`` where they differ."""
 
     def __init__(self, dims: int, eps: float = 1e-5, *, device=None, dtype: torch.dtype = torch.bfloat16):
         super().__init__()
