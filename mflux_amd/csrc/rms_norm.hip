@@ -7,8 +7,8 @@
 // 16, by its length; the weight stays in registers from row to row.
 // A code does not depend on r, so it is decided by the products p alone, and exactly: where the float32 quotient is next to a
 // border between two codes it is taken again in float64, which tells 16-bit types' products apart.
-// A row's sums are float32 for up to 32 terms of a lane, which meet in a tree where registers hold the row and in float64 where they do
-// not, in an order that its length and alignment alone fix.
+// A row's sums are float32 where registers hold it (up to 32 terms a lane, then a tree), and float64, or 32 terms at a time in float32 and
+// these in float64, where they do not: in an order that its length and alignment alone fix.
 #include <type_traits>
 
 #include "rows.h"
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(kLanes > kWave ? kLanes : kThreads) void rows_backw
   }
 }
 
-constexpr int kAtATime = 32;
+constexpr int kAtATime = 32;  // terms of a thread's sums in float32, before they go on in float64 (all of them there: 1.2 times as long in float32)
 
 // rows that no registers hold; a workgroup adds its rows' shares of the weight's gradient up in its own row of `parts`
 template <typename T>
